@@ -303,6 +303,150 @@ extern "C" int fb_sum_slots(const float* slots, int32_t n_slots, int64_t slot_st
   return FB_OK;
 }
 
+// ---- relative position bias ----
+namespace {
+
+// Checks the bias and fills the kernels' copy of it. need_table: the table itself is read.
+int convert_relpos(RelPos& r, const fb_relpos& b, bool need_table) {
+  if (!b.starts || (need_table && !b.table)) return FB_ERR_NULL_ARG;
+  if (b.num_buckets < 2 || b.num_buckets > FB_RELPOS_MAX_BUCKETS) return FB_ERR_RELPOS;
+  if (b.bidirectional != 0 && b.bidirectional != 1) return FB_ERR_RELPOS;
+  if (b.bidirectional && (b.num_buckets < 4 || b.num_buckets % 2 != 0)) return FB_ERR_RELPOS;
+  memset(&r, 0, sizeof(r));
+  r.table = b.table;
+  r.bucket_stride = b.bucket_stride;
+  r.head_stride = b.head_stride;
+  r.nb = b.num_buckets;
+  r.two = b.bidirectional;
+  r.side = r.two ? r.nb / 2 : r.nb;
+  for (int t = 0; t < r.side - 1; ++t) {
+    if (b.starts[t] < 0 || (t > 0 && b.starts[t] < b.starts[t - 1])) return FB_ERR_RELPOS;
+    r.starts[t] = b.starts[t];
+  }
+  return FB_OK;
+}
+
+// The problems the biased attention takes: any of fb_jvp_fwd without row segments and float32 key-side outputs.
+int check_relpos_problem(const fb_problem& pr) {
+  FB_TRY(check_problem(pr));
+  if (pr.seg_rows[0] != 0 || pr.seg_shift[0] != 0) return FB_ERR_MODE;
+  if (pr.flags & (FB_FLAG_KV_OUT_F32 | FB_FLAG_KV_ACCUMULATE | FB_FLAG_SEG_KEYS)) return FB_ERR_MODE;
+  if (pr.seqlen_q > (1 << 30) || pr.seqlen_k > (1 << 30)) return FB_ERR_TOO_LARGE;
+  return FB_OK;
+}
+
+int relpos_tiles(const fb_problem& pr) {
+  const int rows = use_tensor_cores(pr) ? kTcOwnerRows : kSimtOwnerRows;
+  return (pr.seqlen_q + rows - 1) / rows;
+}
+
+int check_bias_sizes(int dtype, int heads, int sq, int sk) {
+  if (dtype != FB_BF16 && dtype != FB_F16 && dtype != FB_F32) return FB_ERR_DTYPE;
+  if (heads <= 0 || sq < 0 || sk < 0) return FB_ERR_SHAPE;
+  if (heads > 65535 || sq > (1 << 20) || sk > (1 << 30)) return FB_ERR_TOO_LARGE;
+  return FB_OK;
+}
+
+}  // namespace
+
+extern "C" int fb_relpos_fwd(const fb_relpos_fwd_args* a, fb_stream_t stream) {
+  tl_launches = 0;
+  if (!a) return FB_ERR_NULL_ARG;
+  FB_TRY(check_relpos_problem(a->prob));
+  RelPos rel;
+  FB_TRY(convert_relpos(rel, a->bias, true));
+  FB_TRY(check_tensor(a->q, true)); FB_TRY(check_tensor(a->k, true)); FB_TRY(check_tensor(a->v, true));
+  FB_TRY(check_tensor(a->out, true));
+  if (!a->lse) return FB_ERR_NULL_ARG;
+  if (a->prob.total_q == 0) return FB_OK;
+  Params p;
+  fill_problem(p, a->prob);
+  FB_TRY(device_setup(&p.status));
+  p.q = cvt(a->q); p.k = cvt(a->k); p.v = cvt(a->v); p.o = cvt(a->out);
+  p.lse = a->lse;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  int n = use_tensor_cores(a->prob) ? launch_tc_fwd_rel(p, rel, s) : launch_simt_fwd_rel(p, rel, s);
+  if (n < 0) { if (n == FB_ERR_CUDA) record_cuda(cudaGetLastError()); return n; }
+  tl_launches = n;
+  return FB_OK;
+}
+
+extern "C" int fb_relpos_bwd(const fb_relpos_bwd_args* a, fb_stream_t stream) {
+  tl_launches = 0;
+  if (!a) return FB_ERR_NULL_ARG;
+  FB_TRY(check_relpos_problem(a->prob));
+  RelPos rel;
+  FB_TRY(convert_relpos(rel, a->bias, true));
+  FB_TRY(check_tensor(a->q, true)); FB_TRY(check_tensor(a->k, true)); FB_TRY(check_tensor(a->v, true));
+  FB_TRY(check_tensor(a->dout, true));
+  FB_TRY(check_tensor(a->dq, false)); FB_TRY(check_tensor(a->dk, false)); FB_TRY(check_tensor(a->dv, false));
+  if (!a->lse || !a->dpsum || (a->dtable && !a->workspace)) return FB_ERR_NULL_ARG;
+  if (a->prob.total_q == 0 || a->prob.total_k == 0) return FB_OK;
+  Params p;
+  fill_problem(p, a->prob);
+  FB_TRY(device_setup(&p.status));
+  p.q = cvt(a->q); p.k = cvt(a->k); p.v = cvt(a->v); p.dout = cvt(a->dout);
+  p.lse = const_cast<float*>(a->lse); p.dpsum = const_cast<float*>(a->dpsum);
+  p.dq = cvt(a->dq); p.dk = cvt(a->dk); p.dv = cvt(a->dv);
+  rel.dpart = a->dtable ? a->workspace : nullptr;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  int n = use_tensor_cores(a->prob) ? launch_tc_bwd_rel(p, rel, s) : launch_simt_bwd_rel(p, rel, s);
+  if (n >= 0 && a->dtable) {
+    const int r = launch_rel_reduce(p.dtype, rel.dpart, p.B, p.Hq, relpos_tiles(a->prob), rel.nb, a->dtable, a->dtable_bucket_stride,
+                                    a->dtable_head_stride, s);
+    n = r < 0 ? r : n + r;
+  }
+  if (n < 0) { if (n == FB_ERR_CUDA) record_cuda(cudaGetLastError()); return n; }
+  tl_launches = n;
+  return FB_OK;
+}
+
+extern "C" size_t fb_relpos_workspace_bytes(const fb_problem* pr, int num_buckets) {
+  if (!pr || check_relpos_problem(*pr) != FB_OK || num_buckets < 2 || num_buckets > FB_RELPOS_MAX_BUCKETS) return 0;
+  return sizeof(float) * (size_t)pr->batch * (size_t)pr->heads_q * (size_t)relpos_tiles(*pr) * (size_t)num_buckets;
+}
+
+extern "C" int fb_relpos_bias(const fb_relpos_bias_args* a, fb_stream_t stream) {
+  tl_launches = 0;
+  if (!a) return FB_ERR_NULL_ARG;
+  FB_TRY(check_bias_sizes(a->dtype, a->heads, a->seqlen_q, a->seqlen_k));
+  RelPos rel;
+  FB_TRY(convert_relpos(rel, a->bias, true));
+  if (!a->out) return FB_ERR_NULL_ARG;
+  if (reinterpret_cast<uintptr_t>(a->out) % 16 != 0) return FB_ERR_ALIGNMENT;
+  if (a->seqlen_q == 0 || a->seqlen_k == 0) return FB_OK;
+  int* status_word = nullptr;
+  FB_TRY(device_setup(&status_word));
+  int n = launch_relpos_fill(a->dtype, rel, a->heads, a->seqlen_q, a->seqlen_k, a->out, reinterpret_cast<cudaStream_t>(stream));
+  if (n < 0) { if (n == FB_ERR_CUDA) record_cuda(cudaGetLastError()); return n; }
+  tl_launches = n;
+  return FB_OK;
+}
+
+extern "C" int fb_relpos_bias_grad(const fb_relpos_bias_grad_args* a, fb_stream_t stream) {
+  tl_launches = 0;
+  if (!a) return FB_ERR_NULL_ARG;
+  FB_TRY(check_bias_sizes(a->dtype, a->heads, a->seqlen_q, a->seqlen_k));
+  RelPos rel;
+  FB_TRY(convert_relpos(rel, a->bias, false));
+  if (!a->grad || !a->dtable || !a->workspace) return FB_ERR_NULL_ARG;
+  if (reinterpret_cast<uintptr_t>(a->grad) % 16 != 0) return FB_ERR_ALIGNMENT;
+  if (a->seqlen_q == 0 || a->seqlen_k == 0) return FB_ERR_SHAPE;
+  int* status_word = nullptr;
+  FB_TRY(device_setup(&status_word));
+  rel.dpart = a->workspace;
+  int n = launch_relpos_grad(a->dtype, rel, a->heads, a->seqlen_q, a->seqlen_k, a->grad, a->dtable, a->dtable_bucket_stride,
+                             a->dtable_head_stride, reinterpret_cast<cudaStream_t>(stream));
+  if (n < 0) { if (n == FB_ERR_CUDA) record_cuda(cudaGetLastError()); return n; }
+  tl_launches = n;
+  return FB_OK;
+}
+
+extern "C" size_t fb_relpos_bias_workspace_bytes(int heads, int sq, int sk, int num_buckets) {
+  if (check_bias_sizes(FB_BF16, heads, sq, sk) != FB_OK || sq == 0 || sk == 0 || num_buckets < 2 || num_buckets > FB_RELPOS_MAX_BUCKETS) return 0;
+  return sizeof(float) * (size_t)heads * (size_t)relpos_bias_parts(heads, sq, sk) * (size_t)num_buckets;
+}
+
 extern "C" int fb_last_launch_count(void) { return tl_launches; }
 
 extern "C" int fb_check_device_status(void) {
@@ -335,6 +479,7 @@ extern "C" const char* fb_status_string(int status) {
     case FB_ERR_CUDA: return "CUDA call failed";
     case FB_ERR_MODE: return "inconsistent combination of optional tensors";
     case FB_ERR_TOO_LARGE: return "size exceeds a documented maximum";
+    case FB_ERR_RELPOS: return "the bias table needs 2 to 128 buckets (even and at least 4 when bidirectional) and ascending bucket starts >= 0";
     case FB_ERR_DEVICE_TIMEOUT: return "a bounded device-side wait gave up";
   }
   return "unknown status";
@@ -382,6 +527,11 @@ extern "C" size_t fb_abi_sizeof(int which) {
     case 4: return sizeof(fb_hvp_args);
     case 5: return sizeof(fb_bwd_noalloc_args);
     case 6: return sizeof(fb_kv_scatter);
+    case 8: return sizeof(fb_relpos);
+    case 9: return sizeof(fb_relpos_fwd_args);
+    case 10: return sizeof(fb_relpos_bwd_args);
+    case 11: return sizeof(fb_relpos_bias_args);
+    case 12: return sizeof(fb_relpos_bias_grad_args);
   }
   return 0;
 }

@@ -57,6 +57,46 @@ struct Params {
   long long wait_budget;  // clock budget of one bounded wait (test hook instantiation only)
 };
 
+// Learned relative position bias (fb_relpos), passed to the kernels that add it as a parameter of its own, so that the
+// others keep theirs as they are.
+struct RelPos {
+  const void* table;  // (bucket, head), the problem's dtype
+  int64_t bucket_stride, head_stride;
+  int nb, side, two;  // buckets in all / per side, 1 = both sides have buckets of their own
+  float* dpart;       // backward: partial table gradients [(batch, query head)][query tile][nb], or nullptr
+  int starts[FB_RELPOS_MAX_BUCKETS - 1];  // side - 1 entries
+};
+struct NoRel {};
+
+// Bucket of relative position r (key - query): the number of bucket starts at or below its distance. Each bucket is one
+// interval of r (r falls monotonically through the buckets of a side), so a range of positions whose ends share a
+// bucket lies in it altogether.
+__device__ __forceinline__ int relpos_bucket(int r, const int* starts, int side, int two) {
+  const int n = two ? abs(r) : max(-r, 0);
+  int lo = 0, hi = side - 1;  // answer in [lo, hi]
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (starts[mid] <= n) lo = mid + 1;
+    else hi = mid;
+  }
+  return lo + ((two && r > 0) ? side : 0);
+}
+// Sum of `v` over the lanes that hold the same key, for keys that form one run of neighbouring lanes each; valid in the
+// first lane of a run. Fixed order.
+__device__ __forceinline__ float run_sum(float v, int key, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const float ov = __shfl_down_sync(0xffffffffu, v, o);
+    const int ok = __shfl_down_sync(0xffffffffu, key, o);
+    if (lane + o < 32 && ok == key) v += ov;
+  }
+  return v;
+}
+__device__ __forceinline__ bool run_head(int key, int lane) {
+  const int prev = __shfl_up_sync(0xffffffffu, key, 1);
+  return lane == 0 || prev != key;
+}
+
 struct SeqInfo {
   int q0, k0;    // first global row of this sequence
   int sq, sk;    // its lengths
@@ -114,6 +154,19 @@ int launch_simt_bwd(const Params& p, cudaStream_t stream);
 int launch_row_stats(const Params& p, cudaStream_t stream);
 int launch_tc_fwd(const Params& p, cudaStream_t stream);
 int launch_tc_bwd(const Params& p, cudaStream_t stream);
+// the same with a relative position bias (first order only); launch_rel_reduce adds up the partial table gradients of
+// `ntiles` query tiles per (batch, head)
+int launch_simt_fwd_rel(const Params& p, const RelPos& rel, cudaStream_t stream);
+int launch_simt_bwd_rel(const Params& p, const RelPos& rel, cudaStream_t stream);
+int launch_tc_fwd_rel(const Params& p, const RelPos& rel, cudaStream_t stream);
+int launch_tc_bwd_rel(const Params& p, const RelPos& rel, cudaStream_t stream);
+int launch_rel_reduce(int dtype, const float* part, int batch, int heads, int ntiles, int nb, void* dtable, int64_t bucket_stride,
+                      int64_t head_stride, cudaStream_t stream);
+int launch_relpos_fill(int dtype, const RelPos& rel, int heads, int sq, int sk, void* out, cudaStream_t stream);
+int launch_relpos_grad(int dtype, const RelPos& rel, int heads, int sq, int sk, const void* grad, void* dtable, int64_t bucket_stride,
+                       int64_t head_stride, cudaStream_t stream);
+int64_t relpos_bias_parts(int heads, int sq, int sk);  // partial table gradients per head of launch_relpos_grad
+constexpr int kTcOwnerRows = 128, kSimtOwnerRows = 16;  // query rows per partial table gradient
 int launch_tc_fwd_wait_hook(const Params& p, cudaStream_t stream);  // test instantiation, see fb_debug_wait_timeout
 int launch_sum_slots(const float* slots, int n_slots, int64_t slot_stride, int64_t count, int64_t period, const int64_t* valid, float* out,
                      cudaStream_t stream);

@@ -60,12 +60,32 @@ __device__ __forceinline__ void store_row(const SeqT& t, int head, int64_t row, 
   for (int i = 0; i < D / 32; ++i) dst[lane + 32 * i] = from_f<T>(acc[i] * mul);
 }
 
+// The relative position bias of one head in shared memory (BIAS kernels): table column, bucket starts and, for the
+// table's gradient, one accumulator per warp and bucket.
+struct RelSmem {
+  float tab[FB_RELPOS_MAX_BUCKETS];
+  int starts[FB_RELPOS_MAX_BUCKETS];
+  float acc[kWarps][FB_RELPOS_MAX_BUCKETS];
+};
+template <typename T>
+__device__ __forceinline__ void rel_load(RelSmem& rs, const RelPos& rel, int h) {
+  for (int t = threadIdx.x; t < rel.nb; t += kThreads) rs.tab[t] = to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + h * rel.head_stride]);
+  for (int t = threadIdx.x; t < rel.side - 1; t += kThreads) rs.starts[t] = rel.starts[t];
+}
+template <bool BIAS> struct RelArg { using type = NoRel; };
+template <> struct RelArg<true> { using type = RelPos; };
+
 // ---------------------------------------------------------------------------------------------
 // Forward / JVP forward
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D, bool TANGENT>
-__global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p) {
+template <typename T, int D, bool TANGENT, bool BIAS>
+__global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __grid_constant__ typename RelArg<BIAS>::type rel) {
   extern __shared__ float smem[];
+  [[maybe_unused]] RelSmem* rs = nullptr;
+  if constexpr (BIAS) {
+    __shared__ RelSmem rs_;
+    rs = &rs_;
+  }
   constexpr int LD = D + 1;
   constexpr int NC = D / 32;
   float* qs = smem;
@@ -81,6 +101,7 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p) {
   if (m0 >= si.sq) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nq = min(kOwn, si.sq - m0);
+  if constexpr (BIAS) rel_load<T>(*rs, rel, h);
   load_rows<T, D>(qs, p.q, h, si.q0 + m0, nq, kOwn);
   if (TANGENT) load_rows<T, D>(qds, p.qd, h, si.q0 + m0, nq, kOwn);
   int n_end = si.sk;
@@ -108,6 +129,10 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p) {
         for (int d = 0; d < D; ++d) s = fmaf(qs[lr * LD + d], ks[lane * LD + d], s);
         s *= p.scale;
         bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j));
+        if constexpr (BIAS) {
+          if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->starts, rel.side, rel.two)];
+          ok = ok && s != -INFINITY;  // a bias of -inf hides the pair
+        }
         if (ok) {
           float mn = fmaxf(m_run[r], s);
           l_run[r] = l_run[r] * expf(m_run[r] - mn) + expf(s - mn);
@@ -152,6 +177,9 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p) {
       }
       s *= p.scale; sd *= p.scale;
       bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j)) && lse[r] != -INFINITY;
+      if constexpr (BIAS) {
+        if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->starts, rel.side, rel.two)];
+      }
       float pr = ok ? expf(s - lse[r]) : 0.f;
       float w = pr * sd;
       zp[r] += w;
@@ -218,9 +246,14 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p) {
 // ---------------------------------------------------------------------------------------------
 // Backward, query-row owner: dQ, dQ_dot
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D, bool TANGENT>
-__global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p) {
+template <typename T, int D, bool TANGENT, bool BIAS>
+__global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p, const __grid_constant__ typename RelArg<BIAS>::type rel) {
   extern __shared__ float smem[];
+  [[maybe_unused]] RelSmem* rs = nullptr;
+  if constexpr (BIAS) {
+    __shared__ RelSmem rs_;
+    rs = &rs_;
+  }
   constexpr int LD = D + 1;
   constexpr int NC = D / 32;
   float* qs = smem;
@@ -235,9 +268,18 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p) {
   const int b = blockIdx.z, h = blockIdx.y, hk = h / (p.Hq / p.Hkv);
   const SeqInfo si = seq_info(p, b);
   const int m0 = blockIdx.x * kOwn;
-  if (m0 >= si.sq) return;
+  if (m0 >= si.sq) {
+    if constexpr (BIAS) {
+      if (rel.dpart && (int)threadIdx.x < rel.nb) rel.dpart[((int64_t)(b * p.Hq + h) * gridDim.x + blockIdx.x) * rel.nb + threadIdx.x] = 0.f;
+    }
+    return;
+  }
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int nq = min(kOwn, si.sq - m0);
+  if constexpr (BIAS) {
+    rel_load<T>(*rs, rel, h);
+    for (int t = threadIdx.x; t < kWarps * FB_RELPOS_MAX_BUCKETS; t += kThreads) (&rs->acc[0][0])[t] = 0.f;
+  }
   load_rows<T, D>(qs, p.q, h, si.q0 + m0, nq, kOwn);
   load_rows<T, D>(dos, p.dout, h, si.q0 + m0, nq, kOwn);
   if (TANGENT) {
@@ -291,9 +333,20 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p) {
       }
       s *= p.scale; sd *= p.scale;
       bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j)) && lse[r] != -INFINITY;
+      [[maybe_unused]] int bucket = 0;
+      if constexpr (BIAS) {
+        bucket = relpos_bucket(j - i - (si.sk - si.sq), rs->starts, rel.side, rel.two);
+        if (ok) s += rs->tab[bucket];
+      }
       float pr = ok ? expf(s - lse[r]) : 0.f;
       float a = dp - dps[r];
       float ds = pr * a;
+      if constexpr (BIAS) {  // neighbouring lanes hold neighbouring positions: equal buckets form runs
+        const bool first = run_head(bucket, lane);
+        const float sum = run_sum(ds, bucket, lane);
+        if (first) rs->acc[warp][bucket] += sum;
+        __syncwarp();
+      }
       float dsd = 0.f;
       if (TANGENT) dsd = pr * (sd - z1[r]) * a + pr * (dpd - ddt[r]);
       for (int jj = 0; jj < kTile; ++jj) {
@@ -315,14 +368,27 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p) {
     store_row<T, D>(p.dq, h, si.q0 + i, lane, acc[r], p.scale);
     if (TANGENT) store_row<T, D>(p.dqd, h, si.q0 + i, lane, accd[r], p.scale);
   }
+  if constexpr (BIAS) {
+    __syncthreads();
+    if (rel.dpart && (int)threadIdx.x < rel.nb) {
+      float sum = 0.f;
+      for (int w = 0; w < kWarps; ++w) sum += rs->acc[w][threadIdx.x];
+      rel.dpart[((int64_t)(b * p.Hq + h) * gridDim.x + blockIdx.x) * rel.nb + threadIdx.x] = sum;
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------------------------
 // Backward, key-row owner: dK, dV, dK_dot, dV_dot (sums over the G query heads of a kv head)
 // ---------------------------------------------------------------------------------------------
-template <typename T, int D, bool TANGENT>
-__global__ void __launch_bounds__(kThreads) simt_dkv_kernel(Params p) {
+template <typename T, int D, bool TANGENT, bool BIAS>
+__global__ void __launch_bounds__(kThreads) simt_dkv_kernel(Params p, const __grid_constant__ typename RelArg<BIAS>::type rel) {
   extern __shared__ float smem[];
+  [[maybe_unused]] RelSmem* rs = nullptr;
+  if constexpr (BIAS) {
+    __shared__ RelSmem rs_;
+    rs = &rs_;
+  }
   constexpr int LD = D + 1;
   constexpr int NC = D / 32;
   float* ks = smem;
@@ -358,6 +424,10 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(Params p) {
 
   for (int g = 0; g < G; ++g) {
     const int h = hk * G + g;
+    if constexpr (BIAS) {
+      __syncthreads();  // the previous head's column is still being read
+      rel_load<T>(*rs, rel, h);
+    }
     for (int m0 = m_start; m0 < si.sq; m0 += kTile) {
       const int nq = min(kTile, si.sq - m0);
       __syncthreads();
@@ -395,6 +465,9 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(Params p) {
         s *= p.scale; sd *= p.scale;
         const float lse = st[lane];
         bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j)) && lse != -INFINITY;
+        if constexpr (BIAS) {
+          if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->starts, rel.side, rel.two)];
+        }
         float pr = ok ? expf(s - lse) : 0.f;
         float a = dp - st[kTile + lane];
         float ds = pr * a;
@@ -468,34 +541,36 @@ int set_smem(K kernel, size_t bytes) {
   return e == cudaSuccess ? 0 : FB_ERR_CUDA;
 }
 
-template <typename T, int D, bool TANGENT>
-int fwd_impl(const Params& p, cudaStream_t s) {
+template <typename T, int D, bool TANGENT, bool BIAS>
+int fwd_impl(const Params& p, const typename RelArg<BIAS>::type& rel, cudaStream_t s) {
   size_t bytes = sizeof(float) * (size_t)(D + 1) * (2 * kOwn + 4 * kTile);
-  auto kern = simt_fwd_kernel<T, D, TANGENT>;
+  auto kern = simt_fwd_kernel<T, D, TANGENT, BIAS>;
   if (set_smem(kern, bytes)) return FB_ERR_CUDA;
   dim3 grid((p.Sq + kOwn - 1) / kOwn, p.Hq, p.B);
-  kern<<<grid, kThreads, bytes, s>>>(p);
+  kern<<<grid, kThreads, bytes, s>>>(p, rel);
   return cudaGetLastError() == cudaSuccess ? 1 : FB_ERR_CUDA;
 }
 
-template <typename T, int D, bool TANGENT>
-int bwd_impl(const Params& p, cudaStream_t s) {
+template <typename T, int D, bool TANGENT, bool BIAS>
+int bwd_impl(const Params& p, const typename RelArg<BIAS>::type& rel, cudaStream_t s) {
   int n = 0;
-  if (p.dq.ptr || p.dqd.ptr) {
+  bool query_side = p.dq.ptr || p.dqd.ptr;
+  if constexpr (BIAS) query_side = query_side || rel.dpart;
+  if (query_side) {
     size_t bytes = sizeof(float) * (size_t)(D + 1) * (4 * kOwn + 4 * kTile);
-    auto kern = simt_dq_kernel<T, D, TANGENT>;
+    auto kern = simt_dq_kernel<T, D, TANGENT, BIAS>;
     if (set_smem(kern, bytes)) return FB_ERR_CUDA;
     dim3 grid((p.Sq + kOwn - 1) / kOwn, p.Hq, p.B);
-    kern<<<grid, kThreads, bytes, s>>>(p);
+    kern<<<grid, kThreads, bytes, s>>>(p, rel);
     if (cudaGetLastError() != cudaSuccess) return FB_ERR_CUDA;
     ++n;
   }
   if (p.dk.ptr || p.dv.ptr || p.dkd.ptr || p.dvd.ptr) {
     size_t bytes = sizeof(float) * ((size_t)(D + 1) * (4 * kOwn + 4 * kTile) + 4 * kTile);
-    auto kern = simt_dkv_kernel<T, D, TANGENT>;
+    auto kern = simt_dkv_kernel<T, D, TANGENT, BIAS>;
     if (set_smem(kern, bytes)) return FB_ERR_CUDA;
     dim3 grid((p.Sk + kOwn - 1) / kOwn, p.Hkv, p.B);
-    kern<<<grid, kThreads, bytes, s>>>(p);
+    kern<<<grid, kThreads, bytes, s>>>(p, rel);
     if (cudaGetLastError() != cudaSuccess) return FB_ERR_CUDA;
     ++n;
   }
@@ -505,14 +580,22 @@ int bwd_impl(const Params& p, cudaStream_t s) {
 template <typename T>
 int fwd_dispatch(const Params& p, cudaStream_t s) {
   const bool t = p.qd.ptr != nullptr;
-  if (p.D == 64) return t ? fwd_impl<T, 64, true>(p, s) : fwd_impl<T, 64, false>(p, s);
-  return t ? fwd_impl<T, 128, true>(p, s) : fwd_impl<T, 128, false>(p, s);
+  if (p.D == 64) return t ? fwd_impl<T, 64, true, false>(p, {}, s) : fwd_impl<T, 64, false, false>(p, {}, s);
+  return t ? fwd_impl<T, 128, true, false>(p, {}, s) : fwd_impl<T, 128, false, false>(p, {}, s);
 }
 template <typename T>
 int bwd_dispatch(const Params& p, cudaStream_t s) {
   const bool t = p.qd.ptr != nullptr;
-  if (p.D == 64) return t ? bwd_impl<T, 64, true>(p, s) : bwd_impl<T, 64, false>(p, s);
-  return t ? bwd_impl<T, 128, true>(p, s) : bwd_impl<T, 128, false>(p, s);
+  if (p.D == 64) return t ? bwd_impl<T, 64, true, false>(p, {}, s) : bwd_impl<T, 64, false, false>(p, {}, s);
+  return t ? bwd_impl<T, 128, true, false>(p, {}, s) : bwd_impl<T, 128, false, false>(p, {}, s);
+}
+template <typename T>
+int fwd_rel_dispatch(const Params& p, const RelPos& rel, cudaStream_t s) {
+  return p.D == 64 ? fwd_impl<T, 64, false, true>(p, rel, s) : fwd_impl<T, 128, false, true>(p, rel, s);
+}
+template <typename T>
+int bwd_rel_dispatch(const Params& p, const RelPos& rel, cudaStream_t s) {
+  return p.D == 64 ? bwd_impl<T, 64, false, true>(p, rel, s) : bwd_impl<T, 128, false, true>(p, rel, s);
 }
 
 }  // namespace
@@ -531,6 +614,25 @@ int launch_simt_bwd(const Params& p, cudaStream_t s) {
     case FB_BF16: return bwd_dispatch<__nv_bfloat16>(p, s);
     case FB_F16: return bwd_dispatch<__half>(p, s);
     case FB_F32: return bwd_dispatch<float>(p, s);
+  }
+  return FB_ERR_DTYPE;
+}
+
+int launch_simt_fwd_rel(const Params& p, const RelPos& rel, cudaStream_t s) {
+  switch (p.dtype) {
+    case FB_BF16: return fwd_rel_dispatch<__nv_bfloat16>(p, rel, s);
+    case FB_F16: return fwd_rel_dispatch<__half>(p, rel, s);
+    case FB_F32: return fwd_rel_dispatch<float>(p, rel, s);
+  }
+  return FB_ERR_DTYPE;
+}
+
+int launch_simt_bwd_rel(const Params& p, const RelPos& rel, cudaStream_t s) {
+  static_assert(kOwn == kSimtOwnerRows, "rows of the partial table gradients");
+  switch (p.dtype) {
+    case FB_BF16: return bwd_rel_dispatch<__nv_bfloat16>(p, rel, s);
+    case FB_F16: return bwd_rel_dispatch<__half>(p, rel, s);
+    case FB_F32: return bwd_rel_dispatch<float>(p, rel, s);
   }
   return FB_ERR_DTYPE;
 }

@@ -61,6 +61,20 @@ static_assert(kRoleThreads * (kLaunchRegs - kRoleRegs) >= kPwThreads * (kPwRegs 
 constexpr int kSmemLimit = 232448;  // 227 KB opt-in maximum per CTA
 constexpr int kMiscBytes = 3072;    // barriers + TMEM slot + abort flag + DKV row statistics (2 buffers); FWD: x2, row-max exchange
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+// Relative position bias: a block of BM owner rows x BN streamed rows spans kRelSpan positions; the statistics warp
+// stages their biases (and, for the table's gradient, their buckets) per block, two buffers.
+constexpr int kRelSpan = BM + BN;  // BM + BN - 1 positions
+enum {                             // byte offsets in the bias area behind the misc area
+  REL_TAB = 0,                                     // this head's table column, in log2 units
+  REL_STARTS = REL_TAB + FB_RELPOS_MAX_BUCKETS * 4,
+  REL_UNI = REL_STARTS + FB_RELPOS_MAX_BUCKETS * 4,  // [2] the bucket all pairs of the block fall in, or -1; [2] its bias
+  REL_BIAS = REL_UNI + 16,                         // [2][kRelSpan]
+  REL_IDS = REL_BIAS + 2 * kRelSpan * 4,           // [2][kRelSpan] (KIND_DQ)
+  REL_DIAG = REL_IDS + 2 * kRelSpan * 4,           // [pointwise warps][32] (KIND_DQ)
+  REL_ACC = REL_DIAG + NWG * 4 * 32 * 4,           // [pointwise warps][FB_RELPOS_MAX_BUCKETS] (KIND_DQ)
+  REL_BYTES = REL_ACC + NWG * 4 * FB_RELPOS_MAX_BUCKETS * 4
+};
 constexpr float kRescaleThreshold = 8.f;  // log2 units: rescale accumulators when the row max grew by > 2^8
 // Experiment, off by default: every kPolyPeriod-th pair of exponentials computed on the FMA pipe
 // (ex2_poly2) instead of the special-function unit (16 ex2 per clock and SM), in the kernels whose
@@ -117,7 +131,7 @@ constexpr int ceil_pow2(int x) {
 // Compile-time shape of one instantiation.
 //   FWD: FIRST = accumulate O with online softmax (false = LSE known, O is an input).
 //   DQ/DKV: FIRST = first-order outputs, TANGENT = directional-derivative outputs, DOD = dO_dot given.
-template <int KIND, int D, bool TANGENT, bool FIRST, bool DOD>
+template <int KIND, int D, bool TANGENT, bool FIRST, bool DOD, bool BIAS = false>
 struct Cfg {
   static constexpr bool kFwd = KIND == KIND_FWD;
   static constexpr int nOuter = kFwd ? (TANGENT ? 2 : 1)
@@ -158,7 +172,7 @@ struct Cfg {
   static constexpr int outerBytes = nOuter * outerTile;
   static constexpr int g0Bytes = nG0 * innerTile;
   static constexpr int g1Bytes = nG1 * innerTile;
-  static constexpr int miscBytes = kMiscBytes;
+  static constexpr int miscBytes = kMiscBytes + (BIAS ? REL_BYTES : 0);
   static constexpr int tileBudget = kSmemLimit - miscBytes;
   // Shared-memory stages. With two TMEM stages the S-like GEMMs of block i+1 are issued before the
   // output GEMMs of block i, so g0 needs two stages and a g1 that also feeds S-like GEMMs three;
@@ -315,9 +329,14 @@ __device__ __forceinline__ void gemm_ts_kmajor(uint32_t d_tmem, uint32_t a_tmem,
 // HOOK = true is a test instantiation: its bounded waits use the budget passed in Params and its
 // producer leaves out the loads of streamed block 1, so that a wait runs out and the CTA takes the
 // abort path (status word set, nothing issued afterwards, resources released) without any fault.
-template <typename T, int KIND, int D, bool TANGENT, bool FIRST, bool DOD, bool HOOK = false>
+//
+// BIAS = true adds a learned relative position bias to S (first-order kernels): the statistics warp stages the biases of
+// every block's positions, handed over with the block's first S-like tile; KIND_DQ also sums dS by bucket.
+template <typename T, int KIND, int D, bool TANGENT, bool FIRST, bool DOD, bool HOOK = false, bool BIAS = false>
 struct TcCta {
-  using C = Cfg<KIND, D, TANGENT, FIRST, DOD>;
+  using C = Cfg<KIND, D, TANGENT, FIRST, DOD, BIAS>;
+  static_assert(!BIAS || !TANGENT, "the bias is built into the first-order kernels");
+  static constexpr bool kStager = KIND == KIND_DKV || BIAS;  // the statistics warp has work
   static constexpr bool kFwd = KIND == KIND_FWD, kDq = KIND == KIND_DQ, kDkv = KIND == KIND_DKV;
   static constexpr int ST = C::ST, SS0 = C::SS0, SS1 = C::SS1, nS = C::nS;
   static constexpr int SS0d = SS0 > 0 ? SS0 : 1;
@@ -354,6 +373,8 @@ struct TcCta {
   static_assert(!kDkv || kSplitA, "the DKV statistics warp signals on the barrier of the first S tile");
 
   // ---- CTA state (same value in every thread) ----
+  const RelPos* rel = nullptr;  // BIAS
+  uint8_t* rel_area;
   const TmaMaps& maps;
   const Params& p;
   uint8_t* const smem;
@@ -380,6 +401,9 @@ struct TcCta {
   float m_used, l_sum, z_sum;   // FWD (l_sum, z_sum: this warpgroup's columns only)
   float lse2, dps, z1v, ddt;    // LSE-known FWD and DQ
   long long pw_wait, pw_work, pw_ld0, pw_st;
+  float2 rel_sum;    // KIND_DQ with a bias: running sum of dS over blocks that lie in bucket rel_cur altogether
+  int rel_cur;
+  int64_t rel_part;  // this tile's row of the partial table gradients
 
   __device__ __forceinline__ TcCta(const TmaMaps& maps_, const Params& p_, uint8_t* smem_) : maps(maps_), p(p_), smem(smem_) {}
 
@@ -438,6 +462,7 @@ struct TcCta {
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::tileBytes + 8 * BAR_COUNT);
     abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     stats_base = reinterpret_cast<float*>(smem + C::tileBytes + 256);
+    rel_area = smem + C::tileBytes + kMiscBytes;
 
     warp = threadIdx.x >> 5;
     lane = threadIdx.x & 31;
@@ -471,7 +496,11 @@ struct TcCta {
     // the most queries; those go first.
     const int tile = (!kDkv && p.causal) ? p.ntiles - 1 - tidx : tidx;
     r0 = tile * BM;
-    if (r0 >= own_len) return false;  // (the same decision in every CTA of a cluster)
+    if (BIAS && kDq) rel_part = (int64_t)(b * p.Hq + head) * p.ntiles + tile;
+    if (r0 >= own_len) {  // (the same decision in every CTA of a cluster)
+      if (BIAS && kDq) zero_table_part();
+      return false;
+    }
     // Causal offset (key j visible to query i iff j <= i + off). A query tile lies inside one query segment
     // (the break is a multiple of BM), so its offset is fixed here; a key tile streams query blocks of both
     // segments and takes the offset per block (pointwise()).
@@ -501,8 +530,9 @@ struct TcCta {
         uint32_t count = 1u;
         if ((i >= BAR_P_FULL && i < BAR_P_FULL + 2) || (i >= BAR_ST_EMPTY && i < BAR_ST_EMPTY + 2) || i == BAR_A_READY || i == BAR_P_HALF) count = NWG * 4;  // one arrival per pointwise warp
         // DKV: the S-like tiles a block's pointwise work starts from are complete when the MMAs have
-        // committed AND the statistics warp has staged the block's row statistics (one wait for both)
-        if (kDkv && (i == BAR_S_FULL || (i == BAR_S_FULL + 1 && !kSplit))) count = 2u;
+        // committed AND the statistics warp has staged the block's row statistics (one wait for both); the same
+        // for the staged biases in every kind
+        if (kStager && (i == BAR_S_FULL || (i == BAR_S_FULL + 1 && !kSplit))) count = 2u;
         mbar_init(bar(i), count);
       }
       *abort_flag = 0;
@@ -550,7 +580,7 @@ struct TcCta {
       } else if (n_it > 0 && warp == 1) {
         if (elect_one()) issuer();
       } else if (warp == kStatsWarp) {
-        if constexpr (kDkv) stats_stager();
+        if constexpr (kStager) stats_stager();
       }
     } else {
       if constexpr (kRealloc) reg_alloc<kPwRegs>();
@@ -827,23 +857,77 @@ struct TcCta {
       }
     }
   }
+  // BIAS: this head's column of the table (in log2 units) and the bucket starts, once per head. A DKV CTA walks
+  // through the query heads of its kv head.
+  __device__ __forceinline__ void rel_load_table(int h) {
+    float* tab = reinterpret_cast<float*>(rel_area + REL_TAB);
+    for (int t = lane; t < rel->nb; t += 32)
+      tab[t] = to_f<T>(reinterpret_cast<const T*>(rel->table)[t * rel->bucket_stride + h * rel->head_stride]) * kLog2e;
+    __syncwarp();
+  }
+  // BIAS: the biases of a block's positions. Entry u belongs to the pairs with (streamed row in block) - (owner row in
+  // tile) = u - (BM - 1). Where the block's first and last position share a bucket all pairs do (the usual case far from
+  // the diagonal) and only that bucket is noted.
+  __device__ __forceinline__ void rel_stage(int it, int buf) {
+    const int blk = kDkv ? blk_begin + (it_base + it) % blk_count : it;
+    const int c0 = blk * BN;
+    const int* starts = reinterpret_cast<const int*>(rel_area + REL_STARTS);
+    const float* tab = reinterpret_cast<const float*>(rel_area + REL_TAB);
+    // FWD, DQ: r = (c0 + c) - (r0 + row + off);  DKV (rows are keys): r = (r0 + row) - (c0 + c + off)
+    const int base = kDkv ? r0 - c0 - off + (BM - 1) : c0 - r0 - off - (BM - 1);
+    auto bucket_at = [&](int u) { return relpos_bucket(kDkv ? base - u : base + u, starts, rel->side, rel->two); };
+    const int mine = bucket_at(lane == 0 ? 0 : kRelSpan - 2);  // lane 0: first position, the others: last
+    const int first = __shfl_sync(0xffffffffu, mine, 0), last = __shfl_sync(0xffffffffu, mine, 1);
+    if (lane == 0) {
+      reinterpret_cast<int*>(rel_area + REL_UNI)[buf] = first == last ? first : -1;
+      reinterpret_cast<float*>(rel_area + REL_UNI)[2 + buf] = tab[first];
+    }
+    if (first != last) {
+      float* dst = reinterpret_cast<float*>(rel_area + REL_BIAS) + buf * kRelSpan;
+      int* ids = reinterpret_cast<int*>(rel_area + REL_IDS) + buf * kRelSpan;
+#pragma unroll
+      for (int i = 0; i < kRelSpan / 32; ++i) {
+        const int u = lane + 32 * i, t = bucket_at(u);
+        dst[u] = tab[t];
+        if (kDq) ids[u] = t;
+      }
+    }
+  }
   __device__ __forceinline__ void stats_stager() {
     float4 cur[BN / 32], nxt[BN / 32];
-    if (n_it > 0) stats_load(0, nxt);
+    int table_head = -1;
+    if constexpr (BIAS) {
+      for (int t = lane; t < rel->side - 1; t += 32) reinterpret_cast<int*>(rel_area + REL_STARTS)[t] = rel->starts[t];
+      __syncwarp();
+    }
+    if (kDkv && n_it > 0) stats_load(0, nxt);
     for (int it = 0; it < n_it; ++it) {
       const int sb_ = it & 1;
+      if (kDkv) {
 #pragma unroll
-      for (int r = 0; r < BN / 32; ++r) cur[r] = nxt[r];
-      if (it + 1 < n_it) stats_load(it + 1, nxt);
+        for (int r = 0; r < BN / 32; ++r) cur[r] = nxt[r];
+        if (it + 1 < n_it) stats_load(it + 1, nxt);
+      }
+      if constexpr (BIAS) {
+        const int h = kDkv ? head * G + (it_base + it) / blk_count : head;
+        if (h != table_head) {
+          __syncwarp();
+          rel_load_table(h);
+          table_head = h;
+        }
+      }
       warp_wait(BAR_ST_EMPTY + sb_, ((it >> 1) & 1) ^ 1);
       if (aborted()) break;
-      float* dst = stats_base + sb_ * (4 * BN);
+      if (kDkv) {
+        float* dst = stats_base + sb_ * (4 * BN);
 #pragma unroll
-      for (int r = 0; r < BN / 32; ++r) {
-        const int rr = lane + 32 * r;
-        dst[rr] = (fabsf(cur[r].x) == INFINITY) ? -INFINITY : -cur[r].x * kLog2e;  // a fully masked row has lse = -inf
-        dst[BN + rr] = -cur[r].y; dst[2 * BN + rr] = -cur[r].z; dst[3 * BN + rr] = -cur[r].w;
+        for (int r = 0; r < BN / 32; ++r) {
+          const int rr = lane + 32 * r;
+          dst[rr] = (fabsf(cur[r].x) == INFINITY) ? -INFINITY : -cur[r].x * kLog2e;  // a fully masked row has lse = -inf
+          dst[BN + rr] = -cur[r].y; dst[2 * BN + rr] = -cur[r].z; dst[3 * BN + rr] = -cur[r].w;
+        }
       }
+      if constexpr (BIAS) rel_stage(it, sb_);
       __syncwarp();
       if (lane == 0) {
         // Second arrival on the barrier the MMA issuer commits block `it`'s first S-like tiles to. Its
@@ -868,7 +952,7 @@ struct TcCta {
     __syncwarp();
     if (lane == 0) {
       mbar_arrive(bar(barrier));
-      if (kDkv && release_stats) mbar_arrive(bar(BAR_ST_EMPTY + (it & 1)));  // this warp is done with the block's statistics
+      if (kStager && release_stats) mbar_arrive(bar(BAR_ST_EMPTY + (it & 1)));  // this warp is done with the block's statistics
     }
   }
 
@@ -1000,8 +1084,31 @@ struct TcCta {
     }
     tmem_ld_wait();
     float pv[HC];
+    // With a bias the scores are brought to log2 units here and the running maximum is kept in them (`unit` = 1);
+    // without one the scale is folded into the exponent's FMA below.
+    const float unit = BIAS ? 1.f : scale2;
+    if constexpr (BIAS) {
+      const float2 sc2 = make_float2(scale2, scale2);
+      const int uni = reinterpret_cast<const int*>(rel_area + REL_UNI)[it & 1];
+      if (uni >= 0) {
+        const float b = reinterpret_cast<const float*>(rel_area + REL_UNI)[2 + (it & 1)];
 #pragma unroll
-    for (int c = 0; c < HC; ++c) pv[c] = __uint_as_float(rs[c]);
+        for (int c = 0; c < HC; c += 2) {
+          const float2 v = __ffma2_rn(make_float2(__uint_as_float(rs[c]), __uint_as_float(rs[c + 1])), sc2, make_float2(b, b));
+          pv[c] = v.x; pv[c + 1] = v.y;
+        }
+      } else {
+        const float* bias = rel_bias(it);
+#pragma unroll
+        for (int c = 0; c < HC; c += 2) {
+          const float2 v = __ffma2_rn(make_float2(__uint_as_float(rs[c]), __uint_as_float(rs[c + 1])), sc2, make_float2(bias[c], bias[c + 1]));
+          pv[c] = v.x; pv[c + 1] = v.y;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < HC; ++c) pv[c] = __uint_as_float(rs[c]);
+    }
     if (need_mask) {
 #pragma unroll
       for (int c = 0; c < HC; ++c) if (cb + c > cmax) pv[c] = -INFINITY;
@@ -1020,10 +1127,10 @@ struct TcCta {
 #pragma unroll
       for (int o = 1; o < NWG; ++o) mloc = fmaxf(mloc, xchg[((it & 1) * NWG + ((wg + o) % NWG)) * 128 + row]);
       const float m_new = fmaxf(m_used, mloc);
-      const bool grow = (m_new - m_used) * scale2 > kRescaleThreshold;  // false when both are -inf (NaN)
+      const bool grow = (m_new - m_used) * unit > kRescaleThreshold;  // false when both are -inf (NaN)
       float alpha = 1.f;
       if (grow) {
-        alpha = (m_used == -INFINITY) ? 0.f : ex2((m_used - m_new) * scale2);
+        alpha = (m_used == -INFINITY) ? 0.f : ex2((m_used - m_new) * unit);
         m_used = m_new;
         l_sum *= alpha;
         z_sum *= alpha;
@@ -1044,16 +1151,17 @@ struct TcCta {
         }
         tmem_st_wait();
       }
-      moff = (m_used == -INFINITY) ? 0.f : m_used * scale2;
+      moff = (m_used == -INFINITY) ? 0.f : m_used * unit;
     } else {
       moff = lse2;
     }
     // packed f32x2 arithmetic: two columns per FMA / add
-    const float2 sc2 = make_float2(scale2, scale2), nmoff = make_float2(-moff, -moff);
+    const float2 sc2 = make_float2(unit, unit), nmoff = make_float2(-moff, -moff);
     float2 ls2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
     for (int c2 = 0; c2 < HC / 2; ++c2) {
-      const float2 e = __ffma2_rn(make_float2(pv[2 * c2], pv[2 * c2 + 1]), sc2, nmoff);
+      const float2 e = BIAS ? __fadd2_rn(make_float2(pv[2 * c2], pv[2 * c2 + 1]), nmoff)
+                            : __ffma2_rn(make_float2(pv[2 * c2], pv[2 * c2 + 1]), sc2, nmoff);
       const float2 pe = exp2_pair(e, c2, !need_mask);
       pv[2 * c2] = pe.x;
       pv[2 * c2 + 1] = pe.y;
@@ -1092,8 +1200,25 @@ struct TcCta {
   // First-order dQ / dK,dV, one block (kernels with tangents take pw_two_phase_block): 16 streamed
   // columns at a time from the S and dP tiles, the TMEM loads of the next group in flight while
   // the current one is processed.
-  __device__ __forceinline__ void pw_bwd_block(int st, bool need_mask, int cmin, int cmax, const float* stats) {
+  // UNI: with a bias, all pairs of the block share a bucket.
+  template <bool UNI>
+  __device__ __forceinline__ void pw_bwd_block(int it, int st, bool need_mask, int cmin, int cmax, const float* stats) {
     static_assert(!TANGENT, "first-order kernels only");
+    const float* bias = nullptr;
+    float2 b2 = make_float2(0.f, 0.f);
+    if constexpr (BIAS) {
+      if constexpr (UNI) {
+        const float b = reinterpret_cast<const float*>(rel_area + REL_UNI)[2 + (it & 1)];
+        b2 = make_float2(b, b);
+      } else {
+        bias = rel_bias(it);
+      }
+    }
+    // KIND_DQ with a bias: sum of dS along the diagonals of this warp's 32 rows x HC columns. The running sum of a
+    // diagonal moves one lane up per column; the one that leaves lane 31 is complete and wraps round to lane 0, which
+    // files it.
+    float diag = 0.f;
+    float* const filed = BIAS ? reinterpret_cast<float*>(rel_area + REL_DIAG) + (warp & 7) * 32 : nullptr;
     constexpr int CW = 16;
     constexpr int NG = HC / CW;
     uint32_t bs[2][CW], bp[2][CW];
@@ -1120,6 +1245,10 @@ struct TcCta {
           nl2 = *reinterpret_cast<const float2*>(&stats[col]);
           ndp = *reinterpret_cast<const float2*>(&stats[BN + col]);
         }
+        if constexpr (BIAS) {
+          if constexpr (!UNI) b2 = make_float2(bias[gi * CW + c], bias[gi * CW + c + 1]);
+          nl2 = __fadd2_rn(nl2, b2);
+        }
         const float2 e = __ffma2_rn(make_float2(__uint_as_float(bs[buf][c]), __uint_as_float(bs[buf][c + 1])), sc2, nl2);
         float2 pe = exp2_pair(e, c2, !need_mask);
         if (need_mask) {
@@ -1127,9 +1256,26 @@ struct TcCta {
           if (col + 1 > cmax || col + 1 < cmin) pe.y = 0.f;
         }
         const float2 a = __fadd2_rn(make_float2(__uint_as_float(bp[buf][c]), __uint_as_float(bp[buf][c + 1])), ndp);
-        const float2 ds = __fmul2_rn(pe, a);
+        float2 ds = __fmul2_rn(pe, a);
+        // a row behind its sequence adds nothing to the table's gradient, whatever the table holds where it points
+        if (BIAS && kDq && !row_ok) ds = make_float2(0.f, 0.f);
         o_p[c2] = pack2<T>(pe.x, pe.y);
         o_ds[c2] = pack2<T>(ds.x, ds.y);
+        if constexpr (BIAS && kDq) {
+          if constexpr (UNI) {
+            rel_sum = __fadd2_rn(rel_sum, ds);
+          } else {
+#pragma unroll
+            for (int e2 = 0; e2 < 2; ++e2) {
+              diag = __shfl_sync(0xffffffffu, diag, (lane + 31) & 31);
+              if (lane == 0) {
+                if (gi * CW + c + e2 > 0) filed[gi * CW + c + e2 - 1] = diag;
+                diag = 0.f;
+              }
+              diag += e2 ? ds.y : ds.x;
+            }
+          }
+        }
       }
       // the packed columns of streamed columns [16*kk, 16*kk+16) live at tile column 16*kk
       const uint32_t pcol = lane_off + cb + gi * CW;
@@ -1145,6 +1291,50 @@ struct TcCta {
         if (prof) pw_ld0 += clock64() - tq2;
       }
     }
+    if constexpr (BIAS && kDq && !UNI) {
+      static_assert(HC == 32, "31 filed diagonals and one per lane");
+      __syncwarp();
+      // entry of (lane 31's row, column 0): the first diagonal
+      const int* ids = reinterpret_cast<const int*>(rel_area + REL_IDS) + (it & 1) * kRelSpan + cb - (warp & 3) * 32 + (BM - 1);
+      rel_add(lane < 31 ? filed[lane] : 0.f, lane < 31 ? ids[lane - 31] : -1);
+      rel_add(diag, ids[31 - lane]);
+    }
+  }
+  // This thread's biases of block `it`: entry c belongs to column cb + c.
+  __device__ __forceinline__ const float* rel_bias(int it) const {
+    return reinterpret_cast<const float*>(rel_area + REL_BIAS) + (it & 1) * kRelSpan + cb - row + (BM - 1);
+  }
+  // KIND_DQ with a bias, one warp: adds every lane's `v` to its bucket (equal buckets sit in neighbouring lanes; -1: none).
+  __device__ __forceinline__ void rel_add(float v, int bucket) {
+    float* acc = reinterpret_cast<float*>(rel_area + REL_ACC) + (warp & 7) * FB_RELPOS_MAX_BUCKETS;
+    const bool first = run_head(bucket, lane);
+    v = run_sum(v, bucket, lane);
+    if (first && bucket >= 0) acc[bucket] += v;
+    __syncwarp();
+  }
+  // The sum of the blocks whose pairs all fall in bucket rel_cur, kept per thread until the bucket changes.
+  __device__ __forceinline__ void rel_flush(int next) {
+    if (next == rel_cur) return;
+    if (rel_cur >= 0) rel_add(rel_sum.x + rel_sum.y, rel_cur);
+    rel_sum = make_float2(0.f, 0.f);
+    rel_cur = next;
+  }
+  // This tile's part of the table's gradient: the warps' sums in a fixed order.
+  __device__ __forceinline__ void rel_store() {
+    rel_flush(-1);
+    named_barrier_sync(8, kPwThreads);
+    const float* acc = reinterpret_cast<const float*>(rel_area + REL_ACC);
+    const int t = threadIdx.x - kRoleThreads;
+    if (rel->dpart && t < rel->nb) {
+      float s = 0.f;
+#pragma unroll
+      for (int w = 0; w < NWG * 4; ++w) s += acc[w * FB_RELPOS_MAX_BUCKETS + t];
+      rel->dpart[rel_part * rel->nb + t] = s;
+    }
+  }
+  __device__ __forceinline__ void zero_table_part() const {  // a tile behind its sequence
+    grid_dependency_wait();
+    if (rel->dpart && (int)threadIdx.x < rel->nb) rel->dpart[rel_part * rel->nb + threadIdx.x] = 0.f;
   }
 
   // Copies the owner operands chosen by Cfg::aOuter from shared memory (K-major, 128-byte swizzle) into
@@ -1195,6 +1385,15 @@ struct TcCta {
       }
     }
     pw_wait = 0; pw_work = 0; pw_ld0 = 0; pw_st = 0;
+    if constexpr (BIAS && kDq) {
+      static_assert(NWG * 4 == 8 && kRoleThreads / 32 % 8 == 4, "warp & 7 numbers the pointwise warps");
+      float* acc = reinterpret_cast<float*>(rel_area + REL_ACC) + (warp & 7) * FB_RELPOS_MAX_BUCKETS;
+#pragma unroll
+      for (int i = 0; i < FB_RELPOS_MAX_BUCKETS / 32; ++i) acc[lane + 32 * i] = 0.f;
+      __syncwarp();
+      rel_cur = -1;
+      rel_sum = make_float2(0.f, 0.f);
+    }
     if constexpr (C::nATmem > 0) {
       if (n_it > 0) stage_a_operands();
     }
@@ -1215,6 +1414,9 @@ struct TcCta {
         const int off_blk = off - (p.seg_keys ? 0 : seg_shift_of(p, c0));  // the block lies inside one query segment
         need_mask = p.causal && (r0 + BM - 1 - off_blk > c0);
         if (p.causal) cmin = orow - off_blk - c0;  // query i visible iff i >= key - off
+        // Queries behind the sequence have lse = inf, which makes their P zero unless a table entry that only they point
+        // at is infinite or NaN.
+        if (BIAS) { need_mask = need_mask || c0 + BN > si.sq; cmax = si.sq - 1 - c0; }
       }
       const float* stats = stats_base + (it & 1) * (4 * BN);  // DKV: this block's staged statistics
       if constexpr (kSplit) {
@@ -1226,12 +1428,23 @@ struct TcCta {
         pw_wait += tw1 - tw;
         tc_fence_after();
         if constexpr (kFwd) pw_fwd_block(it, st, need_mask, cmax);
-        else pw_bwd_block(st, need_mask, cmin, cmax, stats);
+        else if constexpr (BIAS) {
+          const int uni = reinterpret_cast<const int*>(rel_area + REL_UNI)[it & 1];
+          if (uni >= 0) {
+            if constexpr (kDq) rel_flush(uni);
+            pw_bwd_block<true>(it, st, need_mask, cmin, cmax, stats);
+          } else {
+            pw_bwd_block<false>(it, st, need_mask, cmin, cmax, stats);
+          }
+        } else {
+          pw_bwd_block<false>(it, st, need_mask, cmin, cmax, stats);
+        }
         const long long tq1 = prof ? clock64() : 0;
         pw_publish(BAR_P_FULL + st, it, true);
         if (prof) { pw_work += clock64() - tw1; pw_st += clock64() - tq1; }
       }
     }
+    if constexpr (BIAS && kDq) rel_store();
     if (prof && ct == 0) { g_prof[5] = pw_wait; g_prof[6] = pw_work; g_prof[9] = pw_ld0; g_prof[10] = pw_st; }
 
     if (n_it > 0) {
@@ -1381,7 +1594,7 @@ struct TcCta {
       }
     }
     if (row_ok && wg == 0) {
-      if (FIRST) p.lse[srow] = l_sum > 0.f ? m_used * p.scale + logf(l_sum) : -INFINITY;
+      if (FIRST) p.lse[srow] = l_sum > 0.f ? m_used * (BIAS ? kLn2 : p.scale) + logf(l_sum) : -INFINITY;
       if (TANGENT) p.z1[srow] = z1o;
       if (gp) {
         p.dpsum[srow] = dsum;
@@ -1563,6 +1776,21 @@ __global__ void __launch_bounds__(kThreads, 1) tc_kernel(const __grid_constant__
   cta.teardown();
 }
 
+// The first-order kernels with a relative position bias (a parameter of its own: the other kernels keep theirs).
+template <typename T, int KIND, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+tc_rel_kernel(const __grid_constant__ TmaMaps maps, const __grid_constant__ Params p, const __grid_constant__ RelPos rel) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  TcCta<T, KIND, D, false, true, false, false, true> cta(maps, p, smem);
+  cta.rel = &rel;
+  if (!cta.setup()) return;
+  cta.run_role();
+  if constexpr (KIND == KIND_DKV) {
+    if (p.split > 1) cta.cluster_reduce();
+  }
+  cta.teardown();
+}
+
 // ------------------------------------------------------------------------------------------------
 // Host side: tensor maps and dispatch
 // ------------------------------------------------------------------------------------------------
@@ -1735,10 +1963,13 @@ int choose_group(const Params& p, bool dkv, int ntiles, int sm_count) {
   return g < pairs ? (g > 0 ? g : 1) : pairs;
 }
 
-template <typename T, int KIND, int D, bool TANGENT, bool FIRST, bool DOD, bool HOOK = false>
-int launch_one(const TmaMaps& maps, const Params& p_in, cudaStream_t stream) {
-  using C = Cfg<KIND, D, TANGENT, FIRST, DOD>;
-  auto kern = tc_kernel<T, KIND, D, TANGENT, FIRST, DOD, HOOK>;
+template <typename T, int KIND, int D, bool TANGENT, bool FIRST, bool DOD, bool HOOK = false, bool BIAS = false>
+int launch_one(const TmaMaps& maps, const Params& p_in, cudaStream_t stream, const RelPos* rel = nullptr) {
+  using C = Cfg<KIND, D, TANGENT, FIRST, DOD, BIAS>;
+  auto kern = [] {
+    if constexpr (BIAS) return tc_rel_kernel<T, KIND, D>;
+    else return tc_kernel<T, KIND, D, TANGENT, FIRST, DOD, HOOK>;
+  }();
   static bool attr_set[64] = {};  // guarded by g_launch_mutex
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1779,7 +2010,8 @@ int launch_one(const TmaMaps& maps, const Params& p_in, cudaStream_t stream) {
   }
   cfg.attrs = attrs;
   cfg.numAttrs = na;
-  return cudaLaunchKernelEx(&cfg, kern, maps, p) == cudaSuccess ? 1 : FB_ERR_CUDA;
+  if constexpr (BIAS) return cudaLaunchKernelEx(&cfg, kern, maps, p, *rel) == cudaSuccess ? 1 : FB_ERR_CUDA;
+  else return cudaLaunchKernelEx(&cfg, kern, maps, p) == cudaSuccess ? 1 : FB_ERR_CUDA;
 }
 
 template <typename T, int D>
@@ -1876,6 +2108,37 @@ int launch_tc_fwd(const Params& p, cudaStream_t s) {
   if (r) return r;
   if (p.dtype == FB_BF16) return p.D == 64 ? fwd_dispatch<__nv_bfloat16, 64>(maps, p, s) : fwd_dispatch<__nv_bfloat16, 128>(maps, p, s);
   return p.D == 64 ? fwd_dispatch<__half, 64>(maps, p, s) : fwd_dispatch<__half, 128>(maps, p, s);
+}
+
+namespace {
+template <typename T, int KIND, int D>
+int launch_rel(const TmaMaps& maps, const Params& p, const RelPos& rel, cudaStream_t s) {
+  return launch_one<T, KIND, D, false, true, false, false, true>(maps, p, s, &rel);
+}
+template <int KIND>
+int launch_rel_any(const Params& p, const RelPos& rel, cudaStream_t s) {
+  TmaMaps maps;
+  const int r = build_maps(maps, p, KIND);
+  if (r) return r;
+  if (p.dtype == FB_BF16) return p.D == 64 ? launch_rel<__nv_bfloat16, KIND, 64>(maps, p, rel, s) : launch_rel<__nv_bfloat16, KIND, 128>(maps, p, rel, s);
+  return p.D == 64 ? launch_rel<__half, KIND, 64>(maps, p, rel, s) : launch_rel<__half, KIND, 128>(maps, p, rel, s);
+}
+}  // namespace
+
+int launch_tc_fwd_rel(const Params& p, const RelPos& rel, cudaStream_t s) { return launch_rel_any<KIND_FWD>(p, rel, s); }
+
+static_assert(BM == kTcOwnerRows, "rows of the partial table gradients");
+int launch_tc_bwd_rel(const Params& p, const RelPos& rel, cudaStream_t s) {
+  int n = 0, r;
+  if (p.dq.ptr || rel.dpart) {
+    if ((r = launch_rel_any<KIND_DQ>(p, rel, s)) < 0) return r;
+    n += r;
+  }
+  if (p.dk.ptr || p.dv.ptr) {
+    if ((r = launch_rel_any<KIND_DKV>(p, rel, s)) < 0) return r;
+    n += r;
+  }
+  return n;
 }
 
 int launch_tc_bwd(const Params& p, cudaStream_t s) {

@@ -7,5 +7,11 @@ from .interface import (  # noqa: F401
     flashback_attn_jvp,
     flashback_attn_hvp,
 )
+from .relpos import (  # noqa: F401
+    flashback_attn_relpos_func,
+    flashback_attn_relpos_varlen_func,
+    flashback_relpos_bias,
+)
 
-__all__ = ["flashback_attn_func", "flashback_attn_varlen_func", "flashback_attn_jvp", "flashback_attn_hvp"]
+__all__ = ["flashback_attn_func", "flashback_attn_varlen_func", "flashback_attn_jvp", "flashback_attn_hvp",
+           "flashback_attn_relpos_func", "flashback_attn_relpos_varlen_func", "flashback_relpos_bias"]

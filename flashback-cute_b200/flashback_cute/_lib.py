@@ -42,7 +42,7 @@ def FB_FLAG_DKV_SPLIT(n: int) -> int:
 DEFAULT_FLAGS = int(os.environ.get("FLASHBACK_FLAGS", "0"))
 _DTYPES = {torch.bfloat16: FB_BF16, torch.float16: FB_F16, torch.float32: FB_F32}
 
-FB_ERR_DTYPE, FB_ERR_HEAD_DIM, FB_ERR_HEADS, FB_ERR_ARCH = -2, -3, -4, -7
+FB_ERR_DTYPE, FB_ERR_HEAD_DIM, FB_ERR_HEADS, FB_ERR_ARCH, FB_ERR_RELPOS = -2, -3, -4, -7, -12
 
 
 class FbTensor(ctypes.Structure):
@@ -109,12 +109,54 @@ class FbKvScatter(ctypes.Structure):
     ]
 
 
+class FbRelpos(ctypes.Structure):
+    _fields_ = [
+        ("table", ctypes.c_void_p), ("bucket_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+        ("num_buckets", ctypes.c_int32), ("bidirectional", ctypes.c_int32), ("starts", ctypes.c_void_p),
+    ]
+
+
+class FbRelposFwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("prob", FbProblem), ("bias", FbRelpos),
+        ("q", FbTensor), ("k", FbTensor), ("v", FbTensor), ("out", FbTensor), ("lse", ctypes.c_void_p),
+    ]
+
+
+class FbRelposBwdArgs(ctypes.Structure):
+    _fields_ = [
+        ("prob", FbProblem), ("bias", FbRelpos),
+        ("q", FbTensor), ("k", FbTensor), ("v", FbTensor), ("dout", FbTensor),
+        ("lse", ctypes.c_void_p), ("dpsum", ctypes.c_void_p),
+        ("dq", FbTensor), ("dk", FbTensor), ("dv", FbTensor),
+        ("dtable", ctypes.c_void_p), ("dtable_bucket_stride", ctypes.c_int64), ("dtable_head_stride", ctypes.c_int64),
+        ("workspace", ctypes.c_void_p),
+    ]
+
+
+class FbRelposBiasArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("heads", ctypes.c_int32), ("seqlen_q", ctypes.c_int32), ("seqlen_k", ctypes.c_int32),
+        ("bias", FbRelpos), ("out", ctypes.c_void_p),
+    ]
+
+
+class FbRelposBiasGradArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("heads", ctypes.c_int32), ("seqlen_q", ctypes.c_int32), ("seqlen_k", ctypes.c_int32),
+        ("bias", FbRelpos), ("grad", ctypes.c_void_p), ("dtable", ctypes.c_void_p),
+        ("dtable_bucket_stride", ctypes.c_int64), ("dtable_head_stride", ctypes.c_int64), ("workspace", ctypes.c_void_p),
+    ]
+
+
 NOALLOC_MAX_STAT_FLOATS = 1 << 20
+RELPOS_MAX_BUCKETS = 128
 
 EXPORTS = (
     "fb_jvp_fwd", "fb_bwd_row_stats", "fb_hvp_bwd", "fb_bwd_noalloc", "fb_last_launch_count", "fb_check_device_status",
     "fb_status_string", "fb_last_cuda_error", "fb_version", "fb_abi_sizeof", "fb_workspace_bytes", "fb_debug_profile",
     "fb_debug_wait_timeout", "fb_hvp_bwd_scatter", "fb_sum_slots",
+    "fb_relpos_fwd", "fb_relpos_bwd", "fb_relpos_workspace_bytes", "fb_relpos_bias", "fb_relpos_bias_grad", "fb_relpos_bias_workspace_bytes",
 )
 
 
@@ -130,7 +172,8 @@ def load() -> ctypes.CDLL:
                 )
             lib = ctypes.CDLL(str(_LIB_PATH))
             for name, argt in (("fb_jvp_fwd", FbJvpArgs), ("fb_bwd_row_stats", FbStatsArgs), ("fb_hvp_bwd", FbHvpArgs),
-                               ("fb_bwd_noalloc", FbBwdNoAllocArgs)):
+                               ("fb_bwd_noalloc", FbBwdNoAllocArgs), ("fb_relpos_fwd", FbRelposFwdArgs), ("fb_relpos_bwd", FbRelposBwdArgs),
+                               ("fb_relpos_bias", FbRelposBiasArgs), ("fb_relpos_bias_grad", FbRelposBiasGradArgs)):
                 fn = getattr(lib, name)
                 fn.argtypes = [ctypes.POINTER(argt), ctypes.c_void_p]
                 fn.restype = ctypes.c_int
@@ -141,6 +184,10 @@ def load() -> ctypes.CDLL:
             lib.fb_sum_slots.restype = ctypes.c_int
             lib.fb_debug_wait_timeout.argtypes = [ctypes.POINTER(FbJvpArgs), ctypes.c_longlong, ctypes.c_void_p]
             lib.fb_debug_wait_timeout.restype = ctypes.c_int
+            lib.fb_relpos_workspace_bytes.argtypes = [ctypes.POINTER(FbProblem), ctypes.c_int]
+            lib.fb_relpos_workspace_bytes.restype = ctypes.c_size_t
+            lib.fb_relpos_bias_workspace_bytes.argtypes = [ctypes.c_int] * 4
+            lib.fb_relpos_bias_workspace_bytes.restype = ctypes.c_size_t
             lib.fb_abi_sizeof.argtypes = [ctypes.c_int]
             lib.fb_abi_sizeof.restype = ctypes.c_size_t
             lib.fb_status_string.argtypes = [ctypes.c_int]
@@ -170,7 +217,7 @@ def raise_for_status(status: int) -> None:
         raise NotImplementedError(msg)
     if status == FB_ERR_DTYPE:
         raise TypeError(msg)
-    if status == FB_ERR_HEADS:
+    if status in (FB_ERR_HEADS, FB_ERR_RELPOS):
         raise ValueError(msg)
     raise RuntimeError(f"flashback_b200 error {status}: {msg}")
 
@@ -352,3 +399,44 @@ def sum_slots(slots: torch.Tensor, out: torch.Tensor, valid=None, period: int = 
         if status == 0:
             _launches += lib.fb_last_launch_count()
     raise_for_status(status)
+
+
+def relpos(table: Optional[torch.Tensor], num_buckets: int, bidirectional: bool, starts) -> FbRelpos:
+    """`starts`: ctypes int32 array of the bucket starts (the caller keeps it alive through the call)."""
+    if table is None:
+        return FbRelpos(None, 0, 0, num_buckets, int(bidirectional), ctypes.addressof(starts))
+    t = raw(table)
+    return FbRelpos(t.data_ptr(), t.stride(0), t.stride(1), num_buckets, int(bidirectional), ctypes.addressof(starts))
+
+
+def relpos_fwd(prob, bias: FbRelpos, q, k, v, out, lse):
+    _call("fb_relpos_fwd", FbRelposFwdArgs(prob, bias, seq_tensor(q), seq_tensor(k), seq_tensor(v), seq_tensor(out), _fptr(lse)), q)
+
+
+def relpos_bwd(prob, bias: FbRelpos, q, k, v, dout, lse, dpsum, dq, dk, dv, dtable):
+    """dq, dk, dv, dtable: outputs, each optional. The workspace of the table's gradient is allocated here."""
+    work = None
+    if dtable is not None:
+        n = (_lib or load()).fb_relpos_workspace_bytes(ctypes.byref(prob), bias.num_buckets)
+        work = torch.empty(n // 4, dtype=torch.float32, device=q.device)
+    a = FbRelposBwdArgs(
+        prob, bias, seq_tensor(q), seq_tensor(k), seq_tensor(v), seq_tensor(dout), _fptr(lse), _fptr(dpsum),
+        seq_tensor(dq), seq_tensor(dk), seq_tensor(dv),
+        _fptr(dtable), 0 if dtable is None else dtable.stride(0), 0 if dtable is None else dtable.stride(1), _fptr(work),
+    )
+    _call("fb_relpos_bwd", a, q)
+
+
+def relpos_bias(bias: FbRelpos, out: torch.Tensor):
+    """out: contiguous (heads, seqlen_q, seqlen_k)."""
+    h, sq, sk = out.shape
+    _call("fb_relpos_bias", FbRelposBiasArgs(_DTYPES[out.dtype], h, sq, sk, bias, _fptr(out)), out)
+
+
+def relpos_bias_grad(bias: FbRelpos, grad: torch.Tensor, dtable: torch.Tensor):
+    """grad: contiguous (heads, seqlen_q, seqlen_k)."""
+    h, sq, sk = grad.shape
+    n = (_lib or load()).fb_relpos_bias_workspace_bytes(h, sq, sk, bias.num_buckets)
+    work = torch.empty(n // 4, dtype=torch.float32, device=grad.device)
+    a = FbRelposBiasGradArgs(_DTYPES[grad.dtype], h, sq, sk, bias, _fptr(grad), _fptr(dtable), dtable.stride(0), dtable.stride(1), _fptr(work))
+    _call("fb_relpos_bias_grad", a, grad)

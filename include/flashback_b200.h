@@ -48,7 +48,8 @@ typedef enum {
   FB_ERR_CUDA = -8,           /* a CUDA runtime/driver call failed; see fb_last_cuda_error() */
   FB_ERR_MODE = -9,           /* inconsistent combination of optional tensors */
   FB_ERR_TOO_LARGE = -10,     /* size exceeds a documented maximum */
-  FB_ERR_DEVICE_TIMEOUT = -11 /* a bounded device-side wait gave up (reported by fb_check_device_status) */
+  FB_ERR_DEVICE_TIMEOUT = -11, /* a bounded device-side wait gave up (reported by fb_check_device_status) */
+  FB_ERR_RELPOS = -12         /* a bias table's bucket count or bucket starts are not valid (fb_relpos) */
 } fb_status;
 
 typedef enum { FB_BF16 = 0, FB_F16 = 1, FB_F32 = 2 } fb_dtype;
@@ -280,6 +281,83 @@ typedef struct {
 
 int fb_bwd_noalloc(const fb_bwd_noalloc_args* args, fb_stream_t stream);
 
+/*
+ * Attention with a learned relative position bias (no counterpart in the reference, whose attention takes no
+ * additive term):
+ *
+ *   S = c Q K^T + T[bucket(r), h],   r = j - (i + seqlen_k - seqlen_q)   (bottom-right aligned, per sequence)
+ *   P = softmax(S),   O = P V,   LSE = logsumexp(S)
+ *   dT[t, h] = sum of dS over all (sequence, i, j) whose r falls in bucket t
+ *
+ * The bucket of r: a side has `side` buckets, side = num_buckets (bidirectional = 0) or num_buckets / 2, and
+ * `starts` is a HOST array of side - 1 ascending distances >= 0: distance n lies in bucket
+ * #{t : starts[t] <= n} of its side. bidirectional = 0: n = max(-r, 0). bidirectional = 1: n = |r|, and the
+ * buckets of r > 0 follow the `side` buckets of r <= 0. The array is copied during the call.
+ */
+#define FB_RELPOS_MAX_BUCKETS 128
+
+typedef struct {
+  const void* table;      /* device, (num_buckets, heads_q), the problem's dtype */
+  int64_t bucket_stride;  /* elements between consecutive buckets (= heads_q when contiguous) */
+  int64_t head_stride;    /* elements between consecutive heads (= 1 when contiguous) */
+  int32_t num_buckets;    /* 2 .. FB_RELPOS_MAX_BUCKETS; even and >= 4 when bidirectional */
+  int32_t bidirectional;  /* 0 / 1 */
+  const int32_t* starts;  /* HOST, see above */
+} fb_relpos;
+
+/* Forward: O and LSE. `prob` as for fb_jvp_fwd, without row segments. */
+typedef struct {
+  fb_problem prob;
+  fb_relpos bias;
+  fb_tensor q, k, v; /* in */
+  fb_tensor out;     /* out */
+  float* lse;        /* out, [heads_q][total_q], -inf on fully masked rows */
+} fb_relpos_fwd_args;
+
+int fb_relpos_fwd(const fb_relpos_fwd_args* args, fb_stream_t stream);
+
+/* First-order backward. dq, dk, dv and dtable are optional outputs; dtable (problem dtype, the table's shape)
+ * comes out of the kernel that owns the query rows, through `workspace` (fb_relpos_workspace_bytes; required with
+ * dtable, contents irrelevant before and after). Sums are formed in a fixed order: results are deterministic. */
+typedef struct {
+  fb_problem prob;
+  fb_relpos bias;
+  fb_tensor q, k, v, dout; /* in */
+  const float* lse;        /* in */
+  const float* dpsum;      /* in, from fb_bwd_row_stats */
+  fb_tensor dq, dk, dv;    /* out, optional */
+  void* dtable;            /* out, optional */
+  int64_t dtable_bucket_stride, dtable_head_stride;
+  float* workspace;
+} fb_relpos_bwd_args;
+
+int fb_relpos_bwd(const fb_relpos_bwd_args* args, fb_stream_t stream);
+
+/* Bytes of `workspace` for problem `p` and a table of num_buckets; 0 for invalid arguments. */
+size_t fb_relpos_workspace_bytes(const fb_problem* p, int num_buckets);
+
+/* The bias as a tensor: out[h][i][j] = T[bucket(j - (i + seqlen_k - seqlen_q)), h], contiguous (heads, seqlen_q,
+ * seqlen_k), and the gradient of the table for a contiguous gradient of that shape (deterministic). 16-byte aligned. */
+typedef struct {
+  int32_t dtype, heads, seqlen_q, seqlen_k;
+  fb_relpos bias;
+  void* out;
+} fb_relpos_bias_args;
+
+int fb_relpos_bias(const fb_relpos_bias_args* args, fb_stream_t stream);
+
+typedef struct {
+  int32_t dtype, heads, seqlen_q, seqlen_k;
+  fb_relpos bias;    /* num_buckets, bidirectional and starts; the table is not read and may be NULL */
+  const void* grad;  /* in */
+  void* dtable;      /* out */
+  int64_t dtable_bucket_stride, dtable_head_stride;
+  float* workspace;  /* fb_relpos_bias_workspace_bytes */
+} fb_relpos_bias_grad_args;
+
+int fb_relpos_bias_grad(const fb_relpos_bias_grad_args* args, fb_stream_t stream);
+size_t fb_relpos_bias_workspace_bytes(int heads, int seqlen_q, int seqlen_k, int num_buckets);
+
 /* Number of kernels the most recent fb_* call on this thread enqueued (for launch accounting). */
 int fb_last_launch_count(void);
 
@@ -325,7 +403,8 @@ size_t fb_workspace_bytes(const fb_problem* p, int which);
 
 /* sizeof() of the ABI structs as compiled into the library, for bindings to verify their own
  * layout: which = 0 fb_tensor, 1 fb_problem, 2 fb_jvp_args, 3 fb_stats_args, 4 fb_hvp_args,
- * 5 fb_bwd_noalloc_args, 6 fb_kv_scatter. */
+ * 5 fb_bwd_noalloc_args, 6 fb_kv_scatter, 8 fb_relpos, 9 fb_relpos_fwd_args, 10 fb_relpos_bwd_args,
+ * 11 fb_relpos_bias_args, 12 fb_relpos_bias_grad_args. */
 size_t fb_abi_sizeof(int which);
 
 #ifdef __cplusplus

@@ -1,0 +1,271 @@
+"""GPU tests of attention with a learned relative position bias, against the float64 oracle and its bounds
+(oracle/relpos_oracle.py derives them: half a step of the type for every rounding, float32 sums)."""
+
+import itertools
+
+import pytest
+import torch
+
+from flashback_cute import _lib, flashback_attn_func, flashback_attn_relpos_func, flashback_attn_relpos_varlen_func, flashback_relpos_bias
+from oracle import relpos_oracle as orc
+
+pytestmark = pytest.mark.gpu
+if not torch.cuda.is_available():
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+DEV = "cuda"
+BF16, F16, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _device_status_clean():
+    yield
+    torch.cuda.synchronize()
+    _lib.check_device_status()
+
+
+def _within(name, got, want, tol):
+    """|got - want| <= tol, element by element (smallest denormals of float16 aside: half a step of 2^-24)."""
+    assert got.shape == want.shape, name
+    assert torch.isfinite(got).all(), name
+    over = (got.double() - want).abs() - tol - 2.0 ** -25
+    worst = over.max().item() if over.numel() else -1.0
+    assert worst <= 0, f"{name}: {worst:.3e} beyond the bound (largest bound {tol.max().item():.3e}, largest value {want.abs().max().item():.3e})"
+
+
+def _mk(shape, dtype, seed, std=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=DEV) * std).to(dtype)
+
+
+def _check(dtype, d, hq, hkv, causal, batch, sq, sk, num=32, far=128, two=None, seed=0, table=None, packed=None):
+    """Forward and gradients of one dense or packed (`packed`: lists of lengths) problem."""
+    two = (not causal) if two is None else two
+    if packed:
+        q, k, v, do = (_mk((sum(n), h, d), dtype, seed + i) for i, (n, h) in enumerate(zip((packed[0], packed[1], packed[1], packed[0]), (hq, hkv, hkv, hq))))
+        cu = [torch.tensor([0, *itertools.accumulate(n)], dtype=torch.int32, device=DEV) for n in packed]
+    else:
+        q, k, v, do = (_mk((batch, s, h, d), dtype, seed + i) for i, (s, h) in enumerate(((sq, hq), (sk, hkv), (sk, hkv), (sq, hq))))
+    table = _mk((num, hq), dtype, seed + 9) if table is None else table
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, table)]
+    if packed:
+        out = flashback_attn_relpos_varlen_func(*leaves, *cu, max(packed[0]), max(packed[1]), max_distance=far, causal=causal, bidirectional=two)
+    else:
+        out = flashback_attn_relpos_func(*leaves, max_distance=far, causal=causal, bidirectional=two)
+    grads = torch.autograd.grad(out, leaves, do)
+    ref = orc.attention(q, k, v, table, far, two, d ** -0.5, causal, do, *(packed or (None, None)))
+    for name, got, want, tol in zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(), *grads), ref[:5], ref.tol):
+        _within(name, got, want, tol)
+
+
+@pytest.mark.parametrize("sizes", [(1, 1), (1, 300), (128, 128), (129, 65), (200, 333), (300, 97), (64, 640)])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+def test_dense_bf16(d, causal, sizes):
+    _check(BF16, d, 4, 2, causal, 2, *sizes)
+
+
+@pytest.mark.parametrize("heads", [(3, 3), (6, 1)])
+@pytest.mark.parametrize("dtype", [F16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+def test_types_and_heads(d, dtype, heads):
+    _check(dtype, d, *heads, True, 2, 150, 211)
+    _check(dtype, d, *heads, False, 1, 97, 97)
+
+
+@pytest.mark.parametrize("num,far,two", [(2, 2, False), (4, 2, True), (8, 5, True), (32, 17, False), (64, 1024, False), (128, 300, True), (128, 65, False)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_buckets(dtype, num, far, two):
+    """Few and many buckets, borders closer than a tile and beyond the sequence, also both-sided under a causal mask."""
+    _check(dtype, 64, 2, 1, False, 1, 333, 401, num, far, two)
+    _check(dtype, 64, 2, 1, True, 1, 401, 333, num, far, two)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("heads", [(4, 4), (4, 1)])
+def test_packed(heads, causal, dtype):
+    _check(dtype, 64, *heads, causal, None, None, None, packed=([37, 200, 1, 129, 0, 64], [50, 200, 7, 300, 0, 64]))
+    _check(dtype, 128, *heads, causal, None, None, None, packed=([300, 1, 0, 257], [290, 1, 5, 257]))
+
+
+def test_long_rows_share_one_bucket():
+    """Blocks far from the diagonal take the path of a single bucket; 1500 rows cross it on both sides."""
+    _check(BF16, 64, 2, 1, False, 1, 1500, 1500)
+    _check(BF16, 128, 1, 1, True, 1, 1500, 1500, 32, 64)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_entries_that_hide_or_that_nobody_points_at(dtype):
+    """-inf in the table hides its pairs (rows that see nothing give zeros); infinities and NaN in entries that only masked
+    or absent pairs point at do no harm."""
+    hq, num = 2, 32
+    table = _mk((num, hq), dtype, 3)
+    table[0, 0] = -float("inf")  # the query's own position: the first row sees nothing
+    table[5, 1] = -float("inf")
+    _check(dtype, 64, hq, 1, True, 1, 200, 200, table=table)
+    table = _mk((num, hq), dtype, 4)
+    table[num // 2:] = float("nan")  # keys behind the query: masked
+    table[num // 2 + 3:, 0] = float("inf")
+    _check(dtype, 64, hq, 1, True, 2, 77, 77, two=True, table=table)
+    table = _mk((num, hq), dtype, 5)
+    table[12:] = float("inf")  # distances from 12 on: longer than any of these sequences
+    _check(dtype, 64, hq, 1, True, None, None, None, two=False, far=128, table=table, packed=([7, 1, 12, 3], [7, 1, 12, 3]))
+
+
+def test_strides_and_offsets():
+    """Views: heads before rows, sliced heads, an offset into a larger tensor, a transposed table, a broadcast gradient."""
+    b, s, hq, hkv, d = 2, 130, 4, 2, 64
+    q = _mk((b, hq, s, d), BF16, 0).transpose(1, 2)
+    k = _mk((b, s, hkv + 3, d), BF16, 1)[:, :, 1:1 + hkv]
+    v = _mk((b, s, hkv, 2 * d), BF16, 2)[..., d:]
+    odd = _mk((s * hkv * b * d + 1,), BF16, 4)[1:].view(b, s, hkv, d)
+    table = _mk((hq, 32), BF16, 3).t()
+    leaves = [t.requires_grad_() for t in (q, k, v, table)]
+    out = flashback_attn_relpos_func(*leaves, causal=True)
+    grads = torch.autograd.grad(out.float().sum(), leaves)
+    ref = orc.attention(*leaves, 128, False, d ** -0.5, True, torch.ones_like(out))
+    for name, got, want, tol in zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(), *grads), ref[:5], ref.tol):
+        _within(name, got, want, tol)
+    out = flashback_attn_relpos_func(q, odd, odd, table, causal=True)
+    ref = orc.attention(q, odd, odd, table, 128, False, d ** -0.5, True)
+    _within("out", out.detach(), ref.out, ref.tol[0])
+
+
+def test_zero_table_is_plain_attention():
+    q, k, v = _mk((2, 256, 4, 64), BF16, 0), _mk((2, 256, 2, 64), BF16, 1), _mk((2, 256, 2, 64), BF16, 2)
+    got = flashback_attn_relpos_func(q, k, v, torch.zeros(32, 4, dtype=BF16, device=DEV), causal=True)
+    want = flashback_attn_func(q, k, v, causal=True)
+    assert (got.float() - want.float()).abs().max() <= 2 * torch.finfo(BF16).eps * want.abs().max()
+
+
+def test_gradient_of_the_table_against_differences():
+    """Central differences of <O, dO> in the float32 path along a random direction of the table: the step's square times the third derivative
+    and float32 rounding of O over the step are both below 1e-3 of the value here."""
+    q, k, v, do = (_mk((1, 90, 2, 64), F32, i) for i in range(4))
+    table, way = _mk((32, 2), F32, 5), _mk((32, 2), F32, 6)
+    leaf = table.clone().requires_grad_()
+    loss = lambda t: (flashback_attn_relpos_func(q, k, v, t).double() * do.double()).sum()  # noqa: E731
+    g = torch.autograd.grad(loss(leaf), leaf)[0]
+    h = 2.0 ** -6
+    diff = (loss(table + h * way) - loss(table - h * way)) / (2 * h)
+    want = (g.double() * way.double()).sum()
+    assert abs(diff - want) <= 1e-2 * abs(want) + 1e-3 * (g.double() * way.double()).abs().sum()
+
+
+def test_gradients_asked_for_one_by_one():
+    q, k, v, table, do = (_mk(s, BF16, i) for i, s in enumerate([(1, 140, 2, 64), (1, 150, 2, 64), (1, 150, 2, 64), (32, 2), (1, 140, 2, 64)]))
+    every = [t.clone().requires_grad_() for t in (q, k, v, table)]
+    want = torch.autograd.grad(flashback_attn_relpos_func(*every), every, do)
+    for n in range(4):
+        some = [t.clone().requires_grad_(i == n) for i, t in enumerate((q, k, v, table))]
+        got = torch.autograd.grad(flashback_attn_relpos_func(*some), some[n], do)[0]
+        assert torch.equal(got, want[n])
+
+
+def test_deterministic_and_second_order_refused():
+    leaves = [_mk(s, BF16, i).requires_grad_() for i, s in enumerate([(2, 300, 4, 64), (2, 300, 1, 64), (2, 300, 1, 64), (32, 4)])]
+    do = _mk((2, 300, 4, 64), BF16, 8)
+    runs = [torch.autograd.grad(flashback_attn_relpos_func(*leaves, causal=True), leaves, do) for _ in range(3)]
+    for r in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
+    g = torch.autograd.grad(flashback_attn_relpos_func(*leaves), leaves, do.requires_grad_(), create_graph=True)
+    with pytest.raises(RuntimeError):
+        torch.autograd.grad(g[0].float().sum(), leaves[0])
+
+
+def test_empty():
+    table = _mk((32, 2), BF16, 0).requires_grad_()
+    q, k = _mk((1, 5, 2, 64), BF16, 1).requires_grad_(), _mk((1, 0, 2, 64), BF16, 2)
+    out = flashback_attn_relpos_func(q, k, k, table)
+    assert torch.equal(out, torch.zeros_like(out))
+    assert all(torch.equal(g, torch.zeros_like(g)) for g in torch.autograd.grad(out, (q, table), torch.ones_like(out)))
+    out = flashback_attn_relpos_func(q[:, :0], _mk((1, 3, 2, 64), BF16, 2), _mk((1, 3, 2, 64), BF16, 2), table)
+    assert out.shape == (1, 0, 2, 64)
+
+
+def test_rows_behind_the_last_sequence_stay():
+    """Packed tensors longer than the sequences say: the rows behind the last one are not touched."""
+    cu = torch.tensor([0, 70, 150], dtype=torch.int32, device=DEV)
+    q, out = _mk((200, 2, 64), BF16, 0), torch.full((200, 2, 64), 7.0, dtype=BF16, device=DEV)
+    k, table = _mk((200, 2, 64), BF16, 1), _mk((32, 2), BF16, 2)
+    from flashback_cute import relpos
+
+    prob = _lib.problem(q, k, cu, cu, 80, 80, 0.125, True)
+    lse = torch.full((2, 200), 7.0, device=DEV)
+    b = relpos._buckets(32, False, 128)
+    _lib.relpos_fwd(prob, b.bind(table), q, k, k, out, lse)
+    assert (out[150:] == 7.0).all() and (lse[:, 150:] == 7.0).all()
+    ref = orc.attention(q[:150], k[:150], k[:150], table, 128, False, 0.125, True, None, [70, 80], [70, 80])
+    _within("out", out[:150], ref.out, ref.tol[0])
+
+
+def test_captured_and_replayed_on_a_side_stream():
+    """Forward and backward captured into one graph, replayed with new inputs in the same buffers; equal to an eager run."""
+    shapes = [(2, 257, 4, 64), (2, 257, 2, 64), (2, 257, 2, 64), (32, 4), (2, 257, 4, 64)]
+    bufs = [_mk(s, BF16, i) for i, s in enumerate(shapes)]
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in bufs[:4]]
+        out = flashback_attn_relpos_func(*leaves, causal=True)
+        return (out.detach(), *torch.autograd.grad(out, leaves, bufs[4]))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        got = step()
+    for i, s in enumerate(shapes):
+        bufs[i].copy_(_mk(s, BF16, 20 + i))
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, step()))
+
+
+# ---------------------------------------------------------------------------------------------
+# the bias as a tensor
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("sizes", [(1, 1), (1, 4099), (17, 3), (33, 2050), (130, 257), (300, 300)])
+@pytest.mark.parametrize("two", [False, True])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_bias_tensor_and_its_gradient(dtype, two, sizes):
+    sq, sk = sizes
+    for num, far, heads in ((32, 128, 3), (128, 1500, 2), (4, 7, 1)):
+        table = _mk((num, heads), dtype, 0).requires_grad_()
+        which = orc.buckets(sq, sk, num, far, two).to(DEV)
+        bias = flashback_relpos_bias(table, sq, sk, max_distance=far, bidirectional=two)
+        assert torch.equal(bias.detach(), table.detach().t()[:, which])
+        grad = _mk(bias.shape, dtype, 1)
+        got = torch.autograd.grad(bias, table, grad)[0]
+        want, size = (torch.zeros(num, heads, dtype=torch.float64, device=DEV) for _ in range(2))
+        for h in range(heads):
+            want[:, h].index_add_(0, which.flatten(), grad[h].double().flatten())
+            size[:, h].index_add_(0, which.flatten(), grad[h].double().abs().flatten())
+        # float32 sums along a diagonal (at most 512 rows in a row), over the warps and a run of neighbours; then 64 bits; one rounding
+        u = torch.finfo(dtype).eps / 2
+        _within("dtable", got, want, (512 / 8 + 8 + 5 + 8) * 2.0 ** -24 * size * (1 + u) + u * want.abs())
+
+
+def test_bias_tensor_views_and_derivatives():
+    table = _mk((3, 32), F32, 0).t().requires_grad_()
+    bias = flashback_relpos_bias(table, 40, 50)
+    g = torch.autograd.grad(bias.sum(), table, create_graph=True)[0]  # a broadcast gradient
+    which = orc.buckets(40, 50, 32, 128, True).to(DEV)
+    assert torch.equal(g.detach(), torch.bincount(which.flatten(), minlength=32).float()[:, None].expand(-1, 3))
+    w = _mk((3, 40, 50), F32, 1).requires_grad_()
+    first = torch.autograd.grad((flashback_relpos_bias(table, 40, 50) * w).sum(), table, create_graph=True)[0]
+    way = _mk((32, 3), F32, 2)
+    second = torch.autograd.grad((first * way).sum(), w)[0]
+    assert torch.equal(second, way.t()[:, which])
+    _, tangent = torch.func.jvp(lambda t: flashback_relpos_bias(t, 40, 50), (table.detach(),), (way,))
+    assert torch.equal(tangent, way.t()[:, which])
+
+
+def test_bias_tensor_empty():
+    table = _mk((32, 2), BF16, 0).requires_grad_()
+    bias = flashback_relpos_bias(table, 0, 5)
+    assert bias.shape == (2, 0, 5)
+    assert torch.equal(torch.autograd.grad(bias.sum(), table)[0], torch.zeros_like(table))
