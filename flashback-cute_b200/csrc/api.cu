@@ -6,6 +6,7 @@
 #include "fb_params.h"
 
 #include <atomic>
+#include <initializer_list>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
@@ -447,6 +448,71 @@ extern "C" size_t fb_relpos_bias_workspace_bytes(int heads, int sq, int sk, int 
   return sizeof(float) * (size_t)heads * (size_t)relpos_bias_parts(heads, sq, sk) * (size_t)num_buckets;
 }
 
+namespace {
+
+int check_cache(const fb_cache& t) {
+  if (!t.ptr) return FB_ERR_NULL_ARG;
+  if (reinterpret_cast<uintptr_t>(t.ptr) % 16 != 0) return FB_ERR_ALIGNMENT;
+  for (int64_t s : {t.batch_stride, t.row_stride, t.head_stride})
+    if (s < 0 || s % 8 != 0) return FB_ERR_ALIGNMENT;
+  return FB_OK;
+}
+
+int check_decode(const fb_relpos_decode_args& a) {
+  if (a.dtype != FB_BF16 && a.dtype != FB_F16) return FB_ERR_DTYPE;
+  if (a.head_dim != 64 && a.head_dim != 128) return FB_ERR_HEAD_DIM;
+  if (a.heads_q <= 0 || a.heads_kv <= 0 || a.heads_q % a.heads_kv != 0) return FB_ERR_HEADS;
+  if (a.batch < 0 || a.seqlen_q < 0 || a.seqlen_k < 0) return FB_ERR_SHAPE;
+  if (a.batch > 65535 || a.seqlen_k > (1 << 30) || a.heads_q > 65535 || (int64_t)a.seqlen_q * a.heads_q > (1 << 20)) return FB_ERR_TOO_LARGE;
+  return FB_OK;
+}
+
+int splits_of(const fb_relpos_decode_args& a) {
+  return decode_splits(a.batch, a.heads_kv, a.heads_q / a.heads_kv * a.seqlen_q, a.seqlen_k);
+}
+
+}  // namespace
+
+extern "C" size_t fb_relpos_decode_workspace_bytes(const fb_relpos_decode_args* a) {
+  if (!a || check_decode(*a) != FB_OK || a->batch == 0 || a->seqlen_q == 0) return 0;
+  const size_t splits = (size_t)splits_of(*a);
+  return splits == 1 ? 0 : (size_t)a->batch * a->seqlen_q * a->heads_q * splits * (a->head_dim + 2) * sizeof(float);
+}
+
+extern "C" int fb_relpos_decode(const fb_relpos_decode_args* a, fb_stream_t stream) {
+  tl_launches = 0;
+  if (!a) return FB_ERR_NULL_ARG;
+  FB_TRY(check_decode(*a));
+  RelPos rel;
+  FB_TRY(convert_relpos(rel, a->bias, true));
+  FB_TRY(check_cache(a->q)); FB_TRY(check_cache(a->k)); FB_TRY(check_cache(a->v));
+  if (!a->out) return FB_ERR_NULL_ARG;
+  if (reinterpret_cast<uintptr_t>(a->out) % 16 != 0 || reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return FB_ERR_ALIGNMENT;
+  if (a->batch == 0 || a->seqlen_q == 0) return FB_OK;
+  DecodeParams p;
+  memset(&p, 0, sizeof(p));
+  p.B = a->batch; p.Hq = a->heads_q; p.Hkv = a->heads_kv; p.G = a->heads_q / a->heads_kv;
+  p.Sq = a->seqlen_q; p.Sk = a->seqlen_k; p.D = a->head_dim;
+  p.scale = a->softmax_scale;
+  p.q = CacheT{a->q.ptr, a->q.batch_stride, a->q.row_stride, a->q.head_stride};
+  p.k = CacheT{a->k.ptr, a->k.batch_stride, a->k.row_stride, a->k.head_stride};
+  p.v = CacheT{a->v.ptr, a->v.batch_stride, a->v.row_stride, a->v.head_stride};
+  p.lens = a->lens;
+  p.out = a->out;
+  p.splits = splits_of(*a);
+  if (p.splits > 1) {
+    if (!a->workspace) return FB_ERR_NULL_ARG;
+    p.part = a->workspace;  // row length head_dim floats: the (maximum, sum) pairs behind them stay 8-byte aligned
+    p.part_ml = reinterpret_cast<float2*>(a->workspace + (size_t)p.B * p.Sq * p.Hq * p.splits * p.D);
+  }
+  int* status_word = nullptr;
+  FB_TRY(device_setup(&status_word));
+  int n = launch_decode(a->dtype, p, rel, reinterpret_cast<cudaStream_t>(stream));
+  if (n < 0) { if (n == FB_ERR_CUDA) record_cuda(cudaGetLastError()); return n; }
+  tl_launches = n;
+  return FB_OK;
+}
+
 extern "C" int fb_last_launch_count(void) { return tl_launches; }
 
 extern "C" int fb_check_device_status(void) {
@@ -532,6 +598,8 @@ extern "C" size_t fb_abi_sizeof(int which) {
     case 10: return sizeof(fb_relpos_bwd_args);
     case 11: return sizeof(fb_relpos_bias_args);
     case 12: return sizeof(fb_relpos_bias_grad_args);
+    case 13: return sizeof(fb_cache);
+    case 14: return sizeof(fb_relpos_decode_args);
   }
   return 0;
 }

@@ -1,0 +1,381 @@
+// Attention of a few new tokens per sequence against a cache of keys and values, with a learned relative position bias.
+//
+// Bound by HBM: every key and value row up to the sequence's length is read once, 4 D bytes for the 4 rows D flops that the
+// rows = (new tokens) x (query heads per kv head) sharing them need. So the rows of a kv head form ONE 16-row operand (two for
+// more rows) of warp-level MMAs, and the kernel is built around keeping loads in flight:
+//
+//   * a CTA of 4 warps takes a slice of one (sequence, kv head)'s keys; every warp is a flash-attention of its own over every 4th
+//     group of 16 keys (own running maximum, sum and accumulator; own shared-memory stages filled by cp.async), so nothing in
+//     the main loop waits for another warp;
+//   * the slices divide the sequence's OWN length, so ragged batches stay balanced; partial results (float32, unnormalised, with
+//     maximum and sum) are joined by a second kernel in a fixed order. One slice: the first kernel writes the output itself.
+//
+// Far from the newest token all keys of a group share the last bucket and the bias is one number per row.
+#include "fb_params.h"
+#include "ptx_sm100.cuh"
+
+namespace fb {
+namespace {
+
+using namespace ptx;
+
+constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int KG = 16;      // keys per group = MMA k of the second product
+constexpr int kStages = 3;  // groups in flight per warp
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {  // invalid: zero fill, nothing read
+  const int n = valid ? 16 : 0;
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void ldsm4t(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+               : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <typename T> __device__ __forceinline__ uint32_t pack16(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+
+// 16-byte unit u of row r of a [rows][D] 16-bit tile, swizzled so that ldmatrix (8 rows, one unit each) meets 8 different banks
+template <int D>
+__device__ __forceinline__ uint32_t unit_off(int r, int u) { return (uint32_t)(r * D * 2 + ((u ^ (r & 7)) << 4)); }
+
+template <typename T, int D, int MT>
+__global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant__ DecodeParams p, const __grid_constant__ RelPos rel) {
+  constexpr int R = 16 * MT;           // rows per CTA
+  constexpr int U = D / 8;             // 16-byte units per row
+  constexpr int kTile = KG * D * 2;    // bytes of one K or V group
+  constexpr int kWarpBytes = kStages * 2 * kTile;
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t* const qs = smem;                       // [R][D]
+  uint8_t* const stages = smem + R * D * 2;       // per warp [kStages][K, V]
+  __shared__ int starts[FB_RELPOS_MAX_BUCKETS];
+  __shared__ float s_m[kWarps][R], s_l[kWarps][R];
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = blockIdx.x;
+  const int hk = blockIdx.y / p.row_tiles, rt = blockIdx.y - hk * p.row_tiles;
+  const int b = blockIdx.z;
+  const int rows = p.G * p.Sq;
+  for (int t = threadIdx.x; t < rel.side - 1; t += kThreads) starts[t] = rel.starts[t];
+  grid_dependency_wait();
+  grid_launch_dependents();
+  const int len = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
+  // this slice of the sequence's keys: [k0, k1), whole rounds of the CTA's warps
+  const int per = ((len + p.splits - 1) / p.splits + kWarps * KG - 1) / (kWarps * KG) * (kWarps * KG);
+  const int k0 = min(len, split * per), k1 = min(len, k0 + per);
+  const int ngroups = (k1 - k0 + KG - 1) / KG;
+  const int mine = ngroups > warp ? (ngroups - warp + kWarps - 1) / kWarps : 0;
+
+  const T* kb = reinterpret_cast<const T*>(p.k.ptr) + b * p.k.batch_stride + hk * p.k.head_stride;
+  const T* vb = reinterpret_cast<const T*>(p.v.ptr) + b * p.v.batch_stride + hk * p.v.head_stride;
+  const uint32_t my = smem_u32(stages) + warp * kWarpBytes;
+  auto load = [&](int i) {  // group i of this warp into its stage
+    if (i < mine) {
+      const int j0 = k0 + (warp + i * kWarps) * KG;
+      const uint32_t dst = my + (i % kStages) * 2 * kTile;
+#pragma unroll
+      for (int x = 0; x < KG * U / 32; ++x) {
+        const int at = x * 32 + lane, r = at / U, u = at % U;
+        const bool ok = j0 + r < k1;
+        const int64_t j = ok ? j0 + r : k0;
+        cp_async16(dst + unit_off<D>(r, u), kb + j * p.k.row_stride + u * 8, ok);
+        cp_async16(dst + kTile + unit_off<D>(r, u), vb + j * p.v.row_stride + u * 8, ok);
+      }
+    }
+    cp_async_commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) load(i);
+
+  // the queries: row x of the CTA is new token (rt * R + x) / G, query head hk * G + (rt * R + x) % G
+  for (int at = threadIdx.x; at < R * U; at += kThreads) {
+    const int x = at / U, u = at % U, row = rt * R + x;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (row < rows) {
+      const int t = row / p.G, g = row - t * p.G;
+      v = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.q.ptr) + b * p.q.batch_stride + t * p.q.row_stride + (int64_t)(hk * p.G + g) * p.q.head_stride + u * 8);
+    }
+    *reinterpret_cast<uint4*>(qs + unit_off<D>(x, u)) = v;
+  }
+  __syncthreads();
+
+  // this thread's rows of the MMA fragments: lane / 4 and lane / 4 + 8 of every 16
+  const float scale2 = p.scale * kLog2e;
+  const int far = starts[rel.side - 2];  // distances from here on lie in the last bucket of their side
+  int pos[MT][2], head[MT][2];
+  float far_bias[MT][2], m[MT][2], l[MT][2];
+  float o[MT][D / 8][4];
+  int pos_min = INT32_MAX;
+  auto bias_of = [&](int t, int h) { return to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + h * rel.head_stride]) * kLog2e; };
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int row = min(rt * R + mt * 16 + lane / 4 + 8 * x, rows - 1);
+      const int t = row / p.G;
+      head[mt][x] = hk * p.G + row - t * p.G;
+      pos[mt][x] = len - p.Sq + t;  // the new token's place in its sequence
+      far_bias[mt][x] = bias_of(rel.side - 1, head[mt][x]);
+      m[mt][x] = -INFINITY;
+      l[mt][x] = 0.f;
+    }
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
+  }
+  pos_min = len - p.Sq + (rt * R) / p.G;  // the earliest row of the CTA
+
+  for (int i = 0; i < mine; ++i) {
+    load(i + kStages - 1);
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
+    const uint32_t ks = my + (i % kStages) * 2 * kTile, vs = ks + kTile;
+    const int j0 = k0 + (warp + i * kWarps) * KG;
+    float s[MT][2][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mt][n][e] = 0.f;
+    // S = Q K^T: matrices of one x4 load: keys 0-7 | k 0-7, keys 0-7 | k 8-15, keys 8-15 | k 0-7, keys 8-15 | k 8-15
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      uint32_t kf[4];
+      ldsm4(ks + unit_off<D>((lane & 7) + ((lane >> 4) << 3), kk * 2 + ((lane >> 3) & 1)), kf);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        uint32_t qf[4];
+        ldsm4(smem_u32(qs) + unit_off<D>(mt * 16 + (lane & 15), kk * 2 + (lane >> 4)), qf);
+        mma16816<T>(s[mt][0], qf, kf[0], kf[1]);
+        mma16816<T>(s[mt][1], qf, kf[2], kf[3]);
+      }
+    }
+    // bias, mask, running softmax; element e of tile n: row lane / 4 + 8 (e / 2), key j0 + 8 n + 2 (lane % 4) + e % 2
+    const bool all_far = pos_min - (j0 + KG - 1) >= far && j0 + KG <= k1;
+    uint32_t pf[MT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int x = e >> 1, j = j0 + 8 * n + 2 * (lane & 3) + (e & 1);
+          float bias = far_bias[mt][x];
+          if (!all_far) {
+            const int r = j - pos[mt][x];
+            bias = -INFINITY;
+            if (r <= 0 && j < k1) bias = bias_of(relpos_bucket(r, starts, rel.side, rel.two), head[mt][x]);
+          }
+          s[mt][n][e] = fmaf(s[mt][n][e], scale2, bias);
+          mx[x] = fmaxf(mx[x], s[mt][n][e]);
+        }
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
+        mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
+        const float mn = fmaxf(m[mt][x], mx[x]);
+        const float off = mn == -INFINITY ? 0.f : mn;  // nothing visible so far: every exponential below is 0
+        const float alpha = ex2(m[mt][x] - off);       // m = -inf: 0
+        m[mt][x] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 2 * x; e < 2 * x + 2; ++e) {
+            s[mt][n][e] = ex2(s[mt][n][e] - off);
+            sum += s[mt][n][e];
+          }
+        l[mt][x] = l[mt][x] * alpha + sum;  // this lane's keys only; the four lanes of a row are added up at the end
+        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) { o[mt][n][2 * x] *= alpha; o[mt][n][2 * x + 1] *= alpha; }
+        }
+      }
+      // the score fragments of two 8-key tiles are the 16-key operand of the second product
+      pf[mt][0] = pack16<T>(s[mt][0][0], s[mt][0][1]);
+      pf[mt][1] = pack16<T>(s[mt][0][2], s[mt][0][3]);
+      pf[mt][2] = pack16<T>(s[mt][1][0], s[mt][1][1]);
+      pf[mt][3] = pack16<T>(s[mt][1][2], s[mt][1][3]);
+    }
+#pragma unroll
+    for (int n2 = 0; n2 < D / 16; ++n2) {
+      uint32_t vf[4];
+      ldsm4t(vs + unit_off<D>(lane & 15, n2 * 2 + (lane >> 4)), vf);
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        mma16816<T>(o[mt][2 * n2], pf[mt], vf[0], vf[1]);
+        mma16816<T>(o[mt][2 * n2 + 1], pf[mt], vf[2], vf[3]);
+      }
+    }
+    __syncwarp();  // every lane has read the stage before it is filled again
+  }
+
+  // ---- join the warps ----
+  cp_async_wait<0>();
+  __syncthreads();  // the stages are free: [warp][R][D] float32 accumulators
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      l[mt][x] += __shfl_xor_sync(0xffffffffu, l[mt][x], 1);
+      l[mt][x] += __shfl_xor_sync(0xffffffffu, l[mt][x], 2);
+      if ((lane & 3) == 0) {
+        s_m[warp][mt * 16 + lane / 4 + 8 * x] = m[mt][x];
+        s_l[warp][mt * 16 + lane / 4 + 8 * x] = l[mt][x];
+      }
+    }
+  float* const acc = reinterpret_cast<float*>(stages);
+  static_assert(kWarps * R * D * 4 <= kWarps * kWarpBytes, "the accumulators fit the stages");
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        *reinterpret_cast<float2*>(acc + (warp * R + mt * 16 + lane / 4 + 8 * x) * D + n * 8 + 2 * (lane & 3)) = make_float2(o[mt][n][2 * x], o[mt][n][2 * x + 1]);
+  __syncthreads();
+  for (int at = threadIdx.x; at < R * D / 4; at += kThreads) {
+    const int x = at / (D / 4), d4 = at - x * (D / 4), row = rt * R + x;
+    if (row >= rows) break;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][x]);
+    const float off = mm == -INFINITY ? 0.f : mm;
+    float ll = 0.f;
+    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = ex2(s_m[w][x] - off);
+      const float4 a = *reinterpret_cast<const float4*>(acc + (w * R + x) * D + d4 * 4);
+      ll += s_l[w][x] * f;
+      v.x += a.x * f; v.y += a.y * f; v.z += a.z * f; v.w += a.w * f;
+    }
+    const int t = row / p.G, h = hk * p.G + row - t * p.G;
+    if (p.splits == 1) {
+      const float inv = ll > 0.f ? 1.f / ll : 0.f;
+      T* dst = reinterpret_cast<T*>(p.out) + ((int64_t)(b * p.Sq + t) * p.Hq + h) * D + d4 * 4;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<T>(v.x * inv, v.y * inv), pack16<T>(v.z * inv, v.w * inv));
+    } else {
+      const int64_t at_row = ((int64_t)(b * p.Sq + t) * p.Hq + h) * p.splits + split;
+      *reinterpret_cast<float4*>(p.part + at_row * D + d4 * 4) = v;
+      if (d4 == 0) p.part_ml[at_row] = make_float2(mm, ll);
+    }
+  }
+}
+
+// One warp per (sequence, new token, query head): joins the slices in order.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_constant__ DecodeParams p) {
+  constexpr int E = D / 32;  // elements per lane
+  const int lane = threadIdx.x & 31;
+  const int64_t row = (int64_t)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  grid_dependency_wait();
+  if (row >= (int64_t)p.B * p.Sq * p.Hq) return;
+  const float2* ml = p.part_ml + row * p.splits;
+  const float* part = p.part + row * p.splits * D + lane * E;
+  float mm = -INFINITY;
+  for (int s = lane; s < p.splits; s += 32) mm = fmaxf(mm, ml[s].x);
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, x));
+  const float off = mm == -INFINITY ? 0.f : mm;
+  float ll = 0.f, v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < p.splits; ++s) {
+    const float2 x = ml[s];
+    const float f = ex2(x.x - off);
+    ll += x.y * f;
+    if constexpr (E == 4) {
+      const float4 a = *reinterpret_cast<const float4*>(part + (int64_t)s * D);
+      v[0] += a.x * f; v[1] += a.y * f; v[2] += a.z * f; v[3] += a.w * f;
+    } else {
+      const float2 a = *reinterpret_cast<const float2*>(part + (int64_t)s * D);
+      v[0] += a.x * f; v[1] += a.y * f;
+    }
+  }
+  const float inv = ll > 0.f ? 1.f / ll : 0.f;
+  T* dst = reinterpret_cast<T*>(p.out) + row * D + lane * E;
+  if constexpr (E == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<T>(v[0] * inv, v[1] * inv), pack16<T>(v[2] * inv, v[3] * inv));
+  else *reinterpret_cast<uint32_t*>(dst) = pack16<T>(v[0] * inv, v[1] * inv);
+}
+
+template <typename K>
+cudaError_t launch(K kern, dim3 grid, size_t smem, cudaStream_t s, void** args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;  // programmatic dependent launch: both kernels wait for the one before at their start
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kern), args);
+}
+
+template <typename T, int D, int MT>
+int decode_typed(DecodeParams& p, RelPos& rel, cudaStream_t s) {
+  constexpr int R = 16 * MT;
+  constexpr size_t smem = R * D * 2 + kWarps * kStages * 2 * KG * D * 2;
+  auto kern = decode_kernel<T, D, MT>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return FB_ERR_CUDA;
+  p.row_tiles = (p.G * p.Sq + R - 1) / R;
+  void* args[2] = {&p, &rel};
+  if (launch(kern, dim3((unsigned)p.splits, (unsigned)(p.Hkv * p.row_tiles), (unsigned)p.B), smem, s, args) != cudaSuccess) return FB_ERR_CUDA;
+  if (p.splits == 1) return 1;
+  const int64_t rows = (int64_t)p.B * p.Sq * p.Hq;
+  if (launch(decode_join_kernel<T, D>, dim3((unsigned)((rows + kWarps - 1) / kWarps)), 0, s, args) != cudaSuccess) return FB_ERR_CUDA;
+  return 2;
+}
+
+template <typename T>
+int decode_dispatch(DecodeParams& p, RelPos& rel, cudaStream_t s) {
+  if (p.G * p.Sq <= 16) return p.D == 64 ? decode_typed<T, 64, 1>(p, rel, s) : decode_typed<T, 128, 1>(p, rel, s);
+  return p.D == 64 ? decode_typed<T, 64, 2>(p, rel, s) : decode_typed<T, 128, 2>(p, rel, s);
+}
+
+}  // namespace
+
+// Slices of a sequence's keys: enough CTAs for a few waves on the whole GPU, slices of at least one round of the CTA's warps.
+int decode_splits(int batch, int heads_kv, int rows, int seqlen_k) {
+  const int per = rows <= 16 ? 16 : 32;
+  const int64_t base = (int64_t)batch * heads_kv * ((rows + per - 1) / per);
+  const int64_t want = (148 * 2 * 4 + base - 1) / base;
+  const int64_t most = (seqlen_k + kWarps * KG - 1) / (kWarps * KG);
+  const int64_t n = want < most ? want : most;
+  return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+}
+
+int launch_decode(int dtype, DecodeParams& p, RelPos& rel, cudaStream_t s) {
+  return dtype == FB_BF16 ? decode_dispatch<__nv_bfloat16>(p, rel, s) : decode_dispatch<__half>(p, rel, s);
+}
+
+}  // namespace fb

@@ -97,6 +97,22 @@ __device__ __forceinline__ bool run_head(int key, int lane) {
   return lane == 0 || prev != key;
 }
 
+// Decoding against a cache (decode.cu).
+struct CacheT {
+  const void* ptr;
+  int64_t batch_stride, row_stride, head_stride;
+};
+struct DecodeParams {
+  int B, Hq, Hkv, G, Sq, Sk, D;
+  float scale;
+  CacheT q, k, v;
+  const int32_t* lens;  // nullptr: Sk each
+  void* out;            // contiguous (B, Sq, Hq, D)
+  int splits, row_tiles;
+  float* part;          // splits > 1: [(b, token, query head)][split][D] and their (maximum, sum)
+  float2* part_ml;
+};
+
 struct SeqInfo {
   int q0, k0;    // first global row of this sequence
   int sq, sk;    // its lengths
@@ -166,6 +182,8 @@ int launch_relpos_fill(int dtype, const RelPos& rel, int heads, int sq, int sk, 
 int launch_relpos_grad(int dtype, const RelPos& rel, int heads, int sq, int sk, const void* grad, void* dtable, int64_t bucket_stride,
                        int64_t head_stride, cudaStream_t stream);
 int64_t relpos_bias_parts(int heads, int sq, int sk);  // partial table gradients per head of launch_relpos_grad
+int decode_splits(int batch, int heads_kv, int rows, int seqlen_k);
+int launch_decode(int dtype, DecodeParams& p, RelPos& rel, cudaStream_t stream);
 constexpr int kTcOwnerRows = 128, kSimtOwnerRows = 16;  // query rows per partial table gradient
 int launch_tc_fwd_wait_hook(const Params& p, cudaStream_t stream);  // test instantiation, see fb_debug_wait_timeout
 int launch_sum_slots(const float* slots, int n_slots, int64_t slot_stride, int64_t count, int64_t period, const int64_t* valid, float* out,

@@ -149,6 +149,19 @@ class FbRelposBiasGradArgs(ctypes.Structure):
     ]
 
 
+class FbCache(ctypes.Structure):
+    _fields_ = [("ptr", ctypes.c_void_p), ("batch_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64)]
+
+
+class FbRelposDecodeArgs(ctypes.Structure):
+    _fields_ = [
+        ("dtype", ctypes.c_int32), ("batch", ctypes.c_int32), ("heads_q", ctypes.c_int32), ("heads_kv", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("seqlen_q", ctypes.c_int32), ("seqlen_k", ctypes.c_int32), ("softmax_scale", ctypes.c_float),
+        ("bias", FbRelpos), ("q", FbCache), ("k", FbCache), ("v", FbCache),
+        ("lens", ctypes.c_void_p), ("out", ctypes.c_void_p), ("workspace", ctypes.c_void_p),
+    ]
+
+
 NOALLOC_MAX_STAT_FLOATS = 1 << 20
 RELPOS_MAX_BUCKETS = 128
 
@@ -157,6 +170,7 @@ EXPORTS = (
     "fb_status_string", "fb_last_cuda_error", "fb_version", "fb_abi_sizeof", "fb_workspace_bytes", "fb_debug_profile",
     "fb_debug_wait_timeout", "fb_hvp_bwd_scatter", "fb_sum_slots",
     "fb_relpos_fwd", "fb_relpos_bwd", "fb_relpos_workspace_bytes", "fb_relpos_bias", "fb_relpos_bias_grad", "fb_relpos_bias_workspace_bytes",
+    "fb_relpos_decode", "fb_relpos_decode_workspace_bytes",
 )
 
 
@@ -173,7 +187,8 @@ def load() -> ctypes.CDLL:
             lib = ctypes.CDLL(str(_LIB_PATH))
             for name, argt in (("fb_jvp_fwd", FbJvpArgs), ("fb_bwd_row_stats", FbStatsArgs), ("fb_hvp_bwd", FbHvpArgs),
                                ("fb_bwd_noalloc", FbBwdNoAllocArgs), ("fb_relpos_fwd", FbRelposFwdArgs), ("fb_relpos_bwd", FbRelposBwdArgs),
-                               ("fb_relpos_bias", FbRelposBiasArgs), ("fb_relpos_bias_grad", FbRelposBiasGradArgs)):
+                               ("fb_relpos_bias", FbRelposBiasArgs), ("fb_relpos_bias_grad", FbRelposBiasGradArgs),
+                               ("fb_relpos_decode", FbRelposDecodeArgs)):
                 fn = getattr(lib, name)
                 fn.argtypes = [ctypes.POINTER(argt), ctypes.c_void_p]
                 fn.restype = ctypes.c_int
@@ -186,6 +201,8 @@ def load() -> ctypes.CDLL:
             lib.fb_debug_wait_timeout.restype = ctypes.c_int
             lib.fb_relpos_workspace_bytes.argtypes = [ctypes.POINTER(FbProblem), ctypes.c_int]
             lib.fb_relpos_workspace_bytes.restype = ctypes.c_size_t
+            lib.fb_relpos_decode_workspace_bytes.argtypes = [ctypes.POINTER(FbRelposDecodeArgs)]
+            lib.fb_relpos_decode_workspace_bytes.restype = ctypes.c_size_t
             lib.fb_relpos_bias_workspace_bytes.argtypes = [ctypes.c_int] * 4
             lib.fb_relpos_bias_workspace_bytes.restype = ctypes.c_size_t
             lib.fb_abi_sizeof.argtypes = [ctypes.c_int]
@@ -440,3 +457,14 @@ def relpos_bias_grad(bias: FbRelpos, grad: torch.Tensor, dtable: torch.Tensor):
     work = torch.empty(n // 4, dtype=torch.float32, device=grad.device)
     a = FbRelposBiasGradArgs(_DTYPES[grad.dtype], h, sq, sk, bias, _fptr(grad), _fptr(dtable), dtable.stride(0), dtable.stride(1), _fptr(work))
     _call("fb_relpos_bias_grad", a, grad)
+
+
+def relpos_decode(bias: FbRelpos, q, k, v, lens, out, scale):
+    """q (b, sq, hq, d), caches k, v (b, s, hkv, d), lens int32 (b,) or None, out contiguous like q."""
+    cache = lambda t: FbCache(t.data_ptr(), t.stride(0), t.stride(1), t.stride(2))  # noqa: E731
+    a = FbRelposDecodeArgs(_DTYPES[q.dtype], q.shape[0], q.shape[2], k.shape[2], q.shape[3], q.shape[1], k.shape[1], float(scale),
+                           bias, cache(q), cache(k), cache(v), _fptr(lens), out.data_ptr(), None)
+    n = (_lib or load()).fb_relpos_decode_workspace_bytes(ctypes.byref(a))
+    work = torch.empty(n // 4, dtype=torch.float32, device=q.device) if n else None
+    a.workspace = _fptr(work)
+    _call("fb_relpos_decode", a, q)

@@ -6,6 +6,7 @@ aligned, like causal masking). A learned table of shape (num_buckets, heads) hol
     S = scale * Q K^T + table[bucket(r), head],   P = softmax(S),   O = P V
 
   flashback_attn_relpos_func, flashback_attn_relpos_varlen_func   forward, and first-order gradients of q, k, v and the table
+  flashback_attn_relpos_decode                                    a few new tokens per sequence against a cache of keys and values
   flashback_relpos_bias                                            the bias as a tensor (heads, sq, sk), differentiable
 
 Buckets (`bucket_starts`): bidirectional, the first half of the table is for r <= 0 and the second for r > 0, both by
@@ -252,6 +253,50 @@ def flashback_attn_relpos_varlen_func(
     return _RelposAttnFunc.apply(
         q, k, v, bias_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal, b
     )[0]
+
+
+def _cache_ok(t: torch.Tensor) -> bool:
+    return t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(t.stride(i) >= 0 and t.stride(i) % 8 == 0 for i in range(3))
+
+
+def flashback_attn_relpos_decode(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    cache_seqlens: Optional[torch.Tensor],
+    bias_table: torch.Tensor,
+    max_distance: int = 128,
+    softmax_scale: Optional[float] = None,
+    bidirectional: bool = False,
+) -> torch.Tensor:
+    """Attention of the newest tokens of every sequence: q (b, sq, hq, d) against caches (b, s, hkv, d) that already hold
+    their keys and values. cache_seqlens, int32 (b,) on the device of q: keys per sequence, the new tokens included (None: s each; values are
+    clamped to [0, s]). Causal: token t of sequence i sits at position cache_seqlens[i] - sq + t. Cache rows at or behind a
+    sequence's length are not read. bfloat16 or float16; meant for one to a few tokens (every 16 or 32 (token, head) pairs of a kv head read the
+    cache once). No autograd graph."""
+    _validate(q, k_cache, v_cache)
+    _check_shapes(q, k_cache, v_cache, rows=False)
+    _check_table(bias_table, q.shape[2], q)
+    if q.dtype == torch.float32:
+        raise TypeError("decoding takes float16 or bfloat16")
+    if cache_seqlens is not None:
+        if cache_seqlens.dtype != torch.int32:
+            raise TypeError("cache_seqlens must be int32")
+        if cache_seqlens.shape != q.shape[:1] or cache_seqlens.device != q.device or not cache_seqlens.is_contiguous():
+            raise ValueError("cache_seqlens must be contiguous, of shape (batch,) and on the device of q")
+    b = _buckets(bias_table.shape[0], bool(bidirectional), max_distance)
+    if softmax_scale is None:
+        softmax_scale = q.shape[-1] ** -0.5
+    with torch.no_grad():
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        if out.numel() == 0 or k_cache.numel() == 0:
+            return out.zero_()
+        if not (_cache_ok(k_cache) and _cache_ok(v_cache)):
+            raise ValueError("caches need unit stride on head_dim, strides that are multiples of 8 elements and 16-byte alignment")
+        if not _cache_ok(q):
+            q = torch.empty(q.shape, dtype=q.dtype, device=q.device).copy_(q)
+        _lib.relpos_decode(b.bind(bias_table), q, k_cache, v_cache, cache_seqlens, out, softmax_scale)
+    return out
 
 
 def flashback_relpos_bias(

@@ -358,6 +358,30 @@ typedef struct {
 int fb_relpos_bias_grad(const fb_relpos_bias_grad_args* args, fb_stream_t stream);
 size_t fb_relpos_bias_workspace_bytes(int heads, int seqlen_q, int seqlen_k, int num_buckets);
 
+/* Attention of `seqlen_q` new tokens per sequence against a cache of keys and values that already holds them, with the
+ * bias, causal: token t of sequence b sits at position lens[b] - seqlen_q + t and sees the keys at or before it.
+ * 16-bit types, head_dim 64 or 128. A token with a negative position (lens[b] < seqlen_q) sees nothing: zeros.
+ * lens is clamped to [0, seqlen_k]; cache rows at or behind it are not read. */
+typedef struct {
+  const void* ptr;
+  int64_t batch_stride, row_stride, head_stride; /* elements; multiples of 8; head_dim contiguous; 16-byte aligned */
+} fb_cache;
+
+typedef struct {
+  int32_t dtype, batch, heads_q, heads_kv, head_dim;
+  int32_t seqlen_q;      /* new tokens per sequence */
+  int32_t seqlen_k;      /* rows per sequence in the cache */
+  float softmax_scale;
+  fb_relpos bias;
+  fb_cache q, k, v;
+  const int32_t* lens;   /* device int32[batch], keys per sequence (new tokens included), or NULL: seqlen_k each */
+  void* out;             /* contiguous (batch, seqlen_q, heads_q, head_dim) */
+  float* workspace;      /* fb_relpos_decode_workspace_bytes; may be NULL when that is 0; contents irrelevant */
+} fb_relpos_decode_args;
+
+int fb_relpos_decode(const fb_relpos_decode_args* args, fb_stream_t stream);
+size_t fb_relpos_decode_workspace_bytes(const fb_relpos_decode_args* args);
+
 /* Number of kernels the most recent fb_* call on this thread enqueued (for launch accounting). */
 int fb_last_launch_count(void);
 
@@ -404,7 +428,7 @@ size_t fb_workspace_bytes(const fb_problem* p, int which);
 /* sizeof() of the ABI structs as compiled into the library, for bindings to verify their own
  * layout: which = 0 fb_tensor, 1 fb_problem, 2 fb_jvp_args, 3 fb_stats_args, 4 fb_hvp_args,
  * 5 fb_bwd_noalloc_args, 6 fb_kv_scatter, 8 fb_relpos, 9 fb_relpos_fwd_args, 10 fb_relpos_bwd_args,
- * 11 fb_relpos_bias_args, 12 fb_relpos_bias_grad_args. */
+ * 11 fb_relpos_bias_args, 12 fb_relpos_bias_grad_args, 13 fb_cache, 14 fb_relpos_decode_args. */
 size_t fb_abi_sizeof(int which);
 
 #ifdef __cplusplus

@@ -269,3 +269,112 @@ def test_bias_tensor_empty():
     bias = flashback_relpos_bias(table, 0, 5)
     assert bias.shape == (2, 0, 5)
     assert torch.equal(torch.autograd.grad(bias.sum(), table)[0], torch.zeros_like(table))
+
+
+# ---------------------------------------------------------------------------------------------
+# new tokens against a cache
+# ---------------------------------------------------------------------------------------------
+def _decode_ref(q, k, v, lens, table, far, two, scale):
+    out, tol = torch.zeros(q.shape, dtype=torch.float64, device=DEV), torch.zeros(q.shape, dtype=torch.float64, device=DEV)
+    for b, n in enumerate(lens):
+        n = min(max(n, 0), k.shape[1])
+        r = orc.attention(q[b:b + 1], k[b:b + 1, :n], v[b:b + 1, :n], table, far, two, scale, True)
+        out[b], tol[b] = r.out[0], r.tol[0][0]
+    return out, tol
+
+
+def _check_decode(dtype, d, hq, hkv, sq, s, lens, num=32, far=128, two=False, seed=0):
+    from flashback_cute import flashback_attn_relpos_decode
+
+    b = len(lens)
+    q, k, v = _mk((b, sq, hq, d), dtype, seed), _mk((b, s, hkv, d), dtype, seed + 1), _mk((b, s, hkv, d), dtype, seed + 2)
+    table = _mk((num, hq), dtype, seed + 3)
+    for i, n in enumerate(lens):  # rows that must not be read
+        k[i, max(n, 0):], v[i, max(n, 0):] = float("nan"), float("nan")
+    got = flashback_attn_relpos_decode(q, k, v, torch.tensor(lens, dtype=torch.int32, device=DEV), table, max_distance=far, bidirectional=two)
+    want, tol = _decode_ref(q, k, v, lens, table, far, two, d ** -0.5)
+    _within("out", got, want, tol)
+
+
+@pytest.mark.parametrize("sq", [1, 2, 5])
+@pytest.mark.parametrize("heads", [(4, 4), (8, 1), (12, 4)])
+@pytest.mark.parametrize("dtype,d", [(BF16, 64), (BF16, 128), (F16, 64), (F16, 128)])
+def test_decode(dtype, d, heads, sq):
+    _check_decode(dtype, d, *heads, sq, 700, [700, 1, 0, 3, 16, 17, 64, 65, 511, 640, 900, -4])
+
+
+@pytest.mark.parametrize("num,far,two", [(2, 2, False), (64, 2000, False), (32, 60, True), (128, 300, False)])
+def test_decode_buckets(num, far, two):
+    _check_decode(BF16, 128, 8, 2, 3, 2300, [2300, 100, 1555], num, far, two)
+
+
+def test_decode_one_slice_and_many():
+    """One slice per sequence (the kernel writes the output itself), and more slices than keys."""
+    _check_decode(BF16, 64, 32, 8, 1, 300, [300 - 7 * i for i in range(40)])
+    _check_decode(BF16, 64, 160, 160, 1, 90, [90 - i for i in range(16)])
+    _check_decode(F16, 128, 1, 1, 1, 9001, [9001, 5])
+
+
+def test_decode_many_rows():
+    """More (token, head) pairs per kv head than one operand holds."""
+    _check_decode(BF16, 64, 16, 1, 7, 400, [400, 3, 129])
+    _check_decode(F16, 128, 40, 1, 2, 150, [150, 31])
+
+
+def test_decode_agrees_with_the_prompt_path():
+    """The last tokens of a prompt, computed as a prompt and token by token against a growing cache."""
+    from flashback_cute import flashback_attn_relpos_decode
+
+    q, k, v, table = _mk((2, 200, 8, 64), BF16, 0), _mk((2, 256, 2, 64), BF16, 1), _mk((2, 256, 2, 64), BF16, 2), _mk((32, 8), BF16, 3)
+    whole = flashback_attn_relpos_func(q, k[:, :200].contiguous(), v[:, :200].contiguous(), table, causal=True)
+    tol = orc.attention(q, k[:, :200], v[:, :200], table, 128, False, 0.125, True).tol[0]
+    for t in (0, 1, 63, 64, 150, 199):
+        lens = torch.full((2,), t + 1, dtype=torch.int32, device=DEV)
+        one = flashback_attn_relpos_decode(q[:, t:t + 1], k, v, lens, table)
+        assert ((one[:, 0].double() - whole[:, t].double()).abs() <= 2 * tol[:, t]).all()
+
+
+def test_decode_views_and_no_lengths():
+    """Caches as views of one tensor (keys and values side by side, heads before rows); no lengths: every row counts."""
+    from flashback_cute import flashback_attn_relpos_decode
+
+    kv = _mk((3, 2, 4, 333, 64), BF16, 1)  # (b, k or v, heads, rows, d)
+    k, v = kv[:, 0].transpose(1, 2), kv[:, 1].transpose(1, 2)
+    q, table = _mk((3, 8, 2, 64), BF16, 0).transpose(1, 2), _mk((8, 32), BF16, 3).t()
+    got = flashback_attn_relpos_decode(q, k, v, None, table)
+    want, tol = _decode_ref(q, k, v, [333] * 3, table, 128, False, 0.125)
+    _within("out", got, want, tol)
+    with pytest.raises(ValueError):
+        flashback_attn_relpos_decode(q, k.transpose(2, 3).contiguous().transpose(2, 3), v, None, table)
+    with pytest.raises(TypeError):
+        flashback_attn_relpos_decode(q.float(), k.float(), v.float(), None, table.float())
+    with pytest.raises(TypeError):
+        flashback_attn_relpos_decode(q, k, v, torch.zeros(3, dtype=torch.int64, device=DEV), table)
+    with pytest.raises(ValueError):
+        flashback_attn_relpos_decode(q, k, v, torch.zeros(2, dtype=torch.int32, device=DEV), table)
+
+
+def test_decode_captured_with_growing_lengths():
+    """One graph, replayed while the lengths grow: a generation loop."""
+    from flashback_cute import flashback_attn_relpos_decode
+
+    q, k, v, table = _mk((4, 1, 8, 128), BF16, 0), _mk((4, 512, 2, 128), BF16, 1), _mk((4, 512, 2, 128), BF16, 2), _mk((32, 8), BF16, 3)
+    lens = torch.full((4,), 300, dtype=torch.int32, device=DEV)
+    flashback_attn_relpos_decode(q, k, v, lens, table)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = flashback_attn_relpos_decode(q, k, v, lens, table)
+    for _ in range(3):
+        lens += 37
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, flashback_attn_relpos_decode(q, k, v, lens, table))
+
+
+def test_decode_empty():
+    from flashback_cute import flashback_attn_relpos_decode
+
+    q, k, table = _mk((2, 1, 4, 64), BF16, 0), _mk((2, 0, 4, 64), BF16, 1), _mk((32, 4), BF16, 3)
+    assert torch.equal(flashback_attn_relpos_decode(q, k, k, None, table), torch.zeros_like(q))
+    assert flashback_attn_relpos_decode(q[:0], _mk((0, 5, 4, 64), BF16, 1), _mk((0, 5, 4, 64), BF16, 1), None, table).shape == (0, 1, 4, 64)

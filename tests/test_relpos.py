@@ -116,9 +116,31 @@ def test_status_codes():
         _lib.raise_for_status(-12)
 
 
+def test_decode_status_codes():
+    lib = _lib.load()
+    c = _lib.FbCache(0x1000, 1024, 128, 64)
+
+    def args(**kw):
+        base = dict(dtype=0, batch=2, heads_q=4, heads_kv=2, head_dim=64, seqlen_q=1, seqlen_k=500, softmax_scale=0.125, bias=_bias(), q=c, k=c, v=c, out=0x1000)
+        base.update(kw)
+        return _lib.FbRelposDecodeArgs(**base)
+
+    code = lambda **kw: lib.fb_relpos_decode(ctypes.byref(args(**kw)), None)  # noqa: E731
+    assert lib.fb_relpos_decode(None, None) == -1
+    assert code(dtype=2) == -2 and code(head_dim=96) == -3 and code(heads_q=3) == -4 and code(seqlen_q=-1) == -5
+    assert code(batch=70000) == -10 and code(seqlen_q=1 << 20) == -10
+    assert code(bias=_bias(num=1)) == -12
+    assert code(k=_lib.FbCache(0x1008, 1024, 128, 64)) == -6 and code(v=_lib.FbCache(0x1000, 1024, 100, 64)) == -6
+    assert code(out=None) == -1 and code(out=0x1004) == -6
+    assert code() == -1  # slices without a workspace
+    assert lib.fb_relpos_decode_workspace_bytes(ctypes.byref(args())) > 0
+    assert lib.fb_relpos_decode_workspace_bytes(ctypes.byref(args(seqlen_k=40))) == 0 == lib.fb_relpos_decode_workspace_bytes(None)
+
+
 def test_struct_layouts():
     lib = _lib.load()
-    structs = (_lib.FbRelpos, _lib.FbRelposFwdArgs, _lib.FbRelposBwdArgs, _lib.FbRelposBiasArgs, _lib.FbRelposBiasGradArgs)
+    structs = (_lib.FbRelpos, _lib.FbRelposFwdArgs, _lib.FbRelposBwdArgs, _lib.FbRelposBiasArgs, _lib.FbRelposBiasGradArgs,
+               _lib.FbCache, _lib.FbRelposDecodeArgs)
     for i, s in enumerate(structs):
         assert lib.fb_abi_sizeof(8 + i) == ctypes.sizeof(s), s.__name__
 
