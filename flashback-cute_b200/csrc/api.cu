@@ -357,13 +357,13 @@ extern "C" int fb_relpos_fwd(const fb_relpos_fwd_args* a, fb_stream_t stream) {
   RelPos rel;
   FB_TRY(convert_relpos(rel, a->bias, true));
   FB_TRY(check_tensor(a->q, true)); FB_TRY(check_tensor(a->k, true)); FB_TRY(check_tensor(a->v, true));
-  FB_TRY(check_tensor(a->out, true));
-  if (!a->lse) return FB_ERR_NULL_ARG;
+  FB_TRY(check_tensor(a->out, true)); FB_TRY(check_tensor(a->out_low, false));
+  if (a->out_low.ptr && !use_tensor_cores(a->prob)) return FB_ERR_MODE;
   if (a->prob.total_q == 0) return FB_OK;
   Params p;
   fill_problem(p, a->prob);
   FB_TRY(device_setup(&p.status));
-  p.q = cvt(a->q); p.k = cvt(a->k); p.v = cvt(a->v); p.o = cvt(a->out);
+  p.q = cvt(a->q); p.k = cvt(a->k); p.v = cvt(a->v); p.o = cvt(a->out); p.od = cvt(a->out_low);
   p.lse = a->lse;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int n = use_tensor_cores(a->prob) ? launch_tc_fwd_rel(p, rel, s) : launch_simt_fwd_rel(p, rel, s);

@@ -1,0 +1,587 @@
+// Forward of attention with a learned relative position bias on the tensor cores (16-bit types).
+//
+// Online softmax, in log2 units: V_ij = c log2(e) (Q K^T)_ij + log2(e) T[bucket], P = 2^(V - m), O = P V / l.
+//
+// What bounds it: per 128 x 128 scores, S = Q K^T and O += P V keep the tensor pipe busy for 512 clk each (head_dim 128; 256
+// each at 64), the 16384 exponentials keep the special-function units busy for 1024 clk. So a CTA owns TWO tiles of 128
+// query rows and lets them take turns: while the warpgroup of one tile computes exponentials, the tensor pipe works on the
+// other. One thread owns one query row (TMEM lane), 128 scores at a time in registers: row maximum and sum need no exchange between
+// threads. K and V blocks of 128 keys are shared by the two tiles.
+//
+//   warp 0 (one lane)   TMA: Q tiles once, K and V blocks through a ring of stages
+//   warp 1 (one lane)   every tcgen05.mma: PV(t, i) and, right behind it, S(t, i + 1), for the tiles t in turn
+//   warps 2, 3          biases of the next block's positions into shared memory; zeros behind a sequence's last key
+//   warps 4-7, 8-11     softmax, rescaling and epilogue of tile 0 and tile 1
+//
+// TMEM (512 columns): per tile 128 columns of scores, overwritten by P (16 bit) as it is computed, and head_dim of output.
+//
+// The bias. Blocks whose 128 x 128 positions share a bucket (all but a few around the diagonal) take one number, folded into the
+// exponent's FMA. In the others every pair reads its own: entry (key column - row) of 383 staged values. A warp's lanes
+// read neighbouring entries; four copies, each shifted by one entry, let every thread fetch four columns with one
+// 16-byte load whatever its row.
+#include "fb_params.h"
+#include "ptx_sm100.cuh"
+#include "tc_host.h"
+
+#include <cuda.h>
+#include <mutex>
+#include <type_traits>
+
+namespace fb {
+namespace {
+
+using namespace ptx;
+
+constexpr int BM = 128;  // query rows per tile = TMEM lanes
+constexpr int BN = 128;  // keys per block
+constexpr int kRoleThreads = 128, kSoftThreads = 256, kThreads = kRoleThreads + kSoftThreads;
+// The role warps give registers back, the softmax warpgroups take them: no more than the launch left (see tc_kernels.cu).
+constexpr int kLaunchRegs = 168, kRoleRegs = 104, kSoftRegs = 200;
+static_assert(kRoleThreads * (kLaunchRegs - kRoleRegs) >= kSoftThreads * (kSoftRegs - kLaunchRegs), "registers that nobody releases");
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kRescaleThreshold = 8.f;  // log2 units: rescale O only when the row maximum grew by more than 2^8
+constexpr int kSpan = 2 * BM + BN;        // positions of a block seen from both tiles (one more than there are)
+constexpr int kCopyStride = kSpan + 8;    // floats between the shifted copies: 8 banks apart
+
+enum {
+  BAR_Q = 0,        // + tile
+  BAR_K_FULL = 2,   // + stage (up to 3)
+  BAR_K_EMPTY = 5,
+  BAR_V_FULL = 8,
+  BAR_V_EMPTY = 11,
+  BAR_S_FULL = 14,  // + tile: scores complete and biases staged
+  BAR_P_FULL = 16,  // + tile
+  BAR_O_DONE = 18,  // + tile
+  BAR_ST_EMPTY = 20,  // + 2 * buffer + tile: biases of a buffer read
+  BAR_TAIL = 24,    // keys behind the sequence zeroed in the last V block
+  BAR_COUNT = 25
+};
+// Bytes behind the tiles
+enum {
+  M_SLOT = 256,                       // TMEM address, abort flag
+  M_UNI = M_SLOT + 16,                // [2 buffers][2 tiles] flags, then the same of biases
+  M_TAB = M_UNI + 32 + 208,           // 512: table column in log2 units
+  M_STARTS = M_TAB + FB_RELPOS_MAX_BUCKETS * 4,
+  M_BIAS = M_STARTS + FB_RELPOS_MAX_BUCKETS * 4,  // [2][4][kCopyStride]
+  M_BYTES = M_BIAS + 2 * 4 * kCopyStride * 4
+};
+static_assert(M_TAB == 512 && M_BIAS % 16 == 0, "layout");
+
+template <int D>
+struct FwdCfg {
+  static constexpr int kStages = D == 128 ? 2 : 3;
+  static constexpr int qTile = BM * D * 2, kvTile = BN * D * 2;
+  static constexpr int kOff = 2 * qTile, vOff = kOff + kStages * kvTile;
+  static constexpr int tileBytes = vOff + kStages * kvTile;
+  static constexpr int smemBytes = tileBytes + M_BYTES;
+  static_assert(smemBytes <= 232448, "shared memory");
+  static constexpr int tmemCols = 512;  // 2 x (128 scores + D): 384 at head_dim 64, and allocations are powers of two
+};
+
+struct FwdMaps {
+  CUtensorMap q, k, v, o, lo;
+};
+
+template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&v);
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t u);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u)); }
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
+
+template <typename T, int D>
+struct RelFwd {
+  using C = FwdCfg<D>;
+  static constexpr int KS = C::kStages;
+  static constexpr int fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+  static constexpr uint32_t idesc_s = make_idesc(fmt, BM, BN, 0, 0);
+  static constexpr uint32_t idesc_o = make_idesc(fmt, BM, D, 0, 1);
+
+  const FwdMaps& maps;
+  const Params& p;
+  const RelPos& rel;
+  uint8_t* const smem;
+  uint8_t* misc;
+  uint32_t sbase, bar0, tmem_base;
+  volatile int* abort_flag;
+  int warp, lane, head, hk, off, r0, n_it;
+  int n_of[2];  // blocks of the two tiles (0: the tile lies behind its sequence)
+  SeqInfo si;
+
+  __device__ __forceinline__ RelFwd(const FwdMaps& m, const Params& p_, const RelPos& r, uint8_t* s) : maps(m), p(p_), rel(r), smem(s) {}
+
+  __device__ __forceinline__ uint32_t bar(int i) const { return bar0 + 8 * i; }
+  __device__ __forceinline__ bool wait1(int b, int parity) const { return mbar_wait(bar(b), parity, abort_flag); }
+  __device__ __forceinline__ void warp_wait(int b, int parity) const {
+    if (lane == 0) wait1(b, parity);
+    __syncwarp();
+  }
+  __device__ __forceinline__ bool aborted() const { return *abort_flag != 0; }
+  __device__ __forceinline__ uint32_t q_addr(int t) const { return sbase + t * C::qTile; }
+  __device__ __forceinline__ uint32_t k_addr(int s) const { return sbase + C::kOff + s * C::kvTile; }
+  __device__ __forceinline__ uint32_t v_addr(int s) const { return sbase + C::vOff + s * C::kvTile; }
+  __device__ __forceinline__ uint32_t s_cols(int t) const { return tmem_base + t * BN; }
+  __device__ __forceinline__ uint32_t o_cols(int t) const { return tmem_base + 2 * BN + t * D; }
+
+  // False: nothing to do (the whole CTA leaves together).
+  __device__ __forceinline__ bool setup() {
+    sbase = smem_u32(smem);
+    if (sbase & 1023u) {
+      if (threadIdx.x == 0) atomicOr(p.status, 0x100);
+      return false;
+    }
+    if (*reinterpret_cast<volatile int*>(p.status) != 0) return false;  // see tc_kernels.cu
+    misc = smem + C::tileBytes;
+    bar0 = sbase + C::tileBytes;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(misc + M_SLOT);
+    abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    warp = threadIdx.x >> 5;
+    lane = threadIdx.x & 31;
+    // (head, batch) pairs in groups, heaviest tiles of a group first: see tc_kernels.cu
+    const uint32_t lin = blockIdx.x, pairs = (uint32_t)p.Hq * (uint32_t)p.B, gsz = (uint32_t)p.group;
+    const uint32_t grp = lin / (gsz * (uint32_t)p.ntiles), rem = lin - grp * gsz * (uint32_t)p.ntiles;
+    const uint32_t in_grp = min(gsz, pairs - grp * gsz);
+    const int tidx = (int)(rem / in_grp);
+    const uint32_t pair = grp * gsz + rem % in_grp;
+    head = (int)(pair % (uint32_t)p.Hq);
+    hk = head / (p.Hq / p.Hkv);
+    if (p.cu_q) grid_dependency_wait();
+    si = seq_info(p, (int)(pair / (uint32_t)p.Hq));
+    r0 = (p.causal ? p.ntiles - 1 - tidx : tidx) * (2 * BM);
+    if (r0 >= si.sq) return false;
+    off = si.sk - si.sq;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      int kmax = si.sk;
+      if (p.causal) kmax = max(0, min(si.sk, r0 + (t + 1) * BM + off));
+      n_of[t] = r0 + t * BM < si.sq ? (kmax + BN - 1) / BN : 0;
+    }
+    n_it = max(n_of[0], n_of[1]);
+
+    if (threadIdx.x == 0) {
+      for (int i = 0; i < BAR_COUNT; ++i) {
+        uint32_t count = 1;
+        if (i == BAR_S_FULL || i == BAR_S_FULL + 1) count = 3;  // the MMAs and both bias warps
+        if (i == BAR_P_FULL || i == BAR_P_FULL + 1 || (i >= BAR_ST_EMPTY && i < BAR_ST_EMPTY + 4)) count = 4;  // a tile's softmax warps
+        mbar_init(bar(i), count);
+      }
+      *abort_flag = 0;
+      fence_barrier_init();
+      if (n_it > 0) {
+        grid_dependency_wait();
+        prefetch_tmap(&maps.q); prefetch_tmap(&maps.k); prefetch_tmap(&maps.v);
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (n_of[t] == 0) continue;
+          mbar_expect_tx(bar(BAR_Q + t), C::qTile);
+#pragma unroll
+          for (int c = 0; c < D / 64; ++c)
+            tma_load_3d(q_addr(t) + c * (BM * 128), &maps.q, bar(BAR_Q + t), c * 64, si.q0 + r0 + t * BM, head);
+        }
+      }
+    }
+    if (warp == 1) {
+      tmem_alloc(smem_u32(tmem_slot), C::tmemCols);
+      tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    tmem_base = *tmem_slot;
+    grid_launch_dependents();
+    grid_dependency_wait();
+    return true;
+  }
+
+  __device__ __forceinline__ void producer() {
+    for (int it = 0; it < n_it; ++it) {
+      const int s = it % KS, ph = ((it / KS) & 1) ^ 1, row = si.k0 + it * BN;
+      if (!wait1(BAR_K_EMPTY + s, ph)) return;
+      mbar_expect_tx(bar(BAR_K_FULL + s), C::kvTile);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) tma_load_3d(k_addr(s) + c * (BN * 128), &maps.k, bar(BAR_K_FULL + s), c * 64, row, hk);
+      if (!wait1(BAR_V_EMPTY + s, ph)) return;
+      mbar_expect_tx(bar(BAR_V_FULL + s), C::kvTile);
+#pragma unroll
+      for (int c = 0; c < D / 64; ++c) tma_load_3d(v_addr(s) + c * (BN * 128), &maps.v, bar(BAR_V_FULL + s), c * 64, row, hk);
+    }
+  }
+
+  // The last block reaches past the sequence's keys. Their P is 0, but 0 x Inf or 0 x NaN is NaN: whatever lies there (the next
+  // sequence, rows nobody filled) is zeroed in shared memory before the second product reads it.
+  __device__ __forceinline__ bool has_tail() const { return n_it * BN > si.sk; }
+
+  __device__ __forceinline__ void issuer() {
+    bool live = true;
+    const uint32_t kd = smem_desc_lo(k_addr(0), 16), vd = smem_desc_lo(v_addr(0), BN * 128);
+    uint32_t qd[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) qd[t] = smem_desc_lo(q_addr(t), 16);
+    auto issue_s = [&](int t, int it) {
+      const uint32_t o = (uint32_t)(((it % KS) * C::kvTile) >> 4);
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) {
+        const uint32_t a = (uint32_t)(((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4);
+        mma_ss(s_cols(t), qd[t] + a, kd + o + a, idesc_s, kk > 0 ? 1u : 0u);
+      }
+      mma_commit(bar(BAR_S_FULL + t));
+    };
+    auto issue_o = [&](int t, int it) {
+      const uint32_t o = (uint32_t)(((it % KS) * C::kvTile) >> 4);
+#pragma unroll
+      for (int kk = 0; kk < BN / 16; ++kk)
+        mma_ts(o_cols(t), s_cols(t) + kk * 16, vd + o + (uint32_t)((kk * 16 * 128) >> 4), idesc_o, (it > 0 || kk > 0) ? 1u : 0u);
+      if (it == n_of[t] - 1) mma_commit(bar(BAR_O_DONE + t));
+    };
+    live = wait1(BAR_K_FULL + 0, 0);
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      if (n_of[t] == 0) continue;
+      live = wait1(BAR_Q + t, 0) && live;
+      if (!live) return;
+      tc_fence_after();
+      issue_s(t, 0);
+    }
+    mma_commit(bar(BAR_K_EMPTY + 0));
+    for (int it = 0; it < n_it; ++it) {
+      const int s = it % KS, s1 = (it + 1) % KS;
+      live = wait1(BAR_V_FULL + s, (it / KS) & 1) && live;
+      if (it == n_it - 1 && has_tail()) live = wait1(BAR_TAIL, 0) && live;
+      if (it + 1 < n_it) live = wait1(BAR_K_FULL + s1, ((it + 1) / KS) & 1) && live;
+      if (!live) return;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (it >= n_of[t]) continue;
+        if (!wait1(BAR_P_FULL + t, it & 1)) return;
+        tc_fence_after();
+        issue_o(t, it);
+        if (it + 1 < n_of[t]) issue_s(t, it + 1);  // behind PV in the pipe: it overwrites the P that PV reads
+      }
+      mma_commit(bar(BAR_V_EMPTY + s));
+      if (it + 1 < n_it) mma_commit(bar(BAR_K_EMPTY + s1));
+    }
+  }
+
+  // Warps 2 and 3 (w = 0, 1): biases of block `it` into buffer it % 2. Entry u: key column - row = u - (2 BM - 1).
+  __device__ __forceinline__ void bias_warp(int w) {
+    float* tab = reinterpret_cast<float*>(misc + M_TAB);
+    int* starts = reinterpret_cast<int*>(misc + M_STARTS);
+    for (int t = w * 32 + lane; t < rel.nb; t += 64)
+      tab[t] = to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + head * rel.head_stride]) * kLog2e;
+    for (int t = w * 32 + lane; t < rel.side - 1; t += 64) starts[t] = rel.starts[t];
+    named_barrier_sync(1, 64);
+    for (int it = 0; it < n_it; ++it) {
+      const int buf = it & 1;
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (it >= 2 && it - 2 < n_of[t]) warp_wait(BAR_ST_EMPTY + 2 * buf + t, ((it >> 1) & 1) ^ 1);
+      if (aborted()) return;
+      const int base = it * BN - r0 - off - (2 * BM - 1);
+      auto bucket_at = [&](int u) { return relpos_bucket(base + u, starts, rel.side, rel.two); };
+      // first and last positions of tile 1 (u = 0 and BM + BN - 2), tile 0 (BM and 2 BM + BN - 2)
+      const int mine = bucket_at((lane & 1 ? BM + BN - 2 : 0) + (lane & 2 ? 0 : BM));
+      const int f0 = __shfl_sync(0xffffffffu, mine, 0), l0 = __shfl_sync(0xffffffffu, mine, 1);
+      const int f1 = __shfl_sync(0xffffffffu, mine, 2), l1 = __shfl_sync(0xffffffffu, mine, 3);
+      // (with a negative or zero scale the row maximum does not follow the scores': such calls take the general path)
+      const bool uni0 = f0 == l0 && p.scale > 0.f, uni1 = f1 == l1 && p.scale > 0.f;
+      if (w == 0 && lane == 0) {
+        int* flag = reinterpret_cast<int*>(misc + M_UNI) + 2 * buf;
+        float* val = reinterpret_cast<float*>(misc + M_UNI + 16) + 2 * buf;
+        flag[0] = uni0; flag[1] = uni1;
+        val[0] = tab[f0]; val[1] = tab[f1];
+      }
+      if (!(uni0 && uni1)) {
+        float* arr = reinterpret_cast<float*>(misc + M_BIAS) + buf * 4 * kCopyStride;
+#pragma unroll
+        for (int i = 0; i < kSpan / 64; ++i) {
+          const int u = w * (kSpan / 2) + i * 32 + lane;
+          const float b = tab[bucket_at(u)];
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (u >= k) arr[k * kCopyStride + u - k] = b;
+        }
+      }
+      __syncwarp();
+      if (lane == 0) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (it >= n_of[t]) continue;
+          if (it > 0) wait1(BAR_S_FULL + t, (it - 1) & 1);  // this arrival belongs to the next phase
+          mbar_arrive(bar(BAR_S_FULL + t));
+        }
+      }
+      __syncwarp();
+    }
+  }
+  // Warp 3 as well: zeros behind the last key (see has_tail). Runs inside bias_warp's loop order: before the last block's arrival
+  // would be too late for nobody, since only the last PV waits for it.
+  __device__ __forceinline__ void zero_tail() {
+    const int it = n_it - 1, s = it % KS;
+    warp_wait(BAR_V_FULL + s, (it / KS) & 1);
+    if (aborted()) return;
+    const int first = si.sk - it * BN;  // rows first .. BN - 1 of the block
+    uint8_t* v = smem + C::vOff + s * C::kvTile;
+    for (int x = lane; x < (BN - first) * (D / 8); x += 32) {
+      const int r = first + x / (D / 8), u = x % (D / 8);  // whole rows: the swizzle only permutes units inside a row's 128 bytes
+      *reinterpret_cast<uint4*>(v + (u >> 3) * (BN * 128) + r * 128 + (u & 7) * 16) = make_uint4(0, 0, 0, 0);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(BAR_TAIL));
+  }
+
+  // ---- softmax and epilogue of tile t: one thread per row ----
+  __device__ __forceinline__ void softmax(int t) {
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+    const int orow = r0 + t * BM + row;
+    const bool row_ok = orow < si.sq;
+    const float scale2 = p.scale * kLog2e;
+    const float2 sc2 = make_float2(scale2, scale2);
+    const int n = t ? n_of[1] : n_of[0];  // (a dynamic index would put the array into local memory)
+    float m = -INFINITY, l = 0.f;
+    // this row's staged biases: entry a + column, read 4 at a time from the copy that is aligned for it
+    const int a = 2 * BM - 1 - (t * BM + row);
+    const float* bias_row = reinterpret_cast<const float*>(misc + M_BIAS) + (a & 3) * kCopyStride + (a & ~3);
+
+    for (int it = 0; it < n; ++it) {
+      const int buf = it & 1, c0 = it * BN;
+      int cmax = si.sk - 1 - c0;
+      bool need_mask = c0 + BN > si.sk;
+      if (p.causal) {
+        need_mask = need_mask || c0 + BN - 1 > r0 + t * BM + off;
+        cmax = min(cmax, orow + off - c0);
+      }
+      warp_wait(BAR_S_FULL + t, it & 1);
+      tc_fence_after();
+      uint32_t raw[BN / 32][32];
+#pragma unroll
+      for (int q = 0; q < BN / 32; ++q) tmem_ld32(s_cols(t) + lane_off + q * 32, raw[q]);
+      const bool uni = reinterpret_cast<const int*>(misc + M_UNI)[2 * buf + t] != 0;
+      const float ub = reinterpret_cast<const float*>(misc + M_UNI + 16)[2 * buf + t];
+      tmem_ld_wait();
+      float v[BN], mx;
+#pragma unroll
+      for (int c = 0; c < BN; ++c) v[c] = __uint_as_float(raw[c / 32][c % 32]);
+      const bool fold = uni && !need_mask;  // scale and bias folded into the exponent
+      if (fold) {
+        mx = fmaf(row_max(v), scale2, ub);
+      } else if (uni) {
+#pragma unroll
+        for (int c = 0; c < BN; ++c) v[c] = c > cmax ? -INFINITY : fmaf(v[c], scale2, ub);
+        mx = row_max(v);
+      } else {
+        const float4* b4 = reinterpret_cast<const float4*>(bias_row + buf * 4 * kCopyStride);
+#pragma unroll
+        for (int c = 0; c < BN / 4; ++c) {
+          const float4 b = b4[c];
+          const float2 x = __ffma2_rn(make_float2(v[4 * c], v[4 * c + 1]), sc2, make_float2(b.x, b.y));
+          const float2 y = __ffma2_rn(make_float2(v[4 * c + 2], v[4 * c + 3]), sc2, make_float2(b.z, b.w));
+          v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = y.x; v[4 * c + 3] = y.y;
+        }
+        if (need_mask) {
+#pragma unroll
+          for (int c = 0; c < BN; ++c) if (c > cmax) v[c] = -INFINITY;
+        }
+        mx = row_max(v);
+      }
+      const float m_new = fmaxf(m, mx);
+      const bool grow = m_new - m > kRescaleThreshold;  // false when both are -inf (NaN)
+      if (__any_sync(0xffffffffu, grow)) {
+        const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - m_new)) : 1.f;
+        if (grow) { m = m_new; l *= alpha; }
+        if (it > 0) {  // S(it) was issued behind PV(it - 1): O is quiescent
+#pragma unroll 1
+          for (int q = 0; q < D / 32; ++q) {
+            uint32_t o[32];
+            tmem_ld32(o_cols(t) + lane_off + q * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) o[c] = __float_as_uint(__uint_as_float(o[c]) * alpha);
+            tmem_st32(o_cols(t) + lane_off + q * 32, o);
+          }
+        }
+      }
+      const float moff = m == -INFINITY ? 0.f : m;
+      const float2 mul = fold ? sc2 : make_float2(1.f, 1.f);
+      const float2 add = fold ? make_float2(ub - moff, ub - moff) : make_float2(-moff, -moff);
+      float2 ls[4] = {};
+      // 16 keys = one k-step of PV: their 8 packed columns go back over the first 8 of the 16 score columns they came from
+#pragma unroll
+      for (int h = 0; h < BN / 16; ++h) {
+        uint32_t pk[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          const float2 e = __ffma2_rn(make_float2(v[h * 16 + 2 * c], v[h * 16 + 2 * c + 1]), mul, add);
+          const float2 x = make_float2(ex2(e.x), ex2(e.y));
+          ls[c & 3] = __fadd2_rn(ls[c & 3], x);
+          pk[c] = pack2<T>(x.x, x.y);
+        }
+        tmem_st8(s_cols(t) + lane_off + h * 16, pk);
+      }
+      const float2 sum = __fadd2_rn(__fadd2_rn(ls[0], ls[1]), __fadd2_rn(ls[2], ls[3]));
+      l += sum.x + sum.y;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(bar(BAR_P_FULL + t));
+        mbar_arrive(bar(BAR_ST_EMPTY + 2 * buf + t));
+      }
+    }
+    if (r0 + t * BM >= si.sq) return;  // a tile behind its sequence
+    if (n > 0) {
+      warp_wait(BAR_O_DONE + t, 0);
+      tc_fence_after();
+    }
+    // ---- epilogue: O / l; the tile's Q buffer is free (every product that read it is complete) ----
+    const float inv = l > 0.f ? 1.f / l : 0.f;
+    const bool staged = r0 + (t + 1) * BM <= si.sq;
+    const int64_t grow_ = si.q0 + orow;
+    if (p.lse && row_ok) p.lse[(int64_t)head * p.Tq + grow_] = l > 0.f ? m * kLn2 + logf(l) : -INFINITY;
+    write_out(t, row, lane_off, inv, staged, row_ok, grow_, n > 0, false);
+    if (p.od.ptr) write_out(t, row, lane_off, inv, staged, row_ok, grow_, n > 0, true);
+    tc_fence_before();
+  }
+  __device__ __forceinline__ static float row_max(const float (&v)[BN]) {
+    float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+    for (int c = 4; c < BN; ++c) mx[c & 3] = fmaxf(mx[c & 3], v[c]);
+    return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  }
+  // low: what rounding O to 16 bits left out, rounded to 16 bits itself (the backward forms rowsum(dO O) from both)
+  __device__ __forceinline__ void write_out(int t, int row, uint32_t lane_off, float inv, bool staged, bool row_ok, int64_t grow_, bool any, bool low) {
+    const SeqT& dst = low ? p.od : p.o;
+    uint8_t* tile = smem + t * C::qTile;
+    T* rowp = reinterpret_cast<T*>(dst.ptr) + (int64_t)head * dst.head_stride + grow_ * dst.row_stride;
+    if (low && staged) {  // the bulk store of O still reads the buffer
+      if ((threadIdx.x & 127) == 0) bulk_wait_group_read0();
+      named_barrier_sync(2 + t, 128);
+    }
+#pragma unroll 1
+    for (int q = 0; q < D / 32; ++q) {
+      uint32_t o[32];
+      if (any) {
+        tmem_ld32(o_cols(t) + lane_off + q * 32, o);
+        tmem_ld_wait();
+      } else {
+#pragma unroll
+        for (int c = 0; c < 32; ++c) o[c] = 0u;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = __uint_as_float(o[8 * i + 2 * e]) * inv, y = __uint_as_float(o[8 * i + 2 * e + 1]) * inv;
+          w[e] = pack2<T>(x, y);
+          if (low) {
+            const float2 r = unpack2<T>(w[e]);
+            w[e] = pack2<T>(x - r.x, y - r.y);
+          }
+        }
+        const uint4 u = make_uint4(w[0], w[1], w[2], w[3]);
+        if (staged) *reinterpret_cast<uint4*>(tile + (q >> 1) * (BM * 128) + row * 128 + ((((q & 1) * 4 + i) ^ (row & 7)) << 4)) = u;
+        else if (row_ok) *reinterpret_cast<uint4*>(rowp + q * 32 + i * 8) = u;
+      }
+    }
+    if (staged) {
+      fence_proxy_async_smem();
+      named_barrier_sync(2 + t, 128);
+      if ((threadIdx.x & 127) == 0) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) tma_store_3d(low ? &maps.lo : &maps.o, q_addr(t) + c * (BM * 128), c * 64, si.q0 + r0 + t * BM, head);
+        bulk_commit_group();
+        bulk_wait_group_read0();  // shared memory must outlive the reads
+      }
+    }
+  }
+
+  __device__ __forceinline__ void run_role() {
+    if (warp < 4) {
+      reg_dealloc<kRoleRegs>();
+      if (n_it == 0) return;
+      if (warp == 0) {
+        if (elect_one()) producer();
+      } else if (warp == 1) {
+        if (elect_one()) issuer();
+      } else {
+        bias_warp(warp - 2);
+        if (warp == 3 && has_tail() && !aborted()) zero_tail();
+      }
+    } else {
+      reg_alloc<kSoftRegs>();
+      softmax((warp >> 2) - 1);
+    }
+  }
+
+  __device__ __forceinline__ void teardown() {
+    __syncwarp();
+    __syncthreads();
+    if (*abort_flag) {
+      if (threadIdx.x == 0) atomicOr(p.status, 1);
+      for (int i = 0; i < 64; ++i) __nanosleep(20000);  // copies and products in flight land before anything is released
+      __syncthreads();
+    }
+    if (warp == 1) {
+      tc_fence_after();
+      tmem_dealloc(tmem_base, C::tmemCols);
+    }
+  }
+};
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads, 1)
+relpos_fwd_kernel(const __grid_constant__ FwdMaps maps, const __grid_constant__ Params p, const __grid_constant__ RelPos rel) {
+  extern __shared__ __align__(1024) uint8_t smem[];
+  RelFwd<T, D> cta(maps, p, rel, smem);
+  if (!cta.setup()) return;
+  cta.run_role();
+  cta.teardown();
+}
+
+template <typename T, int D>
+int launch_typed(const Params& p_in, const RelPos& rel, cudaStream_t s) {
+  using C = FwdCfg<D>;
+  Params p = p_in;
+  FwdMaps maps;
+  int r;
+  if ((r = tc_tensor_map(&maps.q, p.q, p.dtype, D, p.Tq, p.Hq, BM))) return r;
+  if ((r = tc_tensor_map(&maps.k, p.k, p.dtype, D, p.Tk, p.Hkv, BN))) return r;
+  if ((r = tc_tensor_map(&maps.v, p.v, p.dtype, D, p.Tk, p.Hkv, BN))) return r;
+  if ((r = tc_tensor_map(&maps.o, p.o, p.dtype, D, p.Tq, p.Hq, BM))) return r;
+  if ((r = tc_tensor_map(&maps.lo, p.od, p.dtype, D, p.Tq, p.Hq, BM))) return r;
+  auto kern = relpos_fwd_kernel<T, D>;
+  int sms = 0;
+  if ((r = tc_prepare_launch(reinterpret_cast<const void*>(kern), C::smemBytes, &sms))) return r;
+  p.ntiles = (p.Sq + 2 * BM - 1) / (2 * BM);
+  p.group = tc_choose_group(p, false, p.ntiles, sms);
+  const long long ctas = (long long)p.ntiles * p.Hq * p.B;
+  if (ctas <= 0 || ctas > 0x7fffffffll) return FB_ERR_TOO_LARGE;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.dynamicSmemBytes = C::smemBytes;
+  cfg.stream = s;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, maps, p, rel) == cudaSuccess ? 1 : FB_ERR_CUDA;
+}
+
+}  // namespace
+
+int launch_tc_fwd_rel(const Params& p, const RelPos& rel, cudaStream_t s) {
+  if (p.dtype == FB_BF16) return p.D == 64 ? launch_typed<__nv_bfloat16, 64>(p, rel, s) : launch_typed<__nv_bfloat16, 128>(p, rel, s);
+  return p.D == 64 ? launch_typed<__half, 64>(p, rel, s) : launch_typed<__half, 128>(p, rel, s);
+}
+
+}  // namespace fb

@@ -210,7 +210,7 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
 #pragma unroll
       for (int c = 0; c < NC; ++c) o[c] = acc_o[r][c];
       store_row<T, D>(p.o, h, row, lane, o, 1.f);
-      if (lane == 0) p.lse[srow] = lse[r];
+      if (lane == 0 && (!BIAS || p.lse)) p.lse[srow] = lse[r];
     }
     float od[NC];
     if (TANGENT) {

@@ -30,12 +30,15 @@
 // its producer (24 registers) and MMA warpgroups (240), jvp_fwd_sm90.py:163,433,461.
 #include "fb_params.h"
 #include "ptx_sm100.cuh"
+#include "tc_host.h"
 #include "../../include/flashback_b200.h"
 
 #include <cuda.h>
 #include <cstring>
 #include <mutex>
+#include <set>
 #include <type_traits>
+#include <utility>
 
 namespace fb {
 namespace {
@@ -61,7 +64,6 @@ static_assert(kRoleThreads * (kLaunchRegs - kRoleRegs) >= kPwThreads * (kPwRegs 
 constexpr int kSmemLimit = 232448;  // 227 KB opt-in maximum per CTA
 constexpr int kMiscBytes = 3072;    // barriers + TMEM slot + abort flag + DKV row statistics (2 buffers); FWD: x2, row-max exchange
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 // Relative position bias: a block of BM owner rows x BN streamed rows spans kRelSpan positions; the statistics warp
 // stages their biases (and, for the table's gradient, their buckets) per block, two buffers.
 constexpr int kRelSpan = BM + BN;  // BM + BN - 1 positions
@@ -335,7 +337,7 @@ __device__ __forceinline__ void gemm_ts_kmajor(uint32_t d_tmem, uint32_t a_tmem,
 template <typename T, int KIND, int D, bool TANGENT, bool FIRST, bool DOD, bool HOOK = false, bool BIAS = false>
 struct TcCta {
   using C = Cfg<KIND, D, TANGENT, FIRST, DOD, BIAS>;
-  static_assert(!BIAS || !TANGENT, "the bias is built into the first-order kernels");
+  static_assert(!BIAS || (!TANGENT && KIND != KIND_FWD), "the bias is built into the first-order backward kernels");
   static constexpr bool kStager = KIND == KIND_DKV || BIAS;  // the statistics warp has work
   static constexpr bool kFwd = KIND == KIND_FWD, kDq = KIND == KIND_DQ, kDkv = KIND == KIND_DKV;
   static constexpr int ST = C::ST, SS0 = C::SS0, SS1 = C::SS1, nS = C::nS;
@@ -873,7 +875,7 @@ struct TcCta {
     const int c0 = blk * BN;
     const int* starts = reinterpret_cast<const int*>(rel_area + REL_STARTS);
     const float* tab = reinterpret_cast<const float*>(rel_area + REL_TAB);
-    // FWD, DQ: r = (c0 + c) - (r0 + row + off);  DKV (rows are keys): r = (r0 + row) - (c0 + c + off)
+    // DQ: r = (c0 + c) - (r0 + row + off);  DKV (rows are keys): r = (r0 + row) - (c0 + c + off)
     const int base = kDkv ? r0 - c0 - off + (BM - 1) : c0 - r0 - off - (BM - 1);
     auto bucket_at = [&](int u) { return relpos_bucket(kDkv ? base - u : base + u, starts, rel->side, rel->two); };
     const int mine = bucket_at(lane == 0 ? 0 : kRelSpan - 2);  // lane 0: first position, the others: last
@@ -1084,31 +1086,8 @@ struct TcCta {
     }
     tmem_ld_wait();
     float pv[HC];
-    // With a bias the scores are brought to log2 units here and the running maximum is kept in them (`unit` = 1);
-    // without one the scale is folded into the exponent's FMA below.
-    const float unit = BIAS ? 1.f : scale2;
-    if constexpr (BIAS) {
-      const float2 sc2 = make_float2(scale2, scale2);
-      const int uni = reinterpret_cast<const int*>(rel_area + REL_UNI)[it & 1];
-      if (uni >= 0) {
-        const float b = reinterpret_cast<const float*>(rel_area + REL_UNI)[2 + (it & 1)];
 #pragma unroll
-        for (int c = 0; c < HC; c += 2) {
-          const float2 v = __ffma2_rn(make_float2(__uint_as_float(rs[c]), __uint_as_float(rs[c + 1])), sc2, make_float2(b, b));
-          pv[c] = v.x; pv[c + 1] = v.y;
-        }
-      } else {
-        const float* bias = rel_bias(it);
-#pragma unroll
-        for (int c = 0; c < HC; c += 2) {
-          const float2 v = __ffma2_rn(make_float2(__uint_as_float(rs[c]), __uint_as_float(rs[c + 1])), sc2, make_float2(bias[c], bias[c + 1]));
-          pv[c] = v.x; pv[c + 1] = v.y;
-        }
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < HC; ++c) pv[c] = __uint_as_float(rs[c]);
-    }
+    for (int c = 0; c < HC; ++c) pv[c] = __uint_as_float(rs[c]);
     if (need_mask) {
 #pragma unroll
       for (int c = 0; c < HC; ++c) if (cb + c > cmax) pv[c] = -INFINITY;
@@ -1127,10 +1106,10 @@ struct TcCta {
 #pragma unroll
       for (int o = 1; o < NWG; ++o) mloc = fmaxf(mloc, xchg[((it & 1) * NWG + ((wg + o) % NWG)) * 128 + row]);
       const float m_new = fmaxf(m_used, mloc);
-      const bool grow = (m_new - m_used) * unit > kRescaleThreshold;  // false when both are -inf (NaN)
+      const bool grow = (m_new - m_used) * scale2 > kRescaleThreshold;  // false when both are -inf (NaN)
       float alpha = 1.f;
       if (grow) {
-        alpha = (m_used == -INFINITY) ? 0.f : ex2((m_used - m_new) * unit);
+        alpha = (m_used == -INFINITY) ? 0.f : ex2((m_used - m_new) * scale2);
         m_used = m_new;
         l_sum *= alpha;
         z_sum *= alpha;
@@ -1151,17 +1130,16 @@ struct TcCta {
         }
         tmem_st_wait();
       }
-      moff = (m_used == -INFINITY) ? 0.f : m_used * unit;
+      moff = (m_used == -INFINITY) ? 0.f : m_used * scale2;
     } else {
       moff = lse2;
     }
     // packed f32x2 arithmetic: two columns per FMA / add
-    const float2 sc2 = make_float2(unit, unit), nmoff = make_float2(-moff, -moff);
+    const float2 sc2 = make_float2(scale2, scale2), nmoff = make_float2(-moff, -moff);
     float2 ls2[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
 #pragma unroll
     for (int c2 = 0; c2 < HC / 2; ++c2) {
-      const float2 e = BIAS ? __fadd2_rn(make_float2(pv[2 * c2], pv[2 * c2 + 1]), nmoff)
-                            : __ffma2_rn(make_float2(pv[2 * c2], pv[2 * c2 + 1]), sc2, nmoff);
+      const float2 e = __ffma2_rn(make_float2(pv[2 * c2], pv[2 * c2 + 1]), sc2, nmoff);
       const float2 pe = exp2_pair(e, c2, !need_mask);
       pv[2 * c2] = pe.x;
       pv[2 * c2 + 1] = pe.y;
@@ -1594,7 +1572,7 @@ struct TcCta {
       }
     }
     if (row_ok && wg == 0) {
-      if (FIRST) p.lse[srow] = l_sum > 0.f ? m_used * (BIAS ? kLn2 : p.scale) + logf(l_sum) : -INFINITY;
+      if (FIRST) p.lse[srow] = l_sum > 0.f ? m_used * p.scale + logf(l_sum) : -INFINITY;
       if (TANGENT) p.z1[srow] = z1o;
       if (gp) {
         p.dpsum[srow] = dsum;
@@ -2079,6 +2057,25 @@ int bwd_typed(const Params& p, cudaStream_t s) {
 
 }  // namespace
 
+int tc_tensor_map(CUtensorMap* m, const SeqT& t, int dtype, int D, int64_t rows, int heads, int box_rows) {
+  return make_map(m, t, dtype, D, rows, heads, box_rows);
+}
+
+int tc_prepare_launch(const void* kernel, int smem_bytes, int* sm_count) {
+  static std::set<std::pair<const void*, int>> done;  // guarded by g_launch_mutex
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return FB_ERR_CUDA;
+  *sm_count = device_sm_count(dev);
+  std::lock_guard<std::mutex> lock(g_launch_mutex);
+  if (!done.count({kernel, dev})) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess) return FB_ERR_CUDA;
+    done.insert({kernel, dev});
+  }
+  return FB_OK;
+}
+
+int tc_choose_group(const Params& p, bool dkv, int ntiles, int sm_count) { return choose_group(p, dkv, ntiles, sm_count); }
+
 int read_profile(long long* out16) {
   if (!kProfile) return FB_ERR_MODE;  // the instrumentation is compiled in with -DFB_PROFILE only
   return cudaMemcpyFromSymbol(out16, g_prof, sizeof(long long) * (kProfile ? 16 : 1)) == cudaSuccess ? FB_OK : FB_ERR_CUDA;
@@ -2124,8 +2121,6 @@ int launch_rel_any(const Params& p, const RelPos& rel, cudaStream_t s) {
   return p.D == 64 ? launch_rel<__half, KIND, 64>(maps, p, rel, s) : launch_rel<__half, KIND, 128>(maps, p, rel, s);
 }
 }  // namespace
-
-int launch_tc_fwd_rel(const Params& p, const RelPos& rel, cudaStream_t s) { return launch_rel_any<KIND_FWD>(p, rel, s); }
 
 static_assert(BM == kTcOwnerRows, "rows of the partial table gradients");
 int launch_tc_bwd_rel(const Params& p, const RelPos& rel, cudaStream_t s) {

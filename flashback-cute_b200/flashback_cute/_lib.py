@@ -119,7 +119,7 @@ class FbRelpos(ctypes.Structure):
 class FbRelposFwdArgs(ctypes.Structure):
     _fields_ = [
         ("prob", FbProblem), ("bias", FbRelpos),
-        ("q", FbTensor), ("k", FbTensor), ("v", FbTensor), ("out", FbTensor), ("lse", ctypes.c_void_p),
+        ("q", FbTensor), ("k", FbTensor), ("v", FbTensor), ("out", FbTensor), ("out_low", FbTensor), ("lse", ctypes.c_void_p),
     ]
 
 
@@ -426,8 +426,9 @@ def relpos(table: Optional[torch.Tensor], num_buckets: int, bidirectional: bool,
     return FbRelpos(t.data_ptr(), t.stride(0), t.stride(1), num_buckets, int(bidirectional), ctypes.addressof(starts))
 
 
-def relpos_fwd(prob, bias: FbRelpos, q, k, v, out, lse):
-    _call("fb_relpos_fwd", FbRelposFwdArgs(prob, bias, seq_tensor(q), seq_tensor(k), seq_tensor(v), seq_tensor(out), _fptr(lse)), q)
+def relpos_fwd(prob, bias: FbRelpos, q, k, v, out, lse, out_low=None):
+    a = FbRelposFwdArgs(prob, bias, seq_tensor(q), seq_tensor(k), seq_tensor(v), seq_tensor(out), seq_tensor(out_low), _fptr(lse))
+    _call("fb_relpos_fwd", a, q)
 
 
 def relpos_bwd(prob, bias: FbRelpos, q, k, v, dout, lse, dpsum, dq, dk, dv, dtable):

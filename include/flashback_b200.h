@@ -305,13 +305,15 @@ typedef struct {
   const int32_t* starts;  /* HOST, see above */
 } fb_relpos;
 
-/* Forward: O and LSE. `prob` as for fb_jvp_fwd, without row segments. */
+/* Forward: O and, where asked for, LSE and what rounding O to 16 bits left out (out_low = O - round(O), rounded itself; 16-bit
+ * types only): the backward forms rowsum(dO * O) from both. `prob` as for fb_jvp_fwd, without row segments. */
 typedef struct {
   fb_problem prob;
   fb_relpos bias;
   fb_tensor q, k, v; /* in */
   fb_tensor out;     /* out */
-  float* lse;        /* out, [heads_q][total_q], -inf on fully masked rows */
+  fb_tensor out_low; /* out, optional */
+  float* lse;        /* out, optional, [heads_q][total_q], -inf on fully masked rows */
 } fb_relpos_fwd_args;
 
 int fb_relpos_fwd(const fb_relpos_fwd_args* args, fb_stream_t stream);
