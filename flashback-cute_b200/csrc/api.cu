@@ -341,6 +341,9 @@ int relpos_tiles(const fb_problem& pr) {
   return (pr.seqlen_q + rows - 1) / rows;
 }
 
+// D in the workspace of the backward, rounded up so that what follows is 16-byte aligned
+size_t relpos_dot_floats(const fb_problem& pr) { return ((size_t)pr.heads_q * (size_t)pr.total_q + 3) / 4 * 4; }
+
 int check_bias_sizes(int dtype, int heads, int sq, int sk) {
   if (dtype != FB_BF16 && dtype != FB_F16 && dtype != FB_F32) return FB_ERR_DTYPE;
   if (heads <= 0 || sq < 0 || sk < 0) return FB_ERR_SHAPE;
@@ -379,17 +382,21 @@ extern "C" int fb_relpos_bwd(const fb_relpos_bwd_args* a, fb_stream_t stream) {
   RelPos rel;
   FB_TRY(convert_relpos(rel, a->bias, true));
   FB_TRY(check_tensor(a->q, true)); FB_TRY(check_tensor(a->k, true)); FB_TRY(check_tensor(a->v, true));
-  FB_TRY(check_tensor(a->dout, true));
+  FB_TRY(check_tensor(a->out, true)); FB_TRY(check_tensor(a->dout, true)); FB_TRY(check_tensor(a->out_low, false));
   FB_TRY(check_tensor(a->dq, false)); FB_TRY(check_tensor(a->dk, false)); FB_TRY(check_tensor(a->dv, false));
-  if (!a->lse || !a->dpsum || (a->dtable && !a->workspace)) return FB_ERR_NULL_ARG;
+  if (!a->lse || !a->workspace) return FB_ERR_NULL_ARG;
+  if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return FB_ERR_ALIGNMENT;
+  if (a->out_low.ptr && !use_tensor_cores(a->prob)) return FB_ERR_MODE;
   if (a->prob.total_q == 0 || a->prob.total_k == 0) return FB_OK;
   Params p;
   fill_problem(p, a->prob);
   FB_TRY(device_setup(&p.status));
   p.q = cvt(a->q); p.k = cvt(a->k); p.v = cvt(a->v); p.dout = cvt(a->dout);
-  p.lse = const_cast<float*>(a->lse); p.dpsum = const_cast<float*>(a->dpsum);
+  p.o = cvt(a->out); p.od = cvt(a->out_low);
+  p.lse = const_cast<float*>(a->lse); p.dpsum = a->workspace;
   p.dq = cvt(a->dq); p.dk = cvt(a->dk); p.dv = cvt(a->dv);
-  rel.dpart = a->dtable ? a->workspace : nullptr;
+  if (!a->dtable && !p.dq.ptr && !p.dk.ptr && !p.dv.ptr) return FB_OK;
+  rel.dpart = a->dtable ? a->workspace + relpos_dot_floats(a->prob) : nullptr;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int n = use_tensor_cores(a->prob) ? launch_tc_bwd_rel(p, rel, s) : launch_simt_bwd_rel(p, rel, s);
   if (n >= 0 && a->dtable) {
@@ -404,7 +411,7 @@ extern "C" int fb_relpos_bwd(const fb_relpos_bwd_args* a, fb_stream_t stream) {
 
 extern "C" size_t fb_relpos_workspace_bytes(const fb_problem* pr, int num_buckets) {
   if (!pr || check_relpos_problem(*pr) != FB_OK || num_buckets < 2 || num_buckets > FB_RELPOS_MAX_BUCKETS) return 0;
-  return sizeof(float) * (size_t)pr->batch * (size_t)pr->heads_q * (size_t)relpos_tiles(*pr) * (size_t)num_buckets;
+  return sizeof(float) * (relpos_dot_floats(*pr) + (size_t)pr->batch * (size_t)pr->heads_q * (size_t)relpos_tiles(*pr) * (size_t)num_buckets);
 }
 
 extern "C" int fb_relpos_bias(const fb_relpos_bias_args* a, fb_stream_t stream) {

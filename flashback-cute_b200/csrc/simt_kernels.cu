@@ -296,7 +296,20 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p, const __gri
     bool ok = i < si.sq;
     int64_t srow = (int64_t)h * p.Tq + si.q0 + i;
     lse[r] = ok ? p.lse[srow] : -INFINITY;
-    dps[r] = ok ? p.dpsum[srow] : 0.f;
+    if constexpr (BIAS) {  // D = rowsum(dO * O), also for the dK/dV kernel
+      float d = 0.f;
+      if (ok) {
+        const T* op = reinterpret_cast<const T*>(p.o.ptr) + (int64_t)h * p.o.head_stride + (int64_t)(si.q0 + i) * p.o.row_stride;
+        const T* gp = reinterpret_cast<const T*>(p.dout.ptr) + (int64_t)h * p.dout.head_stride + (int64_t)(si.q0 + i) * p.dout.row_stride;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) d = fmaf(to_f<T>(gp[lane + 32 * c]), to_f<T>(op[lane + 32 * c]), d);
+      }
+      d = warp_sum(d);
+      dps[r] = d;
+      if (ok && lane == 0) p.dpsum[srow] = d;
+    } else {
+      dps[r] = ok ? p.dpsum[srow] : 0.f;
+    }
     z1[r] = (ok && TANGENT) ? p.z1[srow] : 0.f;
     ddt[r] = (ok && TANGENT) ? p.ddot[srow] : 0.f;
   }
@@ -554,9 +567,7 @@ int fwd_impl(const Params& p, const typename RelArg<BIAS>::type& rel, cudaStream
 template <typename T, int D, bool TANGENT, bool BIAS>
 int bwd_impl(const Params& p, const typename RelArg<BIAS>::type& rel, cudaStream_t s) {
   int n = 0;
-  bool query_side = p.dq.ptr || p.dqd.ptr;
-  if constexpr (BIAS) query_side = query_side || rel.dpart;
-  if (query_side) {
+  if (BIAS || p.dq.ptr || p.dqd.ptr) {  // with a bias this kernel also forms D
     size_t bytes = sizeof(float) * (size_t)(D + 1) * (4 * kOwn + 4 * kTile);
     auto kern = simt_dq_kernel<T, D, TANGENT, BIAS>;
     if (set_smem(kern, bytes)) return FB_ERR_CUDA;

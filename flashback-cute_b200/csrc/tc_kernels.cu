@@ -74,7 +74,8 @@ enum {                             // byte offsets in the bias area behind the m
   REL_BIAS = REL_UNI + 16,                         // [2][kRelSpan]
   REL_IDS = REL_BIAS + 2 * kRelSpan * 4,           // [2][kRelSpan] (KIND_DQ)
   REL_DIAG = REL_IDS + 2 * kRelSpan * 4,           // [pointwise warps][32] (KIND_DQ)
-  REL_ACC = REL_DIAG + NWG * 4 * 32 * 4,           // [pointwise warps][FB_RELPOS_MAX_BUCKETS] (KIND_DQ)
+  REL_ROWDOT = REL_DIAG + NWG * 4 * 32 * 4,        // [pointwise warpgroups][BM] (KIND_DQ)
+  REL_ACC = REL_ROWDOT + NWG * BM * 4,             // [pointwise warps][FB_RELPOS_MAX_BUCKETS] (KIND_DQ)
   REL_BYTES = REL_ACC + NWG * 4 * FB_RELPOS_MAX_BUCKETS * 4
 };
 constexpr float kRescaleThreshold = 8.f;  // log2 units: rescale accumulators when the row max grew by > 2^8
@@ -209,7 +210,8 @@ enum {
   BAR_A_READY = 21,   // owner operands copied into TMEM
   BAR_S2_FULL = 22,   // 22 + phase: two-phase kernels, second tile of the pair (S_dot / dP_dot) complete
   BAR_P_HALF = 24,    // two-phase kernels: dS written (dS_dot still to come)
-  BAR_COUNT = 25
+  BAR_TAIL = 25,      // BIAS: rows behind the sequence zeroed in a streamed group
+  BAR_COUNT = 26
 };
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -717,7 +719,11 @@ struct TcCta {
       if (prof) pr_is += clock64() - ts0;
     };
     // Output GEMMs of block `it`: A operands are the 16-bit tiles the pointwise warps left in TMEM.
+    [[maybe_unused]] int tails = 0;
     auto issue_out = [&](int it) {
+      if constexpr (BIAS) {
+        if (is_tail(it)) live = wait1(BAR_TAIL, tails++ & 1) && live;
+      }
       const int s0 = it % SS0d, s1 = it % SS1, st = it % ST;
       const uint32_t o0 = (uint32_t)((s0 * C::g0Bytes) >> 4), o1 = (uint32_t)((s1 * C::g1Bytes) >> 4);
       const bool accu = it > 0;
@@ -895,6 +901,60 @@ struct TcCta {
       }
     }
   }
+  // BIAS: the last streamed block may reach past its sequence. Its P and dS are 0 there, but 0 x Inf and 0 x NaN are NaN: whatever
+  // lies behind the sequence (the next one, rows nobody filled) is zeroed in shared memory before the output GEMMs read
+  // it. (The S-like GEMMs may read it either way: those columns are masked.) DKV: once per query head.
+  __device__ __forceinline__ int stream_len() const { return kDkv ? si.sq : si.sk; }
+  __device__ __forceinline__ bool is_tail(int it) const {
+    if (stream_len() % BN == 0) return false;
+    const int blk = kDkv ? blk_begin + (it_base + it) % blk_count : it;
+    return (blk + 1) * BN > stream_len();
+  }
+  // Called by the statistics warp at block `it`, when block it - 2 has been released: the stage's previous phase (block it - 3) is over,
+  // so the parity is that of this block.
+  __device__ __forceinline__ void zero_tail(int it) {
+    static_assert(SS1 >= 3, "the parity of the stage's phase");
+    const int first = stream_len() % BN, s = it % SS1;
+    warp_wait(BAR_FULL + 3 + s, (it / SS1) & 1);
+    if (aborted()) return;
+    for (int i = 0; i < C::nG1; ++i)
+      for (int x = lane; x < (BN - first) * (D / 8); x += 32) {
+        const int r = first + x / (D / 8), u = x % (D / 8);  // whole rows: the swizzle permutes units inside a row's 128 bytes
+        *reinterpret_cast<uint4*>(smem + (inner_addr(1, s, i) - sbase) + (u >> 3) * ch1 + r * 128 + (u & 7) * 16) = make_uint4(0, 0, 0, 0);
+      }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(bar(BAR_TAIL));
+  }
+  // BIAS, KIND_DQ: D = rowsum(dO * O) of this thread's row, where O = its 16 bits + what their rounding left out. Half the columns per
+  // warpgroup; dO comes from the owner tile, O from global memory (under the first GEMMs). The dK/dV kernel reads D
+  // from memory.
+  __device__ __forceinline__ void row_dot() {
+    float d = 0.f;
+    if (n_it > 0) {
+      warp_wait(BAR_OUTER, 0);
+      const T* op = row_ptr<T>(p.o, head, si.q0 + orow);
+      const T* lp = row_ptr<T>(p.od, head, si.q0 + orow);
+      for (int cc = wg; cc < D / 32; cc += NWG) {
+        float g[32], o[32];
+        unstage32(smem + C::outerTile, cc, g);
+        if (!row_ok) break;
+        load32<T>(op, cc * 32, o);
+#pragma unroll
+        for (int c = 0; c < 32; ++c) d = fmaf(g[c], o[c], d);
+        if (lp) {
+          load32<T>(lp, cc * 32, o);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) d = fmaf(g[c], o[c], d);
+        }
+      }
+    }
+    float* part = reinterpret_cast<float*>(rel_area + REL_ROWDOT);
+    part[wg * BM + row] = d;
+    named_barrier_sync(8, kPwThreads);
+    dps = part[row] + part[BM + row];
+    if (row_ok && wg == 0) p.dpsum[srow] = dps;
+  }
   __device__ __forceinline__ void stats_stager() {
     float4 cur[BN / 32], nxt[BN / 32];
     int table_head = -1;
@@ -937,6 +997,9 @@ struct TcCta {
         // warps release a buffer after they consumed block it-2); with one stage wait for block it-1.
         if (ST == 1 && it > 0) wait1(BAR_S_FULL, (it - 1) & 1);
         mbar_arrive(bar(BAR_S_FULL + it % ST));
+      }
+      if constexpr (BIAS) {
+        if (is_tail(it)) zero_tail(it);
       }
     }
   }
@@ -1233,7 +1296,11 @@ struct TcCta {
           if (col > cmax || col < cmin) pe.x = 0.f;
           if (col + 1 > cmax || col + 1 < cmin) pe.y = 0.f;
         }
-        const float2 a = __fadd2_rn(make_float2(__uint_as_float(bp[buf][c]), __uint_as_float(bp[buf][c + 1])), ndp);
+        float2 a = __fadd2_rn(make_float2(__uint_as_float(bp[buf][c]), __uint_as_float(bp[buf][c + 1])), ndp);
+        if (BIAS && need_mask) {  // dP of a masked pair may come from whatever lies behind the sequence
+          if (col > cmax || col < cmin) a.x = 0.f;
+          if (col + 1 > cmax || col + 1 < cmin) a.y = 0.f;
+        }
         float2 ds = __fmul2_rn(pe, a);
         // a row behind its sequence adds nothing to the table's gradient, whatever the table holds where it points
         if (BIAS && kDq && !row_ok) ds = make_float2(0.f, 0.f);
@@ -1356,7 +1423,7 @@ struct TcCta {
       if (row_ok) {
         float lse = p.lse[srow];
         lse2 = (lse == -INFINITY) ? INFINITY : lse * kLog2e;
-        if (kDq) {
+        if (kDq && !BIAS) {
           dps = p.dpsum[srow];
           if (TANGENT) { z1v = p.z1[srow]; ddt = p.ddot[srow]; }
         }
@@ -1375,6 +1442,7 @@ struct TcCta {
     if constexpr (C::nATmem > 0) {
       if (n_it > 0) stage_a_operands();
     }
+    if constexpr (BIAS && kDq) row_dot();
     for (int it = 0; it < n_it; ++it) {
       const int st = it % ST;
       int blk;  // streamed block index within the sequence
@@ -1798,9 +1866,18 @@ int encode_map(CUtensorMap* m, const SeqT& t, int dtype, int D, int64_t rows, in
   cuuint64_t gstr[2] = {(cuuint64_t)t.row_stride * 2, (cuuint64_t)t.head_stride * 2};
   cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = enc(m, dtype == FB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, t.ptr, gdim, gstr,
-                   box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  auto encode = [&] {
+    return enc(m, dtype == FB_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, t.ptr, gdim, gstr,
+               box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {
+    // A thread that has made no CUDA runtime call yet that needs a context (an autograd worker's first call): the driver
+    // call above does not bind one, cudaSetDevice does.
+    int dev = 0;
+    if (cudaGetDevice(&dev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) r = encode();
+  }
   return r == CUDA_SUCCESS ? FB_OK : FB_ERR_CUDA;
 }
 
@@ -2125,10 +2202,8 @@ int launch_rel_any(const Params& p, const RelPos& rel, cudaStream_t s) {
 static_assert(BM == kTcOwnerRows, "rows of the partial table gradients");
 int launch_tc_bwd_rel(const Params& p, const RelPos& rel, cudaStream_t s) {
   int n = 0, r;
-  if (p.dq.ptr || rel.dpart) {
-    if ((r = launch_rel_any<KIND_DQ>(p, rel, s)) < 0) return r;
-    n += r;
-  }
+  if ((r = launch_rel_any<KIND_DQ>(p, rel, s)) < 0) return r;  // dQ, the table's gradient, and D for the other kernel
+  n += r;
   if (p.dk.ptr || p.dv.ptr) {
     if ((r = launch_rel_any<KIND_DKV>(p, rel, s)) < 0) return r;
     n += r;

@@ -23,10 +23,11 @@ import inspect
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .interface import _Geom, _stat, _validate
+from .interface import _validate
 
 _raw = _lib.raw
 
@@ -51,32 +52,24 @@ def bucket_starts(side: int, max_distance: int) -> tuple:
     return tuple(starts)
 
 
-@functools.lru_cache(maxsize=256)
+@functools.lru_cache(maxsize=None)  # (kept: argument templates hold the arrays' addresses)
 def _starts_array(side: int, max_distance: int):
     s = bucket_starts(side, max_distance)
     return (ctypes.c_int32 * len(s))(*s)
 
 
-class _Buckets:
-    """The bucket function of one call: what the C structure needs besides the table."""
-
-    __slots__ = ("num", "two", "starts")
-
-    def __init__(self, num: int, two: bool, max_distance: int):
-        self.num, self.two = num, two
-        self.starts = _starts_array(num // 2 if two else num, max_distance)
-
-    def bind(self, table: Optional[torch.Tensor]) -> _lib.FbRelpos:
-        return _lib.relpos(table, self.num, self.two, self.starts)
-
-
-def _buckets(num: int, two: bool, max_distance: int) -> _Buckets:
-    max_distance = int(max_distance)
+def _check_buckets(num: int, two: bool, max_distance: int) -> None:
     if not 2 <= num <= _lib.RELPOS_MAX_BUCKETS or (two and (num < 4 or num % 2)):
         raise ValueError(f"bias_table needs 2 to {_lib.RELPOS_MAX_BUCKETS} buckets, even and at least 4 when bidirectional")
     if not (num // 2 if two else num) // 2 < max_distance < 2 ** 30:
         raise ValueError("max_distance must be larger than half the buckets of a side (and below 2**30)")
-    return _Buckets(num, two, max_distance)
+
+
+def _bias(table_shape, table_stride, two: bool, max_distance: int) -> _lib.FbRelpos:
+    """The C structure, without the table's address. The array of bucket starts lives as long as the process."""
+    num = table_shape[0]
+    starts = _starts_array(num // 2 if two else num, max_distance)
+    return _lib.FbRelpos(None, table_stride[0], table_stride[1], num, int(two), ctypes.addressof(starts))
 
 
 def _check_table(table: torch.Tensor, heads: int, like: torch.Tensor) -> None:
@@ -99,105 +92,330 @@ def _check_shapes(q, k, v, rows: bool) -> None:
         raise ValueError("q, k, v must be on one device")
 
 
-def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    """`t` in a layout the kernels take (unit stride on head_dim, batch folded into rows, positive strides that are multiples
-    of 8 elements, 16-byte aligned), copied only if needed."""
-    if t is None or t.numel() == 0 or (_lib.rows_ok(t) and _raw(t).stride(-3) > 0 and _raw(t).stride(-2) > 0):
-        return t
+def _check_cu_seqlens(cu_q, cu_k, q) -> None:
+    for cu in (cu_q, cu_k):
+        if cu.dtype != torch.int32:
+            raise TypeError("cu_seqlens_q and cu_seqlens_k must be int32")
+        if cu.dim() != 1 or cu.numel() < 2 or cu.numel() != cu_q.numel() or cu.device != q.device or not cu.is_contiguous():
+            raise ValueError("cu_seqlens_q and cu_seqlens_k must be contiguous, of one length (batch + 1) and on the device of q")
+
+
+class _Plans:
+    """Plans by geometry, a bounded number of them: shapes, strides, types and options, never addresses."""
+
+    def __init__(self, most: int = 1024):
+        self.most, self.plans = most, {}
+        self.get = self.plans.get
+
+    def add(self, key, plan):
+        if len(self.plans) >= self.most:
+            self.plans.clear()
+        self.plans[key] = plan
+        return plan
+
+
+def _strides_ok(shape, stride) -> bool:
+    """Rows x heads x head_dim as the kernels take it: unit stride on head_dim, batch folded into rows, positive strides that are
+    multiples of 8 elements."""
+    if stride[-1] != 1 or stride[-2] <= 0 or stride[-3] <= 0 or stride[-2] % 8 or stride[-3] % 8:
+        return False
+    return len(shape) == 3 or shape[0] <= 1 or stride[0] == shape[1] * stride[1]
+
+
+def _plain(t: torch.Tensor) -> torch.Tensor:
+    """A copy in the standard layout (torch's .contiguous() may keep odd strides of dimensions of size 1)."""
     return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
 
 
+def _plain_strides(shape):
+    s = [1]
+    for n in reversed(shape[1:]):
+        s.append(s[-1] * n)
+    return tuple(reversed(s))
+
+
+def _raw_ptr(t: torch.Tensor) -> int:
+    return _raw(t).data_ptr()
+
+
+def _address():
+    """data_ptr, through torch.func's wrappers where a transform is active (tensors made inside one are wrappers themselves)."""
+    return _raw_ptr if torch._C._are_functorch_transforms_active() else torch.Tensor.data_ptr
+
+
+_F, _B = _lib.FbRelposFwdArgs, _lib.FbRelposBwdArgs
+_FW = {n: _lib.word(_F, n, "ptr") for n in ("q", "k", "v", "out", "out_low")}
+_FW.update(table=_lib.word(_F, "bias", "table"), lse=_lib.word(_F, "lse"), cu_q=_lib.word(_F, "prob", "cu_seqlens_q"), cu_k=_lib.word(_F, "prob", "cu_seqlens_k"))
+_BW = {n: _lib.word(_B, n, "ptr") for n in ("q", "k", "v", "out", "dout", "out_low", "dq", "dk", "dv")}
+_BW.update(table=_lib.word(_B, "bias", "table"), lse=_lib.word(_B, "lse"), cu_q=_lib.word(_B, "prob", "cu_seqlens_q"), cu_k=_lib.word(_B, "prob", "cu_seqlens_k"),
+           dtable=_lib.word(_B, "dtable"), work=_lib.word(_B, "workspace"))
+
+
+class _AttnPlan:
+    """Everything about one geometry of the attention calls that does not depend on the data: the arguments' checks, templates."""
+
+    def __init__(self, q, k, v, table, cu_q, cu_k, max_q, max_k, max_distance, scale, causal, two):
+        _validate(q, k, v)
+        _check_shapes(q, k, v, rows=cu_q is not None)
+        _check_table(table, q.shape[-2], q)
+        if cu_q is not None:
+            _check_cu_seqlens(cu_q, cu_k, q)
+        q_shape, k_shape, table_shape, dtype, device = tuple(q.shape), tuple(k.shape), tuple(table.shape), q.dtype, q.device
+        q_stride, k_stride, v_stride, table_stride = q.stride(), k.stride(), v.stride(), table.stride()
+        batch = None if cu_q is None else cu_q.shape[0] - 1
+        causal = bool(causal)
+        two = (not causal) if two is None else bool(two)
+        max_distance = int(max_distance)
+        _check_buckets(table_shape[0], two, max_distance)
+        scale = q_shape[-1] ** -0.5 if scale is None else float(scale)
+        self.q_shape, self.dtype, self.device, self.index = q_shape, dtype, device, device.index
+        self.copies = not (_strides_ok(q_shape, q_stride) and _strides_ok(k_shape, k_stride) and _strides_ok(k_shape, v_stride))
+        self.heads = q_shape[-2]
+        packed = batch is not None
+        if packed:
+            total_q, total_k, b, sq, sk = q_shape[0], k_shape[0], batch, int(max_q), int(max_k)
+        else:
+            b, sq, sk = q_shape[0], q_shape[1], k_shape[1]
+            total_q, total_k = b * sq, b * sk
+        self.total_q = total_q
+        self.empty = 0 in q_shape or 0 in k_shape
+        self.low = dtype != torch.float32
+        if self.copies or self.empty:
+            return
+        cu = 16 if packed else None  # an address to come: a problem with cu_seqlens is a packed one
+        prob = _lib.FbProblem(
+            _lib._DTYPES[dtype], b, self.heads, k_shape[-2], q_shape[-1], sq, sk, int(causal), total_q, total_k, cu, cu, scale, _lib.DEFAULT_FLAGS,
+        )
+        bias = _bias(table_shape, table_stride, two, max_distance)
+        t = lambda stride: _lib.FbTensor(None, stride[-3], stride[-2])  # noqa: E731
+        o, k = t(_plain_strides(q_shape)), t(_plain_strides(k_shape))
+        self.fwd = _lib.template(_F(prob, bias, t(q_stride), t(k_stride), t(v_stride), o, o, None))
+        self.bwd = _lib.template(_B(prob, bias, t(q_stride), t(k_stride), t(v_stride), o, o, o, None, o, k, k, None, self.heads, 1, None))
+        self.work = _lib.load().fb_relpos_workspace_bytes(ctypes.byref(prob), table_shape[0]) // 4
+
+    def forward(self, q, k, v, table, cu_q, cu_k, train: bool):
+        """(out, low, lse); the last two are None unless `train` (low: never for float32)."""
+        out = torch.empty(self.q_shape, dtype=self.dtype, device=self.device)
+        low = lse = None
+        if train:
+            lse = torch.empty((self.heads, self.total_q), dtype=torch.float32, device=self.device)
+            if self.low:
+                low = torch.empty(self.q_shape, dtype=self.dtype, device=self.device)
+        if self.empty:
+            return out.zero_(), low, lse
+        ptr, w, i = _address(), self.fwd[:], _FW
+        w[i["q"]], w[i["k"]], w[i["v"]], w[i["table"]], w[i["out"]] = ptr(q), ptr(k), ptr(v), ptr(table), ptr(out)
+        if lse is not None:
+            w[i["lse"]] = ptr(lse)
+        if low is not None:
+            w[i["out_low"]] = ptr(low)
+        if cu_q is not None:
+            w[i["cu_q"]], w[i["cu_k"]] = ptr(cu_q), ptr(cu_k)
+        _lib.call_words("fb_relpos_fwd", w, self.index)
+        return out, low, lse
+
+    def backward(self, q, k, v, table, cu_q, cu_k, out, low, lse, dout, want):
+        """[dq, dk, dv, dtable], None where not wanted."""
+        grads = [torch.empty(t.shape, dtype=self.dtype, device=self.device) if x else None for t, x in zip((q, k, v, table), want)]
+        if self.empty:
+            return [t if t is None else t.zero_() for t in grads]
+        ptr = _address()
+        if ptr(dout) % 16 or not dout.is_contiguous() or dout.stride() != _plain_strides(self.q_shape):
+            dout = _plain(dout)
+        work = torch.empty(self.work, dtype=torch.float32, device=self.device)
+        w, i = self.bwd[:], _BW
+        w[i["q"]], w[i["k"]], w[i["v"]], w[i["table"]], w[i["out"]] = ptr(q), ptr(k), ptr(v), ptr(table), ptr(out)
+        w[i["dout"]], w[i["lse"]], w[i["work"]] = ptr(dout), ptr(lse), ptr(work)
+        if low is not None:
+            w[i["out_low"]] = ptr(low)
+        if cu_q is not None:
+            w[i["cu_q"]], w[i["cu_k"]] = ptr(cu_q), ptr(cu_k)
+        for name, t in zip(("dq", "dk", "dv", "dtable"), grads):
+            if t is not None:
+                w[i[name]] = ptr(t)
+        _lib.call_words("fb_relpos_bwd", w, self.index)
+        return grads
+
+
+_attn_plans = _Plans()
+
+
 class _RelposAttnFunc(torch.autograd.Function):
-    """(q, k, v, table) -> (out, lse); backward gives dq, dk, dv and the table's gradient. First order only."""
+    """(q, k, v, table) -> out; backward gives dq, dk, dv and the table's gradient. First order only."""
 
     @staticmethod
-    def forward(q, k, v, table, cu_q, cu_k, max_q, max_k, scale, causal, buckets):
-        q, k, v = map(_rows, (q, k, v))
-        out, lse = torch.empty(q.shape, dtype=q.dtype, device=q.device), _stat(q, cu_q)
-        g = _Geom(q, k, cu_q, cu_k, max_q, max_k, scale, causal)
-        if g.empty:
-            return out.zero_(), lse.fill_(float("-inf"))
-        _lib.relpos_fwd(g.prob, buckets.bind(table), q, k, v, out, lse)
-        return out, lse
-
-    @staticmethod
-    def setup_context(ctx, inputs, output):
-        q, k, v, table, cu_q, cu_k, max_q, max_k, scale, causal, buckets = inputs
-        out, lse = output
-        ctx.mark_non_differentiable(lse)
-        ctx.save_for_backward(q, k, v, table, out, lse, cu_q, cu_k)
-        ctx.geom, ctx.buckets = (max_q, max_k, scale, causal), buckets
+    def forward(ctx, q, k, v, table, cu_q, cu_k, plan):
+        out, low, lse = plan.forward(q, k, v, table, cu_q, cu_k, True)
+        ctx.save_for_backward(q, k, v, table, cu_q, cu_k, out, low, lse)
+        ctx.plan = plan
+        return out
 
     @staticmethod
     @once_differentiable
-    def backward(ctx, dout, _dlse):
-        q, k, v, table, out, lse, cu_q, cu_k = ctx.saved_tensors
-        want = ctx.needs_input_grad[:4]
-        new = lambda t, wanted: torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted else None  # noqa: E731
-        grads = [new(t, w) for t, w in zip((q, k, v, table), want)]
-        q, k, v, out, dout = map(_rows, (q, k, v, out, dout))
-        g = _Geom(q, k, cu_q, cu_k, *ctx.geom)
-        if g.empty:
-            grads = [t if t is None else t.zero_() for t in grads]
-        elif any(want):
-            dpsum = _stat(q, cu_q)
-            _lib.bwd_row_stats(g.prob, out, dout, None, None, dpsum, None)
-            _lib.relpos_bwd(g.prob, ctx.buckets.bind(table), q, k, v, dout, lse, dpsum, *grads)
-        return (*grads, *((None,) * 7))
+    def backward(ctx, dout):
+        q, k, v, table, cu_q, cu_k, out, low, lse = ctx.saved_tensors
+        return (*ctx.plan.backward(q, k, v, table, cu_q, cu_k, out, low, lse, dout, ctx.needs_input_grad[:4]), None, None, None)
+
+
+class _RelposAttnTransformed(torch.autograd.Function):
+    """The same for torch.func transforms, which ask for setup_context (and for intermediates as outputs)."""
+
+    @staticmethod
+    def forward(q, k, v, table, cu_q, cu_k, plan):
+        return plan.forward(q, k, v, table, cu_q, cu_k, True)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        q, k, v, table, cu_q, cu_k, ctx.plan = inputs
+        ctx.mark_non_differentiable(*(t for t in output[1:] if t is not None))
+        ctx.save_for_backward(q, k, v, table, cu_q, cu_k, *output)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout, *_):
+        q, k, v, table, cu_q, cu_k, out, low, lse = map(_raw, ctx.saved_tensors)
+        return (*ctx.plan.backward(q, k, v, table, cu_q, cu_k, out, low, lse, _raw(dout), ctx.needs_input_grad[:4]), None, None, None)
+
+
+def _attention(q, k, v, table, cu_q, cu_k, max_q, max_k, max_distance, scale, causal, two):
+    while True:
+        key = (
+            q.shape, k.shape, v.shape, table.shape, q.stride(), k.stride(), v.stride(), table.stride(),
+            q.dtype, k.dtype, v.dtype, table.dtype, q.device, k.device, v.device, table.device, max_distance, scale, causal, two,
+        )
+        if cu_q is not None:
+            key += (cu_q.shape, cu_k.shape, cu_q.dtype, cu_k.dtype, cu_q.device, cu_k.device, cu_q.stride(), cu_k.stride(), max_q, max_k)
+        plan = _attn_plans.get(key)
+        if plan is None:
+            plan = _attn_plans.add(key, _AttnPlan(q, k, v, table, cu_q, cu_k, max_q, max_k, max_distance, scale, causal, two))
+        if not plan.copies:
+            break
+        q, k, v = (t if _strides_ok(t.shape, t.stride()) else _Plain.apply(t) for t in (q, k, v))
+    transformed = torch._C._are_functorch_transforms_active()
+    if not transformed and (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
+        return _attention(*(_Plain.apply(t) if t.data_ptr() % 16 else t for t in (q, k, v)), table, cu_q, cu_k, max_q, max_k, max_distance, scale, causal, two)
+    if transformed:
+        return _RelposAttnTransformed.apply(q, k, v, table, cu_q, cu_k, plan)[0]
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad)) or forward_ad._current_level >= 0:
+        return _RelposAttnFunc.apply(q, k, v, table, cu_q, cu_k, plan)
+    return plan.forward(q, k, v, table, cu_q, cu_k, False)[0]
+
+
+class _Plain(torch.autograd.Function):
+    """Copy into the standard layout."""
+
+    @staticmethod
+    def forward(t):
+        return _plain(t)
+
+    @staticmethod
+    def setup_context(ctx, inputs, output):
+        pass
+
+    @staticmethod
+    def backward(ctx, g):
+        return g
+
+    @staticmethod
+    def jvp(ctx, t):
+        return t.clone()
+
+
+class _BiasSpec:
+    """Bucket function and template of flashback_relpos_bias for one geometry."""
+
+    def __init__(self, table, sq, sk, two, max_distance):
+        if table.dim() != 2 or table.shape[1] == 0:
+            raise ValueError("bias_table must have shape (num_buckets, heads)")
+        if table.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+            raise TypeError("bias_table must be float16, bfloat16 or float32")
+        if not table.is_cuda:
+            raise NotImplementedError("flashback_cute (B200 build) has no CPU path: tensors must be CUDA tensors")
+        sq, sk, max_distance = int(sq), int(sk), int(max_distance)
+        if not (0 <= sq <= 1 << 20 and 0 <= sk <= 1 << 30):
+            raise ValueError("seqlen_q must be at most 2**20 and seqlen_k at most 2**30")
+        table_shape, table_stride, dtype, device = tuple(table.shape), table.stride(), table.dtype, table.device
+        _check_buckets(table_shape[0], two, max_distance)
+        self.num, self.heads, self.dtype, self.device, self.index = table_shape[0], table_shape[1], dtype, device, device.index
+        self.shape = (self.heads, sq, sk)
+        lib, code = _lib.load(), _lib._DTYPES[dtype]
+        self.fill = _lib.template(_lib.FbRelposBiasArgs(code, self.heads, sq, sk, _bias(table_shape, table_stride, two, max_distance), None))
+        self.grad = _lib.template(_lib.FbRelposBiasGradArgs(code, self.heads, sq, sk, _bias(table_shape, table_stride, two, max_distance), None, None, self.heads, 1, None))
+        self.work = lib.fb_relpos_bias_workspace_bytes(self.heads, sq, sk, self.num) // 4
+        self.stride = table_stride
+
+    def forward(self, table):
+        if table.stride() != self.stride:  # (tangents and second-order cotangents come in layouts of their own)
+            table = torch.empty_strided(table.shape, self.stride, dtype=table.dtype, device=table.device).copy_(table)
+        out = torch.empty(self.shape, dtype=self.dtype, device=self.device)
+        if out.numel():
+            ptr, w = _address(), self.fill[:]
+            w[_FILL_TABLE], w[_FILL_OUT] = ptr(table), ptr(out)
+            _lib.call_words("fb_relpos_bias", w, self.index)
+        return out
+
+    def backward(self, grad):
+        ptr = _address()
+        if not grad.is_contiguous() or ptr(grad) % 16:
+            grad = _plain(grad)
+        dtable = torch.empty((self.num, self.heads), dtype=self.dtype, device=self.device)
+        if grad.numel() == 0:
+            return dtable.zero_()
+        work = torch.empty(self.work, dtype=torch.float32, device=self.device)
+        w = self.grad[:]
+        w[_GRAD_IN], w[_GRAD_OUT], w[_GRAD_WORK] = ptr(grad), ptr(dtable), ptr(work)
+        _lib.call_words("fb_relpos_bias_grad", w, self.index)
+        return dtable
+
+
+_FILL_TABLE, _FILL_OUT = _lib.word(_lib.FbRelposBiasArgs, "bias", "table"), _lib.word(_lib.FbRelposBiasArgs, "out")
+_GRAD_IN, _GRAD_OUT, _GRAD_WORK = (_lib.word(_lib.FbRelposBiasGradArgs, n) for n in ("grad", "dtable", "workspace"))
+_bias_specs = _Plans()
 
 
 class _RelposBiasFunc(torch.autograd.Function):
     """table (num_buckets, heads) -> bias (heads, sq, sk). Linear: derivatives of any order, both modes."""
 
     @staticmethod
-    def forward(table, sq, sk, buckets):
-        out = torch.empty(table.shape[1], sq, sk, dtype=table.dtype, device=table.device)
-        if out.numel():
-            _lib.relpos_bias(buckets.bind(table), out)
-        return out
+    def forward(table, spec):
+        return spec.forward(table)
 
     @staticmethod
     def setup_context(ctx, inputs, output):
-        _, ctx.sq, ctx.sk, ctx.buckets = inputs
+        ctx.spec = inputs[1]
 
     @staticmethod
     def backward(ctx, grad):
-        return _RelposBiasGradFunc.apply(grad, ctx.buckets), None, None, None
+        if torch.is_grad_enabled() and grad.requires_grad or torch._C._are_functorch_transforms_active():
+            return _RelposBiasGradFunc.apply(grad, ctx.spec), None
+        return ctx.spec.backward(grad), None
 
     @staticmethod
-    def jvp(ctx, table_dot, *_):
-        return _RelposBiasFunc.forward(_raw(table_dot), ctx.sq, ctx.sk, ctx.buckets)
+    def jvp(ctx, table_dot, _):
+        return ctx.spec.forward(_raw(table_dot))
 
 
 class _RelposBiasGradFunc(torch.autograd.Function):
     """The transpose of _RelposBiasFunc: (heads, sq, sk) summed by bucket, (num_buckets, heads)."""
 
     @staticmethod
-    def forward(grad, buckets):
-        grad = grad.contiguous()
-        if grad.data_ptr() % 16:
-            grad = grad.clone()
-        dtable = torch.empty(buckets.num, grad.shape[0], dtype=grad.dtype, device=grad.device)
-        if grad.numel() == 0:
-            return dtable.zero_()
-        _lib.relpos_bias_grad(buckets.bind(None), grad, dtable)
-        return dtable
+    def forward(grad, spec):
+        return spec.backward(grad)
 
     @staticmethod
     def setup_context(ctx, inputs, output):
-        grad, ctx.buckets = inputs
-        ctx.sizes = grad.shape[1:]
+        ctx.spec = inputs[1]
 
     @staticmethod
     def backward(ctx, grad2):
-        return _RelposBiasFunc.apply(grad2, *ctx.sizes, ctx.buckets), None
+        return _RelposBiasFunc.apply(grad2, ctx.spec), None
 
     @staticmethod
-    def jvp(ctx, grad_dot, *_):
-        return _RelposBiasGradFunc.forward(_raw(grad_dot), ctx.buckets)
+    def jvp(ctx, grad_dot, _):
+        return ctx.spec.backward(_raw(grad_dot))
 
 
-for _fn in (_RelposAttnFunc, _RelposBiasFunc, _RelposBiasGradFunc):  # see interface.py
+for _fn in (_RelposAttnTransformed, _Plain, _RelposBiasFunc, _RelposBiasGradFunc):  # see interface.py
     _fn.forward.__signature__ = inspect.signature(_fn.forward)
 
 
@@ -215,13 +433,7 @@ def flashback_attn_relpos_func(
     (num_buckets, hq) of the same dtype (bfloat16, float16 or float32; float32 runs on CUDA cores). bidirectional: whether
     keys behind their query have buckets of their own; by default unless `causal`. Differentiable once, in q, k, v and
     bias_table."""
-    _validate(q, k, v)
-    _check_shapes(q, k, v, rows=False)
-    _check_table(bias_table, q.shape[2], q)
-    b = _buckets(bias_table.shape[0], (not causal) if bidirectional is None else bool(bidirectional), max_distance)
-    if softmax_scale is None:
-        softmax_scale = q.shape[-1] ** -0.5
-    return _RelposAttnFunc.apply(q, k, v, bias_table, None, None, None, None, softmax_scale, causal, b)[0]
+    return _attention(q, k, v, bias_table, None, None, None, None, max_distance, softmax_scale, causal, bidirectional)
 
 
 def flashback_attn_relpos_varlen_func(
@@ -239,24 +451,45 @@ def flashback_attn_relpos_varlen_func(
     bidirectional: Optional[bool] = None,
 ) -> torch.Tensor:
     """The same for packed sequences: q (total_q, hq, d), k/v (total_k, hkv, d), cu_seqlens int32 (b+1,)."""
-    _validate(q, k, v)
-    _check_shapes(q, k, v, rows=True)
-    _check_table(bias_table, q.shape[1], q)
-    for cu in (cu_seqlens_q, cu_seqlens_k):
-        if cu.dtype != torch.int32:
-            raise TypeError("cu_seqlens_q and cu_seqlens_k must be int32")
-        if cu.dim() != 1 or cu.numel() < 2 or cu.numel() != cu_seqlens_q.numel() or cu.device != q.device or not cu.is_contiguous():
-            raise ValueError("cu_seqlens_q and cu_seqlens_k must be contiguous, of one length (batch + 1) and on the device of q")
-    b = _buckets(bias_table.shape[0], (not causal) if bidirectional is None else bool(bidirectional), max_distance)
-    if softmax_scale is None:
-        softmax_scale = q.shape[-1] ** -0.5
-    return _RelposAttnFunc.apply(
-        q, k, v, bias_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, softmax_scale, causal, b
-    )[0]
+    return _attention(
+        q, k, v, bias_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, max_distance, softmax_scale, causal, bidirectional
+    )
 
 
-def _cache_ok(t: torch.Tensor) -> bool:
-    return t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(t.stride(i) >= 0 and t.stride(i) % 8 == 0 for i in range(3))
+_D = _lib.FbRelposDecodeArgs
+_DW = {n: _lib.word(_D, n, "ptr") for n in ("q", "k", "v")}
+_DW.update(table=_lib.word(_D, "bias", "table"), lens=_lib.word(_D, "lens"), out=_lib.word(_D, "out"), work=_lib.word(_D, "workspace"))
+
+
+class _DecodePlan:
+    def __init__(self, q, k, v, lens, table, max_distance, scale, two):
+        _validate(q, k, v)
+        _check_shapes(q, k, v, rows=False)
+        _check_table(table, q.shape[2], q)
+        if q.dtype == torch.float32:
+            raise TypeError("decoding takes float16 or bfloat16")
+        if lens is not None:
+            if lens.dtype != torch.int32:
+                raise TypeError("cache_seqlens must be int32")
+            if lens.shape != q.shape[:1] or lens.device != q.device or not lens.is_contiguous():
+                raise ValueError("cache_seqlens must be contiguous, of shape (batch,) and on the device of q")
+        q_shape, k_shape, table_shape, dtype = tuple(q.shape), tuple(k.shape), tuple(table.shape), q.dtype
+        q_stride, k_stride, v_stride, table_stride = q.stride(), k.stride(), v.stride(), table.stride()
+        max_distance = int(max_distance)
+        _check_buckets(table_shape[0], bool(two), max_distance)
+        ok = lambda s: s[3] == 1 and all(x >= 0 and x % 8 == 0 for x in s[:3])  # noqa: E731
+        if not (ok(k_stride) and ok(v_stride)):
+            raise ValueError("caches need unit stride on head_dim and strides that are multiples of 8 elements")
+        self.copy_q = not ok(q_stride)
+        self.empty = 0 in q_shape or 0 in k_shape
+        cache = lambda s: _lib.FbCache(None, *s[:3])  # noqa: E731
+        args = _D(_lib._DTYPES[dtype], q_shape[0], q_shape[2], k_shape[2], q_shape[3], q_shape[1], k_shape[1], q_shape[-1] ** -0.5 if scale is None else float(scale),
+                  _bias(table_shape, table_stride, bool(two), max_distance), cache(_plain_strides(q_shape) if self.copy_q else q_stride), cache(k_stride), cache(v_stride))
+        self.words = _lib.template(args)
+        self.work = _lib.load().fb_relpos_decode_workspace_bytes(ctypes.byref(args)) // 4
+
+
+_decode_plans = _Plans()
 
 
 def flashback_attn_relpos_decode(
@@ -274,28 +507,32 @@ def flashback_attn_relpos_decode(
     clamped to [0, s]). Causal: token t of sequence i sits at position cache_seqlens[i] - sq + t. Cache rows at or behind a
     sequence's length are not read. bfloat16 or float16; meant for one to a few tokens (every 16 or 32 (token, head) pairs of a kv head read the
     cache once). No autograd graph."""
-    _validate(q, k_cache, v_cache)
-    _check_shapes(q, k_cache, v_cache, rows=False)
-    _check_table(bias_table, q.shape[2], q)
-    if q.dtype == torch.float32:
-        raise TypeError("decoding takes float16 or bfloat16")
+    key = (
+        q.shape, k_cache.shape, v_cache.shape, bias_table.shape, q.stride(), k_cache.stride(), v_cache.stride(), bias_table.stride(),
+        q.dtype, k_cache.dtype, v_cache.dtype, bias_table.dtype, q.device, k_cache.device, v_cache.device, bias_table.device,
+        max_distance, softmax_scale, bidirectional,
+    )
     if cache_seqlens is not None:
-        if cache_seqlens.dtype != torch.int32:
-            raise TypeError("cache_seqlens must be int32")
-        if cache_seqlens.shape != q.shape[:1] or cache_seqlens.device != q.device or not cache_seqlens.is_contiguous():
-            raise ValueError("cache_seqlens must be contiguous, of shape (batch,) and on the device of q")
-    b = _buckets(bias_table.shape[0], bool(bidirectional), max_distance)
-    if softmax_scale is None:
-        softmax_scale = q.shape[-1] ** -0.5
+        key += (cache_seqlens.shape, cache_seqlens.stride(), cache_seqlens.dtype, cache_seqlens.device)
+    plan = _decode_plans.get(key)
+    if plan is None:
+        plan = _decode_plans.add(key, _DecodePlan(q, k_cache, v_cache, cache_seqlens, bias_table, max_distance, softmax_scale, bidirectional))
+    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if plan.empty:
+        return out.zero_()
+    if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
+        raise ValueError("caches need 16-byte alignment")
     with torch.no_grad():
-        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        if out.numel() == 0 or k_cache.numel() == 0:
-            return out.zero_()
-        if not (_cache_ok(k_cache) and _cache_ok(v_cache)):
-            raise ValueError("caches need unit stride on head_dim, strides that are multiples of 8 elements and 16-byte alignment")
-        if not _cache_ok(q):
-            q = torch.empty(q.shape, dtype=q.dtype, device=q.device).copy_(q)
-        _lib.relpos_decode(b.bind(bias_table), q, k_cache, v_cache, cache_seqlens, out, softmax_scale)
+        if plan.copy_q or q.data_ptr() % 16:
+            q = _plain(q) if plan.copy_q else q.clone()
+    w, i = plan.words[:], _DW
+    w[i["q"]], w[i["k"]], w[i["v"]], w[i["table"]], w[i["out"]] = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bias_table.data_ptr(), out.data_ptr()
+    if cache_seqlens is not None:
+        w[i["lens"]] = cache_seqlens.data_ptr()
+    if plan.work:
+        work = torch.empty(plan.work, dtype=torch.float32, device=q.device)
+        w[i["work"]] = work.data_ptr()
+    _lib.call_words("fb_relpos_decode", w, q.device.index)
     return out
 
 
@@ -305,13 +542,11 @@ def flashback_relpos_bias(
     """The bias as a tensor (heads, seqlen_q, seqlen_k) of the table's dtype (bfloat16, float16 or float32): entry (h, i, j) is
     bias_table[bucket(j - (i + seqlen_k - seqlen_q)), h]. For attention that the fused functions do not take (other head
     sizes, masks of its own) and for looking at what was learned. Differentiable in bias_table, any order and mode."""
-    if bias_table.dim() != 2 or bias_table.shape[1] == 0:
-        raise ValueError("bias_table must have shape (num_buckets, heads)")
-    if bias_table.dtype not in (torch.float16, torch.bfloat16, torch.float32):
-        raise TypeError("bias_table must be float16, bfloat16 or float32")
-    if not bias_table.is_cuda:
-        raise NotImplementedError("flashback_cute (B200 build) has no CPU path: tensors must be CUDA tensors")
-    if not (0 <= seqlen_q <= 1 << 20 and 0 <= seqlen_k <= 1 << 30):
-        raise ValueError("seqlen_q must be at most 2**20 and seqlen_k at most 2**30")
-    b = _buckets(bias_table.shape[0], bool(bidirectional), max_distance)
-    return _RelposBiasFunc.apply(bias_table, int(seqlen_q), int(seqlen_k), b)
+    two = bool(bidirectional)
+    key = (bias_table.shape, bias_table.stride(), bias_table.dtype, bias_table.device, seqlen_q, seqlen_k, two, max_distance)
+    spec = _bias_specs.get(key)
+    if spec is None:
+        spec = _bias_specs.add(key, _BiasSpec(bias_table, seqlen_q, seqlen_k, two, max_distance))
+    if not (torch.is_grad_enabled() and bias_table.requires_grad) and forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active():
+        return spec.forward(bias_table)
+    return _RelposBiasFunc.apply(bias_table, spec)

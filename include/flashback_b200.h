@@ -318,15 +318,15 @@ typedef struct {
 
 int fb_relpos_fwd(const fb_relpos_fwd_args* args, fb_stream_t stream);
 
-/* First-order backward. dq, dk, dv and dtable are optional outputs; dtable (problem dtype, the table's shape)
- * comes out of the kernel that owns the query rows, through `workspace` (fb_relpos_workspace_bytes; required with
- * dtable, contents irrelevant before and after). Sums are formed in a fixed order: results are deterministic. */
+/* First-order backward. dq, dk, dv and dtable (problem dtype, the table's shape) are optional outputs. `workspace`
+ * (fb_relpos_workspace_bytes, 16-byte aligned, contents irrelevant before and after) holds D = rowsum(dO * (out + out_low)) and the
+ * query tiles' partial table gradients. Sums are formed in a fixed order: results are deterministic. */
 typedef struct {
   fb_problem prob;
   fb_relpos bias;
-  fb_tensor q, k, v, dout; /* in */
+  fb_tensor q, k, v, out, dout; /* in */
+  fb_tensor out_low;       /* in, optional (16-bit types) */
   const float* lse;        /* in */
-  const float* dpsum;      /* in, from fb_bwd_row_stats */
   fb_tensor dq, dk, dv;    /* out, optional */
   void* dtable;            /* out, optional */
   int64_t dtable_bucket_stride, dtable_head_stride;

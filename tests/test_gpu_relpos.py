@@ -191,13 +191,65 @@ def test_rows_behind_the_last_sequence_stay():
     k, table = _mk((200, 2, 64), BF16, 1), _mk((32, 2), BF16, 2)
     from flashback_cute import relpos
 
+    import ctypes
+
     prob = _lib.problem(q, k, cu, cu, 80, 80, 0.125, True)
     lse = torch.full((2, 200), 7.0, device=DEV)
-    b = relpos._buckets(32, False, 128)
-    _lib.relpos_fwd(prob, b.bind(table), q, k, k, out, lse)
+    bias = relpos._bias(table.shape, table.stride(), False, 128)
+    bias.table = table.data_ptr()
+    a = _lib.FbRelposFwdArgs(prob, bias, *(_lib.seq_tensor(t) for t in (q, k, k, out)), _lib.seq_tensor(None), lse.data_ptr())
+    assert _lib.load().fb_relpos_fwd(ctypes.byref(a), torch.cuda.current_stream().cuda_stream) == 0
     assert (out[150:] == 7.0).all() and (lse[:, 150:] == 7.0).all()
     ref = orc.attention(q[:150], k[:150], k[:150], table, 128, False, 0.125, True, None, [70, 80], [70, 80])
     _within("out", out[:150], ref.out, ref.tol[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_rows_behind_the_last_sequence_may_hold_anything(dtype):
+    """Packed tensors with NaN behind the last sequence: neither the outputs nor any gradient of the sequences' rows sees it."""
+    for causal, lens in ((True, [70, 80, 101]), (False, [64, 1, 130])):
+        total = sum(lens)
+        cu = torch.tensor([0, *itertools.accumulate(lens)], dtype=torch.int32, device=DEV)
+        full = [_mk((total + 40, h, 64), dtype, i) for i, h in enumerate((4, 2, 2, 4))]
+        for t in full:
+            t[total:] = float("nan")
+        table = _mk((32, 4), dtype, 9)
+        leaves = [t.requires_grad_() for t in (*full[:3], table)]
+        out = flashback_attn_relpos_varlen_func(*leaves, cu, cu, max(lens), max(lens), causal=causal)
+        grads = torch.autograd.grad(out, leaves, full[3])
+        q, k, v, do = (t.detach()[:total] for t in full)
+        ref = orc.attention(q, k, v, table, 128, not causal, 0.125, causal, do, lens, lens)
+        for name, got, want, tol in zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(), *grads), ref[:5], ref.tol):
+            _within(name, got[:want.shape[0]], want, tol)
+
+
+def test_a_broken_sequence_leaves_the_others_alone():
+    """NaN in one sequence of a packed batch: the sequences before and behind it are what they are without it."""
+    lens = [100, 70, 90]
+    cu = torch.tensor([0, *itertools.accumulate(lens)], dtype=torch.int32, device=DEV)
+    good = [_mk((260, 2, 64), BF16, i) for i in range(4)]
+    table, res = _mk((32, 2), BF16, 9), []
+    for broken in (False, True):
+        q, k, v, do = (t.clone() for t in good)
+        if broken:
+            for t in (q, k, v, do):
+                t[100:170] = float("nan")
+        leaves = [t.requires_grad_() for t in (q, k, v)]
+        out = flashback_attn_relpos_varlen_func(*leaves, table, cu, cu, 100, 100, causal=True)
+        res.append((out.detach(), *torch.autograd.grad(out, leaves, do)))
+    for a, b in zip(*res):
+        assert torch.equal(a[:100], b[:100]) and torch.equal(a[170:], b[170:])
+
+
+def test_under_torch_func():
+    shapes = [(1, 70, 2, 64), (1, 70, 2, 64), (1, 70, 2, 64), (32, 2)]
+    x = [_mk(s, BF16, i) for i, s in enumerate(shapes)]
+    got = torch.func.grad(lambda *a: flashback_attn_relpos_func(*a).float().sum(), argnums=(0, 1, 2, 3))(*x)
+    leaves = [t.clone().requires_grad_() for t in x]
+    want = torch.autograd.grad(flashback_attn_relpos_func(*leaves).float().sum(), leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    with pytest.raises(RuntimeError):  # no forward mode
+        torch.func.jvp(lambda t: flashback_attn_relpos_func(*x[:3], t), (x[3],), (x[3],))
 
 
 def test_captured_and_replayed_on_a_side_stream():

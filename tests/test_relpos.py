@@ -35,7 +35,7 @@ def test_buckets_agree_with_logarithms_off_the_borders():
 @pytest.mark.parametrize("num,two,far", [(1, False, 128), (129, False, 128), (2, True, 128), (7, True, 128), (32, False, 16), (32, True, 8), (32, False, 2 ** 30)])
 def test_refused_tables(num, two, far):
     with pytest.raises(ValueError):
-        relpos._buckets(num, two, far)
+        relpos._check_buckets(num, two, far)
 
 
 def test_refused_shapes():
@@ -62,13 +62,25 @@ def test_refused_shapes():
         relpos.flashback_attn_relpos_func(t(2, 3, 4, 64), t(2, 3, 4, 64), t(2, 3, 4, 64), t(32, 4))
 
 
-def test_rows_copies_what_the_kernels_cannot_take():
-    x = torch.zeros(1, 8, 1, 64)
-    assert relpos._rows(x) is x
-    for bad in (torch.zeros(64).expand(2, 8, 3, 64), torch.zeros(2, 8, 64, 3).transpose(2, 3), torch.zeros(8 * 64 + 1)[1:].view(1, 8, 1, 64),
+def test_layouts_the_kernels_cannot_take():
+    ok = lambda t: relpos._strides_ok(t.shape, t.stride())  # noqa: E731
+    assert ok(torch.zeros(1, 8, 1, 64)) and ok(torch.zeros(8, 1, 64))
+    for bad in (torch.zeros(64).expand(2, 8, 3, 64), torch.zeros(2, 8, 64, 3).transpose(2, 3),
                 torch.zeros(8, 2, 1, 64).transpose(0, 1), torch.zeros(64).as_strided((1, 1, 1, 64), (1, 1, 1, 1))):
-        y = relpos._rows(bad)
-        assert y is not bad and y.shape == bad.shape and _lib.rows_ok(y) and torch.equal(y, bad)
+        y = relpos._plain(bad)
+        assert not ok(bad) and ok(y) and torch.equal(y, bad) and y.stride() == relpos._plain_strides(tuple(bad.shape))
+
+
+def test_templates_put_pointers_where_the_structures_have_them():
+    for struct, words in ((_lib.FbRelposFwdArgs, relpos._FW), (_lib.FbRelposBwdArgs, relpos._BW), (_lib.FbRelposDecodeArgs, relpos._DW)):
+        w = _lib.template(struct())
+        for n, (name, i) in enumerate(words.items()):
+            w[i] = 4096 + n
+        back = struct.from_buffer_copy(w.tobytes())
+        where = dict(table=lambda a: a.bias.table, cu_q=lambda a: a.prob.cu_seqlens_q, cu_k=lambda a: a.prob.cu_seqlens_k, work=lambda a: a.workspace)
+        for n, name in enumerate(words):
+            x = where.get(name, lambda a: getattr(a, name))(back)
+            assert getattr(x, "ptr", x) == 4096 + n, name
 
 
 def _prob(**kw):
@@ -103,8 +115,8 @@ def test_status_codes():
     assert fwd(bias=_bias(table=None)) == -1
     assert fwd(q=_lib.FbTensor(0x1008, 128, 64)) == -6
     assert fwd(out=_lib.FbTensor(None, 0, 0)) == -1
-    bwd = _lib.FbRelposBwdArgs(prob=_prob(), bias=_bias(), q=t, k=t, v=t, dout=t, lse=0x1000, dpsum=0x1000, dtable=0x1000)
-    assert lib.fb_relpos_bwd(ctypes.byref(bwd), None) == -1  # a table gradient without a workspace
+    bwd = _lib.FbRelposBwdArgs(prob=_prob(), bias=_bias(), q=t, k=t, v=t, out=t, dout=t, lse=0x1000, dtable=0x1000)
+    assert lib.fb_relpos_bwd(ctypes.byref(bwd), None) == -1  # no workspace
     b = _lib.FbRelposBiasArgs(0, 2, 3, 4, _bias(), 0x1004)
     assert lib.fb_relpos_bias(ctypes.byref(b), None) == -6
     b = _lib.FbRelposBiasArgs(0, 2, 3, (1 << 30) + 1, _bias(), 0x1000)
@@ -148,8 +160,8 @@ def test_struct_layouts():
 def test_workspace_bytes():
     lib = _lib.load()
     big = _prob(batch=2, heads_q=16, heads_kv=4, seqlen_q=4096, seqlen_k=4096, total_q=8192, total_k=8192)
-    assert lib.fb_relpos_workspace_bytes(ctypes.byref(big), 32) == 2 * 16 * 32 * 32 * 4
-    assert lib.fb_relpos_workspace_bytes(ctypes.byref(_prob(dtype=2, seqlen_q=17, total_q=17)), 4) == 2 * 2 * 4 * 4
+    assert lib.fb_relpos_workspace_bytes(ctypes.byref(big), 32) == (16 * 8192 + 2 * 16 * 32 * 32) * 4
+    assert lib.fb_relpos_workspace_bytes(ctypes.byref(_prob(dtype=2, seqlen_q=17, total_q=17)), 4) == (2 * 17 + 2 + 2 * 2 * 4) * 4
     assert lib.fb_relpos_workspace_bytes(None, 32) == 0 and lib.fb_relpos_workspace_bytes(ctypes.byref(big), 500) == 0
     assert lib.fb_relpos_bias_workspace_bytes(2, 5, 7, 4) > 0 and lib.fb_relpos_bias_workspace_bytes(2, 0, 7, 4) == 0
 
