@@ -324,6 +324,12 @@ int convert_relpos(RelPos& r, const fb_relpos& b, bool need_table) {
     if (b.starts[t] < 0 || (t > 0 && b.starts[t] < b.starts[t - 1])) return FB_ERR_RELPOS;
     r.starts[t] = b.starts[t];
   }
+  r.far = r.starts[r.side - 2];
+  uint8_t* bytes = reinterpret_cast<uint8_t*>(r.near_words);
+  for (int t = 0, n = 0; t < r.side; ++t) {
+    const int end = t < r.side - 1 && r.starts[t] < kRelNear ? r.starts[t] : kRelNear;
+    if (end > n) { memset(bytes + n, t, (size_t)(end - n)); n = end; }
+  }
   return FB_OK;
 }
 

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
   extern __shared__ __align__(128) uint8_t smem[];
   uint8_t* const qs = smem;                       // [R][D]
   uint8_t* const stages = smem + R * D * 2;       // per warp [kStages][K, V]
-  __shared__ int starts[FB_RELPOS_MAX_BUCKETS];
+  __shared__ RelBuckets buckets;
   __shared__ float s_m[kWarps][R], s_l[kWarps][R];
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -79,7 +79,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
   const int hk = blockIdx.y / p.row_tiles, rt = blockIdx.y - hk * p.row_tiles;
   const int b = blockIdx.z;
   const int rows = p.G * p.Sq;
-  for (int t = threadIdx.x; t < rel.side - 1; t += kThreads) starts[t] = rel.starts[t];
+  relpos_load_buckets(buckets, rel, threadIdx.x, kThreads);
   grid_dependency_wait();
   grid_launch_dependents();
   const int len = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
@@ -124,7 +124,6 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
 
   // this thread's rows of the MMA fragments: lane / 4 and lane / 4 + 8 of every 16
   const float scale2 = p.scale * kLog2e;
-  const int far = starts[rel.side - 2];  // distances from here on lie in the last bucket of their side
   int pos[MT][2], head[MT][2];
   float far_bias[MT][2], m[MT][2], l[MT][2];
   float o[MT][D / 8][4];
@@ -176,7 +175,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
       }
     }
     // bias, mask, running softmax; element e of tile n: row lane / 4 + 8 (e / 2), key j0 + 8 n + 2 (lane % 4) + e % 2
-    const bool all_far = pos_min - (j0 + KG - 1) >= far && j0 + KG <= k1;
+    const bool all_far = pos_min - (j0 + KG - 1) >= rel.far && j0 + KG <= k1;
     uint32_t pf[MT][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -190,7 +189,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
           if (!all_far) {
             const int r = j - pos[mt][x];
             bias = -INFINITY;
-            if (r <= 0 && j < k1) bias = bias_of(relpos_bucket(r, starts, rel.side, rel.two), head[mt][x]);
+            if (r <= 0 && j < k1) bias = bias_of(relpos_bucket(r, buckets, rel), head[mt][x]);
           }
           s[mt][n][e] = fmaf(s[mt][n][e], scale2, bias);
           mx[x] = fmaxf(mx[x], s[mt][n][e]);

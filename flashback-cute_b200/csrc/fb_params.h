@@ -64,22 +64,43 @@ struct RelPos {
   int64_t bucket_stride, head_stride;
   int nb, side, two;  // buckets in all / per side, 1 = both sides have buckets of their own
   float* dpart;       // backward: partial table gradients [(batch, query head)][query tile][nb], or nullptr
+  int far;            // distances from here on lie in the last bucket of their side
   int starts[FB_RELPOS_MAX_BUCKETS - 1];  // side - 1 entries
+  uint32_t near_words[256];  // the buckets of distances 0 .. 1023, a byte each
+};
+// The bucket function in shared memory: a byte per near distance (the usual case: one load), a search beyond them.
+constexpr int kRelNear = 1024;
+struct RelBuckets {
+  uint32_t near_words[kRelNear / 4];
+  int starts[FB_RELPOS_MAX_BUCKETS];
 };
 struct NoRel {};
 
 // Bucket of relative position r (key - query): the number of bucket starts at or below its distance. Each bucket is one
 // interval of r (r falls monotonically through the buckets of a side), so a range of positions whose ends share a
 // bucket lies in it altogether.
-__device__ __forceinline__ int relpos_bucket(int r, const int* starts, int side, int two) {
-  const int n = two ? abs(r) : max(-r, 0);
-  int lo = 0, hi = side - 1;  // answer in [lo, hi]
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    if (starts[mid] <= n) lo = mid + 1;
-    else hi = mid;
+__device__ __forceinline__ int relpos_bucket(int r, const RelBuckets& b, const RelPos& rel) {
+  const int n = min(rel.two ? abs(r) : max(-r, 0), rel.far);
+  int lo;
+  if (n < kRelNear) {
+    lo = reinterpret_cast<const uint8_t*>(b.near_words)[n];
+  } else {
+    lo = 0;
+    int hi = rel.side - 1;  // answer in [lo, hi]
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (b.starts[mid] <= n) lo = mid + 1;
+      else hi = mid;
+    }
   }
-  return lo + ((two && r > 0) ? side : 0);
+  return lo + ((rel.two && r > 0) ? rel.side : 0);
+}
+// Fills `b`, thread `i` of `n`. Only what the search will look at: bytes up to the first far distance.
+__device__ __forceinline__ void relpos_load_buckets(RelBuckets& b, const RelPos& rel, int i, int n) {
+  const int words = min(rel.far, kRelNear - 1) / 4 + 1;
+  for (int t = i; t < words; t += n) b.near_words[t] = rel.near_words[t];
+  if (rel.far >= kRelNear)
+    for (int t = i; t < rel.side - 1; t += n) b.starts[t] = rel.starts[t];
 }
 // Sum of `v` over the lanes that hold the same key, for keys that form one run of neighbouring lanes each; valid in the
 // first lane of a run. Fixed order.

@@ -23,14 +23,14 @@ __global__ void __launch_bounds__(kThreads) relpos_fill_kernel(const __grid_cons
   constexpr int VEC = 16 / sizeof(T);
   __shared__ T val[kRows + kCols];
   __shared__ T tab[FB_RELPOS_MAX_BUCKETS];
-  __shared__ int starts[FB_RELPOS_MAX_BUCKETS];
+  __shared__ RelBuckets buckets;
   const int h = blockIdx.z, i0 = blockIdx.y * kRows, j0 = blockIdx.x * kCols;
   const int rows = min(kRows, sq - i0), cols = min(kCols, sk - j0);
   for (int t = threadIdx.x; t < rel.nb; t += kThreads) tab[t] = reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + h * rel.head_stride];
-  for (int t = threadIdx.x; t < rel.side - 1; t += kThreads) starts[t] = rel.starts[t];
+  relpos_load_buckets(buckets, rel, threadIdx.x, kThreads);
   __syncthreads();
   const int base = j0 - (i0 + rows - 1) - (sk - sq);  // position of entry 0: the tile's last row, first column
-  for (int u = threadIdx.x; u < rows + cols - 1; u += kThreads) val[u] = tab[relpos_bucket(base + u, starts, rel.side, rel.two)];
+  for (int u = threadIdx.x; u < rows + cols - 1; u += kThreads) val[u] = tab[relpos_bucket(base + u, buckets, rel)];
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int r = warp; r < rows; r += kWarps) {
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_cons
   constexpr int PER = kSpan / 32 / VEC;  // vectors per lane and row
   __shared__ float part[kWarps][kSpan + VEC];
   __shared__ float acc[FB_RELPOS_MAX_BUCKETS];
-  __shared__ int starts[FB_RELPOS_MAX_BUCKETS];
+  __shared__ RelBuckets buckets;
   const int h = blockIdx.z;
   const int c0 = blockIdx.x * kSpan;  // first diagonal
   const int ndiag = sq + sk - 1;
@@ -87,7 +87,7 @@ __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_cons
     if ((int)threadIdx.x < rel.nb) out[threadIdx.x] = 0.f;
     return;
   }
-  for (int t = threadIdx.x; t < rel.side - 1; t += kThreads) starts[t] = rel.starts[t];
+  relpos_load_buckets(buckets, rel, threadIdx.x, kThreads);
   if (threadIdx.x < FB_RELPOS_MAX_BUCKETS) acc[threadIdx.x] = 0.f;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const T* g = grad + (int64_t)h * sq * sk;
@@ -144,7 +144,7 @@ __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_cons
   const int c = c0 + threadIdx.x;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) s += part[w][shifts[w] + threadIdx.x];
-  const int bucket = c < ndiag ? relpos_bucket(c - (sq - 1) - (sk - sq), starts, rel.side, rel.two) : -1;
+  const int bucket = c < ndiag ? relpos_bucket(c - (sq - 1) - (sk - sq), buckets, rel) : -1;
   const bool run = run_head(bucket, lane);
   s = run_sum(s, bucket, lane);
   for (int w = 0; w < kWarps; ++w) {

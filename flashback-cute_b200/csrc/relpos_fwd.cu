@@ -61,8 +61,8 @@ enum {
   M_SLOT = 256,                       // TMEM address, abort flag
   M_UNI = M_SLOT + 16,                // [2 buffers][2 tiles] flags, then the same of biases
   M_TAB = M_UNI + 32 + 208,           // 512: table column in log2 units
-  M_STARTS = M_TAB + FB_RELPOS_MAX_BUCKETS * 4,
-  M_BIAS = M_STARTS + FB_RELPOS_MAX_BUCKETS * 4,  // [2][4][kCopyStride]
+  M_BUCKETS = M_TAB + FB_RELPOS_MAX_BUCKETS * 4,  // RelBuckets
+  M_BIAS = M_BUCKETS + (int)sizeof(RelBuckets),   // [2][4][kCopyStride]
   M_BYTES = M_BIAS + 2 * 4 * kCopyStride * 4
 };
 static_assert(M_TAB == 512 && M_BIAS % 16 == 0, "layout");
@@ -271,10 +271,10 @@ struct RelFwd {
   // Warps 2 and 3 (w = 0, 1): biases of block `it` into buffer it % 2. Entry u: key column - row = u - (2 BM - 1).
   __device__ __forceinline__ void bias_warp(int w) {
     float* tab = reinterpret_cast<float*>(misc + M_TAB);
-    int* starts = reinterpret_cast<int*>(misc + M_STARTS);
+    RelBuckets& buckets = *reinterpret_cast<RelBuckets*>(misc + M_BUCKETS);
     for (int t = w * 32 + lane; t < rel.nb; t += 64)
       tab[t] = to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + head * rel.head_stride]) * kLog2e;
-    for (int t = w * 32 + lane; t < rel.side - 1; t += 64) starts[t] = rel.starts[t];
+    relpos_load_buckets(buckets, rel, w * 32 + lane, 64);
     named_barrier_sync(1, 64);
     for (int it = 0; it < n_it; ++it) {
       const int buf = it & 1;
@@ -283,7 +283,7 @@ struct RelFwd {
         if (it >= 2 && it - 2 < n_of[t]) warp_wait(BAR_ST_EMPTY + 2 * buf + t, ((it >> 1) & 1) ^ 1);
       if (aborted()) return;
       const int base = it * BN - r0 - off - (2 * BM - 1);
-      auto bucket_at = [&](int u) { return relpos_bucket(base + u, starts, rel.side, rel.two); };
+      auto bucket_at = [&](int u) { return relpos_bucket(base + u, buckets, rel); };
       // first and last positions of tile 1 (u = 0 and BM + BN - 2), tile 0 (BM and 2 BM + BN - 2)
       const int mine = bucket_at((lane & 1 ? BM + BN - 2 : 0) + (lane & 2 ? 0 : BM));
       const int f0 = __shfl_sync(0xffffffffu, mine, 0), l0 = __shfl_sync(0xffffffffu, mine, 1);

@@ -64,13 +64,13 @@ __device__ __forceinline__ void store_row(const SeqT& t, int head, int64_t row, 
 // table's gradient, one accumulator per warp and bucket.
 struct RelSmem {
   float tab[FB_RELPOS_MAX_BUCKETS];
-  int starts[FB_RELPOS_MAX_BUCKETS];
+  RelBuckets buckets;
   float acc[kWarps][FB_RELPOS_MAX_BUCKETS];
 };
 template <typename T>
 __device__ __forceinline__ void rel_load(RelSmem& rs, const RelPos& rel, int h) {
   for (int t = threadIdx.x; t < rel.nb; t += kThreads) rs.tab[t] = to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + h * rel.head_stride]);
-  for (int t = threadIdx.x; t < rel.side - 1; t += kThreads) rs.starts[t] = rel.starts[t];
+  relpos_load_buckets(rs.buckets, rel, threadIdx.x, kThreads);
 }
 template <bool BIAS> struct RelArg { using type = NoRel; };
 template <> struct RelArg<true> { using type = RelPos; };
@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
         s *= p.scale;
         bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j));
         if constexpr (BIAS) {
-          if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->starts, rel.side, rel.two)];
+          if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->buckets, rel)];
           ok = ok && s != -INFINITY;  // a bias of -inf hides the pair
         }
         if (ok) {
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
       s *= p.scale; sd *= p.scale;
       bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j)) && lse[r] != -INFINITY;
       if constexpr (BIAS) {
-        if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->starts, rel.side, rel.two)];
+        if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->buckets, rel)];
       }
       float pr = ok ? expf(s - lse[r]) : 0.f;
       float w = pr * sd;
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p, const __gri
       bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j)) && lse[r] != -INFINITY;
       [[maybe_unused]] int bucket = 0;
       if constexpr (BIAS) {
-        bucket = relpos_bucket(j - i - (si.sk - si.sq), rs->starts, rel.side, rel.two);
+        bucket = relpos_bucket(j - i - (si.sk - si.sq), rs->buckets, rel);
         if (ok) s += rs->tab[bucket];
       }
       float pr = ok ? expf(s - lse[r]) : 0.f;
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(Params p, const __gr
         const float lse = st[lane];
         bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j)) && lse != -INFINITY;
         if constexpr (BIAS) {
-          if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->starts, rel.side, rel.two)];
+          if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->buckets, rel)];
         }
         float pr = ok ? expf(s - lse) : 0.f;
         float a = dp - st[kTile + lane];

@@ -69,13 +69,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kRelSpan = BM + BN;  // BM + BN - 1 positions
 enum {                             // byte offsets in the bias area behind the misc area
   REL_TAB = 0,                                     // this head's table column, in log2 units
-  REL_STARTS = REL_TAB + FB_RELPOS_MAX_BUCKETS * 4,
-  REL_UNI = REL_STARTS + FB_RELPOS_MAX_BUCKETS * 4,  // [2] the bucket all pairs of the block fall in, or -1; [2] its bias
+  REL_BUCKETS = REL_TAB + FB_RELPOS_MAX_BUCKETS * 4,  // RelBuckets
+  REL_UNI = REL_BUCKETS + (int)sizeof(RelBuckets),  // [2] the bucket all pairs of the block fall in, or -1; [2] its bias
   REL_BIAS = REL_UNI + 16,                         // [2][kRelSpan]
   REL_IDS = REL_BIAS + 2 * kRelSpan * 4,           // [2][kRelSpan] (KIND_DQ)
   REL_DIAG = REL_IDS + 2 * kRelSpan * 4,           // [pointwise warps][32] (KIND_DQ)
-  REL_ROWDOT = REL_DIAG + NWG * 4 * 32 * 4,        // [pointwise warpgroups][BM] (KIND_DQ)
-  REL_ACC = REL_ROWDOT + NWG * BM * 4,             // [pointwise warps][FB_RELPOS_MAX_BUCKETS] (KIND_DQ)
+  REL_ROWDOT = REL_DIAG + NWG * 4 * 32 * 4,        // [BM] (KIND_DQ)
+  REL_ACC = REL_ROWDOT + BM * 4,                 // [pointwise warps][FB_RELPOS_MAX_BUCKETS] (KIND_DQ)
   REL_BYTES = REL_ACC + NWG * 4 * FB_RELPOS_MAX_BUCKETS * 4
 };
 constexpr float kRescaleThreshold = 8.f;  // log2 units: rescale accumulators when the row max grew by > 2^8
@@ -879,11 +879,11 @@ struct TcCta {
   __device__ __forceinline__ void rel_stage(int it, int buf) {
     const int blk = kDkv ? blk_begin + (it_base + it) % blk_count : it;
     const int c0 = blk * BN;
-    const int* starts = reinterpret_cast<const int*>(rel_area + REL_STARTS);
+    const RelBuckets& buckets = *reinterpret_cast<const RelBuckets*>(rel_area + REL_BUCKETS);
     const float* tab = reinterpret_cast<const float*>(rel_area + REL_TAB);
     // DQ: r = (c0 + c) - (r0 + row + off);  DKV (rows are keys): r = (r0 + row) - (c0 + c + off)
     const int base = kDkv ? r0 - c0 - off + (BM - 1) : c0 - r0 - off - (BM - 1);
-    auto bucket_at = [&](int u) { return relpos_bucket(kDkv ? base - u : base + u, starts, rel->side, rel->two); };
+    auto bucket_at = [&](int u) { return relpos_bucket(kDkv ? base - u : base + u, buckets, *rel); };
     const int mine = bucket_at(lane == 0 ? 0 : kRelSpan - 2);  // lane 0: first position, the others: last
     const int first = __shfl_sync(0xffffffffu, mine, 0), last = __shfl_sync(0xffffffffu, mine, 1);
     if (lane == 0) {
@@ -926,40 +926,55 @@ struct TcCta {
     __syncwarp();
     if (lane == 0) mbar_arrive(bar(BAR_TAIL));
   }
-  // BIAS, KIND_DQ: D = rowsum(dO * O) of this thread's row, where O = its 16 bits + what their rounding left out. Half the columns per
-  // warpgroup; dO comes from the owner tile, O from global memory (under the first GEMMs). The dK/dV kernel reads D
-  // from memory.
+  // BIAS, KIND_DQ: D = rowsum(dO * O) of the tile's rows, where O = its 16 bits + what their rounding left out. dO comes from the owner tile, O from global memory (under the first GEMMs): D / 8 lanes read a row, so that
+  // a load covers whole rows, and all of a warp's loads are in flight together. The dK/dV kernel reads D from memory.
   __device__ __forceinline__ void row_dot() {
-    float d = 0.f;
-    if (n_it > 0) {
-      warp_wait(BAR_OUTER, 0);
-      const T* op = row_ptr<T>(p.o, head, si.q0 + orow);
-      const T* lp = row_ptr<T>(p.od, head, si.q0 + orow);
-      for (int cc = wg; cc < D / 32; cc += NWG) {
-        float g[32], o[32];
-        unstage32(smem + C::outerTile, cc, g);
-        if (!row_ok) break;
-        load32<T>(op, cc * 32, o);
+    float* dots = reinterpret_cast<float*>(rel_area + REL_ROWDOT);  // [BM]
+    constexpr int U = D / 8, RPI = 32 / U;                 // 16-byte units per row, rows per load
+    constexpr int kWarpRows = BM / (NWG * 4), NL = kWarpRows / RPI;
+    const int first = (warp & 7) * kWarpRows + lane / U, u = lane % U;
+    uint4 o[NL], l[NL];
 #pragma unroll
-        for (int c = 0; c < 32; ++c) d = fmaf(g[c], o[c], d);
-        if (lp) {
-          load32<T>(lp, cc * 32, o);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) d = fmaf(g[c], o[c], d);
-        }
+    for (int j = 0; j < NL; ++j) {
+      const int r = first + j * RPI;
+      o[j] = l[j] = make_uint4(0, 0, 0, 0);
+      if (n_it > 0 && r0 + r < own_len) {
+        o[j] = *reinterpret_cast<const uint4*>(row_ptr<T>(p.o, head, si.q0 + r0 + r) + u * 8);
+        if (p.od.ptr) l[j] = *reinterpret_cast<const uint4*>(row_ptr<T>(p.od, head, si.q0 + r0 + r) + u * 8);
       }
     }
-    float* part = reinterpret_cast<float*>(rel_area + REL_ROWDOT);
-    part[wg * BM + row] = d;
+    if (n_it > 0) warp_wait(BAR_OUTER, 0);
+#pragma unroll
+    for (int j = 0; j < NL; ++j) {
+      const int r = first + j * RPI;
+      float d = 0.f;
+      if (n_it > 0 && r0 + r < own_len) {
+        const uint4 g = *reinterpret_cast<const uint4*>(smem + C::outerTile + (u >> 3) * (BM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4));
+        const uint32_t gw[4] = {g.x, g.y, g.z, g.w}, ow[4] = {o[j].x, o[j].y, o[j].z, o[j].w}, lw[4] = {l[j].x, l[j].y, l[j].z, l[j].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float2 gv = unpack2<T>(gw[e]), ov = unpack2<T>(ow[e]), lv = unpack2<T>(lw[e]);
+          d = fmaf(gv.x, ov.x, d);
+          d = fmaf(gv.y, ov.y, d);
+          d = fmaf(gv.x, lv.x, d);
+          d = fmaf(gv.y, lv.y, d);
+        }
+      }
+#pragma unroll
+      for (int x = U / 2; x > 0; x >>= 1) d += __shfl_xor_sync(0xffffffffu, d, x);
+      if (u == 0) {
+        dots[r] = d;
+        if (r0 + r < own_len) p.dpsum[(int64_t)head * p.Tq + si.q0 + r0 + r] = d;
+      }
+    }
     named_barrier_sync(8, kPwThreads);
-    dps = part[row] + part[BM + row];
-    if (row_ok && wg == 0) p.dpsum[srow] = dps;
+    dps = dots[row];
   }
   __device__ __forceinline__ void stats_stager() {
     float4 cur[BN / 32], nxt[BN / 32];
     int table_head = -1;
     if constexpr (BIAS) {
-      for (int t = lane; t < rel->side - 1; t += 32) reinterpret_cast<int*>(rel_area + REL_STARTS)[t] = rel->starts[t];
+      relpos_load_buckets(*reinterpret_cast<RelBuckets*>(rel_area + REL_BUCKETS), *rel, lane, 32);
       __syncwarp();
     }
     if (kDkv && n_it > 0) stats_load(0, nxt);
