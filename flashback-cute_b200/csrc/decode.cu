@@ -124,6 +124,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
 
   // this thread's rows of the MMA fragments: lane / 4 and lane / 4 + 8 of every 16
   const float scale2 = p.scale * kLog2e;
+  const RelFn bucket_of(rel, buckets);
   int pos[MT][2], head[MT][2];
   float far_bias[MT][2], m[MT][2], l[MT][2];
   float o[MT][D / 8][4];
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
       }
     }
     // bias, mask, running softmax; element e of tile n: row lane / 4 + 8 (e / 2), key j0 + 8 n + 2 (lane % 4) + e % 2
-    const bool all_far = pos_min - (j0 + KG - 1) >= rel.far && j0 + KG <= k1;
+    const bool all_far = pos_min - (j0 + KG - 1) >= bucket_of.far && j0 + KG <= k1;
     uint32_t pf[MT][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
           if (!all_far) {
             const int r = j - pos[mt][x];
             bias = -INFINITY;
-            if (r <= 0 && j < k1) bias = bias_of(relpos_bucket(r, buckets, rel), head[mt][x]);
+            if (r <= 0 && j < k1) bias = bias_of(bucket_of(r), head[mt][x]);
           }
           s[mt][n][e] = fmaf(s[mt][n][e], scale2, bias);
           mx[x] = fmaxf(mx[x], s[mt][n][e]);

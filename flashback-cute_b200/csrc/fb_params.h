@@ -79,22 +79,29 @@ struct NoRel {};
 // Bucket of relative position r (key - query): the number of bucket starts at or below its distance. Each bucket is one
 // interval of r (r falls monotonically through the buckets of a side), so a range of positions whose ends share a
 // bucket lies in it altogether.
-__device__ __forceinline__ int relpos_bucket(int r, const RelBuckets& b, const RelPos& rel) {
-  const int n = min(rel.two ? abs(r) : max(-r, 0), rel.far);
-  int lo;
-  if (n < kRelNear) {
-    lo = reinterpret_cast<const uint8_t*>(b.near_words)[n];
-  } else {
-    lo = 0;
-    int hi = rel.side - 1;  // answer in [lo, hi]
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (b.starts[mid] <= n) lo = mid + 1;
-      else hi = mid;
+// (its parameters by value: read once, not again behind every barrier)
+struct RelFn {
+  const RelBuckets* b;
+  int two, far, side;
+  RelFn() = default;
+  __device__ __forceinline__ RelFn(const RelPos& rel, const RelBuckets& buckets) : b(&buckets), two(rel.two), far(rel.far), side(rel.side) {}
+  __device__ __forceinline__ int operator()(int r) const {
+    const int n = min(two ? abs(r) : max(-r, 0), far);
+    int lo;
+    if (n < kRelNear) {
+      lo = reinterpret_cast<const uint8_t*>(b->near_words)[n];
+    } else {
+      lo = 0;
+      int hi = side - 1;  // answer in [lo, hi]
+      while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (b->starts[mid] <= n) lo = mid + 1;
+        else hi = mid;
+      }
     }
+    return lo + ((two && r > 0) ? side : 0);
   }
-  return lo + ((rel.two && r > 0) ? rel.side : 0);
-}
+};
 // Fills `b`, thread `i` of `n`. Only what the search will look at: bytes up to the first far distance.
 __device__ __forceinline__ void relpos_load_buckets(RelBuckets& b, const RelPos& rel, int i, int n) {
   const int words = min(rel.far, kRelNear - 1) / 4 + 1;

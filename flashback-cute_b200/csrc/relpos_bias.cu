@@ -29,8 +29,9 @@ __global__ void __launch_bounds__(kThreads) relpos_fill_kernel(const __grid_cons
   for (int t = threadIdx.x; t < rel.nb; t += kThreads) tab[t] = reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + h * rel.head_stride];
   relpos_load_buckets(buckets, rel, threadIdx.x, kThreads);
   __syncthreads();
+  const RelFn bucket_of(rel, buckets);
   const int base = j0 - (i0 + rows - 1) - (sk - sq);  // position of entry 0: the tile's last row, first column
-  for (int u = threadIdx.x; u < rows + cols - 1; u += kThreads) val[u] = tab[relpos_bucket(base + u, buckets, rel)];
+  for (int u = threadIdx.x; u < rows + cols - 1; u += kThreads) val[u] = tab[bucket_of(base + u)];
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int r = warp; r < rows; r += kWarps) {
@@ -144,7 +145,7 @@ __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_cons
   const int c = c0 + threadIdx.x;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) s += part[w][shifts[w] + threadIdx.x];
-  const int bucket = c < ndiag ? relpos_bucket(c - (sq - 1) - (sk - sq), buckets, rel) : -1;
+  const int bucket = c < ndiag ? RelFn(rel, buckets)(c - (sq - 1) - (sk - sq)) : -1;
   const bool run = run_head(bucket, lane);
   s = run_sum(s, bucket, lane);
   for (int w = 0; w < kWarps; ++w) {

@@ -276,6 +276,7 @@ struct RelFwd {
       tab[t] = to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + head * rel.head_stride]) * kLog2e;
     relpos_load_buckets(buckets, rel, w * 32 + lane, 64);
     named_barrier_sync(1, 64);
+    const RelFn bucket_of(rel, buckets);
     for (int it = 0; it < n_it; ++it) {
       const int buf = it & 1;
 #pragma unroll
@@ -283,7 +284,7 @@ struct RelFwd {
         if (it >= 2 && it - 2 < n_of[t]) warp_wait(BAR_ST_EMPTY + 2 * buf + t, ((it >> 1) & 1) ^ 1);
       if (aborted()) return;
       const int base = it * BN - r0 - off - (2 * BM - 1);
-      auto bucket_at = [&](int u) { return relpos_bucket(base + u, buckets, rel); };
+      auto bucket_at = [&](int u) { return bucket_of(base + u); };
       // first and last positions of tile 1 (u = 0 and BM + BN - 2), tile 0 (BM and 2 BM + BN - 2)
       const int mine = bucket_at((lane & 1 ? BM + BN - 2 : 0) + (lane & 2 ? 0 : BM));
       const int f0 = __shfl_sync(0xffffffffu, mine, 0), l0 = __shfl_sync(0xffffffffu, mine, 1);

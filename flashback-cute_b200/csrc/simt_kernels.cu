@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
         s *= p.scale;
         bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j));
         if constexpr (BIAS) {
-          if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->buckets, rel)];
+          if (ok) s += rs->tab[RelFn(rel, rs->buckets)(j - i - (si.sk - si.sq))];
           ok = ok && s != -INFINITY;  // a bias of -inf hides the pair
         }
         if (ok) {
@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
       s *= p.scale; sd *= p.scale;
       bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j)) && lse[r] != -INFINITY;
       if constexpr (BIAS) {
-        if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->buckets, rel)];
+        if (ok) s += rs->tab[RelFn(rel, rs->buckets)(j - i - (si.sk - si.sq))];
       }
       float pr = ok ? expf(s - lse[r]) : 0.f;
       float w = pr * sd;
@@ -348,7 +348,7 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p, const __gri
       bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j)) && lse[r] != -INFINITY;
       [[maybe_unused]] int bucket = 0;
       if constexpr (BIAS) {
-        bucket = relpos_bucket(j - i - (si.sk - si.sq), rs->buckets, rel);
+        bucket = RelFn(rel, rs->buckets)(j - i - (si.sk - si.sq));
         if (ok) s += rs->tab[bucket];
       }
       float pr = ok ? expf(s - lse[r]) : 0.f;
@@ -479,7 +479,7 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(Params p, const __gr
         const float lse = st[lane];
         bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j)) && lse != -INFINITY;
         if constexpr (BIAS) {
-          if (ok) s += rs->tab[relpos_bucket(j - i - (si.sk - si.sq), rs->buckets, rel)];
+          if (ok) s += rs->tab[RelFn(rel, rs->buckets)(j - i - (si.sk - si.sq))];
         }
         float pr = ok ? expf(s - lse) : 0.f;
         float a = dp - st[kTile + lane];

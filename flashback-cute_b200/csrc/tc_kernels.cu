@@ -876,14 +876,13 @@ struct TcCta {
   // BIAS: the biases of a block's positions. Entry u belongs to the pairs with (streamed row in block) - (owner row in
   // tile) = u - (BM - 1). Where the block's first and last position share a bucket all pairs do (the usual case far from
   // the diagonal) and only that bucket is noted.
-  __device__ __forceinline__ void rel_stage(int it, int buf) {
+  __device__ __forceinline__ void rel_stage(int it, int buf, const RelFn& bucket_of) {
     const int blk = kDkv ? blk_begin + (it_base + it) % blk_count : it;
     const int c0 = blk * BN;
-    const RelBuckets& buckets = *reinterpret_cast<const RelBuckets*>(rel_area + REL_BUCKETS);
     const float* tab = reinterpret_cast<const float*>(rel_area + REL_TAB);
     // DQ: r = (c0 + c) - (r0 + row + off);  DKV (rows are keys): r = (r0 + row) - (c0 + c + off)
     const int base = kDkv ? r0 - c0 - off + (BM - 1) : c0 - r0 - off - (BM - 1);
-    auto bucket_at = [&](int u) { return relpos_bucket(kDkv ? base - u : base + u, buckets, *rel); };
+    auto bucket_at = [&](int u) { return bucket_of(kDkv ? base - u : base + u); };
     const int mine = bucket_at(lane == 0 ? 0 : kRelSpan - 2);  // lane 0: first position, the others: last
     const int first = __shfl_sync(0xffffffffu, mine, 0), last = __shfl_sync(0xffffffffu, mine, 1);
     if (lane == 0) {
@@ -977,6 +976,8 @@ struct TcCta {
       relpos_load_buckets(*reinterpret_cast<RelBuckets*>(rel_area + REL_BUCKETS), *rel, lane, 32);
       __syncwarp();
     }
+    RelFn bucket_of;
+    if constexpr (BIAS) bucket_of = RelFn(*rel, *reinterpret_cast<const RelBuckets*>(rel_area + REL_BUCKETS));
     if (kDkv && n_it > 0) stats_load(0, nxt);
     for (int it = 0; it < n_it; ++it) {
       const int sb_ = it & 1;
@@ -1004,7 +1005,7 @@ struct TcCta {
           dst[BN + rr] = -cur[r].y; dst[2 * BN + rr] = -cur[r].z; dst[3 * BN + rr] = -cur[r].w;
         }
       }
-      if constexpr (BIAS) rel_stage(it, sb_);
+      if constexpr (BIAS) rel_stage(it, sb_, bucket_of);
       __syncwarp();
       if (lane == 0) {
         // Second arrival on the barrier the MMA issuer commits block `it`'s first S-like tiles to. Its
@@ -1256,9 +1257,10 @@ struct TcCta {
   // First-order dQ / dK,dV, one block (kernels with tangents take pw_two_phase_block): 16 streamed
   // columns at a time from the S and dP tiles, the TMEM loads of the next group in flight while
   // the current one is processed.
-  // UNI: with a bias, all pairs of the block share a bucket.
-  template <bool UNI>
-  __device__ __forceinline__ void pw_bwd_block(int it, int st, bool need_mask, int cmin, int cmax, const float* stats) {
+  // With a bias: UNI = all pairs of the block share a bucket, MASK = some are masked (without one need_mask says so at run time).
+  template <bool UNI, bool MASK>
+  __device__ __forceinline__ void pw_bwd_block(int it, int st, bool need_mask_, int cmin, int cmax, const float* stats) {
+    const bool need_mask = BIAS ? MASK : need_mask_;
     static_assert(!TANGENT, "first-order kernels only");
     const float* bias = nullptr;
     float2 b2 = make_float2(0.f, 0.f);
@@ -1318,7 +1320,7 @@ struct TcCta {
         }
         float2 ds = __fmul2_rn(pe, a);
         // a row behind its sequence adds nothing to the table's gradient, whatever the table holds where it points
-        if (BIAS && kDq && !row_ok) ds = make_float2(0.f, 0.f);
+        if (BIAS && MASK && kDq && !row_ok) ds = make_float2(0.f, 0.f);
         o_p[c2] = pack2<T>(pe.x, pe.y);
         o_ds[c2] = pack2<T>(ds.x, ds.y);
         if constexpr (BIAS && kDq) {
@@ -1467,7 +1469,7 @@ struct TcCta {
       bool need_mask;
       int cmin = 0, cmax = BN - 1;  // this thread's visible streamed-column range [cmin, cmax] (block local)
       if (!kDkv) {
-        need_mask = (c0 + BN > si.sk) || (p.causal && c0 + BN - 1 > r0 + off);
+        need_mask = (c0 + BN > si.sk) || (p.causal && c0 + BN - 1 > r0 + off) || (BIAS && r0 + BM > si.sq);
         int jmax = si.sk - 1;
         if (p.causal) jmax = min(jmax, orow + off);
         cmax = jmax - c0;
@@ -1493,12 +1495,15 @@ struct TcCta {
           const int uni = reinterpret_cast<const int*>(rel_area + REL_UNI)[it & 1];
           if (uni >= 0) {
             if constexpr (kDq) rel_flush(uni);
-            pw_bwd_block<true>(it, st, need_mask, cmin, cmax, stats);
+            if (need_mask) pw_bwd_block<true, true>(it, st, true, cmin, cmax, stats);
+            else pw_bwd_block<true, false>(it, st, false, cmin, cmax, stats);
+          } else if (need_mask) {
+            pw_bwd_block<false, true>(it, st, true, cmin, cmax, stats);
           } else {
-            pw_bwd_block<false>(it, st, need_mask, cmin, cmax, stats);
+            pw_bwd_block<false, false>(it, st, false, cmin, cmax, stats);
           }
         } else {
-          pw_bwd_block<false>(it, st, need_mask, cmin, cmax, stats);
+          pw_bwd_block<false, false>(it, st, need_mask, cmin, cmax, stats);
         }
         const long long tq1 = prof ? clock64() : 0;
         pw_publish(BAR_P_FULL + st, it, true);
