@@ -279,10 +279,7 @@ struct RelFwd {
     const RelFn bucket_of(rel, buckets);
     for (int it = 0; it < n_it; ++it) {
       const int buf = it & 1;
-#pragma unroll
-      for (int t = 0; t < 2; ++t)
-        if (it >= 2 && it - 2 < n_of[t]) warp_wait(BAR_ST_EMPTY + 2 * buf + t, ((it >> 1) & 1) ^ 1);
-      if (aborted()) return;
+      // looked up into registers before the wait for the buffer (see rel_look_up in tc_kernels.cu)
       const int base = it * BN - r0 - off - (2 * BM - 1);
       auto bucket_at = [&](int u) { return bucket_of(base + u); };
       // first and last positions of tile 1 (u = 0 and BM + BN - 2), tile 0 (BM and 2 BM + BN - 2)
@@ -291,21 +288,30 @@ struct RelFwd {
       const int f1 = __shfl_sync(0xffffffffu, mine, 2), l1 = __shfl_sync(0xffffffffu, mine, 3);
       // (with a negative or zero scale the row maximum does not follow the scores': such calls take the general path)
       const bool uni0 = f0 == l0 && p.scale > 0.f, uni1 = f1 == l1 && p.scale > 0.f;
+      const float v0 = tab[f0], v1 = tab[f1];
+      float bias[kSpan / 64];
+      if (!(uni0 && uni1)) {
+#pragma unroll
+        for (int i = 0; i < kSpan / 64; ++i) bias[i] = tab[bucket_at(w * (kSpan / 2) + i * 32 + lane)];
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t)
+        if (it >= 2 && it - 2 < n_of[t]) warp_wait(BAR_ST_EMPTY + 2 * buf + t, ((it >> 1) & 1) ^ 1);
+      if (aborted()) return;
       if (w == 0 && lane == 0) {
         int* flag = reinterpret_cast<int*>(misc + M_UNI) + 2 * buf;
         float* val = reinterpret_cast<float*>(misc + M_UNI + 16) + 2 * buf;
         flag[0] = uni0; flag[1] = uni1;
-        val[0] = tab[f0]; val[1] = tab[f1];
+        val[0] = v0; val[1] = v1;
       }
       if (!(uni0 && uni1)) {
         float* arr = reinterpret_cast<float*>(misc + M_BIAS) + buf * 4 * kCopyStride;
 #pragma unroll
         for (int i = 0; i < kSpan / 64; ++i) {
           const int u = w * (kSpan / 2) + i * 32 + lane;
-          const float b = tab[bucket_at(u)];
 #pragma unroll
           for (int k = 0; k < 4; ++k)
-            if (u >= k) arr[k * kCopyStride + u - k] = b;
+            if (u >= k) arr[k * kCopyStride + u - k] = bias[i];
         }
       }
       __syncwarp();

@@ -875,9 +875,15 @@ struct TcCta {
   }
   // BIAS: the biases of a block's positions. Entry u belongs to the pairs with (streamed row in block) - (owner row in
   // tile) = u - (BM - 1). Where the block's first and last position share a bucket all pairs do (the usual case far from
-  // the diagonal) and only that bucket is noted.
-  __device__ __forceinline__ void rel_stage(int it, int buf, const RelFn& bucket_of) {
-    const int blk = kDkv ? blk_begin + (it_base + it) % blk_count : it;
+  // the diagonal) and only that bucket is noted. Looked up into registers before the wait for the buffer: a shared-memory load takes 100
+  // clk and more beside the MMAs' operand reads, so that a chain of them behind the wait delayed every block.
+  struct RelStaged {
+    int uni;      // the common bucket, or -1
+    float value;  // its bias
+    float bias[kRelSpan / 32];
+    int ids[kRelSpan / 32];
+  };
+  __device__ __forceinline__ void rel_look_up(int blk, const RelFn& bucket_of, RelStaged& o) const {
     const int c0 = blk * BN;
     const float* tab = reinterpret_cast<const float*>(rel_area + REL_TAB);
     // DQ: r = (c0 + c) - (r0 + row + off);  DKV (rows are keys): r = (r0 + row) - (c0 + c + off)
@@ -885,18 +891,28 @@ struct TcCta {
     auto bucket_at = [&](int u) { return bucket_of(kDkv ? base - u : base + u); };
     const int mine = bucket_at(lane == 0 ? 0 : kRelSpan - 2);  // lane 0: first position, the others: last
     const int first = __shfl_sync(0xffffffffu, mine, 0), last = __shfl_sync(0xffffffffu, mine, 1);
-    if (lane == 0) {
-      reinterpret_cast<int*>(rel_area + REL_UNI)[buf] = first == last ? first : -1;
-      reinterpret_cast<float*>(rel_area + REL_UNI)[2 + buf] = tab[first];
-    }
+    o.uni = first == last ? first : -1;
+    o.value = tab[first];
     if (first != last) {
+#pragma unroll
+      for (int i = 0; i < kRelSpan / 32; ++i) {
+        o.ids[i] = bucket_at(lane + 32 * i);
+        o.bias[i] = tab[o.ids[i]];
+      }
+    }
+  }
+  __device__ __forceinline__ void rel_store_staged(int buf, const RelStaged& o) const {
+    if (lane == 0) {
+      reinterpret_cast<int*>(rel_area + REL_UNI)[buf] = o.uni;
+      reinterpret_cast<float*>(rel_area + REL_UNI)[2 + buf] = o.value;
+    }
+    if (o.uni < 0) {
       float* dst = reinterpret_cast<float*>(rel_area + REL_BIAS) + buf * kRelSpan;
       int* ids = reinterpret_cast<int*>(rel_area + REL_IDS) + buf * kRelSpan;
 #pragma unroll
       for (int i = 0; i < kRelSpan / 32; ++i) {
-        const int u = lane + 32 * i, t = bucket_at(u);
-        dst[u] = tab[t];
-        if (kDq) ids[u] = t;
+        dst[lane + 32 * i] = o.bias[i];
+        if (kDq) ids[lane + 32 * i] = o.ids[i];
       }
     }
   }
@@ -986,13 +1002,16 @@ struct TcCta {
         for (int r = 0; r < BN / 32; ++r) cur[r] = nxt[r];
         if (it + 1 < n_it) stats_load(it + 1, nxt);
       }
+      [[maybe_unused]] RelStaged staged;
       if constexpr (BIAS) {
-        const int h = kDkv ? head * G + (it_base + it) / blk_count : head;
+        const int gi = it_base + it, g = kDkv ? gi / blk_count : 0;
+        const int h = kDkv ? head * G + g : head;
         if (h != table_head) {
           __syncwarp();
           rel_load_table(h);
           table_head = h;
         }
+        rel_look_up(kDkv ? blk_begin + gi - g * blk_count : it, bucket_of, staged);
       }
       warp_wait(BAR_ST_EMPTY + sb_, ((it >> 1) & 1) ^ 1);
       if (aborted()) break;
@@ -1005,7 +1024,7 @@ struct TcCta {
           dst[BN + rr] = -cur[r].y; dst[2 * BN + rr] = -cur[r].z; dst[3 * BN + rr] = -cur[r].w;
         }
       }
-      if constexpr (BIAS) rel_stage(it, sb_, bucket_of);
+      if constexpr (BIAS) rel_store_staged(sb_, staged);
       __syncwarp();
       if (lane == 0) {
         // Second arrival on the barrier the MMA issuer commits block `it`'s first S-like tiles to. Its
