@@ -2,23 +2,28 @@
 //
 // Online softmax, in log2 units: V_ij = c log2(e) (Q K^T)_ij + log2(e) T[bucket], P = 2^(V - m), O = P V / l.
 //
-// What bounds it: per 128 x 128 scores, S = Q K^T and O += P V keep the tensor pipe busy for 512 clk each (head_dim 128; 256
-// each at 64), the 16384 exponentials keep the special-function units busy for 1024 clk. So a CTA owns TWO tiles of 128
-// query rows and lets them take turns: while the warpgroup of one tile computes exponentials, the tensor pipe works on the
-// other. One thread owns one query row (TMEM lane), 128 scores at a time in registers: row maximum and sum need no exchange between
-// threads. K and V blocks of 128 keys are shared by the two tiles.
+// What bounds it: per 128 x 64 scores, S = Q K^T and O += P V keep the tensor pipe busy for 384 + 256 clk (head_dim 128; 192 +
+// 128 at 64), the 8192 exponentials the special-function units for 512 clk, and the softmax warps need about 1100 clk from
+// a tile's scores to its P, plus several hundred clk for every hand-over. So a CTA owns TWO tiles of 128 query rows with
+// two buffers of scores each: while the warpgroup of a tile works on one block of 64 keys, the tensor pipe computes its next one and
+// the other tile's. One thread owns one query row (TMEM lane) and has 64 scores at a time in registers: row maximum and sum need no
+// exchange between threads. K and V blocks are shared by the two tiles.
 //
-//   warp 0 (one lane)   TMA: Q tiles once, K and V blocks through a ring of stages
-//   warp 1 (one lane)   every tcgen05.mma: PV(t, i) and, right behind it, S(t, i + 1), for the tiles t in turn
-//   warps 2, 3          biases of the next block's positions into shared memory; zeros behind a sequence's last key
+//   warp 0 (one lane)   TMA: Q tiles once, K and V blocks through three stages
+//   warp 1 (one lane)   every tcgen05.mma: PV(t, j) and, right behind it, S(t, j + 2) into the buffer it read, for the tiles t in turn
+//   warps 2, 3          biases of the coming blocks' positions into shared memory; zeros behind a sequence's last key
 //   warps 4-7, 8-11     softmax, rescaling and epilogue of tile 0 and tile 1
 //
-// TMEM (512 columns): per tile 128 columns of scores, overwritten by P (16 bit) as it is computed, and head_dim of output.
+// TMEM (512 columns): per tile 2 x 64 columns of scores, overwritten by P (16 bit) as it is computed, and head_dim of output.
 //
-// The bias. Blocks whose 128 x 128 positions share a bucket (all but a few around the diagonal) take one number, folded into the
-// exponent's FMA. In the others every pair reads its own: entry (key column - row) of 383 staged values. A warp's lanes
+// The bias. Blocks whose 128 x 64 positions share a bucket (all but a few around the diagonal) take one number, folded into the
+// exponent's FMA. In the others every pair reads its own: entry (key column - row) of 319 staged values. A warp's lanes
 // read neighbouring entries; four copies, each shifted by one entry, let every thread fetch four columns with one
 // 16-byte load whatever its row.
+//
+// Tried (non-causal B2 Hq16 Hkv4 S4096 D128): blocks of 128 keys with one buffer of scores per tile 340 us (a tile waits 1550 of 3800 clk
+// for its scores); the same with the exponentials started on the maximum known so far, 348 us; two CTAs per SM with one
+// tile each and two warps per row, 372 us.
 #include "fb_params.h"
 #include "ptx_sm100.cuh"
 #include "tc_host.h"
@@ -33,7 +38,7 @@ namespace {
 using namespace ptx;
 
 constexpr int BM = 128;  // query rows per tile = TMEM lanes
-constexpr int BN = 128;  // keys per block
+constexpr int BN = 64;   // keys per block
 constexpr int kRoleThreads = 128, kSoftThreads = 256, kThreads = kRoleThreads + kSoftThreads;
 // The role warps give registers back, the softmax warpgroups take them: no more than the launch left (see tc_kernels.cu).
 constexpr int kLaunchRegs = 168, kRoleRegs = 104, kSoftRegs = 200;
@@ -43,18 +48,20 @@ constexpr float kRescaleThreshold = 8.f;  // log2 units: rescale O only when the
 constexpr int kSpan = 2 * BM + BN;        // positions of a block seen from both tiles (one more than there are)
 constexpr int kCopyStride = kSpan + 8;    // floats between the shifted copies: 8 banks apart
 
+constexpr int KS = 3;                     // stages of K and of V
 enum {
-  BAR_Q = 0,        // + tile
-  BAR_K_FULL = 2,   // + stage (up to 3)
+  BAR_Q = 0,            // + tile
+  BAR_K_FULL = 2,       // + stage
   BAR_K_EMPTY = 5,
   BAR_V_FULL = 8,
   BAR_V_EMPTY = 11,
-  BAR_S_FULL = 14,  // + tile: scores complete and biases staged
-  BAR_P_FULL = 16,  // + tile
-  BAR_O_DONE = 18,  // + tile
-  BAR_ST_EMPTY = 20,  // + 2 * buffer + tile: biases of a buffer read
-  BAR_TAIL = 24,    // keys behind the sequence zeroed in the last V block
-  BAR_COUNT = 25
+  BAR_S_FULL = 14,      // + 2 * tile + slot: scores complete and biases staged
+  BAR_P_FULL = 18,      // + 2 * tile + slot
+  BAR_ST_EMPTY = 22,    // + 2 * tile + slot: biases read
+  BAR_PV_DONE = 26,     // + tile
+  BAR_O_DONE = 28,      // + tile
+  BAR_TAIL = 30,        // keys behind the sequence zeroed in the last V block
+  BAR_COUNT = 31
 };
 // Bytes behind the tiles
 enum {
@@ -69,13 +76,13 @@ static_assert(M_TAB == 512 && M_BIAS % 16 == 0, "layout");
 
 template <int D>
 struct FwdCfg {
-  static constexpr int kStages = D == 128 ? 2 : 3;
   static constexpr int qTile = BM * D * 2, kvTile = BN * D * 2;
-  static constexpr int kOff = 2 * qTile, vOff = kOff + kStages * kvTile;
-  static constexpr int tileBytes = vOff + kStages * kvTile;
-  static constexpr int smemBytes = tileBytes + M_BYTES;
+  static constexpr int kOff = 2 * qTile, vOff = kOff + KS * kvTile;
+  static constexpr int tileBytes = vOff + KS * kvTile;
+  // at least half of shared memory: TMEM takes one CTA per SM
+  static constexpr int smemBytes = tileBytes + M_BYTES < 120 * 1024 ? 120 * 1024 : tileBytes + M_BYTES;
   static_assert(smemBytes <= 232448, "shared memory");
-  static constexpr int tmemCols = 512;  // 2 x (128 scores + D): 384 at head_dim 64, and allocations are powers of two
+  static constexpr int tmemCols = 512;  // 2 x (2 x 64 scores + D): 384 at head_dim 64, and allocations are powers of two
 };
 
 struct FwdMaps {
@@ -98,7 +105,6 @@ template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { retu
 template <typename T, int D>
 struct RelFwd {
   using C = FwdCfg<D>;
-  static constexpr int KS = C::kStages;
   static constexpr int fmt = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
   static constexpr uint32_t idesc_s = make_idesc(fmt, BM, BN, 0, 0);
   static constexpr uint32_t idesc_o = make_idesc(fmt, BM, D, 0, 1);
@@ -126,8 +132,8 @@ struct RelFwd {
   __device__ __forceinline__ uint32_t q_addr(int t) const { return sbase + t * C::qTile; }
   __device__ __forceinline__ uint32_t k_addr(int s) const { return sbase + C::kOff + s * C::kvTile; }
   __device__ __forceinline__ uint32_t v_addr(int s) const { return sbase + C::vOff + s * C::kvTile; }
-  __device__ __forceinline__ uint32_t s_cols(int t) const { return tmem_base + t * BN; }
-  __device__ __forceinline__ uint32_t o_cols(int t) const { return tmem_base + 2 * BN + t * D; }
+  __device__ __forceinline__ uint32_t s_cols(int t, int slot) const { return tmem_base + (2 * t + slot) * BN; }
+  __device__ __forceinline__ uint32_t o_cols(int t) const { return tmem_base + 4 * BN + t * D; }
 
   // False: nothing to do (the whole CTA leaves together).
   __device__ __forceinline__ bool setup() {
@@ -167,8 +173,8 @@ struct RelFwd {
     if (threadIdx.x == 0) {
       for (int i = 0; i < BAR_COUNT; ++i) {
         uint32_t count = 1;
-        if (i == BAR_S_FULL || i == BAR_S_FULL + 1) count = 3;  // the MMAs and both bias warps
-        if (i == BAR_P_FULL || i == BAR_P_FULL + 1 || (i >= BAR_ST_EMPTY && i < BAR_ST_EMPTY + 4)) count = 4;  // a tile's softmax warps
+        if (i >= BAR_S_FULL && i < BAR_S_FULL + 4) count = 3;    // the MMAs and both bias warps
+        if (i >= BAR_P_FULL && i < BAR_ST_EMPTY + 4) count = 4;  // a tile's softmax warps
         mbar_init(bar(i), count);
       }
       *abort_flag = 0;
@@ -226,45 +232,48 @@ struct RelFwd {
     auto issue_s = [&](int t, int it) {
       const uint32_t o = (uint32_t)(((it % KS) * C::kvTile) >> 4);
 #pragma unroll
-      for (int kk = 0; kk < D / 16; ++kk) {
-        const uint32_t a = (uint32_t)(((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4);
-        mma_ss(s_cols(t), qd[t] + a, kd + o + a, idesc_s, kk > 0 ? 1u : 0u);
-      }
-      mma_commit(bar(BAR_S_FULL + t));
+      for (int kk = 0; kk < D / 16; ++kk)
+        mma_ss(s_cols(t, it & 1), qd[t] + (uint32_t)(((kk >> 2) * (BM * 128) + (kk & 3) * 32) >> 4),
+               kd + o + (uint32_t)(((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4), idesc_s, kk > 0 ? 1u : 0u);
+      mma_commit(bar(BAR_S_FULL + 2 * t + (it & 1)));
     };
     auto issue_o = [&](int t, int it) {
       const uint32_t o = (uint32_t)(((it % KS) * C::kvTile) >> 4);
 #pragma unroll
       for (int kk = 0; kk < BN / 16; ++kk)
-        mma_ts(o_cols(t), s_cols(t) + kk * 16, vd + o + (uint32_t)((kk * 16 * 128) >> 4), idesc_o, (it > 0 || kk > 0) ? 1u : 0u);
-      if (it == n_of[t] - 1) mma_commit(bar(BAR_O_DONE + t));
+        mma_ts(o_cols(t), s_cols(t, it & 1) + kk * 16, vd + o + (uint32_t)((kk * 16 * 128) >> 4), idesc_o, (it > 0 || kk > 0) ? 1u : 0u);
+      mma_commit(bar((it == n_of[t] - 1 ? BAR_O_DONE : BAR_PV_DONE) + t));
     };
-    live = wait1(BAR_K_FULL + 0, 0);
 #pragma unroll
-    for (int t = 0; t < 2; ++t) {
-      if (n_of[t] == 0) continue;
-      live = wait1(BAR_Q + t, 0) && live;
-      if (!live) return;
-      tc_fence_after();
-      issue_s(t, 0);
+    for (int it = 0; it < 2; ++it) {
+      if (it >= n_it) break;
+      live = wait1(BAR_K_FULL + it, 0) && live;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if (it >= n_of[t]) continue;
+        if (it == 0) live = wait1(BAR_Q + t, 0) && live;
+        if (!live) return;
+        tc_fence_after();
+        issue_s(t, it);
+      }
+      mma_commit(bar(BAR_K_EMPTY + it));
     }
-    mma_commit(bar(BAR_K_EMPTY + 0));
     for (int it = 0; it < n_it; ++it) {
-      const int s = it % KS, s1 = (it + 1) % KS;
+      const int s = it % KS, s2 = (it + 2) % KS;
       live = wait1(BAR_V_FULL + s, (it / KS) & 1) && live;
       if (it == n_it - 1 && has_tail()) live = wait1(BAR_TAIL, 0) && live;
-      if (it + 1 < n_it) live = wait1(BAR_K_FULL + s1, ((it + 1) / KS) & 1) && live;
+      if (it + 2 < n_it) live = wait1(BAR_K_FULL + s2, ((it + 2) / KS) & 1) && live;
       if (!live) return;
 #pragma unroll
       for (int t = 0; t < 2; ++t) {
         if (it >= n_of[t]) continue;
-        if (!wait1(BAR_P_FULL + t, it & 1)) return;
+        if (!wait1(BAR_P_FULL + 2 * t + (it & 1), (it >> 1) & 1)) return;
         tc_fence_after();
         issue_o(t, it);
-        if (it + 1 < n_of[t]) issue_s(t, it + 1);  // behind PV in the pipe: it overwrites the P that PV reads
+        if (it + 2 < n_of[t]) issue_s(t, it + 2);  // behind PV in the pipe: it overwrites the P that PV reads
       }
       mma_commit(bar(BAR_V_EMPTY + s));
-      if (it + 1 < n_it) mma_commit(bar(BAR_K_EMPTY + s1));
+      if (it + 2 < n_it) mma_commit(bar(BAR_K_EMPTY + s2));
     }
   }
 
@@ -296,7 +305,7 @@ struct RelFwd {
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t)
-        if (it >= 2 && it - 2 < n_of[t]) warp_wait(BAR_ST_EMPTY + 2 * buf + t, ((it >> 1) & 1) ^ 1);
+        if (it >= 2 && it - 2 < n_of[t]) warp_wait(BAR_ST_EMPTY + 2 * t + buf, ((it >> 1) & 1) ^ 1);  // (then their barrier's phase is over too)
       if (aborted()) return;
       if (w == 0 && lane == 0) {
         int* flag = reinterpret_cast<int*>(misc + M_UNI) + 2 * buf;
@@ -318,18 +327,19 @@ struct RelFwd {
       if (lane == 0) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (it >= n_of[t]) continue;
-          if (it > 0) wait1(BAR_S_FULL + t, (it - 1) & 1);  // this arrival belongs to the next phase
-          mbar_arrive(bar(BAR_S_FULL + t));
+          if (it < n_of[t]) mbar_arrive(bar(BAR_S_FULL + 2 * t + buf));
         }
       }
       __syncwarp();
     }
   }
-  // Warp 3 as well: zeros behind the last key (see has_tail). Runs inside bias_warp's loop order: before the last block's arrival
-  // would be too late for nobody, since only the last PV waits for it.
+  // Warp 3 as well: zeros behind the last key (see has_tail).
   __device__ __forceinline__ void zero_tail() {
     const int it = n_it - 1, s = it % KS;
+    // Parities repeat: the stage's previous phase (block it - KS) has to be over. It is once S(it - 1), which was issued behind
+    // PV(it - 3), is complete; that barrier has no phase behind the one waited for, and block it - 3 of its slot has been read.
+    static_assert(KS == 3, "the parity of the last V stage");
+    if (it >= KS) warp_wait(BAR_S_FULL + 2 * (n_of[1] == n_it ? 1 : 0) + ((it - 1) & 1), ((it - 1) >> 1) & 1);
     warp_wait(BAR_V_FULL + s, (it / KS) & 1);
     if (aborted()) return;
     const int first = si.sk - it * BN;  // rows first .. BN - 1 of the block
@@ -365,11 +375,11 @@ struct RelFwd {
         need_mask = need_mask || c0 + BN - 1 > r0 + t * BM + off;
         cmax = min(cmax, orow + off - c0);
       }
-      warp_wait(BAR_S_FULL + t, it & 1);
+      warp_wait(BAR_S_FULL + 2 * t + buf, (it >> 1) & 1);
       tc_fence_after();
       uint32_t raw[BN / 32][32];
 #pragma unroll
-      for (int q = 0; q < BN / 32; ++q) tmem_ld32(s_cols(t) + lane_off + q * 32, raw[q]);
+      for (int q = 0; q < BN / 32; ++q) tmem_ld32(s_cols(t, buf) + lane_off + q * 32, raw[q]);
       const bool uni = reinterpret_cast<const int*>(misc + M_UNI)[2 * buf + t] != 0;
       const float ub = reinterpret_cast<const float*>(misc + M_UNI + 16)[2 * buf + t];
       tmem_ld_wait();
@@ -403,7 +413,9 @@ struct RelFwd {
       if (__any_sync(0xffffffffu, grow)) {
         const float alpha = grow ? (m == -INFINITY ? 0.f : ex2(m - m_new)) : 1.f;
         if (grow) { m = m_new; l *= alpha; }
-        if (it > 0) {  // S(it) was issued behind PV(it - 1): O is quiescent
+        if (it > 0) {
+          warp_wait(BAR_PV_DONE + t, (it - 1) & 1);  // (PV(it - 2) is complete: S(it) was issued behind it)
+          tc_fence_after();
 #pragma unroll 1
           for (int q = 0; q < D / 32; ++q) {
             uint32_t o[32];
@@ -430,7 +442,7 @@ struct RelFwd {
           ls[c & 3] = __fadd2_rn(ls[c & 3], x);
           pk[c] = pack2<T>(x.x, x.y);
         }
-        tmem_st8(s_cols(t) + lane_off + h * 16, pk);
+        tmem_st8(s_cols(t, buf) + lane_off + h * 16, pk);
       }
       const float2 sum = __fadd2_rn(__fadd2_rn(ls[0], ls[1]), __fadd2_rn(ls[2], ls[3]));
       l += sum.x + sum.y;
@@ -438,8 +450,8 @@ struct RelFwd {
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(bar(BAR_P_FULL + t));
-        mbar_arrive(bar(BAR_ST_EMPTY + 2 * buf + t));
+        mbar_arrive(bar(BAR_P_FULL + 2 * t + buf));
+        mbar_arrive(bar(BAR_ST_EMPTY + 2 * t + buf));
       }
     }
     if (r0 + t * BM >= si.sq) return;  // a tile behind its sequence
