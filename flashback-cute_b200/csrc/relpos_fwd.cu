@@ -430,6 +430,9 @@ struct RelFwd {
       const float moff = m == -INFINITY ? 0.f : m;
       const float2 mul = fold ? sc2 : make_float2(1.f, 1.f);
       const float2 add = fold ? make_float2(ub - moff, ub - moff) : make_float2(-moff, -moff);
+      // The two tiles' exponentials alternate: the warps of a TMEM lane quadrant share a scheduler and its special-function unit.
+      const int pairs = min(n_of[0], n_of[1]);
+      if (it < pairs && (t == 1 || it > 0)) named_barrier_sync(4 + 4 * t + (warp & 3), 64);
       float2 ls[4] = {};
       // 16 keys = one k-step of PV: their 8 packed columns go back over the first 8 of the 16 score columns they came from
 #pragma unroll
@@ -444,6 +447,7 @@ struct RelFwd {
         }
         tmem_st8(s_cols(t, buf) + lane_off + h * 16, pk);
       }
+      if (it < pairs && (t == 0 || it + 1 < pairs)) named_barrier_arrive(8 - 4 * t + (warp & 3), 64);
       const float2 sum = __fadd2_rn(__fadd2_rn(ls[0], ls[1]), __fadd2_rn(ls[2], ls[3]));
       l += sum.x + sum.y;
       tmem_st_wait();
