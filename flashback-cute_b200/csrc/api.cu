@@ -456,9 +456,9 @@ extern "C" int fb_relpos_bias_grad(const fb_relpos_bias_grad_args* a, fb_stream_
   return FB_OK;
 }
 
-extern "C" size_t fb_relpos_bias_workspace_bytes(int heads, int sq, int sk, int num_buckets) {
-  if (check_bias_sizes(FB_BF16, heads, sq, sk) != FB_OK || sq == 0 || sk == 0 || num_buckets < 2 || num_buckets > FB_RELPOS_MAX_BUCKETS) return 0;
-  return sizeof(float) * (size_t)heads * (size_t)relpos_bias_parts(heads, sq, sk) * (size_t)num_buckets;
+extern "C" size_t fb_relpos_bias_workspace_bytes(int dtype, int heads, int sq, int sk, int num_buckets) {
+  if (check_bias_sizes(dtype, heads, sq, sk) != FB_OK || sq == 0 || sk == 0 || num_buckets < 2 || num_buckets > FB_RELPOS_MAX_BUCKETS) return 0;
+  return sizeof(float) * (size_t)heads * (size_t)relpos_bias_parts(dtype, heads, sq, sk) * (size_t)num_buckets;
 }
 
 namespace {
@@ -477,9 +477,13 @@ int check_decode(const fb_relpos_decode_args& a) {
   if (a.heads_q <= 0 || a.heads_kv <= 0 || a.heads_q % a.heads_kv != 0) return FB_ERR_HEADS;
   if (a.batch < 0 || a.seqlen_q < 0 || a.seqlen_k < 0) return FB_ERR_SHAPE;
   if (a.batch > 65535 || a.seqlen_k > (1 << 30) || a.heads_q > 65535 || (int64_t)a.seqlen_q * a.heads_q > (1 << 20)) return FB_ERR_TOO_LARGE;
+  if ((int64_t)(a.heads_q / a.heads_kv) * a.bias.num_buckets > kDecodeMaxTable) return FB_ERR_TOO_LARGE;
   return FB_OK;
 }
 
+bool cluster_of(const fb_relpos_decode_args& a) {
+  return decode_cluster(a.batch, a.heads_kv, a.heads_q / a.heads_kv * a.seqlen_q, a.seqlen_k);
+}
 int splits_of(const fb_relpos_decode_args& a) {
   return decode_splits(a.batch, a.heads_kv, a.heads_q / a.heads_kv * a.seqlen_q, a.seqlen_k);
 }
@@ -489,7 +493,7 @@ int splits_of(const fb_relpos_decode_args& a) {
 extern "C" size_t fb_relpos_decode_workspace_bytes(const fb_relpos_decode_args* a) {
   if (!a || check_decode(*a) != FB_OK || a->batch == 0 || a->seqlen_q == 0) return 0;
   const size_t splits = (size_t)splits_of(*a);
-  return splits == 1 ? 0 : (size_t)a->batch * a->seqlen_q * a->heads_q * splits * (a->head_dim + 2) * sizeof(float);
+  return splits == 1 || cluster_of(*a) ? 0 : (size_t)a->batch * a->seqlen_q * a->heads_q * splits * (a->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int fb_relpos_decode(const fb_relpos_decode_args* a, fb_stream_t stream) {
@@ -513,7 +517,8 @@ extern "C" int fb_relpos_decode(const fb_relpos_decode_args* a, fb_stream_t stre
   p.lens = a->lens;
   p.out = a->out;
   p.splits = splits_of(*a);
-  if (p.splits > 1) {
+  p.cluster = cluster_of(*a) ? 1 : 0;
+  if (p.splits > 1 && !p.cluster) {
     if (!a->workspace) return FB_ERR_NULL_ARG;
     p.part = a->workspace;  // row length head_dim floats: the (maximum, sum) pairs behind them stay 8-byte aligned
     p.part_ml = reinterpret_cast<float2*>(a->workspace + (size_t)p.B * p.Sq * p.Hq * p.splits * p.D);

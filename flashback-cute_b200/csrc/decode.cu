@@ -7,8 +7,10 @@
 //   * a CTA of 4 warps takes a slice of one (sequence, kv head)'s keys; every warp is a flash-attention of its own over every 4th
 //     group of 16 keys (own running maximum, sum and accumulator; own shared-memory stages filled by cp.async), so nothing in
 //     the main loop waits for another warp;
-//   * the slices divide the sequence's OWN length, so ragged batches stay balanced; partial results (float32, unnormalised, with
-//     maximum and sum) are joined by a second kernel in a fixed order. One slice: the first kernel writes the output itself.
+//   * the slices divide the sequence's OWN length, so ragged batches stay balanced. Up to 8 slices are one thread-block cluster: its CTAs
+//     leave their partial results (float32, unnormalised, with maximum and sum) in shared memory and join them through
+//     distributed shared memory, each a part of the rows. More slices (few sequences with long caches) go through a
+//     workspace and a second kernel. Fixed order either way.
 //
 // Far from the newest token all keys of a group share the last bucket and the bias is one number per row.
 #include "fb_params.h"
@@ -22,6 +24,8 @@ using namespace ptx;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int KG = 16;      // keys per group = MMA k of the second product
 constexpr int kStages = 3;  // groups in flight per warp
+constexpr int kMaxTable = kDecodeMaxTable;  // entries of the table's columns that a CTA keeps
+constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {  // invalid: zero fill, nothing read
@@ -62,6 +66,13 @@ template <> __device__ __forceinline__ uint32_t pack16<__half>(float lo, float h
 template <int D>
 __device__ __forceinline__ uint32_t unit_off(int r, int u) { return (uint32_t)(r * D * 2 + ((u ^ (r & 7)) << 4)); }
 
+template <typename T, int D>
+__device__ __forceinline__ void store_out(const DecodeParams& p, int b, int t, int h, int d4, float4 v, float l) {
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  T* dst = reinterpret_cast<T*>(p.out) + ((int64_t)(b * p.Sq + t) * p.Hq + h) * D + d4 * 4;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<T>(v.x * inv, v.y * inv), pack16<T>(v.z * inv, v.w * inv));
+}
+
 template <typename T, int D, int MT>
 __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant__ DecodeParams p, const __grid_constant__ RelPos rel) {
   constexpr int R = 16 * MT;           // rows per CTA
@@ -73,6 +84,8 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
   uint8_t* const stages = smem + R * D * 2;       // per warp [kStages][K, V]
   __shared__ RelBuckets buckets;
   __shared__ float s_m[kWarps][R], s_l[kWarps][R];
+  __shared__ float2 joint_ml[R];
+  float* const tab = reinterpret_cast<float*>(smem + R * D * 2 + kWarps * kWarpBytes);  // [heads of the CTA's rows][nb], log2 units
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x;
@@ -110,6 +123,11 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) load(i);
 
+  // the table's columns of this kv head's query heads
+  for (int at = threadIdx.x; at < p.G * rel.nb; at += kThreads) {
+    const int g = at / rel.nb, t = at - g * rel.nb;
+    tab[at] = to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + (int64_t)(hk * p.G + g) * rel.head_stride]) * kLog2e;
+  }
   // the queries: row x of the CTA is new token (rt * R + x) / G, query head hk * G + (rt * R + x) % G
   for (int at = threadIdx.x; at < R * U; at += kThreads) {
     const int x = at / U, u = at % U, row = rt * R + x;
@@ -125,20 +143,20 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
   // this thread's rows of the MMA fragments: lane / 4 and lane / 4 + 8 of every 16
   const float scale2 = p.scale * kLog2e;
   const RelFn bucket_of(rel, buckets);
-  int pos[MT][2], head[MT][2];
+  int pos[MT][2];
+  const float* row_tab[MT][2];
   float far_bias[MT][2], m[MT][2], l[MT][2];
   float o[MT][D / 8][4];
   int pos_min = INT32_MAX;
-  auto bias_of = [&](int t, int h) { return to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + h * rel.head_stride]) * kLog2e; };
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
     for (int x = 0; x < 2; ++x) {
       const int row = min(rt * R + mt * 16 + lane / 4 + 8 * x, rows - 1);
       const int t = row / p.G;
-      head[mt][x] = hk * p.G + row - t * p.G;
+      row_tab[mt][x] = tab + (row - t * p.G) * rel.nb;
       pos[mt][x] = len - p.Sq + t;  // the new token's place in its sequence
-      far_bias[mt][x] = bias_of(rel.side - 1, head[mt][x]);
+      far_bias[mt][x] = row_tab[mt][x][rel.side - 1];
       m[mt][x] = -INFINITY;
       l[mt][x] = 0.f;
     }
@@ -189,8 +207,8 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
           float bias = far_bias[mt][x];
           if (!all_far) {
             const int r = j - pos[mt][x];
-            bias = -INFINITY;
-            if (r <= 0 && j < k1) bias = bias_of(bucket_of(r), head[mt][x]);
+            bias = row_tab[mt][x][bucket_of(min(r, 0))];
+            if (r > 0 || j >= k1) bias = -INFINITY;
           }
           s[mt][n][e] = fmaf(s[mt][n][e], scale2, bias);
           mx[x] = fmaxf(mx[x], s[mt][n][e]);
@@ -251,7 +269,8 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
       }
     }
   float* const acc = reinterpret_cast<float*>(stages);
-  static_assert(kWarps * R * D * 4 <= kWarps * kWarpBytes, "the accumulators fit the stages");
+  float* const joint = acc + kWarps * R * D;  // [R][D], cluster: this slice's sum
+  static_assert((kWarps + 1) * R * D * 4 <= kWarps * kWarpBytes, "the accumulators fit the stages");
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -278,14 +297,49 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
     }
     const int t = row / p.G, h = hk * p.G + row - t * p.G;
     if (p.splits == 1) {
-      const float inv = ll > 0.f ? 1.f / ll : 0.f;
-      T* dst = reinterpret_cast<T*>(p.out) + ((int64_t)(b * p.Sq + t) * p.Hq + h) * D + d4 * 4;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<T>(v.x * inv, v.y * inv), pack16<T>(v.z * inv, v.w * inv));
+      store_out<T, D>(p, b, t, h, d4, v, ll);
+    } else if (p.cluster) {
+      *reinterpret_cast<float4*>(joint + x * D + d4 * 4) = v;
+      if (d4 == 0) joint_ml[x] = make_float2(mm, ll);
     } else {
       const int64_t at_row = ((int64_t)(b * p.Sq + t) * p.Hq + h) * p.splits + split;
       *reinterpret_cast<float4*>(p.part + at_row * D + d4 * 4) = v;
       if (d4 == 0) p.part_ml[at_row] = make_float2(mm, ll);
     }
+  }
+  if (p.cluster) {
+    cluster_sync_all();  // every slice's result is in its CTA's shared memory
+    const uint32_t my_joint = smem_u32(joint), my_ml = smem_u32(joint_ml);
+    for (int at = split * kThreads + threadIdx.x; at < R * D / 4; at += p.splits * kThreads) {
+      const int x = at / (D / 4), d4 = at - x * (D / 4), row = rt * R + x;
+      if (row >= rows) break;
+      float mm = -INFINITY;
+      float2 ml[kMaxCluster];
+      float4 a[kMaxCluster];
+#pragma unroll
+      for (int s = 0; s < kMaxCluster; ++s) {
+        ml[s] = make_float2(-INFINITY, 0.f);
+        if (s < p.splits) {
+          ml[s] = ld_cluster_f2(map_to_cta(my_ml + x * 8, (uint32_t)s));
+          a[s] = ld_cluster_f4(map_to_cta(my_joint + (x * D + d4 * 4) * 4, (uint32_t)s));
+          mm = fmaxf(mm, ml[s].x);
+        }
+      }
+      const float off = mm == -INFINITY ? 0.f : mm;
+      float ll = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int s = 0; s < kMaxCluster; ++s) {
+        if (s < p.splits) {
+          const float f = ex2(ml[s].x - off);
+          ll += ml[s].y * f;
+          v.x += a[s].x * f; v.y += a[s].y * f; v.z += a[s].z * f; v.w += a[s].w * f;
+        }
+      }
+      const int t = row / p.G, h = hk * p.G + row - t * p.G;
+      store_out<T, D>(p, b, t, h, d4, v, ll);
+    }
+    cluster_sync_all();  // nobody reads this CTA's shared memory any more
   }
 }
 
@@ -327,32 +381,37 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_cons
 }
 
 template <typename K>
-cudaError_t launch(K kern, dim3 grid, size_t smem, cudaStream_t s, void** args) {
+cudaError_t launch(K kern, dim3 grid, size_t smem, int cluster, cudaStream_t s, void** args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaLaunchAttribute attr;  // programmatic dependent launch: both kernels wait for the one before at their start
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];  // programmatic dependent launch: both kernels wait for the one before at their start
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
   return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kern), args);
 }
 
 template <typename T, int D, int MT>
 int decode_typed(DecodeParams& p, RelPos& rel, cudaStream_t s) {
   constexpr int R = 16 * MT;
-  constexpr size_t smem = R * D * 2 + kWarps * kStages * 2 * KG * D * 2;
+  constexpr size_t tiles = R * D * 2 + kWarps * kStages * 2 * KG * D * 2;
+  const size_t smem = tiles + (size_t)p.G * rel.nb * sizeof(float);
   auto kern = decode_kernel<T, D, MT>;
-  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return FB_ERR_CUDA;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(tiles + kMaxTable * sizeof(float))) != cudaSuccess) return FB_ERR_CUDA;
   p.row_tiles = (p.G * p.Sq + R - 1) / R;
   void* args[2] = {&p, &rel};
-  if (launch(kern, dim3((unsigned)p.splits, (unsigned)(p.Hkv * p.row_tiles), (unsigned)p.B), smem, s, args) != cudaSuccess) return FB_ERR_CUDA;
-  if (p.splits == 1) return 1;
+  if (launch(kern, dim3((unsigned)p.splits, (unsigned)(p.Hkv * p.row_tiles), (unsigned)p.B), smem, p.cluster ? p.splits : 1, s, args) != cudaSuccess)
+    return FB_ERR_CUDA;
+  if (p.splits == 1 || p.cluster) return 1;
   const int64_t rows = (int64_t)p.B * p.Sq * p.Hq;
-  if (launch(decode_join_kernel<T, D>, dim3((unsigned)((rows + kWarps - 1) / kWarps)), 0, s, args) != cudaSuccess) return FB_ERR_CUDA;
+  if (launch(decode_join_kernel<T, D>, dim3((unsigned)((rows + kWarps - 1) / kWarps)), 0, 1, s, args) != cudaSuccess) return FB_ERR_CUDA;
   return 2;
 }
 
@@ -364,14 +423,27 @@ int decode_dispatch(DecodeParams& p, RelPos& rel, cudaStream_t s) {
 
 }  // namespace
 
-// Slices of a sequence's keys: enough CTAs for a few waves on the whole GPU, slices of at least one round of the CTA's warps.
+// Slices of a sequence's keys: enough CTAs for a few waves on the whole GPU, slices of at least one round of the CTA's warps. A
+// power of two up to 8 (a cluster: one launch) for small batches whose slices then have at most 8 rounds; otherwise a workspace and a
+// second launch, since a cluster holds its SMs until its last CTA is done: 48 sequences of up to 8192 keys, 8 kv heads of 128
+// in 4 slices each: 171 us as clusters, 152 + 5 us through the workspace.
 int decode_splits(int batch, int heads_kv, int rows, int seqlen_k) {
   const int per = rows <= 16 ? 16 : 32;
   const int64_t base = (int64_t)batch * heads_kv * ((rows + per - 1) / per);
   const int64_t want = (148 * 2 * 4 + base - 1) / base;
-  const int64_t most = (seqlen_k + kWarps * KG - 1) / (kWarps * KG);
-  const int64_t n = want < most ? want : most;
+  const int64_t rounds = (seqlen_k + kWarps * KG - 1) / (kWarps * KG);
+  if (base < 2 * 148 && rounds <= 8 * kMaxCluster) {
+    int n = 1;
+    while (n < kMaxCluster && n < want && 2 * n <= rounds) n *= 2;
+    return n;
+  }
+  const int64_t n = want < rounds ? want : rounds;
   return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
+}
+bool decode_cluster(int batch, int heads_kv, int rows, int seqlen_k) {
+  const int per = rows <= 16 ? 16 : 32;
+  const int n = decode_splits(batch, heads_kv, rows, seqlen_k);
+  return n > 1 && n <= kMaxCluster && (int64_t)batch * heads_kv * ((rows + per - 1) / per) < 2 * 148;
 }
 
 int launch_decode(int dtype, DecodeParams& p, RelPos& rel, cudaStream_t s) {

@@ -137,6 +137,7 @@ struct DecodeParams {
   const int32_t* lens;  // nullptr: Sk each
   void* out;            // contiguous (B, Sq, Hq, D)
   int splits, row_tiles;
+  int cluster;          // the slices of a sequence are one thread-block cluster
   float* part;          // splits > 1: [(b, token, query head)][split][D] and their (maximum, sum)
   float2* part_ml;
 };
@@ -209,8 +210,10 @@ int launch_rel_reduce(int dtype, const float* part, int batch, int heads, int nt
 int launch_relpos_fill(int dtype, const RelPos& rel, int heads, int sq, int sk, void* out, cudaStream_t stream);
 int launch_relpos_grad(int dtype, const RelPos& rel, int heads, int sq, int sk, const void* grad, void* dtable, int64_t bucket_stride,
                        int64_t head_stride, cudaStream_t stream);
-int64_t relpos_bias_parts(int heads, int sq, int sk);  // partial table gradients per head of launch_relpos_grad
+int64_t relpos_bias_parts(int dtype, int heads, int sq, int sk);  // partial table gradients per head of launch_relpos_grad
 int decode_splits(int batch, int heads_kv, int rows, int seqlen_k);
+bool decode_cluster(int batch, int heads_kv, int rows, int seqlen_k);  // those slices are one cluster (and need no workspace)
+constexpr int kDecodeMaxTable = 4096;  // query heads per kv head x buckets
 int launch_decode(int dtype, DecodeParams& p, RelPos& rel, cudaStream_t stream);
 constexpr int kTcOwnerRows = 128, kSimtOwnerRows = 16;  // query rows per partial table gradient
 int launch_tc_fwd_wait_hook(const Params& p, cudaStream_t stream);  // test instantiation, see fb_debug_wait_timeout

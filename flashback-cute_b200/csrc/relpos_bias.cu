@@ -15,13 +15,17 @@ constexpr int kWarps = kThreads / 32;
 // ---------------------------------------------------------------------------------------------------
 // One CTA = kRows rows x kCols columns of one head. The values depend on j - i alone: the kRows + kCols - 1 of them that
 // the tile needs are looked up once, into shared memory, and a warp per row copies its stretch out in 16-byte stores
-// (aligned in the flat tensor, since rows of odd length start anywhere; the ends of a row go out one by one).
-constexpr int kRows = 32, kCols = 2048;
+// (aligned in the flat tensor, since rows of odd length start anywhere; the ends of a row go out one by one). The stretch of a row
+// starts at any element: one copy of the values per element of a 16-byte unit, each shifted by one more, gives every
+// row 16-byte loads too. (One copy and an element at a time was bound by shared memory: 168 us for 16 x 4095 x 4099 bf16.)
+constexpr int kRows = 64, kCols = 2048;
 
 template <typename T>
 __global__ void __launch_bounds__(kThreads) relpos_fill_kernel(const __grid_constant__ RelPos rel, int sq, int sk, T* __restrict__ out) {
   constexpr int VEC = 16 / sizeof(T);
-  __shared__ T val[kRows + kCols];
+  constexpr int LEN = kRows + kCols + VEC;  // entries per copy, whole units
+  extern __shared__ __align__(16) uint8_t smem[];
+  T* const val = reinterpret_cast<T*>(smem);  // [VEC][LEN]: copy k, entry u = value u + k
   __shared__ T tab[FB_RELPOS_MAX_BUCKETS];
   __shared__ RelBuckets buckets;
   const int h = blockIdx.z, i0 = blockIdx.y * kRows, j0 = blockIdx.x * kCols;
@@ -30,26 +34,34 @@ __global__ void __launch_bounds__(kThreads) relpos_fill_kernel(const __grid_cons
   relpos_load_buckets(buckets, rel, threadIdx.x, kThreads);
   __syncthreads();
   const RelFn bucket_of(rel, buckets);
-  const int base = j0 - (i0 + rows - 1) - (sk - sq);  // position of entry 0: the tile's last row, first column
-  for (int u = threadIdx.x; u < rows + cols - 1; u += kThreads) val[u] = tab[bucket_of(base + u)];
+  const int base = j0 - (i0 + rows - 1) - (sk - sq);  // position of value 0: the tile's last row, first column
+  for (int x = threadIdx.x; x < (rows + cols - 1 + VEC - 1) / VEC; x += kThreads) {
+    T v[2 * VEC];  // values VEC x .. VEC x + 2 VEC - 1
+#pragma unroll
+    for (int e = 0; e < 2 * VEC; ++e) v[e] = tab[bucket_of(base + x * VEC + e)];
+#pragma unroll
+    for (int k = 0; k < VEC; ++k) {
+      alignas(16) T w[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) w[e] = v[k + e];
+      *reinterpret_cast<uint4*>(val + k * LEN + x * VEC) = *reinterpret_cast<const uint4*>(w);
+    }
+  }
   __syncthreads();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int r = warp; r < rows; r += kWarps) {
     const int64_t flat = ((int64_t)h * sq + i0 + r) * sk + j0;
-    const T* src = val + (rows - 1 - r);
+    const int first = rows - 1 - r;  // value of the row's first column
     T* dst = out + flat;
     const int head = min(cols, (int)((VEC - flat % VEC) % VEC));
-    if (lane < head) dst[lane] = src[lane];
-    const int nvec = (cols - head) / VEC;
-    for (int k = lane; k < nvec; k += 32) {
-      const int j = head + k * VEC;
-      alignas(16) T v[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[e] = src[j + e];
-      *reinterpret_cast<uint4*>(dst + j) = *reinterpret_cast<const uint4*>(v);
-    }
+    if (lane < head) dst[lane] = val[first + lane];
+    const int nvec = (cols - head) / VEC, start = first + head;
+    const uint4* src = reinterpret_cast<const uint4*>(val + (start % VEC) * LEN + start / VEC * VEC);
+    uint4* to = reinterpret_cast<uint4*>(dst + head);
+#pragma unroll 4
+    for (int k = lane; k < nvec; k += 32) to[k] = src[k];
     const int j = head + nvec * VEC + lane;
-    if (j < cols) dst[j] = src[j];
+    if (j < cols) dst[j] = val[first + j];
   }
 }
 
@@ -58,21 +70,22 @@ __global__ void __launch_bounds__(kThreads) relpos_fill_kernel(const __grid_cons
 // ---------------------------------------------------------------------------------------------------
 // The sum over a bucket is a sum over diagonals. Diagonal c = j - i + (sq - 1) of row i sits at flat offset
 // i * (sk + 1) + c - (sq - 1): rows that are VEC = 16 bytes / element apart keep their place relative to a 16-byte
-// boundary. So a CTA takes kDiag diagonals x a stretch of rows, each of VEC residues of the row index gets an equal share of
+// boundary. So a CTA takes kSpan diagonals x a stretch of rows, each of VEC residues of the row index gets an equal share of
 // the warps, and a thread adds up VEC neighbouring diagonals in registers over its rows with 16-byte loads: no
 // atomics, no reordering, every element read once. At the end the CTA adds up its warps' diagonals, then those of
 // each bucket (neighbours), and leaves one number per bucket in the workspace.
-constexpr int kSpan = 256;  // diagonals per warp: 32 lanes x 8 elements (16 bit); 32 x 4 x 2 (float32)
+// PER vectors per lane: long stretches of a row per warp where the problem is large, more CTAs where it is small.
 
 template <typename T> struct Vec;
 template <> struct Vec<__nv_bfloat16> { static constexpr int n = 8; };
 template <> struct Vec<__half> { static constexpr int n = 8; };
 template <> struct Vec<float> { static constexpr int n = 4; };
 
-template <typename T>
+template <typename T, int PER>
 __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_constant__ RelPos rel, int sq, int sk, int rows_per_cta, const T* __restrict__ grad) {
   constexpr int VEC = Vec<T>::n;
-  constexpr int PER = kSpan / 32 / VEC;  // vectors per lane and row
+  constexpr int kSpan = 32 * VEC * PER;  // diagonals per CTA
+  constexpr int kBatch = 8 / PER;        // rows of a warp in flight
   __shared__ float part[kWarps][kSpan + VEC];
   __shared__ float acc[FB_RELPOS_MAX_BUCKETS];
   __shared__ RelBuckets buckets;
@@ -123,12 +136,35 @@ __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_cons
         if (j + e >= 0 && j + e < sk) s[e] += to_f<T>(g[(int64_t)i * sk + j + e]);
     }
   };
-#pragma unroll 4
-  for (int i = first; i < i_hi; i += kWarps) {
+  auto edge = [&](int i) {
 #pragma unroll
     for (int q = 0; q < PER; ++q) add(sum[q], i, c0 - shift + (q * 32 + lane) * VEC);
-    if (shift > 0 && lane == 0) add(tail, i, c0 - shift + kSpan);
+  };
+  // Rows in which all of the warp's vectors lie inside [0, sk): unconditional loads, kBatch rows' in flight together. The few
+  // rows before and behind them are checked vector by vector.
+  const int lo = c0 - shift - (sq - 1);  // column of the first vector in row 0
+  const int in_lo = -lo, in_hi = sk - kSpan - lo;  // interior rows [in_lo, in_hi]
+  int i = first;
+  for (; i < i_hi && i < in_lo; i += kWarps) edge(i);
+  for (; i + (kBatch - 1) * kWarps < i_hi && i + (kBatch - 1) * kWarps <= in_hi; i += kBatch * kWarps) {
+    uint4 u[kBatch][PER];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+      for (int q = 0; q < PER; ++q)
+        u[b][q] = *reinterpret_cast<const uint4*>(g + (int64_t)(i + b * kWarps) * sk + (lo + i + b * kWarps + (q * 32 + lane) * VEC));
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+#pragma unroll
+      for (int q = 0; q < PER; ++q) {
+        const T* v = reinterpret_cast<const T*>(&u[b][q]);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) sum[q][e] += to_f<T>(v[e]);
+      }
   }
+  for (; i < i_hi; i += kWarps) edge(i);
+  if (shift > 0 && lane == 0)
+    for (i = first; i < i_hi; i += kWarps) add(tail, i, c0 - shift + kSpan);
 #pragma unroll
   for (int q = 0; q < PER; ++q)
 #pragma unroll
@@ -140,17 +176,22 @@ __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_cons
   __shared__ int shifts[kWarps];
   if (lane == 0) shifts[warp] = shift;
   __syncthreads();
-  // thread t: diagonal c0 + t, the warps' sums in a fixed order; then the diagonals of a bucket, warp by warp
-  float s = 0.f;
-  const int c = c0 + threadIdx.x;
+  // diagonal c0 + t, the warps' sums in a fixed order; then the diagonals of a bucket, warp by warp
+  for (int t0 = 0; t0 < kSpan; t0 += kThreads) {
+    const int t = t0 + threadIdx.x, c = c0 + t;
+    float s = 0.f;
+    int bucket = -1;
+    if (t < kSpan) {
 #pragma unroll
-  for (int w = 0; w < kWarps; ++w) s += part[w][shifts[w] + threadIdx.x];
-  const int bucket = c < ndiag ? RelFn(rel, buckets)(c - (sq - 1) - (sk - sq)) : -1;
-  const bool run = run_head(bucket, lane);
-  s = run_sum(s, bucket, lane);
-  for (int w = 0; w < kWarps; ++w) {
-    if (w == warp && run && bucket >= 0) acc[bucket] += s;
-    __syncthreads();
+      for (int w = 0; w < kWarps; ++w) s += part[w][shifts[w] + t];
+      if (c < ndiag) bucket = RelFn(rel, buckets)(c - (sq - 1) - (sk - sq));
+    }
+    const bool run = run_head(bucket, lane);
+    s = run_sum(s, bucket, lane);
+    for (int w = 0; w < kWarps; ++w) {
+      if (w == warp && run && bucket >= 0) acc[bucket] += s;
+      __syncthreads();
+    }
   }
   if ((int)threadIdx.x < rel.nb) out[threadIdx.x] = acc[threadIdx.x];
 }
@@ -188,7 +229,9 @@ template <typename T>
 int fill_typed(const RelPos& rel, int heads, int sq, int sk, void* out, cudaStream_t s) {
   const dim3 grid((sk + kCols - 1) / kCols, (sq + kRows - 1) / kRows, heads);
   if (grid.y > 65535 || grid.z > 65535) return FB_ERR_TOO_LARGE;
-  relpos_fill_kernel<T><<<grid, kThreads, 0, s>>>(rel, sq, sk, reinterpret_cast<T*>(out));
+  constexpr int VEC = 16 / sizeof(T), smem = VEC * (kRows + kCols + VEC) * (int)sizeof(T);
+  static_assert(smem <= 48 * 1024, "without an opt-in");
+  relpos_fill_kernel<T><<<grid, kThreads, smem, s>>>(rel, sq, sk, reinterpret_cast<T*>(out));
   return cudaGetLastError() == cudaSuccess ? 1 : FB_ERR_CUDA;
 }
 
@@ -198,21 +241,30 @@ int reduce_typed(const float* part, int batch, int heads, int ntiles, int nb, vo
   return cudaGetLastError() == cudaSuccess ? 1 : FB_ERR_CUDA;
 }
 
-// Rows per CTA of the gradient: long stretches spread the end of a CTA (its sums by bucket) over more reads, short ones
-// fill the GPU. The same rule sizes the workspace.
-int grad_rows(int heads, int sq, int sk) {
-  const long long spans = (sq + sk - 1 + kSpan - 1) / kSpan;
-  int rows = 512;
-  while (rows > 32 && spans * heads * ((sq + rows - 1) / rows) < 148 * 8) rows /= 2;
-  return rows;
+// Shape of the gradient's CTAs: long stretches of rows spread the end of a CTA (its sums by bucket) over more reads, short ones
+// fill the GPU; wide spans read longer stretches of a row. The same rule sizes the workspace.
+struct GradShape {
+  int per, rows, spans, row_blocks;
+};
+GradShape grad_shape(int dtype, int heads, int sq, int sk) {
+  const int vec = dtype == FB_F32 ? 4 : 8;
+  GradShape g;
+  g.per = (int64_t)heads * sq * sk >= (1 << 24) ? 2 : 1;
+  const int span = 32 * vec * g.per;
+  g.spans = (sq + sk - 1 + span - 1) / span;
+  g.rows = 512;
+  while (g.rows > 32 && (int64_t)g.spans * heads * ((sq + g.rows - 1) / g.rows) < 148 * 8) g.rows /= 2;
+  g.row_blocks = (sq + g.rows - 1) / g.rows;
+  return g;
 }
 
 template <typename T>
-int grad_typed(const RelPos& rel, int heads, int sq, int sk, const void* grad, cudaStream_t s) {
-  const int rows = grad_rows(heads, sq, sk);
-  const dim3 grid((sq + sk - 1 + kSpan - 1) / kSpan, (sq + rows - 1) / rows, heads);
+int grad_typed(const RelPos& rel, const GradShape& g, int heads, int sq, int sk, const void* grad, cudaStream_t s) {
+  const dim3 grid(g.spans, g.row_blocks, heads);
   if (grid.y > 65535 || grid.z > 65535) return FB_ERR_TOO_LARGE;
-  relpos_grad_kernel<T><<<grid, kThreads, 0, s>>>(rel, sq, sk, rows, reinterpret_cast<const T*>(grad));
+  const T* in = reinterpret_cast<const T*>(grad);
+  if (g.per == 2) relpos_grad_kernel<T, 2><<<grid, kThreads, 0, s>>>(rel, sq, sk, g.rows, in);
+  else relpos_grad_kernel<T, 1><<<grid, kThreads, 0, s>>>(rel, sq, sk, g.rows, in);
   return cudaGetLastError() == cudaSuccess ? 1 : FB_ERR_CUDA;
 }
 
@@ -227,9 +279,9 @@ int launch_rel_reduce(int dtype, const float* part, int batch, int heads, int nt
   return FB_ERR_DTYPE;
 }
 
-int64_t relpos_bias_parts(int heads, int sq, int sk) {
-  const int rows = grad_rows(heads, sq, sk);
-  return (int64_t)((sq + sk - 1 + kSpan - 1) / kSpan) * ((sq + rows - 1) / rows);
+int64_t relpos_bias_parts(int dtype, int heads, int sq, int sk) {
+  const GradShape g = grad_shape(dtype, heads, sq, sk);
+  return (int64_t)g.spans * g.row_blocks;
 }
 
 int launch_relpos_fill(int dtype, const RelPos& rel, int heads, int sq, int sk, void* out, cudaStream_t s) {
@@ -242,15 +294,16 @@ int launch_relpos_fill(int dtype, const RelPos& rel, int heads, int sq, int sk, 
 }
 
 int launch_relpos_grad(int dtype, const RelPos& rel, int heads, int sq, int sk, const void* grad, void* dtable, int64_t bs, int64_t hs, cudaStream_t s) {
+  const GradShape g = grad_shape(dtype, heads, sq, sk);
   int r;
   switch (dtype) {
-    case FB_BF16: r = grad_typed<__nv_bfloat16>(rel, heads, sq, sk, grad, s); break;
-    case FB_F16: r = grad_typed<__half>(rel, heads, sq, sk, grad, s); break;
-    case FB_F32: r = grad_typed<float>(rel, heads, sq, sk, grad, s); break;
+    case FB_BF16: r = grad_typed<__nv_bfloat16>(rel, g, heads, sq, sk, grad, s); break;
+    case FB_F16: r = grad_typed<__half>(rel, g, heads, sq, sk, grad, s); break;
+    case FB_F32: r = grad_typed<float>(rel, g, heads, sq, sk, grad, s); break;
     default: return FB_ERR_DTYPE;
   }
   if (r < 0) return r;
-  const int r2 = launch_rel_reduce(dtype, rel.dpart, 1, heads, (int)relpos_bias_parts(heads, sq, sk), rel.nb, dtable, bs, hs, s);
+  const int r2 = launch_rel_reduce(dtype, rel.dpart, 1, heads, g.spans * g.row_blocks, rel.nb, dtable, bs, hs, s);
   return r2 < 0 ? r2 : r + r2;
 }
 

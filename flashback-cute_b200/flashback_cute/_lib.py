@@ -204,7 +204,7 @@ def load() -> ctypes.CDLL:
             lib.fb_relpos_workspace_bytes.restype = ctypes.c_size_t
             lib.fb_relpos_decode_workspace_bytes.argtypes = [ctypes.POINTER(FbRelposDecodeArgs)]
             lib.fb_relpos_decode_workspace_bytes.restype = ctypes.c_size_t
-            lib.fb_relpos_bias_workspace_bytes.argtypes = [ctypes.c_int] * 4
+            lib.fb_relpos_bias_workspace_bytes.argtypes = [ctypes.c_int] * 5
             lib.fb_relpos_bias_workspace_bytes.restype = ctypes.c_size_t
             lib.fb_abi_sizeof.argtypes = [ctypes.c_int]
             lib.fb_abi_sizeof.restype = ctypes.c_size_t

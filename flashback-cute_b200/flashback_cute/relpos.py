@@ -341,7 +341,7 @@ class _BiasSpec:
         lib, code = _lib.load(), _lib._DTYPES[dtype]
         self.fill = _lib.template(_lib.FbRelposBiasArgs(code, self.heads, sq, sk, _bias(table_shape, table_stride, two, max_distance), None))
         self.grad = _lib.template(_lib.FbRelposBiasGradArgs(code, self.heads, sq, sk, _bias(table_shape, table_stride, two, max_distance), None, None, self.heads, 1, None))
-        self.work = lib.fb_relpos_bias_workspace_bytes(self.heads, sq, sk, self.num) // 4
+        self.work = lib.fb_relpos_bias_workspace_bytes(code, self.heads, sq, sk, self.num) // 4
         self.stride = table_stride
 
     def forward(self, table):
@@ -393,6 +393,21 @@ class _RelposBiasFunc(torch.autograd.Function):
     @staticmethod
     def jvp(ctx, table_dot, _):
         return ctx.spec.forward(_raw(table_dot))
+
+
+class _RelposBiasEager(torch.autograd.Function):
+    """The same outside torch.func transforms, in the form that costs less per call (no setup_context)."""
+
+    @staticmethod
+    def forward(ctx, table, spec):
+        ctx.spec = spec
+        return spec.forward(table)
+
+    @staticmethod
+    def backward(ctx, grad):
+        if torch.is_grad_enabled() and grad.requires_grad:
+            return _RelposBiasGradFunc.apply(grad, ctx.spec), None
+        return ctx.spec.backward(grad), None
 
 
 class _RelposBiasGradFunc(torch.autograd.Function):
@@ -547,6 +562,8 @@ def flashback_relpos_bias(
     spec = _bias_specs.get(key)
     if spec is None:
         spec = _bias_specs.add(key, _BiasSpec(bias_table, seqlen_q, seqlen_k, two, max_distance))
-    if not (torch.is_grad_enabled() and bias_table.requires_grad) and forward_ad._current_level < 0 and not torch._C._are_functorch_transforms_active():
-        return spec.forward(bias_table)
-    return _RelposBiasFunc.apply(bias_table, spec)
+    if forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active():
+        return _RelposBiasFunc.apply(bias_table, spec)
+    if torch.is_grad_enabled() and bias_table.requires_grad:
+        return _RelposBiasEager.apply(bias_table, spec)
+    return spec.forward(bias_table)

@@ -358,11 +358,11 @@ typedef struct {
 } fb_relpos_bias_grad_args;
 
 int fb_relpos_bias_grad(const fb_relpos_bias_grad_args* args, fb_stream_t stream);
-size_t fb_relpos_bias_workspace_bytes(int heads, int seqlen_q, int seqlen_k, int num_buckets);
+size_t fb_relpos_bias_workspace_bytes(int dtype, int heads, int seqlen_q, int seqlen_k, int num_buckets);
 
 /* Attention of `seqlen_q` new tokens per sequence against a cache of keys and values that already holds them, with the
  * bias, causal: token t of sequence b sits at position lens[b] - seqlen_q + t and sees the keys at or before it.
- * 16-bit types, head_dim 64 or 128. A token with a negative position (lens[b] < seqlen_q) sees nothing: zeros.
+ * 16-bit types, head_dim 64 or 128, (heads_q / heads_kv) * num_buckets <= 4096. A token with a negative position (lens[b] < seqlen_q) sees nothing: zeros.
  * lens is clamped to [0, seqlen_k]; cache rows at or behind it are not read. */
 typedef struct {
   const void* ptr;

@@ -144,8 +144,8 @@ def test_decode_status_codes():
     assert code(bias=_bias(num=1)) == -12
     assert code(k=_lib.FbCache(0x1008, 1024, 128, 64)) == -6 and code(v=_lib.FbCache(0x1000, 1024, 100, 64)) == -6
     assert code(out=None) == -1 and code(out=0x1004) == -6
-    assert code() == -1  # slices without a workspace
-    assert lib.fb_relpos_decode_workspace_bytes(ctypes.byref(args())) > 0
+    assert code(seqlen_k=50000, batch=1) == -1  # more slices than a cluster holds, without a workspace
+    assert lib.fb_relpos_decode_workspace_bytes(ctypes.byref(args(seqlen_k=50000, batch=1))) > 0
     assert lib.fb_relpos_decode_workspace_bytes(ctypes.byref(args(seqlen_k=40))) == 0 == lib.fb_relpos_decode_workspace_bytes(None)
 
 
@@ -163,7 +163,7 @@ def test_workspace_bytes():
     assert lib.fb_relpos_workspace_bytes(ctypes.byref(big), 32) == (16 * 8192 + 2 * 16 * 32 * 32) * 4
     assert lib.fb_relpos_workspace_bytes(ctypes.byref(_prob(dtype=2, seqlen_q=17, total_q=17)), 4) == (2 * 17 + 2 + 2 * 2 * 4) * 4
     assert lib.fb_relpos_workspace_bytes(None, 32) == 0 and lib.fb_relpos_workspace_bytes(ctypes.byref(big), 500) == 0
-    assert lib.fb_relpos_bias_workspace_bytes(2, 5, 7, 4) > 0 and lib.fb_relpos_bias_workspace_bytes(2, 0, 7, 4) == 0
+    assert lib.fb_relpos_bias_workspace_bytes(0, 2, 5, 7, 4) > 0 and lib.fb_relpos_bias_workspace_bytes(0, 2, 0, 7, 4) == 0
 
 
 def test_oracle_gradients_are_the_formulas():
