@@ -105,9 +105,14 @@ struct RelFn {
 // Fills `b`, thread `i` of `n`. Only what the search will look at: bytes up to the first far distance.
 __device__ __forceinline__ void relpos_load_buckets(RelBuckets& b, const RelPos& rel, int i, int n) {
   const int words = min(rel.far, kRelNear - 1) / 4 + 1;
-  for (int t = i; t < words; t += n) b.near_words[t] = rel.near_words[t];
+  // Through generic addresses: as constant-bank reads with a different index per lane these would be served one lane at a time.
+  const uint32_t* near_words = rel.near_words;
+  const int* starts = rel.starts;
+  asm("" : "+l"(near_words));
+  asm("" : "+l"(starts));
+  for (int t = i; t < words; t += n) b.near_words[t] = near_words[t];
   if (rel.far >= kRelNear)
-    for (int t = i; t < rel.side - 1; t += n) b.starts[t] = rel.starts[t];
+    for (int t = i; t < rel.side - 1; t += n) b.starts[t] = starts[t];
 }
 // Sum of `v` over the lanes that hold the same key, for keys that form one run of neighbouring lanes each; valid in the
 // first lane of a run. Fixed order.
