@@ -16,14 +16,17 @@
 #include "fb_params.h"
 #include "ptx_sm100.cuh"
 
+#include <type_traits>
+
 namespace fb {
 namespace {
 
 using namespace ptx;
 
-constexpr int kWarps = 4, kThreads = kWarps * 32;
+constexpr int kWarps = 4, kThreads = kWarps * 32;  // of the join kernel; the decode kernel has 4 or 8 warps
 constexpr int KG = 16;      // keys per group = MMA k of the second product
 constexpr int kStages = 3;  // groups in flight per warp
+constexpr float kRescaleThreshold = 8.f;  // log2 units
 constexpr int kMaxTable = kDecodeMaxTable;  // entries of the table's columns that a CTA keeps
 constexpr int kMaxCluster = 8;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -73,8 +76,9 @@ __device__ __forceinline__ void store_out(const DecodeParams& p, int b, int t, i
   *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<T>(v.x * inv, v.y * inv), pack16<T>(v.z * inv, v.w * inv));
 }
 
-template <typename T, int D, int MT>
-__global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant__ DecodeParams p, const __grid_constant__ RelPos rel) {
+template <typename T, int D, int MT, int NW>
+__global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__ DecodeParams p, const __grid_constant__ RelPos rel) {
+  constexpr int NT = NW * 32;
   constexpr int R = 16 * MT;           // rows per CTA
   constexpr int U = D / 8;             // 16-byte units per row
   constexpr int kTile = KG * D * 2;    // bytes of one K or V group
@@ -83,31 +87,31 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
   uint8_t* const qs = smem;                       // [R][D]
   uint8_t* const stages = smem + R * D * 2;       // per warp [kStages][K, V]
   __shared__ RelBuckets buckets;
-  __shared__ float s_m[kWarps][R], s_l[kWarps][R];
+  __shared__ float s_m[NW][R], s_l[NW][R];
   __shared__ float2 joint_ml[R];
-  float* const tab = reinterpret_cast<float*>(smem + R * D * 2 + kWarps * kWarpBytes);  // [heads of the CTA's rows][nb], log2 units
+  float* const tab = reinterpret_cast<float*>(smem + R * D * 2 + NW * kWarpBytes);  // [heads of the CTA's rows][nb], log2 units
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = blockIdx.x;
   const int hk = blockIdx.y / p.row_tiles, rt = blockIdx.y - hk * p.row_tiles;
   const int b = blockIdx.z;
   const int rows = p.G * p.Sq;
-  relpos_load_buckets(buckets, rel, threadIdx.x, kThreads);
+  relpos_load_buckets(buckets, rel, threadIdx.x, NT);
   grid_dependency_wait();
   grid_launch_dependents();
   const int len = p.lens ? min(max(p.lens[b], 0), p.Sk) : p.Sk;
   // this slice of the sequence's keys: [k0, k1), whole rounds of the CTA's warps
-  const int per = ((len + p.splits - 1) / p.splits + kWarps * KG - 1) / (kWarps * KG) * (kWarps * KG);
+  const int per = ((len + p.splits - 1) / p.splits + NW * KG - 1) / (NW * KG) * (NW * KG);
   const int k0 = min(len, split * per), k1 = min(len, k0 + per);
   const int ngroups = (k1 - k0 + KG - 1) / KG;
-  const int mine = ngroups > warp ? (ngroups - warp + kWarps - 1) / kWarps : 0;
+  const int mine = ngroups > warp ? (ngroups - warp + NW - 1) / NW : 0;
 
   const T* kb = reinterpret_cast<const T*>(p.k.ptr) + b * p.k.batch_stride + hk * p.k.head_stride;
   const T* vb = reinterpret_cast<const T*>(p.v.ptr) + b * p.v.batch_stride + hk * p.v.head_stride;
   const uint32_t my = smem_u32(stages) + warp * kWarpBytes;
   auto load = [&](int i) {  // group i of this warp into its stage
     if (i < mine) {
-      const int j0 = k0 + (warp + i * kWarps) * KG;
+      const int j0 = k0 + (warp + i * NW) * KG;
       const uint32_t dst = my + (i % kStages) * 2 * kTile;
 #pragma unroll
       for (int x = 0; x < KG * U / 32; ++x) {
@@ -124,12 +128,12 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
   for (int i = 0; i < kStages - 1; ++i) load(i);
 
   // the table's columns of this kv head's query heads
-  for (int at = threadIdx.x; at < p.G * rel.nb; at += kThreads) {
+  for (int at = threadIdx.x; at < p.G * rel.nb; at += NT) {
     const int g = at / rel.nb, t = at - g * rel.nb;
     tab[at] = to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + (int64_t)(hk * p.G + g) * rel.head_stride]) * kLog2e;
   }
   // the queries: row x of the CTA is new token (rt * R + x) / G, query head hk * G + (rt * R + x) % G
-  for (int at = threadIdx.x; at < R * U; at += kThreads) {
+  for (int at = threadIdx.x; at < R * U; at += NT) {
     const int x = at / U, u = at % U, row = rt * R + x;
     uint4 v = make_uint4(0, 0, 0, 0);
     if (row < rows) {
@@ -167,12 +171,22 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
   }
   pos_min = len - p.Sq + (rt * R) / p.G;  // the earliest row of the CTA
 
+  // the query fragments stay in registers unless the accumulators need them
+  constexpr bool kQRegs = MT * D <= 128;
+  uint32_t q_regs[kQRegs ? MT : 1][kQRegs ? D / 16 : 1][4];
+  if constexpr (kQRegs) {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int kk = 0; kk < D / 16; ++kk) ldsm4(smem_u32(qs) + unit_off<D>(mt * 16 + (lane & 15), kk * 2 + (lane >> 4)), q_regs[mt][kk]);
+  }
+
   for (int i = 0; i < mine; ++i) {
     load(i + kStages - 1);
     cp_async_wait<kStages - 1>();
     __syncwarp();
     const uint32_t ks = my + (i % kStages) * 2 * kTile, vs = ks + kTile;
-    const int j0 = k0 + (warp + i * kWarps) * KG;
+    const int j0 = k0 + (warp + i * NW) * KG;
     float s[MT][2][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -188,52 +202,78 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
         uint32_t qf[4];
-        ldsm4(smem_u32(qs) + unit_off<D>(mt * 16 + (lane & 15), kk * 2 + (lane >> 4)), qf);
+        if constexpr (kQRegs) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) qf[e] = q_regs[mt][kk][e];
+        } else {
+          ldsm4(smem_u32(qs) + unit_off<D>(mt * 16 + (lane & 15), kk * 2 + (lane >> 4)), qf);
+        }
         mma16816<T>(s[mt][0], qf, kf[0], kf[1]);
         mma16816<T>(s[mt][1], qf, kf[2], kf[3]);
       }
     }
-    // bias, mask, running softmax; element e of tile n: row lane / 4 + 8 (e / 2), key j0 + 8 n + 2 (lane % 4) + e % 2
+    // bias and mask; element e of tile n: row lane / 4 + 8 (e / 2), key j0 + 8 n + 2 (lane % 4) + e % 2
     const bool all_far = pos_min - (j0 + KG - 1) >= bucket_of.far && j0 + KG <= k1;
-    uint32_t pf[MT][4];
+    float mx[MT][2];
+    auto add_bias = [&](auto which) {
+    constexpr int mode = decltype(which)::value;  // 0: one bucket per row, 1: by the byte table, 2: with a search
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      float mx[2] = {-INFINITY, -INFINITY};
+      mx[mt][0] = mx[mt][1] = -INFINITY;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int x = e >> 1, j = j0 + 8 * n + 2 * (lane & 3) + (e & 1);
           float bias = far_bias[mt][x];
-          if (!all_far) {
+          if (mode != 0) {
             const int r = j - pos[mt][x];
-            bias = row_tab[mt][x][bucket_of(min(r, 0))];
+            bias = row_tab[mt][x][mode == 1 ? bucket_of.near(min(r, 0)) : bucket_of(min(r, 0))];
             if (r > 0 || j >= k1) bias = -INFINITY;
           }
           s[mt][n][e] = fmaf(s[mt][n][e], scale2, bias);
-          mx[x] = fmaxf(mx[x], s[mt][n][e]);
+          mx[mt][x] = fmaxf(mx[mt][x], s[mt][n][e]);
         }
+    }
+    };
+    if (all_far) add_bias(std::integral_constant<int, 0>{});
+    else if (bucket_of.byte_table()) add_bias(std::integral_constant<int, 1>{});
+    else add_bias(std::integral_constant<int, 2>{});
+    // running maximum, every row's steps side by side; it moves (and the accumulators are rescaled) only when it grew by more than 2^8
+    bool grow = false;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 1));
-        mx[x] = fmaxf(mx[x], __shfl_xor_sync(0xffffffffu, mx[x], 2));
-        const float mn = fmaxf(m[mt][x], mx[x]);
-        const float off = mn == -INFINITY ? 0.f : mn;  // nothing visible so far: every exponential below is 0
-        const float alpha = ex2(m[mt][x] - off);       // m = -inf: 0
-        m[mt][x] = mn;
-        float sum = 0.f;
+        mx[mt][x] = fmaxf(mx[mt][x], __shfl_xor_sync(0xffffffffu, mx[mt][x], 1));
+        mx[mt][x] = fmaxf(mx[mt][x], __shfl_xor_sync(0xffffffffu, mx[mt][x], 2));
+        grow = grow || mx[mt][x] - m[mt][x] > kRescaleThreshold;  // (false when both are -inf: NaN)
+      }
+    if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+      for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-          for (int e = 2 * x; e < 2 * x + 2; ++e) {
-            s[mt][n][e] = ex2(s[mt][n][e] - off);
-            sum += s[mt][n][e];
-          }
-        l[mt][x] = l[mt][x] * alpha + sum;  // this lane's keys only; the four lanes of a row are added up at the end
-        if (__any_sync(0xffffffffu, alpha != 1.f)) {
+        for (int x = 0; x < 2; ++x) {
+          if (!(mx[mt][x] - m[mt][x] > kRescaleThreshold)) continue;
+          const float alpha = ex2(m[mt][x] - mx[mt][x]);  // m = -inf: 0
+          m[mt][x] = mx[mt][x];
+          l[mt][x] *= alpha;
 #pragma unroll
           for (int n = 0; n < D / 8; ++n) { o[mt][n][2 * x] *= alpha; o[mt][n][2 * x + 1] *= alpha; }
         }
+    }
+    uint32_t pf[MT][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const float off = m[mt][x] == -INFINITY ? 0.f : m[mt][x];  // nothing visible so far: every exponential is 0
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 2 * x; e < 2 * x + 2; ++e) s[mt][n][e] = ex2(s[mt][n][e] - off);
+        // this lane's keys only; the four lanes of a row are added up at the end
+        l[mt][x] += (s[mt][0][2 * x] + s[mt][0][2 * x + 1]) + (s[mt][1][2 * x] + s[mt][1][2 * x + 1]);
       }
       // the score fragments of two 8-key tiles are the 16-key operand of the second product
       pf[mt][0] = pack16<T>(s[mt][0][0], s[mt][0][1]);
@@ -269,8 +309,8 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
       }
     }
   float* const acc = reinterpret_cast<float*>(stages);
-  float* const joint = acc + kWarps * R * D;  // [R][D], cluster: this slice's sum
-  static_assert((kWarps + 1) * R * D * 4 <= kWarps * kWarpBytes, "the accumulators fit the stages");
+  float* const joint = acc + NW * R * D;  // [R][D], cluster: this slice's sum
+  static_assert((NW + 1) * R * D * 4 <= NW * kWarpBytes, "the accumulators fit the stages");
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
@@ -279,17 +319,17 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
       for (int x = 0; x < 2; ++x)
         *reinterpret_cast<float2*>(acc + (warp * R + mt * 16 + lane / 4 + 8 * x) * D + n * 8 + 2 * (lane & 3)) = make_float2(o[mt][n][2 * x], o[mt][n][2 * x + 1]);
   __syncthreads();
-  for (int at = threadIdx.x; at < R * D / 4; at += kThreads) {
+  for (int at = threadIdx.x; at < R * D / 4; at += NT) {
     const int x = at / (D / 4), d4 = at - x * (D / 4), row = rt * R + x;
     if (row >= rows) break;
     float mm = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w][x]);
+    for (int w = 0; w < NW; ++w) mm = fmaxf(mm, s_m[w][x]);
     const float off = mm == -INFINITY ? 0.f : mm;
     float ll = 0.f;
     float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float f = ex2(s_m[w][x] - off);
       const float4 a = *reinterpret_cast<const float4*>(acc + (w * R + x) * D + d4 * 4);
       ll += s_l[w][x] * f;
@@ -310,7 +350,7 @@ __global__ void __launch_bounds__(kThreads) decode_kernel(const __grid_constant_
   if (p.cluster) {
     cluster_sync_all();  // every slice's result is in its CTA's shared memory
     const uint32_t my_joint = smem_u32(joint), my_ml = smem_u32(joint_ml);
-    for (int at = split * kThreads + threadIdx.x; at < R * D / 4; at += p.splits * kThreads) {
+    for (int at = split * NT + threadIdx.x; at < R * D / 4; at += p.splits * NT) {
       const int x = at / (D / 4), d4 = at - x * (D / 4), row = rt * R + x;
       if (row >= rows) break;
       float mm = -INFINITY;
@@ -381,10 +421,10 @@ __global__ void __launch_bounds__(kThreads) decode_join_kernel(const __grid_cons
 }
 
 template <typename K>
-cudaError_t launch(K kern, dim3 grid, size_t smem, int cluster, cudaStream_t s, void** args) {
+cudaError_t launch(K kern, dim3 grid, int threads, size_t smem, int cluster, cudaStream_t s, void** args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3((unsigned)threads, 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute attr[2];  // programmatic dependent launch: both kernels wait for the one before at their start
@@ -398,27 +438,32 @@ cudaError_t launch(K kern, dim3 grid, size_t smem, int cluster, cudaStream_t s, 
   return cudaLaunchKernelExC(&cfg, reinterpret_cast<const void*>(kern), args);
 }
 
-template <typename T, int D, int MT>
+template <typename T, int D, int MT, int NW>
 int decode_typed(DecodeParams& p, RelPos& rel, cudaStream_t s) {
   constexpr int R = 16 * MT;
-  constexpr size_t tiles = R * D * 2 + kWarps * kStages * 2 * KG * D * 2;
+  constexpr size_t tiles = R * D * 2 + NW * kStages * 2 * KG * D * 2;
   const size_t smem = tiles + (size_t)p.G * rel.nb * sizeof(float);
-  auto kern = decode_kernel<T, D, MT>;
+  auto kern = decode_kernel<T, D, MT, NW>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(tiles + kMaxTable * sizeof(float))) != cudaSuccess) return FB_ERR_CUDA;
   p.row_tiles = (p.G * p.Sq + R - 1) / R;
   void* args[2] = {&p, &rel};
-  if (launch(kern, dim3((unsigned)p.splits, (unsigned)(p.Hkv * p.row_tiles), (unsigned)p.B), smem, p.cluster ? p.splits : 1, s, args) != cudaSuccess)
+  if (launch(kern, dim3((unsigned)p.splits, (unsigned)(p.Hkv * p.row_tiles), (unsigned)p.B), NW * 32, smem, p.cluster ? p.splits : 1, s, args) != cudaSuccess)
     return FB_ERR_CUDA;
   if (p.splits == 1 || p.cluster) return 1;
   const int64_t rows = (int64_t)p.B * p.Sq * p.Hq;
-  if (launch(decode_join_kernel<T, D>, dim3((unsigned)((rows + kWarps - 1) / kWarps)), 0, 1, s, args) != cudaSuccess) return FB_ERR_CUDA;
+  if (launch(decode_join_kernel<T, D>, dim3((unsigned)((rows + kWarps - 1) / kWarps)), kThreads, 0, 1, s, args) != cudaSuccess) return FB_ERR_CUDA;
   return 2;
 }
 
 template <typename T>
 int decode_dispatch(DecodeParams& p, RelPos& rel, cudaStream_t s) {
-  if (p.G * p.Sq <= 16) return p.D == 64 ? decode_typed<T, 64, 1>(p, rel, s) : decode_typed<T, 128, 1>(p, rel, s);
-  return p.D == 64 ? decode_typed<T, 64, 2>(p, rel, s) : decode_typed<T, 128, 2>(p, rel, s);
+  // A cluster's problem is small: one CTA per SM, whose 8 warps have the schedulers to themselves.
+  if (p.cluster) {
+    if (p.G * p.Sq <= 16) return p.D == 64 ? decode_typed<T, 64, 1, 8>(p, rel, s) : decode_typed<T, 128, 1, 8>(p, rel, s);
+    return p.D == 64 ? decode_typed<T, 64, 2, 8>(p, rel, s) : decode_typed<T, 128, 2, 8>(p, rel, s);
+  }
+  if (p.G * p.Sq <= 16) return p.D == 64 ? decode_typed<T, 64, 1, 4>(p, rel, s) : decode_typed<T, 128, 1, 4>(p, rel, s);
+  return p.D == 64 ? decode_typed<T, 64, 2, 4>(p, rel, s) : decode_typed<T, 128, 2, 4>(p, rel, s);
 }
 
 }  // namespace
@@ -432,9 +477,10 @@ int decode_splits(int batch, int heads_kv, int rows, int seqlen_k) {
   const int64_t base = (int64_t)batch * heads_kv * ((rows + per - 1) / per);
   const int64_t want = (148 * 2 * 4 + base - 1) / base;
   const int64_t rounds = (seqlen_k + kWarps * KG - 1) / (kWarps * KG);
-  if (base < 2 * 148 && rounds <= 8 * kMaxCluster) {
+  const int64_t rounds8 = (rounds + 1) / 2;  // of 8 warps
+  if (base < 2 * 148 && rounds8 <= 8 * kMaxCluster) {
     int n = 1;
-    while (n < kMaxCluster && n < want && 2 * n <= rounds) n *= 2;
+    while (n < kMaxCluster && n < want && 2 * n <= rounds8) n *= 2;
     return n;
   }
   const int64_t n = want < rounds ? want : rounds;

@@ -85,6 +85,12 @@ struct RelFn {
   int two, far, side;
   RelFn() = default;
   __device__ __forceinline__ RelFn(const RelPos& rel, const RelBuckets& buckets) : b(&buckets), two(rel.two), far(rel.far), side(rel.side) {}
+  // Without a branch, so that several look-ups overlap; only where `byte_table()`.
+  __device__ __forceinline__ bool byte_table() const { return far < kRelNear; }
+  __device__ __forceinline__ int near(int r) const {
+    const int n = min(two ? abs(r) : max(-r, 0), far);
+    return reinterpret_cast<const uint8_t*>(b->near_words)[n] + ((two && r > 0) ? side : 0);
+  }
   __device__ __forceinline__ int operator()(int r) const {
     const int n = min(two ? abs(r) : max(-r, 0), far);
     int lo;

@@ -37,8 +37,13 @@ __global__ void __launch_bounds__(kThreads) relpos_fill_kernel(const __grid_cons
   const int base = j0 - (i0 + rows - 1) - (sk - sq);  // position of value 0: the tile's last row, first column
   for (int x = threadIdx.x; x < (rows + cols - 1 + VEC - 1) / VEC; x += kThreads) {
     T v[2 * VEC];  // values VEC x .. VEC x + 2 VEC - 1
+    if (bucket_of.byte_table()) {
 #pragma unroll
-    for (int e = 0; e < 2 * VEC; ++e) v[e] = tab[bucket_of(base + x * VEC + e)];
+      for (int e = 0; e < 2 * VEC; ++e) v[e] = tab[bucket_of.near(base + x * VEC + e)];
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2 * VEC; ++e) v[e] = tab[bucket_of(base + x * VEC + e)];
+    }
 #pragma unroll
     for (int k = 0; k < VEC; ++k) {
       alignas(16) T w[VEC];

@@ -300,8 +300,14 @@ struct RelFwd {
       const float v0 = tab[f0], v1 = tab[f1];
       float bias[kSpan / 64];
       if (!(uni0 && uni1)) {
+        const int r = base + w * (kSpan / 2) + lane;
+        if (bucket_of.byte_table()) {
 #pragma unroll
-        for (int i = 0; i < kSpan / 64; ++i) bias[i] = tab[bucket_at(w * (kSpan / 2) + i * 32 + lane)];
+          for (int i = 0; i < kSpan / 64; ++i) bias[i] = tab[bucket_of.near(r + i * 32)];
+        } else {
+#pragma unroll
+          for (int i = 0; i < kSpan / 64; ++i) bias[i] = tab[bucket_of(r + i * 32)];
+        }
       }
 #pragma unroll
       for (int t = 0; t < 2; ++t)

@@ -894,11 +894,15 @@ struct TcCta {
     o.uni = first == last ? first : -1;
     o.value = tab[first];
     if (first != last) {
+      if (bucket_of.byte_table()) {
 #pragma unroll
-      for (int i = 0; i < kRelSpan / 32; ++i) {
-        o.ids[i] = bucket_at(lane + 32 * i);
-        o.bias[i] = tab[o.ids[i]];
+        for (int i = 0; i < kRelSpan / 32; ++i) o.ids[i] = bucket_of.near(kDkv ? base - lane - 32 * i : base + lane + 32 * i);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kRelSpan / 32; ++i) o.ids[i] = bucket_at(lane + 32 * i);
       }
+#pragma unroll
+      for (int i = 0; i < kRelSpan / 32; ++i) o.bias[i] = tab[o.ids[i]];
     }
   }
   __device__ __forceinline__ void rel_store_staged(int buf, const RelStaged& o) const {
