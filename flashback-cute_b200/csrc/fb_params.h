@@ -120,20 +120,19 @@ __device__ __forceinline__ void relpos_load_buckets(RelBuckets& b, const RelPos&
   if (rel.far >= kRelNear)
     for (int t = i; t < rel.side - 1; t += n) b.starts[t] = starts[t];
 }
-// Sum of `v` over the lanes that hold the same key, for keys that form one run of neighbouring lanes each; valid in the
-// first lane of a run. Fixed order.
-__device__ __forceinline__ float run_sum(float v, int key, int lane) {
+// Sum of `v` over the lanes that hold the same key, for keys that form one run of neighbouring lanes each. Returns whether this lane
+// is the first of its run; `v` is the run's sum there. Fixed order.
+__device__ __forceinline__ bool run_sum(float& v, int key, int lane) {
+  const int prev = __shfl_up_sync(0xffffffffu, key, 1);
+  const bool head = lane == 0 || prev != key;
+  const uint32_t behind = __ballot_sync(0xffffffffu, head) & ~((2u << lane) - 1u);  // first lanes of later runs
+  const int left = (behind ? __ffs((int)behind) - 2 : 31) - lane;                   // lanes of this run behind this one
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const float ov = __shfl_down_sync(0xffffffffu, v, o);
-    const int ok = __shfl_down_sync(0xffffffffu, key, o);
-    if (lane + o < 32 && ok == key) v += ov;
+    if (o <= left) v += ov;
   }
-  return v;
-}
-__device__ __forceinline__ bool run_head(int key, int lane) {
-  const int prev = __shfl_up_sync(0xffffffffu, key, 1);
-  return lane == 0 || prev != key;
+  return head;
 }
 
 // Decoding against a cache (decode.cu).

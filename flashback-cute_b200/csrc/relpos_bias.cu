@@ -191,8 +191,7 @@ __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_cons
       for (int w = 0; w < kWarps; ++w) s += part[w][shifts[w] + t];
       if (c < ndiag) bucket = RelFn(rel, buckets)(c - (sq - 1) - (sk - sq));
     }
-    const bool run = run_head(bucket, lane);
-    s = run_sum(s, bucket, lane);
+    const bool run = run_sum(s, bucket, lane);
     for (int w = 0; w < kWarps; ++w) {
       if (w == warp && run && bucket >= 0) acc[bucket] += s;
       __syncthreads();

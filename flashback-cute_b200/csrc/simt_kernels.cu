@@ -355,8 +355,8 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p, const __gri
       float a = dp - dps[r];
       float ds = pr * a;
       if constexpr (BIAS) {  // neighbouring lanes hold neighbouring positions: equal buckets form runs
-        const bool first = run_head(bucket, lane);
-        const float sum = run_sum(ds, bucket, lane);
+        float sum = ds;
+        const bool first = run_sum(sum, bucket, lane);
         if (first) rs->acc[warp][bucket] += sum;
         __syncwarp();
       }

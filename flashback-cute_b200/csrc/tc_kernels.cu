@@ -67,12 +67,13 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Relative position bias: a block of BM owner rows x BN streamed rows spans kRelSpan positions; the statistics warp
 // stages their biases (and, for the table's gradient, their buckets) per block, two buffers.
 constexpr int kRelSpan = BM + BN;  // BM + BN - 1 positions
+constexpr int kRelCopy = kRelSpan + 8;  // 8 banks apart: see relpos_fwd.cu
 enum {                             // byte offsets in the bias area behind the misc area
   REL_TAB = 0,                                     // this head's table column, in log2 units
   REL_BUCKETS = REL_TAB + FB_RELPOS_MAX_BUCKETS * 4,  // RelBuckets
   REL_UNI = REL_BUCKETS + (int)sizeof(RelBuckets),  // [2] the bucket all pairs of the block fall in, or -1; [2] its bias
-  REL_BIAS = REL_UNI + 16,                         // [2][kRelSpan]
-  REL_IDS = REL_BIAS + 2 * kRelSpan * 4,           // [2][kRelSpan] (KIND_DQ)
+  REL_BIAS = REL_UNI + 16,                         // [2][4][kRelCopy]: four copies, each shifted by one entry more
+  REL_IDS = REL_BIAS + 2 * 4 * kRelCopy * 4,       // [2][kRelSpan] (KIND_DQ)
   REL_DIAG = REL_IDS + 2 * kRelSpan * 4,           // [pointwise warps][32] (KIND_DQ)
   REL_ROWDOT = REL_DIAG + NWG * 4 * 32 * 4,        // [BM] (KIND_DQ)
   REL_ACC = REL_ROWDOT + BM * 4,                 // [pointwise warps][FB_RELPOS_MAX_BUCKETS] (KIND_DQ)
@@ -911,11 +912,13 @@ struct TcCta {
       reinterpret_cast<float*>(rel_area + REL_UNI)[2 + buf] = o.value;
     }
     if (o.uni < 0) {
-      float* dst = reinterpret_cast<float*>(rel_area + REL_BIAS) + buf * kRelSpan;
+      float* dst = reinterpret_cast<float*>(rel_area + REL_BIAS) + buf * 4 * kRelCopy;
       int* ids = reinterpret_cast<int*>(rel_area + REL_IDS) + buf * kRelSpan;
 #pragma unroll
       for (int i = 0; i < kRelSpan / 32; ++i) {
-        dst[lane + 32 * i] = o.bias[i];
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i > 0 || lane >= k) dst[k * kRelCopy + lane + 32 * i - k] = o.bias[i];
         if (kDq) ids[lane + 32 * i] = o.ids[i];
       }
     }
@@ -1285,7 +1288,8 @@ struct TcCta {
   __device__ __forceinline__ void pw_bwd_block(int it, int st, bool need_mask_, int cmin, int cmax, const float* stats) {
     const bool need_mask = BIAS ? MASK : need_mask_;
     static_assert(!TANGENT, "first-order kernels only");
-    const float* bias = nullptr;
+    const float4* bias = nullptr;
+    float4 b4;
     float2 b2 = make_float2(0.f, 0.f);
     if constexpr (BIAS) {
       if constexpr (UNI) {
@@ -1297,8 +1301,8 @@ struct TcCta {
     }
     // KIND_DQ with a bias: sum of dS along the diagonals of this warp's 32 rows x HC columns. The running sum of a
     // diagonal moves one lane up per column; the one that leaves lane 31 is complete and wraps round to lane 0, which
-    // files it.
-    float diag = 0.f;
+    // files it. Two chains, one per 16 columns, halve the latency of the shuffles; they are put together at the end.
+    float diags[2] = {0.f, 0.f};
     float* const filed = BIAS ? reinterpret_cast<float*>(rel_area + REL_DIAG) + (warp & 7) * 32 : nullptr;
     constexpr int CW = 16;
     constexpr int NG = HC / CW;
@@ -1327,7 +1331,10 @@ struct TcCta {
           ndp = *reinterpret_cast<const float2*>(&stats[BN + col]);
         }
         if constexpr (BIAS) {
-          if constexpr (!UNI) b2 = make_float2(bias[gi * CW + c], bias[gi * CW + c + 1]);
+          if constexpr (!UNI) {
+            if (c % 4 == 0) b4 = bias[(gi * CW + c) / 4];
+            b2 = c % 4 == 0 ? make_float2(b4.x, b4.y) : make_float2(b4.z, b4.w);
+          }
           nl2 = __fadd2_rn(nl2, b2);
         }
         const float2 e = __ffma2_rn(make_float2(__uint_as_float(bs[buf][c]), __uint_as_float(bs[buf][c + 1])), sc2, nl2);
@@ -1352,9 +1359,10 @@ struct TcCta {
           } else {
 #pragma unroll
             for (int e2 = 0; e2 < 2; ++e2) {
+              float& diag = diags[gi];
               diag = __shfl_sync(0xffffffffu, diag, (lane + 31) & 31);
               if (lane == 0) {
-                if (gi * CW + c + e2 > 0) filed[gi * CW + c + e2 - 1] = diag;
+                if (c + e2 > 0) filed[gi * CW + c + e2 - 1] = diag;
                 diag = 0.f;
               }
               diag += e2 ? ds.y : ds.x;
@@ -1377,23 +1385,28 @@ struct TcCta {
       }
     }
     if constexpr (BIAS && kDq && !UNI) {
-      static_assert(HC == 32, "31 filed diagonals and one per lane");
+      static_assert(HC == 32 && CW == 16, "two chains of 16 columns");
       __syncwarp();
-      // entry of (lane 31's row, column 0): the first diagonal
+      // Diagonal (column - lane) of 32 x 32: -31 + k is filed as k by the chain of columns 0-15 (k < 15) and that of columns 16-31
+      // (15 < k < 31); lane i ends up holding 15 - i of the first chain and 31 - i of the second.
+      const float a_low = __shfl_sync(0xffffffffu, diags[0], (46 - lane) & 31), a_high = __shfl_sync(0xffffffffu, diags[0], (lane - 16) & 31);
+      float low = lane != 15 && lane < 31 ? filed[lane] : 0.f;
+      if (lane >= 15 && lane < 31) low += a_low;
+      // entry of (lane 0's row, column 0)
       const int* ids = reinterpret_cast<const int*>(rel_area + REL_IDS) + (it & 1) * kRelSpan + cb - (warp & 3) * 32 + (BM - 1);
-      rel_add(lane < 31 ? filed[lane] : 0.f, lane < 31 ? ids[lane - 31] : -1);
-      rel_add(diag, ids[31 - lane]);
+      rel_add(low, lane < 31 ? ids[lane - 31] : -1);
+      rel_add(diags[1] + (lane >= 16 ? a_high : 0.f), ids[31 - lane]);
     }
   }
-  // This thread's biases of block `it`: entry c belongs to column cb + c.
-  __device__ __forceinline__ const float* rel_bias(int it) const {
-    return reinterpret_cast<const float*>(rel_area + REL_BIAS) + (it & 1) * kRelSpan + cb - row + (BM - 1);
+  // This thread's biases of block `it`, four columns a load: entry c belongs to columns cb + 4 c .. + 3.
+  __device__ __forceinline__ const float4* rel_bias(int it) const {
+    const int a = cb - row + (BM - 1);
+    return reinterpret_cast<const float4*>(reinterpret_cast<const float*>(rel_area + REL_BIAS) + ((it & 1) * 4 + (a & 3)) * kRelCopy + (a & ~3));
   }
   // KIND_DQ with a bias, one warp: adds every lane's `v` to its bucket (equal buckets sit in neighbouring lanes; -1: none).
   __device__ __forceinline__ void rel_add(float v, int bucket) {
     float* acc = reinterpret_cast<float*>(rel_area + REL_ACC) + (warp & 7) * FB_RELPOS_MAX_BUCKETS;
-    const bool first = run_head(bucket, lane);
-    v = run_sum(v, bucket, lane);
+    const bool first = run_sum(v, bucket, lane);
     if (first && bucket >= 0) acc[bucket] += v;
     __syncwarp();
   }
