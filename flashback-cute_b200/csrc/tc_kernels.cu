@@ -536,8 +536,8 @@ struct TcCta {
         if ((i >= BAR_P_FULL && i < BAR_P_FULL + 2) || (i >= BAR_ST_EMPTY && i < BAR_ST_EMPTY + 2) || i == BAR_A_READY || i == BAR_P_HALF) count = NWG * 4;  // one arrival per pointwise warp
         // DKV: the S-like tiles a block's pointwise work starts from are complete when the MMAs have
         // committed AND the statistics warp has staged the block's row statistics (one wait for both); the same
-        // for the staged biases in every kind
-        if (kStager && (i == BAR_S_FULL || (i == BAR_S_FULL + 1 && !kSplit))) count = 2u;
+        // for the staged biases in every kind (DKV: by another warp)
+        if (kStager && (i == BAR_S_FULL || (i == BAR_S_FULL + 1 && !kSplit))) count = kDkv && BIAS ? 3u : 2u;
         mbar_init(bar(i), count);
       }
       *abort_flag = 0;
@@ -585,7 +585,10 @@ struct TcCta {
       } else if (n_it > 0 && warp == 1) {
         if (elect_one()) issuer();
       } else if (warp == kStatsWarp) {
-        if constexpr (kStager) stats_stager();
+        if constexpr (kDkv) stats_stager();
+        else if constexpr (BIAS) bias_stager();
+      } else if (warp == kStatsWarp + 1) {
+        if constexpr (kDkv && BIAS) bias_stager();
       }
     } else {
       if constexpr (kRealloc) reg_alloc<kPwRegs>();
@@ -994,44 +997,21 @@ struct TcCta {
   }
   __device__ __forceinline__ void stats_stager() {
     float4 cur[BN / 32], nxt[BN / 32];
-    int table_head = -1;
-    if constexpr (BIAS) {
-      relpos_load_buckets(*reinterpret_cast<RelBuckets*>(rel_area + REL_BUCKETS), *rel, lane, 32);
-      __syncwarp();
-    }
-    RelFn bucket_of;
-    if constexpr (BIAS) bucket_of = RelFn(*rel, *reinterpret_cast<const RelBuckets*>(rel_area + REL_BUCKETS));
-    if (kDkv && n_it > 0) stats_load(0, nxt);
+    if (n_it > 0) stats_load(0, nxt);
     for (int it = 0; it < n_it; ++it) {
       const int sb_ = it & 1;
-      if (kDkv) {
 #pragma unroll
-        for (int r = 0; r < BN / 32; ++r) cur[r] = nxt[r];
-        if (it + 1 < n_it) stats_load(it + 1, nxt);
-      }
-      [[maybe_unused]] RelStaged staged;
-      if constexpr (BIAS) {
-        const int gi = it_base + it, g = kDkv ? gi / blk_count : 0;
-        const int h = kDkv ? head * G + g : head;
-        if (h != table_head) {
-          __syncwarp();
-          rel_load_table(h);
-          table_head = h;
-        }
-        rel_look_up(kDkv ? blk_begin + gi - g * blk_count : it, bucket_of, staged);
-      }
+      for (int r = 0; r < BN / 32; ++r) cur[r] = nxt[r];
+      if (it + 1 < n_it) stats_load(it + 1, nxt);
       warp_wait(BAR_ST_EMPTY + sb_, ((it >> 1) & 1) ^ 1);
       if (aborted()) break;
-      if (kDkv) {
-        float* dst = stats_base + sb_ * (4 * BN);
+      float* dst = stats_base + sb_ * (4 * BN);
 #pragma unroll
-        for (int r = 0; r < BN / 32; ++r) {
-          const int rr = lane + 32 * r;
-          dst[rr] = (fabsf(cur[r].x) == INFINITY) ? -INFINITY : -cur[r].x * kLog2e;  // a fully masked row has lse = -inf
-          dst[BN + rr] = -cur[r].y; dst[2 * BN + rr] = -cur[r].z; dst[3 * BN + rr] = -cur[r].w;
-        }
+      for (int r = 0; r < BN / 32; ++r) {
+        const int rr = lane + 32 * r;
+        dst[rr] = (fabsf(cur[r].x) == INFINITY) ? -INFINITY : -cur[r].x * kLog2e;  // a fully masked row has lse = -inf
+        dst[BN + rr] = -cur[r].y; dst[2 * BN + rr] = -cur[r].z; dst[3 * BN + rr] = -cur[r].w;
       }
-      if constexpr (BIAS) rel_store_staged(sb_, staged);
       __syncwarp();
       if (lane == 0) {
         // Second arrival on the barrier the MMA issuer commits block `it`'s first S-like tiles to. Its
@@ -1040,9 +1020,31 @@ struct TcCta {
         if (ST == 1 && it > 0) wait1(BAR_S_FULL, (it - 1) & 1);
         mbar_arrive(bar(BAR_S_FULL + it % ST));
       }
-      if constexpr (BIAS) {
-        if (is_tail(it)) zero_tail(it);
+    }
+  }
+  // BIAS: one warp (KIND_DKV: beside the statistics warp) that stages the biases of every block the same way, and zeroes the tails.
+  __device__ __forceinline__ void bias_stager() {
+    static_assert(ST == 2 || !BIAS, "the wait for the buffer implies the previous phase of S_FULL");
+    int table_head = -1;
+    relpos_load_buckets(*reinterpret_cast<RelBuckets*>(rel_area + REL_BUCKETS), *rel, lane, 32);
+    __syncwarp();
+    const RelFn bucket_of(*rel, *reinterpret_cast<const RelBuckets*>(rel_area + REL_BUCKETS));
+    for (int it = 0; it < n_it; ++it) {
+      const int gi = it_base + it, g = kDkv ? gi / blk_count : 0;
+      const int h = kDkv ? head * G + g : head;
+      if (h != table_head) {
+        __syncwarp();
+        rel_load_table(h);
+        table_head = h;
       }
+      RelStaged staged;
+      rel_look_up(kDkv ? blk_begin + gi - g * blk_count : it, bucket_of, staged);
+      warp_wait(BAR_ST_EMPTY + (it & 1), ((it >> 1) & 1) ^ 1);
+      if (aborted()) break;
+      rel_store_staged(it & 1, staged);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar(BAR_S_FULL + it % ST));
+      if (is_tail(it)) zero_tail(it);
     }
   }
 
@@ -1285,7 +1287,8 @@ struct TcCta {
   // the current one is processed.
   // With a bias: UNI = all pairs of the block share a bucket, MASK = some are masked (without one need_mask says so at run time).
   template <bool UNI, bool MASK>
-  __device__ __forceinline__ void pw_bwd_block(int it, int st, bool need_mask_, int cmin, int cmax, const float* stats) {
+  __device__ __forceinline__ void pw_bwd_block(int it, int st, bool need_mask_, int cmin, int cmax, const float* stats,
+                                               float (&dsv)[BIAS && kDq ? HC : 1]) {
     const bool need_mask = BIAS ? MASK : need_mask_;
     static_assert(!TANGENT, "first-order kernels only");
     const float4* bias = nullptr;
@@ -1299,11 +1302,6 @@ struct TcCta {
         bias = rel_bias(it);
       }
     }
-    // KIND_DQ with a bias: sum of dS along the diagonals of this warp's 32 rows x HC columns. The running sum of a
-    // diagonal moves one lane up per column; the one that leaves lane 31 is complete and wraps round to lane 0, which
-    // files it. Two chains, one per 16 columns, halve the latency of the shuffles; they are put together at the end.
-    float diags[2] = {0.f, 0.f};
-    float* const filed = BIAS ? reinterpret_cast<float*>(rel_area + REL_DIAG) + (warp & 7) * 32 : nullptr;
     constexpr int CW = 16;
     constexpr int NG = HC / CW;
     uint32_t bs[2][CW], bp[2][CW];
@@ -1357,16 +1355,8 @@ struct TcCta {
           if constexpr (UNI) {
             rel_sum = __fadd2_rn(rel_sum, ds);
           } else {
-#pragma unroll
-            for (int e2 = 0; e2 < 2; ++e2) {
-              float& diag = diags[gi];
-              diag = __shfl_sync(0xffffffffu, diag, (lane + 31) & 31);
-              if (lane == 0) {
-                if (c + e2 > 0) filed[gi * CW + c + e2 - 1] = diag;
-                diag = 0.f;
-              }
-              diag += e2 ? ds.y : ds.x;
-            }
+            dsv[gi * CW + c] = ds.x;
+            dsv[gi * CW + c + 1] = ds.y;
           }
         }
       }
@@ -1384,18 +1374,48 @@ struct TcCta {
         if (prof) pw_ld0 += clock64() - tq2;
       }
     }
-    if constexpr (BIAS && kDq && !UNI) {
-      static_assert(HC == 32 && CW == 16, "two chains of 16 columns");
+  }
+  // KIND_DQ with a bias: adds this warp's 32 rows x 32 columns of dS to their buckets, diagonal by diagonal. The running sum of a
+  // diagonal moves one lane up per column; the one that leaves lane 31 is complete and wraps round to lane 0, which files it. Four
+  // chains of 8 columns each hide each other's shuffles; they are put together at the end. Runs after the block's dS has
+  // been handed over.
+  __device__ __forceinline__ void rel_diagonals(int it, const float (&dsv)[BIAS && kDq ? HC : 1]) {
+    if constexpr (BIAS && kDq) {
+      static_assert(HC == 32, "32 columns");
+      constexpr int NCH = 4, CC = HC / NCH;
+      float* const filed = reinterpret_cast<float*>(rel_area + REL_DIAG) + (warp & 7) * 32;
+      float diag[NCH] = {};
+#pragma unroll
+      for (int s = 0; s < CC; ++s) {
+#pragma unroll
+        for (int q = 0; q < NCH; ++q) {
+          if (s > 0) {
+            const float moved = __shfl_sync(0xffffffffu, diag[q], (lane + 31) & 31);
+            if (lane == 0) filed[q * CC + s - 1] = moved;
+            diag[q] = (lane == 0 ? 0.f : moved) + dsv[q * CC + s];
+          } else {
+            diag[q] = dsv[q * CC];
+          }
+        }
+      }
       __syncwarp();
-      // Diagonal (column - lane) of 32 x 32: -31 + k is filed as k by the chain of columns 0-15 (k < 15) and that of columns 16-31
-      // (15 < k < 31); lane i ends up holding 15 - i of the first chain and 31 - i of the second.
-      const float a_low = __shfl_sync(0xffffffffu, diags[0], (46 - lane) & 31), a_high = __shfl_sync(0xffffffffu, diags[0], (lane - 16) & 31);
-      float low = lane != 15 && lane < 31 ? filed[lane] : 0.f;
-      if (lane >= 15 && lane < 31) low += a_low;
+      // Diagonal (column - lane): -31 + k is filed as k (not k = 7, 15, 23); lane i holds CC q + 7 - i of chain q. Turned by 8 (3 - q) lanes,
+      // lane i holds 31 - i of every chain, or, where the turn wrapped round (i < 8 (3 - q)), -1 - i.
+      float high = diag[NCH - 1], low = 0.f;
+#pragma unroll
+      for (int q = 0; q < NCH - 1; ++q) {
+        const int turn = CC * (NCH - 1 - q);
+        const float v = __shfl_sync(0xffffffffu, diag[q], (lane - turn) & 31);
+        if (lane >= turn) high += v;
+        else low += v;
+      }
+      low = __shfl_sync(0xffffffffu, low, (30 - lane) & 31);
+      if (lane == 31) low = 0.f;
+      if ((lane & (CC - 1)) != CC - 1) low += filed[lane];
       // entry of (lane 0's row, column 0)
       const int* ids = reinterpret_cast<const int*>(rel_area + REL_IDS) + (it & 1) * kRelSpan + cb - (warp & 3) * 32 + (BM - 1);
       rel_add(low, lane < 31 ? ids[lane - 31] : -1);
-      rel_add(diags[1] + (lane >= 16 ? a_high : 0.f), ids[31 - lane]);
+      rel_add(high, ids[31 - lane]);
     }
   }
   // This thread's biases of block `it`, four columns a load: entry c belongs to columns cb + 4 c .. + 3.
@@ -1528,18 +1548,25 @@ struct TcCta {
         tc_fence_after();
         if constexpr (kFwd) pw_fwd_block(it, st, need_mask, cmax);
         else if constexpr (BIAS) {
+          float dsv[kDq ? HC : 1];
           const int uni = reinterpret_cast<const int*>(rel_area + REL_UNI)[it & 1];
           if (uni >= 0) {
             if constexpr (kDq) rel_flush(uni);
-            if (need_mask) pw_bwd_block<true, true>(it, st, true, cmin, cmax, stats);
-            else pw_bwd_block<true, false>(it, st, false, cmin, cmax, stats);
-          } else if (need_mask) {
-            pw_bwd_block<false, true>(it, st, true, cmin, cmax, stats);
+            if (need_mask) pw_bwd_block<true, true>(it, st, true, cmin, cmax, stats, dsv);
+            else pw_bwd_block<true, false>(it, st, false, cmin, cmax, stats, dsv);
           } else {
-            pw_bwd_block<false, false>(it, st, false, cmin, cmax, stats);
+            if (need_mask) pw_bwd_block<false, true>(it, st, true, cmin, cmax, stats, dsv);
+            else pw_bwd_block<false, false>(it, st, false, cmin, cmax, stats, dsv);
+            if constexpr (kDq) {
+              pw_publish(BAR_P_FULL + st, it, false);
+              rel_diagonals(it, dsv);
+              if (lane == 0) mbar_arrive(bar(BAR_ST_EMPTY + (it & 1)));  // the staged buckets have been read
+              continue;
+            }
           }
         } else {
-          pw_bwd_block<false, false>(it, st, need_mask, cmin, cmax, stats);
+          float none[1];
+          pw_bwd_block<false, false>(it, st, need_mask, cmin, cmax, stats, none);
         }
         const long long tq1 = prof ? clock64() : 0;
         pw_publish(BAR_P_FULL + st, it, true);
