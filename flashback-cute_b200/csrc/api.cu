@@ -367,8 +367,8 @@ extern "C" int fb_relpos_fwd(const fb_relpos_fwd_args* a, fb_stream_t stream) {
   FB_TRY(convert_relpos(rel, a->bias, true));
   FB_TRY(check_tensor(a->q, true)); FB_TRY(check_tensor(a->k, true)); FB_TRY(check_tensor(a->v, true));
   FB_TRY(check_tensor(a->out, true)); FB_TRY(check_tensor(a->out_low, false));
-  if (a->out_low.ptr && !use_tensor_cores(a->prob)) return FB_ERR_MODE;
   if (a->prob.total_q == 0) return FB_OK;
+  if (a->prob.total_k == 0) return FB_ERR_SHAPE;
   Params p;
   fill_problem(p, a->prob);
   FB_TRY(device_setup(&p.status));
@@ -392,8 +392,7 @@ extern "C" int fb_relpos_bwd(const fb_relpos_bwd_args* a, fb_stream_t stream) {
   FB_TRY(check_tensor(a->dq, false)); FB_TRY(check_tensor(a->dk, false)); FB_TRY(check_tensor(a->dv, false));
   if (!a->lse || !a->workspace) return FB_ERR_NULL_ARG;
   if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return FB_ERR_ALIGNMENT;
-  if (a->out_low.ptr && !use_tensor_cores(a->prob)) return FB_ERR_MODE;
-  if (a->prob.total_q == 0 || a->prob.total_k == 0) return FB_OK;
+  if (a->prob.total_q == 0 || a->prob.total_k == 0) return FB_ERR_SHAPE;
   Params p;
   fill_problem(p, a->prob);
   FB_TRY(device_setup(&p.status));
@@ -477,6 +476,7 @@ int check_decode(const fb_relpos_decode_args& a) {
   if (a.heads_q <= 0 || a.heads_kv <= 0 || a.heads_q % a.heads_kv != 0) return FB_ERR_HEADS;
   if (a.batch < 0 || a.seqlen_q < 0 || a.seqlen_k < 0) return FB_ERR_SHAPE;
   if (a.batch > 65535 || a.seqlen_k > (1 << 30) || a.heads_q > 65535 || (int64_t)a.seqlen_q * a.heads_q > (1 << 20)) return FB_ERR_TOO_LARGE;
+  if ((int64_t)a.heads_kv * (((int64_t)(a.heads_q / a.heads_kv) * a.seqlen_q + 15) / 16) > 65535) return FB_ERR_TOO_LARGE;  // grid
   if ((int64_t)(a.heads_q / a.heads_kv) * a.bias.num_buckets > kDecodeMaxTable) return FB_ERR_TOO_LARGE;
   return FB_OK;
 }

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
   // the table's columns of this kv head's query heads
   for (int at = threadIdx.x; at < p.G * rel.nb; at += NT) {
     const int g = at / rel.nb, t = at - g * rel.nb;
-    tab[at] = to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + (int64_t)(hk * p.G + g) * rel.head_stride]) * kLog2e;
+    tab[at] = relpos_entry<T>(rel, t, hk * p.G + g) * kLog2e;
   }
   // the queries: row x of the CTA is new token (rt * R + x) / G, query head hk * G + (rt * R + x) % G
   for (int at = threadIdx.x; at < R * U; at += NT) {

@@ -57,6 +57,16 @@ struct Params {
   long long wait_budget;  // clock budget of one bounded wait (test hook instantiation only)
 };
 
+template <typename T> __device__ __forceinline__ float to_f(T x);
+template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+template <> __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
+
+template <typename T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
+
 // Learned relative position bias (fb_relpos), passed to the kernels that add it as a parameter of its own, so that the
 // others keep theirs as they are.
 struct RelPos {
@@ -108,6 +118,15 @@ struct RelFn {
     return lo + ((two && r > 0) ? side : 0);
   }
 };
+// A table entry as the attention kernels use it. Entries at or below -2^100 (the lowest bfloat16 and float32 values among them) hide their
+// pairs like -inf: kept as numbers they would swallow the scores of a row that sees nothing else and make its log-sum-exp
+// useless for the backward.
+constexpr float kRelHidden = -1.2676506002282294e30f;  // -2^100
+template <typename T>
+__device__ __forceinline__ float relpos_entry(const RelPos& rel, int bucket, int head) {
+  const float x = to_f<T>(reinterpret_cast<const T*>(rel.table)[bucket * rel.bucket_stride + head * rel.head_stride]);
+  return x <= kRelHidden ? -INFINITY : x;
+}
 // Fills `b`, thread `i` of `n`. Only what the search will look at: bytes up to the first far distance.
 __device__ __forceinline__ void relpos_load_buckets(RelBuckets& b, const RelPos& rel, int i, int n) {
   const int words = min(rel.far, kRelNear - 1) / 4 + 1;
@@ -192,16 +211,6 @@ __device__ __forceinline__ int first_query_of_key(const Params& p, const SeqInfo
   }
   return max(lo, j - off);
 }
-
-template <typename T> __device__ __forceinline__ float to_f(T x);
-template <> __device__ __forceinline__ float to_f<float>(float x) { return x; }
-template <> __device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-template <> __device__ __forceinline__ float to_f<__half>(__half x) { return __half2float(x); }
-
-template <typename T> __device__ __forceinline__ T from_f(float x);
-template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
-template <> __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
-template <> __device__ __forceinline__ __half from_f<__half>(float x) { return __float2half_rn(x); }
 
 // host-side launchers (each returns the number of kernels enqueued, or a negative fb_status)
 int launch_simt_fwd(const Params& p, cudaStream_t stream);

@@ -282,7 +282,7 @@ struct RelFwd {
     float* tab = reinterpret_cast<float*>(misc + M_TAB);
     RelBuckets& buckets = *reinterpret_cast<RelBuckets*>(misc + M_BUCKETS);
     for (int t = w * 32 + lane; t < rel.nb; t += 64)
-      tab[t] = to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + head * rel.head_stride]) * kLog2e;
+      tab[t] = relpos_entry<T>(rel, t, head) * kLog2e;
     relpos_load_buckets(buckets, rel, w * 32 + lane, 64);
     named_barrier_sync(1, 64);
     const RelFn bucket_of(rel, buckets);

@@ -69,7 +69,7 @@ struct RelSmem {
 };
 template <typename T>
 __device__ __forceinline__ void rel_load(RelSmem& rs, const RelPos& rel, int h) {
-  for (int t = threadIdx.x; t < rel.nb; t += kThreads) rs.tab[t] = to_f<T>(reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + h * rel.head_stride]);
+  for (int t = threadIdx.x; t < rel.nb; t += kThreads) rs.tab[t] = relpos_entry<T>(rel, t, h);
   relpos_load_buckets(rs.buckets, rel, threadIdx.x, kThreads);
 }
 template <bool BIAS> struct RelArg { using type = NoRel; };
@@ -210,6 +210,14 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
 #pragma unroll
       for (int c = 0; c < NC; ++c) o[c] = acc_o[r][c];
       store_row<T, D>(p.o, h, row, lane, o, 1.f);
+      if constexpr (BIAS) {
+        if (p.od.ptr) {  // what rounding O left out
+          float low[NC];
+#pragma unroll
+          for (int c = 0; c < NC; ++c) low[c] = o[c] - to_f<T>(from_f<T>(o[c]));
+          store_row<T, D>(p.od, h, row, lane, low, 1.f);
+        }
+      }
       if (lane == 0 && (!BIAS || p.lse)) p.lse[srow] = lse[r];
     }
     float od[NC];
@@ -303,6 +311,11 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p, const __gri
         const T* gp = reinterpret_cast<const T*>(p.dout.ptr) + (int64_t)h * p.dout.head_stride + (int64_t)(si.q0 + i) * p.dout.row_stride;
 #pragma unroll
         for (int c = 0; c < NC; ++c) d = fmaf(to_f<T>(gp[lane + 32 * c]), to_f<T>(op[lane + 32 * c]), d);
+        if (p.od.ptr) {
+          const T* lp = reinterpret_cast<const T*>(p.od.ptr) + (int64_t)h * p.od.head_stride + (int64_t)(si.q0 + i) * p.od.row_stride;
+#pragma unroll
+          for (int c = 0; c < NC; ++c) d = fmaf(to_f<T>(gp[lane + 32 * c]), to_f<T>(lp[lane + 32 * c]), d);
+        }
       }
       d = warp_sum(d);
       dps[r] = d;

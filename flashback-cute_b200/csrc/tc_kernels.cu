@@ -36,9 +36,8 @@
 #include <cuda.h>
 #include <cstring>
 #include <mutex>
-#include <set>
 #include <type_traits>
-#include <utility>
+
 
 namespace fb {
 namespace {
@@ -874,7 +873,7 @@ struct TcCta {
   __device__ __forceinline__ void rel_load_table(int h) {
     float* tab = reinterpret_cast<float*>(rel_area + REL_TAB);
     for (int t = lane; t < rel->nb; t += 32)
-      tab[t] = to_f<T>(reinterpret_cast<const T*>(rel->table)[t * rel->bucket_stride + h * rel->head_stride]) * kLog2e;
+      tab[t] = relpos_entry<T>(*rel, t, h) * kLog2e;
     __syncwarp();
   }
   // BIAS: the biases of a block's positions. Entry u belongs to the pairs with (streamed row in block) - (owner row in
@@ -2222,15 +2221,16 @@ int tc_tensor_map(CUtensorMap* m, const SeqT& t, int dtype, int D, int64_t rows,
 }
 
 int tc_prepare_launch(const void* kernel, int smem_bytes, int* sm_count) {
-  static std::set<std::pair<const void*, int>> done;  // guarded by g_launch_mutex
+  static struct { const void* kernel; int dev; } done[64];  // guarded by g_launch_mutex; when full, set again per call
+  static int n_done = 0;
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return FB_ERR_CUDA;
   *sm_count = device_sm_count(dev);
   std::lock_guard<std::mutex> lock(g_launch_mutex);
-  if (!done.count({kernel, dev})) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess) return FB_ERR_CUDA;
-    done.insert({kernel, dev});
-  }
+  for (int i = 0; i < n_done; ++i)
+    if (done[i].kernel == kernel && done[i].dev == dev) return FB_OK;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes) != cudaSuccess) return FB_ERR_CUDA;
+  if (n_done < 64) { done[n_done].kernel = kernel; done[n_done].dev = dev; ++n_done; }
   return FB_OK;
 }
 

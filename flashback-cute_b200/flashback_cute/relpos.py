@@ -446,8 +446,9 @@ def flashback_attn_relpos_func(
 ) -> torch.Tensor:
     """Softmax attention with a learned relative position bias: q (b, sq, hq, d), k/v (b, sk, hkv, d), bias_table
     (num_buckets, hq) of the same dtype (bfloat16, float16 or float32; float32 runs on CUDA cores). bidirectional: whether
-    keys behind their query have buckets of their own; by default unless `causal`. Differentiable once, in q, k, v and
-    bias_table."""
+    keys behind their query have buckets of their own; by default unless `causal`. An entry of -inf, or at or below -2^100 (the
+    lowest bfloat16 or float32 value), hides its pairs; a row that sees nothing gives zeros. Differentiable once, in q, k, v
+    and bias_table (a second derivative raises)."""
     return _attention(q, k, v, bias_table, None, None, None, None, max_distance, softmax_scale, causal, bidirectional)
 
 

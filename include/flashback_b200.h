@@ -305,8 +305,9 @@ typedef struct {
   const int32_t* starts;  /* HOST, see above */
 } fb_relpos;
 
-/* Forward: O and, where asked for, LSE and what rounding O to 16 bits left out (out_low = O - round(O), rounded itself; 16-bit
- * types only): the backward forms rowsum(dO * O) from both. `prob` as for fb_jvp_fwd, without row segments. */
+/* Forward: O and, where asked for, LSE and what rounding O to the dtype left out (out_low = O - round(O), rounded itself):
+ * the backward forms rowsum(dO * O) from both. `prob` as for fb_jvp_fwd, without row segments; total_k > 0. A table entry
+ * at or below -2^100 hides its pairs like -inf. */
 typedef struct {
   fb_problem prob;
   fb_relpos bias;
@@ -318,14 +319,14 @@ typedef struct {
 
 int fb_relpos_fwd(const fb_relpos_fwd_args* args, fb_stream_t stream);
 
-/* First-order backward. dq, dk, dv and dtable (problem dtype, the table's shape) are optional outputs. `workspace`
+/* First-order backward (total_q, total_k > 0). dq, dk, dv and dtable (problem dtype, the table's shape) are optional outputs. `workspace`
  * (fb_relpos_workspace_bytes, 16-byte aligned, contents irrelevant before and after) holds D = rowsum(dO * (out + out_low)) and the
  * query tiles' partial table gradients. Sums are formed in a fixed order: results are deterministic. */
 typedef struct {
   fb_problem prob;
   fb_relpos bias;
   fb_tensor q, k, v, out, dout; /* in */
-  fb_tensor out_low;       /* in, optional (16-bit types) */
+  fb_tensor out_low;       /* in, optional */
   const float* lse;        /* in */
   fb_tensor dq, dk, dv;    /* out, optional */
   void* dtable;            /* out, optional */

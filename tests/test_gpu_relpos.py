@@ -113,6 +113,67 @@ def test_entries_that_hide_or_that_nobody_points_at(dtype):
     _check(dtype, 64, hq, 1, True, None, None, None, two=False, far=128, table=table, packed=([7, 1, 12, 3], [7, 1, 12, 3]))
 
 
+def test_lowest_values_hide():
+    """The lowest bfloat16 / float32 value hides like -inf, also where a row sees nothing else; the lowest float16 value is a number."""
+    for dtype in (BF16, F32):
+        table = _mk((32, 2), dtype, 3)
+        table[0, 0] = torch.finfo(dtype).min
+        table[7, 1] = torch.finfo(dtype).min
+        hidden = table.clone()
+        hidden[0, 0] = hidden[7, 1] = -float("inf")
+        q, k, v, do = (_mk((1, 150, 2, 64), dtype, i) for i in range(4))
+        res = []
+        for t in (table, hidden):
+            leaves = [x.clone().requires_grad_() for x in (q, k, v, t)]
+            out = flashback_attn_relpos_func(*leaves, causal=True)
+            res.append((out.detach(), *torch.autograd.grad(out, leaves, do)))
+        assert all(torch.equal(a, b) for a, b in zip(*res)) and (res[0][0][:, 0, 0] == 0).all()
+    table = _mk((32, 2), F16, 3)
+    table[9] = torch.finfo(F16).min
+    _check(F16, 64, 2, 1, False, 1, 150, 150, table=table)
+
+
+@pytest.mark.parametrize("scale", [-0.2, 0.0, 1.5])
+def test_scales(scale):
+    """Negative, zero and large scales (the row maximum follows the bias and the scaled scores)."""
+    q, k, v, do = (_mk((2, 190, 2, 64), BF16, i) for i in range(4))
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, _mk((32, 2), BF16, 8))]
+    for causal in (False, True):
+        out = flashback_attn_relpos_func(*leaves, softmax_scale=scale, causal=causal)
+        grads = torch.autograd.grad(out, leaves, do)
+        ref = orc.attention(q, k, v, leaves[3], 128, not causal, scale, causal, do)
+        for name, got, want, tol in zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(), *grads), ref[:5], ref.tol):
+            _within(name, got, want, tol)
+
+
+def test_broadcast_inputs():
+    """One set of keys for every batch entry, one column for every head: gradients are summed by what expanded them."""
+    q, k, v, do = _mk((3, 100, 4, 64), BF16, 0), _mk((1, 100, 2, 64), BF16, 1), _mk((1, 100, 2, 64), BF16, 2), _mk((3, 100, 4, 64), BF16, 3)
+    column = _mk((32, 1), BF16, 4)
+    leaves = [t.clone().requires_grad_() for t in (q, k, v, column)]
+    out = flashback_attn_relpos_func(leaves[0], leaves[1].expand(3, -1, -1, -1), leaves[2].expand(3, -1, -1, -1), leaves[3].expand(-1, 4))
+    grads = torch.autograd.grad(out, leaves, do)
+    ref = orc.attention(q, k.expand(3, -1, -1, -1), v.expand(3, -1, -1, -1), column.expand(-1, 4), 128, True, 0.125, False, do)
+    sums = [ref.dq, ref.dk.sum(0, True), ref.dv.sum(0, True), ref.dt.sum(1, True)]
+    tols = [ref.tol[1], ref.tol[2].sum(0, True), ref.tol[3].sum(0, True), ref.tol[4].sum(1, True)]
+    for name, got, want, tol in zip(("dq", "dk", "dv", "dcolumn"), grads, sums, tols):
+        _within(name, got, want, tol * 1.01 + 3 * torch.finfo(BF16).eps / 2 * want.abs())  # torch adds the parts in bfloat16 steps
+
+
+def test_cuda_core_kernels_agree():
+    """The CUDA-core kernels on 16-bit inputs (FB_FLAG_FORCE_SIMT), a second implementation, within the same bounds."""
+    flags, _lib.DEFAULT_FLAGS = _lib.DEFAULT_FLAGS, _lib.FB_FLAG_FORCE_SIMT
+    from flashback_cute import relpos
+
+    relpos._attn_plans.plans.clear()
+    try:
+        _check(BF16, 64, 4, 2, True, 1, 77, 90)
+        _check(F16, 128, 2, 1, False, None, None, None, packed=([33, 1, 50], [33, 4, 50]))
+    finally:
+        _lib.DEFAULT_FLAGS = flags
+        relpos._attn_plans.plans.clear()
+
+
 def test_strides_and_offsets():
     """Views: heads before rows, sliced heads, an offset into a larger tensor, a transposed table, a broadcast gradient."""
     b, s, hq, hkv, d = 2, 130, 4, 2, 64

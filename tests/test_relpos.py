@@ -117,6 +117,11 @@ def test_status_codes():
     assert fwd(out=_lib.FbTensor(None, 0, 0)) == -1
     bwd = _lib.FbRelposBwdArgs(prob=_prob(), bias=_bias(), q=t, k=t, v=t, out=t, dout=t, lse=0x1000, dtable=0x1000)
     assert lib.fb_relpos_bwd(ctypes.byref(bwd), None) == -1  # no workspace
+    assert fwd(_prob(seqlen_k=0, total_k=0)) == -5
+    bwd.workspace, bwd.prob = 0x1000, _prob(seqlen_k=0, total_k=0)
+    assert lib.fb_relpos_bwd(ctypes.byref(bwd), None) == -5
+    bwd.workspace = 0x1008
+    assert lib.fb_relpos_bwd(ctypes.byref(bwd), None) == -6
     b = _lib.FbRelposBiasArgs(0, 2, 3, 4, _bias(), 0x1004)
     assert lib.fb_relpos_bias(ctypes.byref(b), None) == -6
     b = _lib.FbRelposBiasArgs(0, 2, 3, (1 << 30) + 1, _bias(), 0x1000)
@@ -141,6 +146,8 @@ def test_decode_status_codes():
     assert lib.fb_relpos_decode(None, None) == -1
     assert code(dtype=2) == -2 and code(head_dim=96) == -3 and code(heads_q=3) == -4 and code(seqlen_q=-1) == -5
     assert code(batch=70000) == -10 and code(seqlen_q=1 << 20) == -10
+    assert code(heads_q=256, heads_kv=2, bias=_bias(num=100, starts=tuple(range(1, 100)))) == -10  # 128 x 100 table entries per kv head
+    assert code(heads_q=40000, heads_kv=40000, seqlen_q=20) == -10
     assert code(bias=_bias(num=1)) == -12
     assert code(k=_lib.FbCache(0x1008, 1024, 128, 64)) == -6 and code(v=_lib.FbCache(0x1000, 1024, 100, 64)) == -6
     assert code(out=None) == -1 and code(out=0x1004) == -6
