@@ -18,18 +18,19 @@ constexpr int kWarps = kThreads / 32;
 // (aligned in the flat tensor, since rows of odd length start anywhere; the ends of a row go out one by one). The stretch of a row
 // starts at any element: one copy of the values per element of a 16-byte unit, each shifted by one more, gives every
 // row 16-byte loads too. (One copy and an element at a time was bound by shared memory: 168 us for 16 x 4095 x 4099 bf16.)
-constexpr int kRows = 64, kCols = 2048;
+// The columns are split evenly into stretches of at most kCols.
+constexpr int kRows = 128, kCols = 2304;
 
 template <typename T>
-__global__ void __launch_bounds__(kThreads) relpos_fill_kernel(const __grid_constant__ RelPos rel, int sq, int sk, T* __restrict__ out) {
+__global__ void __launch_bounds__(kThreads) relpos_fill_kernel(const __grid_constant__ RelPos rel, int sq, int sk, int rows_per_cta, int cols_per_cta, T* __restrict__ out) {
   constexpr int VEC = 16 / sizeof(T);
   constexpr int LEN = kRows + kCols + VEC;  // entries per copy, whole units
   extern __shared__ __align__(16) uint8_t smem[];
   T* const val = reinterpret_cast<T*>(smem);  // [VEC][LEN]: copy k, entry u = value u + k
   __shared__ T tab[FB_RELPOS_MAX_BUCKETS];
   __shared__ RelBuckets buckets;
-  const int h = blockIdx.z, i0 = blockIdx.y * kRows, j0 = blockIdx.x * kCols;
-  const int rows = min(kRows, sq - i0), cols = min(kCols, sk - j0);
+  const int h = blockIdx.z, i0 = blockIdx.y * rows_per_cta, j0 = blockIdx.x * cols_per_cta;
+  const int rows = min(rows_per_cta, sq - i0), cols = min(cols_per_cta, sk - j0);
   for (int t = threadIdx.x; t < rel.nb; t += kThreads) tab[t] = reinterpret_cast<const T*>(rel.table)[t * rel.bucket_stride + h * rel.head_stride];
   relpos_load_buckets(buckets, rel, threadIdx.x, kThreads);
   __syncthreads();
@@ -79,18 +80,20 @@ __global__ void __launch_bounds__(kThreads) relpos_fill_kernel(const __grid_cons
 // the warps, and a thread adds up VEC neighbouring diagonals in registers over its rows with 16-byte loads: no
 // atomics, no reordering, every element read once. At the end the CTA adds up its warps' diagonals, then those of
 // each bucket (neighbours), and leaves one number per bucket in the workspace.
-// PER vectors per lane: long stretches of a row per warp where the problem is large, more CTAs where it is small.
+// A warp reads one 16-byte vector per lane and row, 512 bytes of it; 4 rows in flight, 256 rows per CTA. Measured on 16 x 4095 x 4099 bf16
+// (537 MB): 140 us; 8 rows in flight 153; 512 / 1024 rows per CTA 178 / 196; 1 KB of a row per warp 158, 2 KB 222. Many small
+// CTAs that read one region of the tensor at a time beat fewer, longer ones.
 
 template <typename T> struct Vec;
 template <> struct Vec<__nv_bfloat16> { static constexpr int n = 8; };
 template <> struct Vec<__half> { static constexpr int n = 8; };
 template <> struct Vec<float> { static constexpr int n = 4; };
 
-template <typename T, int PER>
+template <typename T>
 __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_constant__ RelPos rel, int sq, int sk, int rows_per_cta, const T* __restrict__ grad) {
   constexpr int VEC = Vec<T>::n;
-  constexpr int kSpan = 32 * VEC * PER;  // diagonals per CTA
-  constexpr int kBatch = 8 / PER;        // rows of a warp in flight
+  constexpr int kSpan = 32 * VEC;  // diagonals per CTA
+  constexpr int kBatch = 4;        // rows of a warp in flight
   __shared__ float part[kWarps][kSpan + VEC];
   __shared__ float acc[FB_RELPOS_MAX_BUCKETS];
   __shared__ RelBuckets buckets;
@@ -116,64 +119,54 @@ __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_cons
   const int first = i_lo + warp;
   // vectors start where (g_at + i * (sk + 1) + c - (sq - 1)) is a multiple of VEC: diagonal c0 - shift + VEC * k
   const int shift = (int)(((g_at + (int64_t)first * (sk + 1) + c0 - (sq - 1)) % VEC + VEC) % VEC);
-  float sum[PER][VEC];
+  float sum[VEC], tail[VEC];
 #pragma unroll
-  for (int q = 0; q < PER; ++q)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) sum[q][e] = 0.f;
+  for (int e = 0; e < VEC; ++e) sum[e] = tail[e] = 0.f;
   // One residue needs kSpan + VEC diagonals when shift > 0: the first `shift` of its first vector belong to the CTA before
   // and are masked, the last vector's are masked by the next; so the span of a warp is [c0 - shift, c0 - shift + kSpan)
   // plus one more vector, which lane 0 takes.
-  float tail[VEC];
-#pragma unroll
-  for (int e = 0; e < VEC; ++e) tail[e] = 0.f;
 
-  auto add = [&](float (&s)[VEC], int i, int c) {  // the vector that starts at diagonal c of row i
-    const int j = c - (sq - 1) + i;
-    if (j >= 0 && j + VEC <= sk) {
-      const uint4 u = *reinterpret_cast<const uint4*>(g + (int64_t)i * sk + j);
-      const T* v = reinterpret_cast<const T*>(&u);
+  // a vector in row i whose first column is j and that an end of the row cuts; where both do, the first call takes it
+  auto cut = [&](float (&s)[VEC], int i, int j, int end) {
+    if (end == 1 && j < 0) return;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) s[e] += to_f<T>(v[e]);
-    } else if (j + VEC > 0 && j < sk) {
+    for (int e = 0; e < VEC; ++e)
+      if (j + e >= 0 && j + e < sk) s[e] += to_f<T>(g[(int64_t)i * sk + j + e]);
+  };
+  // Vectors that lie inside [0, sk) altogether, kBatch rows' in flight together (predicated, no branches between the loads)
+  const int lo = c0 - shift - (sq - 1) + lane * VEC;  // this lane's first column, in row 0
+  for (int i = first; i < i_hi; i += kBatch * kWarps) {
+    uint4 u[kBatch];
 #pragma unroll
-      for (int e = 0; e < VEC; ++e)
-        if (j + e >= 0 && j + e < sk) s[e] += to_f<T>(g[(int64_t)i * sk + j + e]);
+    for (int b = 0; b < kBatch; ++b) {
+      const int row = i + b * kWarps, j = lo + row;
+      u[b] = make_uint4(0, 0, 0, 0);
+      if (row < i_hi && j >= 0 && j + VEC <= sk) u[b] = *reinterpret_cast<const uint4*>(g + (int64_t)row * sk + j);
     }
-  };
-  auto edge = [&](int i) {
 #pragma unroll
-    for (int q = 0; q < PER; ++q) add(sum[q], i, c0 - shift + (q * 32 + lane) * VEC);
-  };
-  // Rows in which all of the warp's vectors lie inside [0, sk): unconditional loads, kBatch rows' in flight together. The few
-  // rows before and behind them are checked vector by vector.
-  const int lo = c0 - shift - (sq - 1);  // column of the first vector in row 0
-  const int in_lo = -lo, in_hi = sk - kSpan - lo;  // interior rows [in_lo, in_hi]
-  int i = first;
-  for (; i < i_hi && i < in_lo; i += kWarps) edge(i);
-  for (; i + (kBatch - 1) * kWarps < i_hi && i + (kBatch - 1) * kWarps <= in_hi; i += kBatch * kWarps) {
-    uint4 u[kBatch][PER];
+    for (int b = 0; b < kBatch; ++b) {
+      const T* v = reinterpret_cast<const T*>(&u[b]);
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-      for (int q = 0; q < PER; ++q)
-        u[b][q] = *reinterpret_cast<const uint4*>(g + (int64_t)(i + b * kWarps) * sk + (lo + i + b * kWarps + (q * 32 + lane) * VEC));
-#pragma unroll
-    for (int b = 0; b < kBatch; ++b)
-#pragma unroll
-      for (int q = 0; q < PER; ++q) {
-        const T* v = reinterpret_cast<const T*>(&u[b][q]);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) sum[q][e] += to_f<T>(v[e]);
-      }
+      for (int e = 0; e < VEC; ++e) sum[e] += to_f<T>(v[e]);
+    }
   }
-  for (; i < i_hi; i += kWarps) edge(i);
+  // ... and those that an end of their row cuts: the column moves by kWarps per row of this warp, so that happens at most once per end
+  static_assert(kWarps >= VEC, "a vector is cut in one row per end at most");
+#pragma unroll
+  for (int end = 0; end < 2; ++end) {
+    // the row whose column lies in (edge - VEC, edge)
+    const int edge = end ? sk : 0, ahead = edge - 1 - (lo + first), k = ahead / kWarps;
+    const int row = first + k * kWarps, at = lo + row;
+    if (ahead >= 0 && row < i_hi && at > edge - VEC && (at < 0 || at + VEC > sk)) cut(sum, row, at, end);
+  }
   if (shift > 0 && lane == 0)
-    for (i = first; i < i_hi; i += kWarps) add(tail, i, c0 - shift + kSpan);
+    for (int i = first; i < i_hi; i += kWarps) {
+      const int j = lo + kSpan + i;
+      for (int e = 0; e < VEC; ++e)
+        if (j + e >= 0 && j + e < sk && e < shift) tail[e] += to_f<T>(g[(int64_t)i * sk + j + e]);
+    }
 #pragma unroll
-  for (int q = 0; q < PER; ++q)
-#pragma unroll
-    for (int e = 0; e < VEC; ++e) part[warp][(q * 32 + lane) * VEC + e] = sum[q][e];
+  for (int e = 0; e < VEC; ++e) part[warp][lane * VEC + e] = sum[e];
   if (lane == 0) {
 #pragma unroll
     for (int e = 0; e < VEC; ++e) part[warp][kSpan + e] = tail[e];
@@ -182,20 +175,19 @@ __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_cons
   if (lane == 0) shifts[warp] = shift;
   __syncthreads();
   // diagonal c0 + t, the warps' sums in a fixed order; then the diagonals of a bucket, warp by warp
-  for (int t0 = 0; t0 < kSpan; t0 += kThreads) {
-    const int t = t0 + threadIdx.x, c = c0 + t;
-    float s = 0.f;
-    int bucket = -1;
-    if (t < kSpan) {
+  const int t = threadIdx.x, c = c0 + t;
+  float s = 0.f;
+  int bucket = -1;
+  if (t < kSpan) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) s += part[w][shifts[w] + t];
-      if (c < ndiag) bucket = RelFn(rel, buckets)(c - (sq - 1) - (sk - sq));
-    }
-    const bool run = run_sum(s, bucket, lane);
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp && run && bucket >= 0) acc[bucket] += s;
-      __syncthreads();
-    }
+    for (int w = 0; w < kWarps; ++w) s += part[w][shifts[w] + t];
+    if (c < ndiag) bucket = RelFn(rel, buckets)(c - (sq - 1) - (sk - sq));
+  }
+  static_assert(kSpan <= kThreads, "a thread per diagonal");
+  const bool run = run_sum(s, bucket, lane);
+  for (int w = 0; w < kWarps; ++w) {
+    if (w == warp && run && bucket >= 0) acc[bucket] += s;
+    __syncthreads();
   }
   if ((int)threadIdx.x < rel.nb) out[threadIdx.x] = acc[threadIdx.x];
 }
@@ -215,7 +207,7 @@ __global__ void __launch_bounds__(kReduceThreads) relpos_reduce_kernel(const flo
   double s = 0.0;
   if (slice < slices) {
     const int rows = batch * ntiles;
-#pragma unroll 4
+#pragma unroll 8
     for (int r = slice; r < rows; r += slices) {
       const int b = r / ntiles, tile = r - b * ntiles;
       s += (double)part[((int64_t)(b * heads + h) * ntiles + tile) * nb + t];
@@ -231,11 +223,14 @@ __global__ void __launch_bounds__(kReduceThreads) relpos_reduce_kernel(const flo
 
 template <typename T>
 int fill_typed(const RelPos& rel, int heads, int sq, int sk, void* out, cudaStream_t s) {
-  const dim3 grid((sk + kCols - 1) / kCols, (sq + kRows - 1) / kRows, heads);
+  const int n = (sk + kCols - 1) / kCols, cols = ((sk + n - 1) / n + 7) / 8 * 8;
+  int rows = kRows;
+  while (rows > 16 && (int64_t)n * heads * ((sq + rows - 1) / rows) < 148 * 4) rows /= 2;  // small: more CTAs
+  const dim3 grid((sk + cols - 1) / cols, (sq + rows - 1) / rows, heads);
   if (grid.y > 65535 || grid.z > 65535) return FB_ERR_TOO_LARGE;
   constexpr int VEC = 16 / sizeof(T), smem = VEC * (kRows + kCols + VEC) * (int)sizeof(T);
   static_assert(smem <= 48 * 1024, "without an opt-in");
-  relpos_fill_kernel<T><<<grid, kThreads, smem, s>>>(rel, sq, sk, reinterpret_cast<T*>(out));
+  relpos_fill_kernel<T><<<grid, kThreads, smem, s>>>(rel, sq, sk, rows, cols, reinterpret_cast<T*>(out));
   return cudaGetLastError() == cudaSuccess ? 1 : FB_ERR_CUDA;
 }
 
@@ -245,18 +240,15 @@ int reduce_typed(const float* part, int batch, int heads, int ntiles, int nb, vo
   return cudaGetLastError() == cudaSuccess ? 1 : FB_ERR_CUDA;
 }
 
-// Shape of the gradient's CTAs: long stretches of rows spread the end of a CTA (its sums by bucket) over more reads, short ones
-// fill the GPU; wide spans read longer stretches of a row. The same rule sizes the workspace.
+// Shape of the gradient's CTAs: 256 rows, fewer where the problem would not fill the GPU. The same rule sizes the workspace.
 struct GradShape {
-  int per, rows, spans, row_blocks;
+  int rows, spans, row_blocks;
 };
 GradShape grad_shape(int dtype, int heads, int sq, int sk) {
-  const int vec = dtype == FB_F32 ? 4 : 8;
   GradShape g;
-  g.per = (int64_t)heads * sq * sk >= (1 << 24) ? 2 : 1;
-  const int span = 32 * vec * g.per;
+  const int span = 32 * (dtype == FB_F32 ? 4 : 8);
   g.spans = (sq + sk - 1 + span - 1) / span;
-  g.rows = 512;
+  g.rows = 256;
   while (g.rows > 32 && (int64_t)g.spans * heads * ((sq + g.rows - 1) / g.rows) < 148 * 8) g.rows /= 2;
   g.row_blocks = (sq + g.rows - 1) / g.rows;
   return g;
@@ -267,8 +259,7 @@ int grad_typed(const RelPos& rel, const GradShape& g, int heads, int sq, int sk,
   const dim3 grid(g.spans, g.row_blocks, heads);
   if (grid.y > 65535 || grid.z > 65535) return FB_ERR_TOO_LARGE;
   const T* in = reinterpret_cast<const T*>(grad);
-  if (g.per == 2) relpos_grad_kernel<T, 2><<<grid, kThreads, 0, s>>>(rel, sq, sk, g.rows, in);
-  else relpos_grad_kernel<T, 1><<<grid, kThreads, 0, s>>>(rel, sq, sk, g.rows, in);
+  relpos_grad_kernel<T><<<grid, kThreads, 0, s>>>(rel, sq, sk, g.rows, in);
   return cudaGetLastError() == cudaSuccess ? 1 : FB_ERR_CUDA;
 }
 
