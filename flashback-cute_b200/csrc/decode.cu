@@ -12,6 +12,8 @@
 //     distributed shared memory, each a part of the rows. More slices (few sequences with long caches) go through a
 //     workspace and a second kernel. Fixed order either way.
 //
+// Measured: 48 sequences of up to 8192 keys, 32 / 8 heads of 128, bf16 (897 MB): 141 + 7 us, 6.0 TB/s, 92 % of the measured copy bandwidth.
+//
 // Far from the newest token all keys of a group share the last bucket and the bias is one number per row.
 #include "fb_params.h"
 #include "ptx_sm100.cuh"
