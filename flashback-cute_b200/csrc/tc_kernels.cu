@@ -210,8 +210,8 @@ enum {
   BAR_A_READY = 21,   // owner operands copied into TMEM
   BAR_S2_FULL = 22,   // 22 + phase: two-phase kernels, second tile of the pair (S_dot / dP_dot) complete
   BAR_P_HALF = 24,    // two-phase kernels: dS written (dS_dot still to come)
-  BAR_TAIL = 25,      // BIAS: rows behind the sequence zeroed in a streamed group
-  BAR_COUNT = 26
+  BAR_TAIL = 25,      // 25 + s, BIAS: rows behind the sequence zeroed in stage s of group g1
+  BAR_COUNT = 28
 };
 
 template <typename T> __device__ __forceinline__ uint32_t pack2(float lo, float hi);
@@ -722,10 +722,15 @@ struct TcCta {
       if (prof) pr_is += clock64() - ts0;
     };
     // Output GEMMs of block `it`: A operands are the 16-bit tiles the pointwise warps left in TMEM.
-    [[maybe_unused]] int tails = 0;
+    [[maybe_unused]] uint32_t tails = 0;  // bit s: parity of the next tail in stage s
     auto issue_out = [&](int it) {
       if constexpr (BIAS) {
-        if (is_tail(it)) live = wait1(BAR_TAIL, tails++ & 1) && live;
+        // One barrier per stage: a stage's next tail is zeroed after the stage was refilled, that is after this wait. (On a single
+        // barrier the zeroing warp may run two phases ahead, one short block per query head, and the wait never ends.)
+        if (is_tail(it)) {
+          live = wait1(BAR_TAIL + it % SS1, (tails >> (it % SS1)) & 1) && live;
+          tails ^= 1u << (it % SS1);
+        }
       }
       const int s0 = it % SS0d, s1 = it % SS1, st = it % ST;
       const uint32_t o0 = (uint32_t)((s0 * C::g0Bytes) >> 4), o1 = (uint32_t)((s1 * C::g1Bytes) >> 4);
@@ -937,7 +942,7 @@ struct TcCta {
   // Called by the statistics warp at block `it`, when block it - 2 has been released: the stage's previous phase (block it - 3) is over,
   // so the parity is that of this block.
   __device__ __forceinline__ void zero_tail(int it) {
-    static_assert(SS1 >= 3, "the parity of the stage's phase");
+    static_assert(SS1 == 3, "the parity of the stage's phase; three tail barriers");
     const int first = stream_len() % BN, s = it % SS1;
     warp_wait(BAR_FULL + 3 + s, (it / SS1) & 1);
     if (aborted()) return;
@@ -948,7 +953,7 @@ struct TcCta {
       }
     fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) mbar_arrive(bar(BAR_TAIL));
+    if (lane == 0) mbar_arrive(bar(BAR_TAIL + s));
   }
   // BIAS, KIND_DQ: D = rowsum(dO * O) of the tile's rows, where O = its 16 bits + what their rounding left out. dO comes from the owner tile, O from global memory (under the first GEMMs): D / 8 lanes read a row, so that
   // a load covers whole rows, and all of a warp's loads are in flight together. The dK/dV kernel reads D from memory.

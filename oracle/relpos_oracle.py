@@ -14,6 +14,8 @@ also what D is computed from).
     D                       dD = u rowsum(|dO| |O|) + (1 + u) (rowsum(|dO| (u + ep + n e) P|V|) + d e |dO| |O|)
     dS                      ds = |dS| ep + P (dD + d e |dO|.|V| )
     dQ                      c (ds + (u + n e) |dS|) |K| + u |dQ|;  dK, dV, dT alike (dT has no operand rounding)
+float16 operands (P, dS) below 2^-14 are subnormal: their rounding is off by up to half a step of 2^-24, an absolute w = 2^-25 beside
+the relative u. It adds w rowsum(|V|) to O, c w rowsum(|K|) to dQ, and so on; 0 for the other types, whose range is float32's.
 """
 
 from __future__ import annotations
@@ -57,7 +59,7 @@ class Head(NamedTuple):
     tol_dt: Optional[torch.Tensor]
 
 
-def head(q, k, v, table, which, scale, causal, u, dout=None) -> Head:
+def head(q, k, v, table, which, scale, causal, u, dout=None, w=0.0) -> Head:
     """q (sq, d), k/v (sk, d), table (num,), which (sq, sk) long; everything float64 on one device."""
     e = 2.0 ** -24
     sq, sk, d = q.shape[0], k.shape[0], q.shape[1]
@@ -75,7 +77,8 @@ def head(q, k, v, table, which, scale, causal, u, dout=None) -> Head:
     es = (d + 8) * e * mag
     ep = (2 * es.amax(-1, keepdim=True) + 16 * e) if sk else torch.zeros(sq, 1, dtype=q.dtype, device=q.device)
     pv = p @ v.abs()
-    tol_out = (u + ep + sk * e) * pv + u * out.abs() * (1 + 2 * u)
+    seen = (p > 0).to(q.dtype)
+    tol_out = (u + ep + sk * e) * pv + w * (seen @ v.abs()) + u * out.abs() * (1 + 2 * u)
     if dout is None:
         return Head(out, None, None, None, None, tol_out, None, None, None, None)
     g = dout
@@ -84,12 +87,12 @@ def head(q, k, v, table, which, scale, causal, u, dout=None) -> Head:
     ds = p * (dp - dd)
     err_d = ((g.abs() * tol_out).sum(-1, keepdim=True)) + d * e * (g.abs() * out.abs()).sum(-1, keepdim=True) * (1 + u)
     err_s = ds.abs() * ep * (1 + ep) + p * (err_d + d * e * (g.abs() @ v.abs().T) + 2 * e * (dp.abs() + dd.abs())) * (1 + ep)
-    op = err_s + (u + 4 * e) * (ds.abs() + err_s)  # dS as an operand
+    op = err_s + (u + 4 * e) * (ds.abs() + err_s) + w * seen  # dS as an operand
     dq, dk, dv = scale * ds @ k, scale * ds.T @ q, p.T @ g
     c = abs(scale)
     tol_dq = c * (op + sk * e * ds.abs()) @ k.abs() * (1 + u) + (u + 2 * e) * dq.abs()
     tol_dk = c * (op + sq * e * ds.abs()).T @ q.abs() * (1 + u) + (u + 2 * e) * dk.abs()
-    tol_dv = (p * (ep + u + sq * e)).T @ g.abs() * (1 + u) + u * dv.abs()
+    tol_dv = (p * (ep + u + sq * e) + w * seen).T @ g.abs() * (1 + u) + u * dv.abs()
     num = table.shape[0]
     # the table's gradient: float32 sums over a warp's diagonals, a tile, then in 64 bits over the tiles; at most sk + 256 summands in a row
     dt = torch.zeros(num, dtype=q.dtype, device=q.device).index_add_(0, which.flatten(), ds.flatten())
@@ -110,8 +113,9 @@ def attention(q, k, v, table, far, two, scale, causal, dout=None, lens_q=None, l
     """Dense (b, s, h, d), or packed (total, h, d) with lens_q, lens_k; inputs of any type, results float64."""
     u = torch.finfo(q.dtype).eps / 2
     packed = q.dim() == 3
-    w = lambda t: None if t is None else t.detach().double()  # noqa: E731
-    q, k, v, table, dout = map(w, (q, k, v, table, dout))
+    w = 2.0 ** -25 if q.dtype == torch.float16 else 0.0
+    wide = lambda t: None if t is None else t.detach().double()  # noqa: E731
+    q, k, v, table, dout = map(wide, (q, k, v, table, dout))
     shape_q, shape_k = q.shape, k.shape
     if not packed:
         lens_q, lens_k = [q.shape[1]] * q.shape[0], [k.shape[1]] * k.shape[0]
@@ -128,7 +132,7 @@ def attention(q, k, v, table, far, two, scale, causal, dout=None, lens_q=None, l
         sl, kl = slice(iq, iq + nq), slice(ik, ik + nk)
         for h in range(q.shape[1]):
             hk = h // group
-            r = head(q[sl, h], k[kl, hk], v[kl, hk], table[:, h], which, scale, causal, u, None if dout is None else dout[sl, h])
+            r = head(q[sl, h], k[kl, hk], v[kl, hk], table[:, h], which, scale, causal, u, None if dout is None else dout[sl, h], w)
             out[sl, h], tol_out[sl, h] = r.out, r.tol_out
             if dout is not None:
                 dq[sl, h], tol_dq[sl, h] = r.dq, r.tol_dq

@@ -284,6 +284,15 @@ def test_rows_behind_the_last_sequence_may_hold_anything(dtype):
             _within(name, got[:want.shape[0]], want, tol)
 
 
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F16, 64)])
+def test_every_streamed_block_is_a_tail(dtype, d):
+    """Short queries under many heads: the dK/dV kernel meets the end of the sequence in every block it streams."""
+    for hq, sq, sk, causal in ((8, 52, 15, True), (16, 1, 200, False), (12, 33, 70, True), (16, 63, 300, False)):
+        for seed in range(3):
+            _check(dtype, d, hq, 1, causal, 2, sq, sk, 64, 91, False, seed)
+    _check(dtype, d, 8, 1, True, None, None, None, packed=([5, 60, 1, 33, 100], [5, 60, 1, 33, 100]))
+
+
 def test_a_broken_sequence_leaves_the_others_alone():
     """NaN in one sequence of a packed batch: the sequences before and behind it are what they are without it."""
     lens = [100, 70, 90]
