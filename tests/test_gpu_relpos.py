@@ -311,6 +311,94 @@ def test_a_broken_sequence_leaves_the_others_alone():
         assert torch.equal(a[:100], b[:100]) and torch.equal(a[170:], b[170:])
 
 
+def _step(seed, d=64, s=300, causal=True):
+    from flashback_cute import flashback_attn_relpos_decode
+
+    leaves = [_mk(x, BF16, seed + i).requires_grad_() for i, x in enumerate([(2, s, 4, d), (2, s, 2, d), (2, s, 2, d), (32, 4)])]
+    out = flashback_attn_relpos_func(*leaves, causal=causal)
+    grads = torch.autograd.grad(out, leaves, _mk((2, s, 4, d), BF16, seed + 5))
+    lens = torch.tensor([s, 17], dtype=torch.int32, device=DEV)
+    q, k, v, table = (t.detach() for t in leaves)
+    one = flashback_attn_relpos_decode(q[:, -1:], k, v, lens, table)
+    long_k = _mk((1, 20000, 2, d), BF16, seed + 6)
+    many = flashback_attn_relpos_decode(q[:1, -1:], long_k, long_k, None, table)
+    bias = flashback_relpos_bias(leaves[3], 200, 333)
+    return [out.detach(), *grads, one, many, bias.detach(), torch.autograd.grad(bias, leaves[3], _mk((4, 200, 333), BF16, seed + 7))[0]]
+
+
+def test_several_streams_at_once():
+    """The same work on four streams at once (CTAs of different kernels and calls share the SMs), against one after the other."""
+    want = [_step(10 * i, 128 if i % 2 else 64, 300 + 50 * i, i < 2) for i in range(4)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    for _ in range(3):
+        got = [None] * 4
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i] = _step(10 * i, 128 if i % 2 else 64, 300 + 50 * i, i < 2)
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_workspaces_may_hold_anything():
+    """Outputs and workspaces come from memory full of NaN: nothing is read before it is written, nothing is left unwritten."""
+    want = _step(3)
+    for _ in range(2):
+        torch.cuda.synchronize()
+        poison = [torch.full((n,), float("nan"), device=DEV) for n in (1 << 24, 1 << 20, 1 << 18, 1 << 16, 1 << 14, 1 << 12, 128, 64)]
+        poison += [torch.full((n,), float("nan"), device=DEV) for n in (1 << 20, 1 << 18, 1 << 16, 1 << 14, 1 << 12, 128, 64) for _ in range(8)]
+        del poison
+        assert all(torch.equal(a, b) for a, b in zip(_step(3), want))
+
+
+def test_several_threads_at_once():
+    """Calls from several host threads: plans, argument templates and the library's look-ups are shared between them."""
+    import concurrent.futures
+
+    want = [_step(7 * i, s=180 + i) for i in range(4)]
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            got = [_step(7 * i, s=180 + i) for _ in range(3)]
+            torch.cuda.current_stream().synchronize()
+        return got
+
+    with concurrent.futures.ThreadPoolExecutor(4) as pool:
+        for i, runs in enumerate(pool.map(work, range(4))):
+            for r in runs:
+                assert all(torch.equal(a, b) for a, b in zip(r, want[i]))
+
+
+def test_two_captured_graphs():
+    """Two graphs over the same buffers, replayed in turn and with eager calls between: each has workspaces of its own."""
+    bufs = [_mk(x, BF16, i) for i, x in enumerate([(2, 150, 4, 64), (2, 150, 2, 64), (2, 150, 2, 64), (32, 4), (2, 150, 4, 64)])]
+
+    def step(causal):
+        leaves = [t.detach().requires_grad_() for t in bufs[:4]]
+        out = flashback_attn_relpos_func(*leaves, causal=causal)
+        return (out.detach(), *torch.autograd.grad(out, leaves, bufs[4]))
+
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        step(True), step(False)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for causal in (True, False):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(step(causal))
+        graphs.append(g)
+    for round_ in range(3):
+        for i in range(5):
+            bufs[i].copy_(_mk(bufs[i].shape, BF16, 40 * round_ + i))
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for got, causal in zip(outs, (True, False)):
+            assert all(torch.equal(a, b) for a, b in zip(got, step(causal)))
+
+
 def test_under_torch_func():
     shapes = [(1, 70, 2, 64), (1, 70, 2, 64), (1, 70, 2, 64), (32, 2)]
     x = [_mk(s, BF16, i) for i, s in enumerate(shapes)]
