@@ -957,25 +957,35 @@ struct TcCta {
   }
   // BIAS, KIND_DQ: D = rowsum(dO * O) of the tile's rows, where O = its 16 bits + what their rounding left out. dO comes from the owner tile, O from global memory (under the first GEMMs): D / 8 lanes read a row, so that
   // a load covers whole rows, and all of a warp's loads are in flight together. The dK/dV kernel reads D from memory.
-  __device__ __forceinline__ void row_dot() {
-    float* dots = reinterpret_cast<float*>(rel_area + REL_ROWDOT);  // [BM]
-    constexpr int U = D / 8, RPI = 32 / U;                 // 16-byte units per row, rows per load
-    constexpr int kWarpRows = BM / (NWG * 4), NL = kWarpRows / RPI;
-    const int first = (warp & 7) * kWarpRows + lane / U, u = lane % U;
-    uint4 o[NL], l[NL];
+  static constexpr int kDotUnits = D / 8, kDotRows = 32 / kDotUnits;  // 16-byte units per row, rows per load
+  static constexpr int kDotLoads = BM / (NWG * 4) / kDotRows;
+  struct RowDot {
+    uint4 o[kDotLoads], l[kDotLoads];
+  };
+  __device__ __forceinline__ void row_dot_load(RowDot& x) const {  // ahead of the wait for the owner tiles
+    const int first = (warp & 7) * (BM / (NWG * 4)) + lane / kDotUnits, u = lane % kDotUnits;
+    uint4(&o)[kDotLoads] = x.o;
+    uint4(&l)[kDotLoads] = x.l;
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      const int r = first + j * RPI;
+    for (int j = 0; j < kDotLoads; ++j) {
+      const int r = first + j * kDotRows;
       o[j] = l[j] = make_uint4(0, 0, 0, 0);
       if (n_it > 0 && r0 + r < own_len) {
         o[j] = *reinterpret_cast<const uint4*>(row_ptr<T>(p.o, head, si.q0 + r0 + r) + u * 8);
         if (p.od.ptr) l[j] = *reinterpret_cast<const uint4*>(row_ptr<T>(p.od, head, si.q0 + r0 + r) + u * 8);
       }
     }
+  }
+  __device__ __forceinline__ void row_dot(const RowDot& x) {
+    float* dots = reinterpret_cast<float*>(rel_area + REL_ROWDOT);  // [BM]
+    constexpr int U = kDotUnits;
+    const int first = (warp & 7) * (BM / (NWG * 4)) + lane / U, u = lane % U;
+    const uint4(&o)[kDotLoads] = x.o;
+    const uint4(&l)[kDotLoads] = x.l;
     if (n_it > 0) warp_wait(BAR_OUTER, 0);
 #pragma unroll
-    for (int j = 0; j < NL; ++j) {
-      const int r = first + j * RPI;
+    for (int j = 0; j < kDotLoads; ++j) {
+      const int r = first + j * kDotRows;
       float d = 0.f;
       if (n_it > 0 && r0 + r < own_len) {
         const uint4 g = *reinterpret_cast<const uint4*>(smem + C::outerTile + (u >> 3) * (BM * 128) + r * 128 + (((u & 7) ^ (r & 7)) << 4));
@@ -1516,10 +1526,12 @@ struct TcCta {
       rel_cur = -1;
       rel_sum = make_float2(0.f, 0.f);
     }
+    [[maybe_unused]] RowDot row_dots;
+    if constexpr (BIAS && kDq) row_dot_load(row_dots);
     if constexpr (C::nATmem > 0) {
       if (n_it > 0) stage_a_operands();
     }
-    if constexpr (BIAS && kDq) row_dot();
+    if constexpr (BIAS && kDq) row_dot(row_dots);
     for (int it = 0; it < n_it; ++it) {
       const int st = it % ST;
       int blk;  // streamed block index within the sequence
