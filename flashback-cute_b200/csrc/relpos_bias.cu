@@ -135,29 +135,43 @@ __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_cons
   };
   // Vectors that lie inside [0, sk) altogether, kBatch rows' in flight together (predicated, no branches between the loads)
   const int lo = c0 - shift - (sq - 1) + lane * VEC;  // this lane's first column, in row 0
-  for (int i = first; i < i_hi; i += kBatch * kWarps) {
-    uint4 u[kBatch];
+  const int warp_lo = lo - lane * VEC;
+  const int64_t step = (int64_t)kWarps * (sk + 1);  // elements from a row's vector to that of the warp's next row
+  const T* at = g + (int64_t)first * sk + first + lo;
+  float2 sum2[VEC / 2];
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int row = i + b * kWarps, j = lo + row;
-      u[b] = make_uint4(0, 0, 0, 0);
-      if (row < i_hi && j >= 0 && j + VEC <= sk) u[b] = *reinterpret_cast<const uint4*>(g + (int64_t)row * sk + j);
+  for (int e = 0; e < VEC / 2; ++e) sum2[e] = make_float2(0.f, 0.f);
+  for (int i = first; i < i_hi; i += kBatch * kWarps, at += kBatch * step) {
+    const int last = i + (kBatch - 1) * kWarps;
+    uint4 u[kBatch];
+    if (last < i_hi && warp_lo + i >= 0 && warp_lo + kSpan + last <= sk) {  // every lane's vectors of these rows
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) u[b] = *reinterpret_cast<const uint4*>(at + b * step);
+    } else {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int row = i + b * kWarps, j = lo + row;
+        u[b] = make_uint4(0, 0, 0, 0);
+        if (row < i_hi && j >= 0 && j + VEC <= sk) u[b] = *reinterpret_cast<const uint4*>(at + b * step);
+      }
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const T* v = reinterpret_cast<const T*>(&u[b]);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) sum[e] += to_f<T>(v[e]);
+      for (int e = 0; e < VEC / 2; ++e) sum2[e] = __fadd2_rn(sum2[e], make_float2(to_f<T>(v[2 * e]), to_f<T>(v[2 * e + 1])));
     }
   }
+#pragma unroll
+  for (int e = 0; e < VEC / 2; ++e) { sum[2 * e] = sum2[e].x; sum[2 * e + 1] = sum2[e].y; }
   // ... and those that an end of their row cuts: the column moves by kWarps per row of this warp, so that happens at most once per end
   static_assert(kWarps >= VEC, "a vector is cut in one row per end at most");
 #pragma unroll
   for (int end = 0; end < 2; ++end) {
     // the row whose column lies in (edge - VEC, edge)
     const int edge = end ? sk : 0, ahead = edge - 1 - (lo + first), k = ahead / kWarps;
-    const int row = first + k * kWarps, at = lo + row;
-    if (ahead >= 0 && row < i_hi && at > edge - VEC && (at < 0 || at + VEC > sk)) cut(sum, row, at, end);
+    const int row = first + k * kWarps, col = lo + row;
+    if (ahead >= 0 && row < i_hi && col > edge - VEC && (col < 0 || col + VEC > sk)) cut(sum, row, col, end);
   }
   if (shift > 0 && lane == 0)
     for (int i = first; i < i_hi; i += kWarps) {
