@@ -153,7 +153,6 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
   const float* row_tab[MT][2];
   float far_bias[MT][2], m[MT][2], l[MT][2];
   float o[MT][D / 8][4];
-  int pos_min = INT32_MAX;
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
 #pragma unroll
@@ -171,7 +170,7 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[mt][n][e] = 0.f;
   }
-  pos_min = len - p.Sq + (rt * R) / p.G;  // the earliest row of the CTA
+  const int pos_min = len - p.Sq + (rt * R) / p.G;  // the earliest row of the CTA
 
   // the query fragments stay in registers unless the accumulators need them
   constexpr bool kQRegs = MT * D <= 128;
@@ -218,25 +217,25 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
     const bool all_far = pos_min - (j0 + KG - 1) >= bucket_of.far && j0 + KG <= k1;
     float mx[MT][2];
     auto add_bias = [&](auto which) {
-    constexpr int mode = decltype(which)::value;  // 0: one bucket per row, 1: by the byte table, 2: with a search
+      constexpr int mode = decltype(which)::value;  // 0: one bucket per row, 1: by the byte table, 2: with a search
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      mx[mt][0] = mx[mt][1] = -INFINITY;
+      for (int mt = 0; mt < MT; ++mt) {
+        mx[mt][0] = mx[mt][1] = -INFINITY;
 #pragma unroll
-      for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < 2; ++n)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int x = e >> 1, j = j0 + 8 * n + 2 * (lane & 3) + (e & 1);
-          float bias = far_bias[mt][x];
-          if (mode != 0) {
-            const int r = j - pos[mt][x];
-            bias = row_tab[mt][x][mode == 1 ? bucket_of.near(min(r, 0)) : bucket_of(min(r, 0))];
-            if (r > 0 || j >= k1) bias = -INFINITY;
+          for (int e = 0; e < 4; ++e) {
+            const int x = e >> 1, j = j0 + 8 * n + 2 * (lane & 3) + (e & 1);
+            float bias = far_bias[mt][x];
+            if (mode != 0) {
+              const int r = j - pos[mt][x];
+              bias = row_tab[mt][x][mode == 1 ? bucket_of.near(min(r, 0)) : bucket_of(min(r, 0))];
+              if (r > 0 || j >= k1) bias = -INFINITY;
+            }
+            s[mt][n][e] = fmaf(s[mt][n][e], scale2, bias);
+            mx[mt][x] = fmaxf(mx[mt][x], s[mt][n][e]);
           }
-          s[mt][n][e] = fmaf(s[mt][n][e], scale2, bias);
-          mx[mt][x] = fmaxf(mx[mt][x], s[mt][n][e]);
-        }
-    }
+      }
     };
     if (all_far) add_bias(std::integral_constant<int, 0>{});
     else if (bucket_of.byte_table()) add_bias(std::integral_constant<int, 1>{});

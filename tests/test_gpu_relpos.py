@@ -588,3 +588,56 @@ def test_decode_empty():
     q, k, table = _mk((2, 1, 4, 64), BF16, 0), _mk((2, 0, 4, 64), BF16, 1), _mk((32, 4), BF16, 3)
     assert torch.equal(flashback_attn_relpos_decode(q, k, k, None, table), torch.zeros_like(q))
     assert flashback_attn_relpos_decode(q[:0], _mk((0, 5, 4, 64), BF16, 1), _mk((0, 5, 4, 64), BF16, 1), None, table).shape == (0, 1, 4, 64)
+
+
+# ---------------------------------------------------------------------------------------------
+# offsets that pass 32 bits, long rows
+# ---------------------------------------------------------------------------------------------
+def test_decode_offsets_beyond_32_bits():
+    """A cache of more than 2^31 elements; the last kv head of the last rows against the oracle's formula."""
+    from flashback_cute import flashback_attn_relpos_decode
+
+    s, hkv, d = 1_060_000, 16, 128
+    assert s * hkv * d > 2 ** 31
+    k, v = (torch.empty(1, s, hkv, d, dtype=BF16, device=DEV).normal_() for _ in range(2))
+    q, table = _mk((1, 1, hkv, d), BF16, 0), _mk((32, hkv), BF16, 1)
+    got = flashback_attn_relpos_decode(q, k, v, None, table)
+    which = torch.full((1, s), 31, device=DEV)
+    which[0, -200:] = orc.buckets(1, 200, 32, 128, False)[0].to(DEV)
+    for h in (0, hkv - 1):
+        w = lambda t: t[0, :, h].double()  # noqa: E731
+        r = orc.head(w(q), w(k), w(v), table[:, h].double(), which, d ** -0.5, True, 2.0 ** -8)
+        _within("out", got[0, :, h], r.out, r.tol_out)
+
+
+def test_bias_tensor_offsets_beyond_32_bits():
+    n, heads = 16_411, 8
+    assert n * n * heads > 2 ** 31
+    table = _mk((32, heads), BF16, 0).requires_grad_()
+    bias = flashback_relpos_bias(table, n, n, bidirectional=False)
+    row = orc.buckets(1, n, 32, 128, False)[0].to(DEV)  # the last query's
+    assert torch.equal(bias[heads - 1, -1].detach(), table.detach()[:, heads - 1][row])
+    grad = torch.zeros_like(bias)
+    grad[heads - 1, -1] = 1
+    got = torch.autograd.grad(bias, table, grad)[0]
+    want = torch.zeros(32, heads, device=DEV)
+    want[:, heads - 1] = torch.bincount(row, minlength=32).float()
+    assert torch.equal(got, want.to(BF16))
+
+
+def test_long_sequence():
+    """32768 keys: the last 256 queries' outputs and gradients, and the last keys' (no earlier query sees them)."""
+    s, n = 32768, 256
+    q, k, v, do = (_mk((1, s, 1, 64), BF16, i) for i in range(4))
+    do[:, :-n] = 0  # then only these queries have gradients
+    leaves = [t.requires_grad_() for t in (q, k, v, _mk((32, 1), BF16, 7))]
+    out = flashback_attn_relpos_func(*leaves, causal=True)
+    grads = torch.autograd.grad(out, leaves, do)
+    which = torch.full((n, s), 31, device=DEV)
+    which[:, -n - 200:] = orc.buckets(n, n + 200, 32, 128, False).to(DEV)
+    w = lambda t, m=s: t.detach()[0, -m:, 0].double()  # noqa: E731
+    r = orc.head(w(q, n), w(k), w(v), leaves[3].detach()[:, 0].double(), which, 0.125, True, 2.0 ** -8, w(do, n))
+    _within("out", out.detach()[0, -n:, 0], r.out, r.tol_out)
+    for name, got, want, tol in (("dq", grads[0][0, -n:, 0], r.dq, r.tol_dq), ("dk", grads[1][0, :, 0], r.dk, r.tol_dk), ("dv", grads[2][0, :, 0], r.dv, r.tol_dv),
+                                 ("dtable", grads[3][:, 0], r.dt, r.tol_dt + 2.0 ** -8 * (r.dt.abs() + r.tol_dt))):
+        _within(name, got, want, tol)
