@@ -523,6 +523,9 @@ def flashback_attn_relpos_decode(
     clamped to [0, s]). Causal: token t of sequence i sits at position cache_seqlens[i] - sq + t. Cache rows at or behind a
     sequence's length are not read. bfloat16 or float16; meant for one to a few tokens (every 16 or 32 (token, head) pairs of a kv head read the
     cache once). No autograd graph."""
+    if q.data_ptr() % 16:  # a copy in the standard layout, with the plan of that layout (a clone may have strides of its own)
+        with torch.no_grad():
+            q = _plain(q)
     key = (
         q.shape, k_cache.shape, v_cache.shape, bias_table.shape, q.stride(), k_cache.stride(), v_cache.stride(), bias_table.stride(),
         q.dtype, k_cache.dtype, v_cache.dtype, bias_table.dtype, q.device, k_cache.device, v_cache.device, bias_table.device,
@@ -538,9 +541,9 @@ def flashback_attn_relpos_decode(
         return out.zero_()
     if (k_cache.data_ptr() | v_cache.data_ptr()) % 16:
         raise ValueError("caches need 16-byte alignment")
-    with torch.no_grad():
-        if plan.copy_q or q.data_ptr() % 16:
-            q = _plain(q) if plan.copy_q else q.clone()
+    if plan.copy_q:
+        with torch.no_grad():
+            q = _plain(q)
     w, i = plan.words[:], _DW
     w[i["q"]], w[i["k"]], w[i["v"]], w[i["table"]], w[i["out"]] = q.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), bias_table.data_ptr(), out.data_ptr()
     if cache_seqlens is not None:

@@ -641,3 +641,19 @@ def test_long_sequence():
     for name, got, want, tol in (("dq", grads[0][0, -n:, 0], r.dq, r.tol_dq), ("dk", grads[1][0, :, 0], r.dk, r.tol_dk), ("dv", grads[2][0, :, 0], r.dv, r.tol_dv),
                                  ("dtable", grads[3][:, 0], r.dt, r.tol_dt + 2.0 ** -8 * (r.dt.abs() + r.tol_dt))):
         _within(name, got, want, tol)
+
+
+def test_decode_queries_at_any_address():
+    """Queries 8 bytes off an aligned address: slices of wider heads, of a fused buffer, transposed, one for all."""
+    from flashback_cute import flashback_attn_relpos_decode
+    from tests.test_relpos_host import odd_queries
+
+    for q in odd_queries().values():
+        flat = q.as_strided((q.untyped_storage().nbytes() // 2,), (1,), 0).to(DEV)
+        q = flat.as_strided(q.shape, q.stride(), q.storage_offset())
+        assert q.data_ptr() % 16 == 8
+        k, v, table = _mk((q.shape[0], 90, 4, 64), BF16, 1), _mk((q.shape[0], 90, 4, 64), BF16, 2), _mk((32, 8), BF16, 3)
+        lens = [90, 31, 2][:q.shape[0]]
+        got = flashback_attn_relpos_decode(q, k, v, torch.tensor(lens, dtype=torch.int32, device=DEV), table)
+        want, tol = _decode_ref(q, k, v, lens, table, 128, False, 0.125)
+        _within("out", got, want, tol)
