@@ -100,6 +100,11 @@ def _check_cu_seqlens(cu_q, cu_k, q) -> None:
             raise ValueError("cu_seqlens_q and cu_seqlens_k must be contiguous, of one length (batch + 1) and on the device of q")
 
 
+def _numbers(max_distance, scale):
+    """The options as Python numbers. Plans are found by their values: a tensor among them would be found by its identity, whatever it holds by then."""
+    return int(max_distance), None if scale is None else float(scale)
+
+
 class _Plans:
     """Plans by geometry, a bounded number of them: shapes, strides, types and options, never addresses."""
 
@@ -163,17 +168,15 @@ class _AttnPlan:
         q_shape, k_shape, table_shape, dtype, device = tuple(q.shape), tuple(k.shape), tuple(table.shape), q.dtype, q.device
         q_stride, k_stride, v_stride, table_stride = q.stride(), k.stride(), v.stride(), table.stride()
         batch = None if cu_q is None else cu_q.shape[0] - 1
-        causal = bool(causal)
-        two = (not causal) if two is None else bool(two)
-        max_distance = int(max_distance)
+        two = (not causal) if two is None else two
         _check_buckets(table_shape[0], two, max_distance)
-        scale = q_shape[-1] ** -0.5 if scale is None else float(scale)
+        scale = q_shape[-1] ** -0.5 if scale is None else scale
         self.q_shape, self.dtype, self.device, self.index = q_shape, dtype, device, device.index
         self.copies = not (_strides_ok(q_shape, q_stride) and _strides_ok(k_shape, k_stride) and _strides_ok(k_shape, v_stride))
         self.heads = q_shape[-2]
         packed = batch is not None
         if packed:
-            total_q, total_k, b, sq, sk = q_shape[0], k_shape[0], batch, int(max_q), int(max_k)
+            total_q, total_k, b, sq, sk = q_shape[0], k_shape[0], batch, max_q, max_k
         else:
             b, sq, sk = q_shape[0], q_shape[1], k_shape[1]
             total_q, total_k = b * sq, b * sk
@@ -278,6 +281,12 @@ class _RelposAttnTransformed(torch.autograd.Function):
 
 
 def _attention(q, k, v, table, cu_q, cu_k, max_q, max_k, max_distance, scale, causal, two):
+    max_distance, scale = _numbers(max_distance, scale)
+    causal = bool(causal)
+    if two is not None:
+        two = bool(two)
+    if cu_q is not None:
+        max_q, max_k = int(max_q), int(max_k)
     while True:
         key = (
             q.shape, k.shape, v.shape, table.shape, q.stride(), k.stride(), v.stride(), table.stride(),
@@ -331,7 +340,6 @@ class _BiasSpec:
             raise TypeError("bias_table must be float16, bfloat16 or float32")
         if not table.is_cuda:
             raise NotImplementedError("flashback_cute (B200 build) has no CPU path: tensors must be CUDA tensors")
-        sq, sk, max_distance = int(sq), int(sk), int(max_distance)
         if not (0 <= sq <= 1 << 20 and 0 <= sk <= 1 << 30):
             raise ValueError("seqlen_q must be at most 2**20 and seqlen_k at most 2**30")
         table_shape, table_stride, dtype, device = tuple(table.shape), table.stride(), table.dtype, table.device
@@ -491,16 +499,15 @@ class _DecodePlan:
                 raise ValueError("cache_seqlens must be contiguous, of shape (batch,) and on the device of q")
         q_shape, k_shape, table_shape, dtype = tuple(q.shape), tuple(k.shape), tuple(table.shape), q.dtype
         q_stride, k_stride, v_stride, table_stride = q.stride(), k.stride(), v.stride(), table.stride()
-        max_distance = int(max_distance)
-        _check_buckets(table_shape[0], bool(two), max_distance)
+        _check_buckets(table_shape[0], two, max_distance)
         ok = lambda s: s[3] == 1 and all(x >= 0 and x % 8 == 0 for x in s[:3])  # noqa: E731
         if not (ok(k_stride) and ok(v_stride)):
             raise ValueError("caches need unit stride on head_dim and strides that are multiples of 8 elements")
         self.copy_q = not ok(q_stride)
         self.empty = 0 in q_shape or 0 in k_shape
         cache = lambda s: _lib.FbCache(None, *s[:3])  # noqa: E731
-        args = _D(_lib._DTYPES[dtype], q_shape[0], q_shape[2], k_shape[2], q_shape[3], q_shape[1], k_shape[1], q_shape[-1] ** -0.5 if scale is None else float(scale),
-                  _bias(table_shape, table_stride, bool(two), max_distance), cache(_plain_strides(q_shape) if self.copy_q else q_stride), cache(k_stride), cache(v_stride))
+        args = _D(_lib._DTYPES[dtype], q_shape[0], q_shape[2], k_shape[2], q_shape[3], q_shape[1], k_shape[1], q_shape[-1] ** -0.5 if scale is None else scale,
+                  _bias(table_shape, table_stride, two, max_distance), cache(_plain_strides(q_shape) if self.copy_q else q_stride), cache(k_stride), cache(v_stride))
         self.words = _lib.template(args)
         self.work = _lib.load().fb_relpos_decode_workspace_bytes(ctypes.byref(args)) // 4
 
@@ -523,6 +530,8 @@ def flashback_attn_relpos_decode(
     clamped to [0, s]). Causal: token t of sequence i sits at position cache_seqlens[i] - sq + t. Cache rows at or behind a
     sequence's length are not read. bfloat16 or float16; meant for one to a few tokens (every 16 or 32 (token, head) pairs of a kv head read the
     cache once). No autograd graph."""
+    max_distance, softmax_scale = _numbers(max_distance, softmax_scale)
+    bidirectional = bool(bidirectional)
     if q.data_ptr() % 16:  # a copy in the standard layout, with the plan of that layout (a clone may have strides of its own)
         with torch.no_grad():
             q = _plain(q)
@@ -561,7 +570,7 @@ def flashback_relpos_bias(
     """The bias as a tensor (heads, seqlen_q, seqlen_k) of the table's dtype (bfloat16, float16 or float32): entry (h, i, j) is
     bias_table[bucket(j - (i + seqlen_k - seqlen_q)), h]. For attention that the fused functions do not take (other head
     sizes, masks of its own) and for looking at what was learned. Differentiable in bias_table, any order and mode."""
-    two = bool(bidirectional)
+    seqlen_q, seqlen_k, max_distance, two = int(seqlen_q), int(seqlen_k), int(max_distance), bool(bidirectional)
     key = (bias_table.shape, bias_table.stride(), bias_table.dtype, bias_table.device, seqlen_q, seqlen_k, two, max_distance)
     spec = _bias_specs.get(key)
     if spec is None:

@@ -1,9 +1,12 @@
 """CPU tests of the biased attention's host side (checks, plans, copies, autograd glue) with the library replaced by a double."""
 
+import ctypes
+from types import SimpleNamespace
+
 import pytest
 import torch
 
-from flashback_cute import flashback_attn_relpos_decode
+from flashback_cute import flashback_attn_relpos_decode, flashback_attn_relpos_varlen_func, flashback_relpos_bias, relpos
 from oracle import relpos_oracle as orc
 from tests import relpos_double as double
 
@@ -42,3 +45,40 @@ def test_decode_takes_queries_at_any_address(which):
     assert all(a.q.ptr % 16 == 0 for _, a in calls)
     assert torch.equal(got, _decode_want(q, k, v, table))
     assert torch.equal(again, _decode_want(_mk(q.shape, 13), k, v, table))
+
+
+# ---------------------------------------------------------------------------------------------
+# options that are tensors and change between calls
+# ---------------------------------------------------------------------------------------------
+def test_options_count_by_their_value():
+    """Lengths, scales, distances and sizes handed over as 0-dim tensors, changed in place: the call uses what they hold."""
+    longest, scale, far = torch.tensor(40), torch.tensor(0.125), torch.tensor(128)
+    q, k, v, table = _mk((160, 8, 64), 0), _mk((160, 4, 64), 1), _mk((160, 4, 64), 2), _mk((32, 8), 3)
+    cu = torch.tensor([0, 40, 60], dtype=torch.int32)
+    qd, kd = _mk((2, 1, 8, 64), 4), _mk((2, 9, 4, 64), 5)
+    spec = relpos._BiasSpec
+    with double.library() as calls:
+        for n, c, f in ((40, 0.125, 128), (100, 1.0, 64)):
+            longest.fill_(n), scale.fill_(c), far.fill_(f)
+            cu[1:] = torch.tensor([n, n + 20])
+            calls.far = f
+            flashback_attn_relpos_varlen_func(q, k, v, table, cu, cu, longest, longest, max_distance=far, softmax_scale=scale, causal=torch.tensor(True))
+            flashback_attn_relpos_decode(qd, kd, kd, None, table, max_distance=far, softmax_scale=scale)
+            fwd, dec = calls[-2][1], calls[-1][1]
+            assert (fwd.prob.seqlen_q, fwd.prob.seqlen_k, fwd.prob.softmax_scale, fwd.prob.causal) == (n, n, c, 1)
+            assert dec.softmax_scale == c
+            starts = relpos.bucket_starts(32, f)
+            for a in (fwd, dec):
+                assert tuple((ctypes.c_int32 * 31).from_address(a.bias.starts)) == starts
+    # the sizes of the bias tensor: the look-up, with the plan's device check out of the way
+    made = []
+    relpos._BiasSpec = lambda table, sq, sk, two, far: made.append((sq, sk, two, far)) or SimpleNamespace(forward=lambda t: (sq, sk, far))
+    try:
+        size = torch.tensor(5)
+        for n in (5, 9):
+            size.fill_(n), far.fill_(100 + n)
+            assert flashback_relpos_bias(table, size, size, max_distance=far) == (n, n, 100 + n)
+        assert all(type(x) in (int, bool) for m in made for x in m)
+    finally:
+        relpos._BiasSpec = spec
+        relpos._bias_specs.plans.clear()
