@@ -121,7 +121,9 @@ class _Plans:
 
 def _strides_ok(shape, stride) -> bool:
     """Rows x heads x head_dim as the kernels take it: unit stride on head_dim, batch folded into rows, positive strides that are
-    multiples of 8 elements."""
+    multiples of 8 elements. A tensor without elements is never read."""
+    if 0 in shape:
+        return True
     if stride[-1] != 1 or stride[-2] <= 0 or stride[-3] <= 0 or stride[-2] % 8 or stride[-3] % 8:
         return False
     return len(shape) == 3 or shape[0] <= 1 or stride[0] == shape[1] * stride[1]
@@ -172,7 +174,6 @@ class _AttnPlan:
         _check_buckets(table_shape[0], two, max_distance)
         scale = q_shape[-1] ** -0.5 if scale is None else scale
         self.q_shape, self.dtype, self.device, self.index = q_shape, dtype, device, device.index
-        self.copies = not (_strides_ok(q_shape, q_stride) and _strides_ok(k_shape, k_stride) and _strides_ok(k_shape, v_stride))
         self.heads = q_shape[-2]
         packed = batch is not None
         if packed:
@@ -181,7 +182,8 @@ class _AttnPlan:
             b, sq, sk = q_shape[0], q_shape[1], k_shape[1]
             total_q, total_k = b * sq, b * sk
         self.total_q = total_q
-        self.empty = 0 in q_shape or 0 in k_shape
+        self.empty = 0 in q_shape or 0 in k_shape  # nothing is read, whatever the layouts
+        self.copies = not (self.empty or (_strides_ok(q_shape, q_stride) and _strides_ok(k_shape, k_stride) and _strides_ok(k_shape, v_stride)))
         self.low = dtype != torch.float32
         if self.copies or self.empty:
             return
@@ -287,7 +289,7 @@ def _attention(q, k, v, table, cu_q, cu_k, max_q, max_k, max_distance, scale, ca
         two = bool(two)
     if cu_q is not None:
         max_q, max_k = int(max_q), int(max_k)
-    while True:
+    for again in (True, False):
         key = (
             q.shape, k.shape, v.shape, table.shape, q.stride(), k.stride(), v.stride(), table.stride(),
             q.dtype, k.dtype, v.dtype, table.dtype, q.device, k.device, v.device, table.device, max_distance, scale, causal, two,
@@ -299,6 +301,7 @@ def _attention(q, k, v, table, cu_q, cu_k, max_q, max_k, max_distance, scale, ca
             plan = _attn_plans.add(key, _AttnPlan(q, k, v, table, cu_q, cu_k, max_q, max_k, max_distance, scale, causal, two))
         if not plan.copies:
             break
+        assert again, "the standard layout is one that the kernels take"
         q, k, v = (t if _strides_ok(t.shape, t.stride()) else _Plain.apply(t) for t in (q, k, v))
     transformed = torch._C._are_functorch_transforms_active()
     if not transformed and (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:

@@ -657,3 +657,12 @@ def test_decode_queries_at_any_address():
         got = flashback_attn_relpos_decode(q, k, v, torch.tensor(lens, dtype=torch.int32, device=DEV), table)
         want, tol = _decode_ref(q, k, v, lens, table, 128, False, 0.125)
         _within("out", got, want, tol)
+
+
+def test_empty_sequences_in_batches():
+    """Two dense sequences of length zero: queries, keys, both."""
+    for sq, sk in ((0, 5), (5, 0), (0, 0)):
+        leaves = [t.requires_grad_() for t in (_mk((2, sq, 4, 64), BF16, 0), _mk((2, sk, 2, 64), BF16, 1), _mk((2, sk, 2, 64), BF16, 2), _mk((32, 4), BF16, 3))]
+        out = flashback_attn_relpos_func(*leaves)
+        assert out.shape == (2, sq, 4, 64) and (out == 0).all()
+        assert all((g == 0).all() for g in torch.autograd.grad(out, leaves, torch.ones_like(out)))

@@ -6,7 +6,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from flashback_cute import flashback_attn_relpos_decode, flashback_attn_relpos_varlen_func, flashback_relpos_bias, relpos
+from flashback_cute import flashback_attn_relpos_decode, flashback_attn_relpos_func, flashback_attn_relpos_varlen_func, flashback_relpos_bias, relpos
 from oracle import relpos_oracle as orc
 from tests import relpos_double as double
 
@@ -82,3 +82,23 @@ def test_options_count_by_their_value():
     finally:
         relpos._BiasSpec = spec
         relpos._bias_specs.plans.clear()
+
+
+# ---------------------------------------------------------------------------------------------
+# sequences of length zero
+# ---------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("b", [1, 2, 3])
+@pytest.mark.parametrize("sq,sk", [(0, 5), (5, 0), (0, 0)])
+def test_dense_batches_of_empty_sequences(b, sq, sk, monkeypatch):
+    """No loop of copies (torch's strides of an empty tensor are not those of rows folded into the batch)."""
+    copies, plain = [], relpos._plain
+    monkeypatch.setattr(relpos, "_plain", lambda t: copies.append(t) or (plain(t) if len(copies) < 20 else pytest.fail("copies without end")))
+    for turned in (False, True):
+        mk = lambda s, h, seed: _mk((b, h, s, 64), seed).transpose(1, 2) if turned else _mk((b, s, h, 64), seed)  # noqa: E731
+        leaves = [t.requires_grad_() for t in (mk(sq, 4, 0), mk(sk, 2, 1), mk(sk, 2, 2), _mk((32, 4), 3))]
+        with double.library() as calls:
+            out = flashback_attn_relpos_func(*leaves, causal=True)
+            grads = torch.autograd.grad(out, leaves, torch.ones_like(out))
+            assert flashback_attn_relpos_decode(leaves[0], leaves[1], leaves[2], None, leaves[3]).shape == out.shape
+        assert not calls and out.shape == (b, sq, 4, 64) and (out == 0).all()
+        assert all(g.shape == t.shape and (g == 0).all() for g, t in zip(grads, leaves))
