@@ -292,7 +292,7 @@ def _attention(q, k, v, table, cu_q, cu_k, max_q, max_k, max_distance, scale, ca
     for again in (True, False):
         key = (
             q.shape, k.shape, v.shape, table.shape, q.stride(), k.stride(), v.stride(), table.stride(),
-            q.dtype, k.dtype, v.dtype, table.dtype, q.device, k.device, v.device, table.device, max_distance, scale, causal, two,
+            q.dtype, k.dtype, v.dtype, table.dtype, q.device, k.device, v.device, table.device, max_distance, scale, causal, two, _lib.DEFAULT_FLAGS,
         )
         if cu_q is not None:
             key += (cu_q.shape, cu_k.shape, cu_q.dtype, cu_k.dtype, cu_q.device, cu_k.device, cu_q.stride(), cu_k.stride(), max_q, max_k)

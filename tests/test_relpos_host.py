@@ -6,7 +6,7 @@ from types import SimpleNamespace
 import pytest
 import torch
 
-from flashback_cute import flashback_attn_relpos_decode, flashback_attn_relpos_func, flashback_attn_relpos_varlen_func, flashback_relpos_bias, relpos
+from flashback_cute import _lib, flashback_attn_relpos_decode, flashback_attn_relpos_func, flashback_attn_relpos_varlen_func, flashback_relpos_bias, relpos
 from oracle import relpos_oracle as orc
 from tests import relpos_double as double
 
@@ -102,3 +102,17 @@ def test_dense_batches_of_empty_sequences(b, sq, sk, monkeypatch):
             assert flashback_attn_relpos_decode(leaves[0], leaves[1], leaves[2], None, leaves[3]).shape == out.shape
         assert not calls and out.shape == (b, sq, 4, 64) and (out == 0).all()
         assert all(g.shape == t.shape and (g == 0).all() for g, t in zip(grads, leaves))
+
+
+# ---------------------------------------------------------------------------------------------
+# flags of the binding
+# ---------------------------------------------------------------------------------------------
+def test_flags_of_the_call_count(monkeypatch):
+    """`_lib.DEFAULT_FLAGS` as it is at the call, like the rest of the binding, also for a layout seen before."""
+    q, k, table = _mk((1, 5, 4, 64), 0), _mk((1, 5, 2, 64), 1), _mk((32, 4), 2)
+    with double.library() as calls:
+        for flags in (0, _lib.FB_FLAG_FORCE_SIMT, 0):
+            monkeypatch.setattr(_lib, "DEFAULT_FLAGS", flags)
+            leaf = q.clone().requires_grad_()
+            torch.autograd.grad(flashback_attn_relpos_func(leaf, k, k, table).sum(), leaf)
+            assert [a.prob.flags for _, a in calls[-2:]] == [flags, flags]
