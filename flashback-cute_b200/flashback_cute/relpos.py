@@ -303,9 +303,9 @@ def _attention(q, k, v, table, cu_q, cu_k, max_q, max_k, max_distance, scale, ca
             break
         assert again, "the standard layout is one that the kernels take"
         q, k, v = (t if _strides_ok(t.shape, t.stride()) else _Plain.apply(t) for t in (q, k, v))
-    transformed = torch._C._are_functorch_transforms_active()
-    if not transformed and (q.data_ptr() | k.data_ptr() | v.data_ptr()) % 16:
-        return _attention(*(_Plain.apply(t) if t.data_ptr() % 16 else t for t in (q, k, v)), table, cu_q, cu_k, max_q, max_k, max_distance, scale, causal, two)
+    transformed, ptr = torch._C._are_functorch_transforms_active(), _address()
+    if (ptr(q) | ptr(k) | ptr(v)) % 16:
+        return _attention(*(_Plain.apply(t) if ptr(t) % 16 else t for t in (q, k, v)), table, cu_q, cu_k, max_q, max_k, max_distance, scale, causal, two)
     if transformed:
         return _RelposAttnTransformed.apply(q, k, v, table, cu_q, cu_k, plan)[0]
     if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or table.requires_grad)) or forward_ad._current_level >= 0:

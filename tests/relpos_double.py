@@ -8,6 +8,7 @@ import ctypes
 from contextlib import contextmanager
 
 import torch
+from torch._functorch.pyfunctorch import temporarily_clear_interpreter_stack
 
 from flashback_cute import _lib, relpos
 from oracle import relpos_oracle as orc
@@ -40,7 +41,8 @@ class Calls(list):
                   "fb_relpos_bias": _lib.FbRelposBiasArgs, "fb_relpos_bias_grad": _lib.FbRelposBiasGradArgs}[name]
         a = struct.from_buffer_copy(words.tobytes())
         self.append((name, a))
-        getattr(self, name, lambda a: None)(a)
+        with temporarily_clear_interpreter_stack():  # the library knows nothing of torch.func
+            getattr(self, name, lambda a: None)(a)
 
     def _attention(self, a, dout=None):
         p, dtype = a.prob, TYPES[a.prob.dtype]

@@ -666,3 +666,13 @@ def test_empty_sequences_in_batches():
         out = flashback_attn_relpos_func(*leaves)
         assert out.shape == (2, sq, 4, 64) and (out == 0).all()
         assert all((g == 0).all() for g in torch.autograd.grad(out, leaves, torch.ones_like(out)))
+
+
+def test_misaligned_inputs_under_torch_func():
+    off = lambda shape, seed: torch.cat([_mk((4,), BF16, 0), _mk(shape, BF16, seed).flatten()])[4:].view(shape)  # noqa: E731
+    x = (off((2, 50, 4, 64), 0), off((2, 60, 2, 64), 1), off((2, 60, 2, 64), 2), _mk((32, 4), BF16, 3))
+    assert x[0].data_ptr() % 16 == 8
+    got = torch.func.grad(lambda *a: flashback_attn_relpos_func(*a).float().sum(), argnums=(0, 1, 2, 3))(*x)
+    leaves = [t.clone().requires_grad_() for t in x]
+    want = torch.autograd.grad(flashback_attn_relpos_func(*leaves).float().sum(), leaves)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))

@@ -1,6 +1,7 @@
 """CPU tests of the biased attention's host side (checks, plans, copies, autograd glue) with the library replaced by a double."""
 
 import ctypes
+import math
 from types import SimpleNamespace
 
 import pytest
@@ -116,3 +117,19 @@ def test_flags_of_the_call_count(monkeypatch):
             leaf = q.clone().requires_grad_()
             torch.autograd.grad(flashback_attn_relpos_func(leaf, k, k, table).sum(), leaf)
             assert [a.prob.flags for _, a in calls[-2:]] == [flags, flags]
+
+
+# ---------------------------------------------------------------------------------------------
+# addresses under torch.func
+# ---------------------------------------------------------------------------------------------
+def test_misaligned_inputs_under_torch_func():
+    off = lambda shape, seed: _mk((math.prod(shape) + 4,), seed)[4:].view(shape)  # noqa: E731
+    q, k, v, table = off((2, 5, 4, 64), 0), off((2, 6, 2, 64), 1), off((2, 6, 2, 64), 2), _mk((32, 4), 3)
+    assert all(t.data_ptr() % 16 == 8 for t in (q, k, v))
+    loss = lambda *a: flashback_attn_relpos_func(*a, causal=True).float().sum()  # noqa: E731
+    with double.library() as calls:
+        got = torch.func.grad(loss, argnums=(0, 1, 2, 3))(q, k, v, table)
+        leaves = [t.clone().requires_grad_() for t in (q, k, v, table)]
+        want = torch.autograd.grad(loss(*leaves), leaves)
+    assert all(t.ptr % 16 == 0 for _, a in calls for t in (a.q, a.k, a.v))
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
