@@ -353,11 +353,11 @@ class _BiasSpec:
         self.fill = _lib.template(_lib.FbRelposBiasArgs(code, self.heads, sq, sk, _bias(table_shape, table_stride, two, max_distance), None))
         self.grad = _lib.template(_lib.FbRelposBiasGradArgs(code, self.heads, sq, sk, _bias(table_shape, table_stride, two, max_distance), None, None, self.heads, 1, None))
         self.work = lib.fb_relpos_bias_workspace_bytes(code, self.heads, sq, sk, self.num) // 4
-        self.stride = table_stride
+        self.stride, self.options = table_stride, (sq, sk, two, max_distance)
 
     def forward(self, table):
         if table.stride() != self.stride:  # (tangents and second-order cotangents come in layouts of their own)
-            table = torch.empty_strided(table.shape, self.stride, dtype=table.dtype, device=table.device).copy_(table)
+            return _bias_spec(table, *self.options).forward(table)
         out = torch.empty(self.shape, dtype=self.dtype, device=self.device)
         if out.numel():
             ptr, w = _address(), self.fill[:]
@@ -382,6 +382,14 @@ class _BiasSpec:
 _FILL_TABLE, _FILL_OUT = _lib.word(_lib.FbRelposBiasArgs, "bias", "table"), _lib.word(_lib.FbRelposBiasArgs, "out")
 _GRAD_IN, _GRAD_OUT, _GRAD_WORK = (_lib.word(_lib.FbRelposBiasGradArgs, n) for n in ("grad", "dtable", "workspace"))
 _bias_specs = _Plans()
+
+
+def _bias_spec(table, sq, sk, two, max_distance):
+    key = (table.shape, table.stride(), table.dtype, table.device, sq, sk, two, max_distance)
+    spec = _bias_specs.get(key)
+    if spec is None:
+        spec = _bias_specs.add(key, _BiasSpec(table, sq, sk, two, max_distance))
+    return spec
 
 
 class _RelposBiasFunc(torch.autograd.Function):
@@ -574,10 +582,7 @@ def flashback_relpos_bias(
     bias_table[bucket(j - (i + seqlen_k - seqlen_q)), h]. For attention that the fused functions do not take (other head
     sizes, masks of its own) and for looking at what was learned. Differentiable in bias_table, any order and mode."""
     seqlen_q, seqlen_k, max_distance, two = int(seqlen_q), int(seqlen_k), int(max_distance), bool(bidirectional)
-    key = (bias_table.shape, bias_table.stride(), bias_table.dtype, bias_table.device, seqlen_q, seqlen_k, two, max_distance)
-    spec = _bias_specs.get(key)
-    if spec is None:
-        spec = _bias_specs.add(key, _BiasSpec(bias_table, seqlen_q, seqlen_k, two, max_distance))
+    spec = _bias_spec(bias_table, seqlen_q, seqlen_k, two, max_distance)
     if forward_ad._current_level >= 0 or torch._C._are_functorch_transforms_active():
         return _RelposBiasFunc.apply(bias_table, spec)
     if torch.is_grad_enabled() and bias_table.requires_grad:

@@ -85,6 +85,20 @@ class Calls(list):
         for i, n in enumerate(lens):
             out[i] = orc.attention(q[i:i + 1], k[i:i + 1, :n], v[i:i + 1, :n], _table(a.bias, hq, dtype), self.far, bool(a.bias.bidirectional), a.softmax_scale, True).out[0].to(dtype)
 
+    which = None  # (sq, sk) buckets of the bias tensor's calls
+
+    def fb_relpos_bias(self, a):
+        dtype = TYPES[a.dtype]
+        out = memory(a.out, (a.heads, a.seqlen_q, a.seqlen_k), (a.seqlen_q * a.seqlen_k, a.seqlen_k, 1), dtype)
+        out.copy_(_table(a.bias, a.heads, dtype).t()[:, self.which])
+
+    def fb_relpos_bias_grad(self, a):
+        dtype = TYPES[a.dtype]
+        grad = memory(a.grad, (a.heads, a.seqlen_q, a.seqlen_k), (a.seqlen_q * a.seqlen_k, a.seqlen_k, 1), dtype)
+        out = memory(a.dtable, (a.bias.num_buckets, a.heads), (a.dtable_bucket_stride, a.dtable_head_stride), dtype)
+        for h in range(a.heads):
+            out[:, h] = torch.zeros(a.bias.num_buckets, dtype=torch.float64).index_add_(0, self.which.flatten(), grad[h].double().flatten()).to(dtype)
+
 
 @contextmanager
 def library():

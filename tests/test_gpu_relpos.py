@@ -676,3 +676,13 @@ def test_misaligned_inputs_under_torch_func():
     leaves = [t.clone().requires_grad_() for t in x]
     want = torch.autograd.grad(flashback_attn_relpos_func(*leaves).float().sum(), leaves)
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_bias_tensor_of_a_broadcast_table():
+    column, way = _mk((32, 1), F32, 0), _mk((32, 1), F32, 1)
+    which = orc.buckets(40, 50, 32, 128, True).to(DEV)
+    _, tangent = torch.func.jvp(lambda c: flashback_relpos_bias(c.expand(-1, 3), 40, 50), (column,), (way,))
+    assert torch.equal(tangent, way.expand(-1, 3).t()[:, which])
+    leaf, w, spread = column.expand(-1, 3).detach().requires_grad_(), _mk((3, 40, 50), F32, 2).requires_grad_(), _mk((32, 3), F32, 3)
+    first = torch.autograd.grad((flashback_relpos_bias(leaf, 40, 50) * w).sum(), leaf, create_graph=True)[0]
+    assert torch.equal(torch.autograd.grad((first * spread).sum(), w)[0], spread.t()[:, which])

@@ -133,3 +133,24 @@ def test_misaligned_inputs_under_torch_func():
         want = torch.autograd.grad(loss(*leaves), leaves)
     assert all(t.ptr % 16 == 0 for _, a in calls for t in (a.q, a.k, a.v))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+# ---------------------------------------------------------------------------------------------
+# the bias tensor of a broadcast table
+# ---------------------------------------------------------------------------------------------
+def test_derivatives_of_the_bias_of_a_broadcast_table(monkeypatch):
+    """One column for every head (stride 0): tangents and second-order cotangents have layouts of their own."""
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda t: True))
+    column = _mk((8, 1), 0, torch.float32)
+    which = orc.buckets(5, 7, 8, 6, True)
+    bias = lambda c: flashback_relpos_bias(c.expand(-1, 3), 5, 7, max_distance=6)  # noqa: E731
+    way, w = _mk((8, 1), 1, torch.float32), _mk((3, 5, 7), 2, torch.float32).requires_grad_()
+    with double.library() as calls:
+        calls.which = which
+        _, tangent = torch.func.jvp(bias, (column,), (way,))
+        assert torch.equal(tangent, way.expand(-1, 3).t()[:, which])
+        spread = torch.randn(8, 3)
+        leaf = column.expand(-1, 3).detach().requires_grad_()
+        assert leaf.stride() == (1, 0)
+        first = torch.autograd.grad((flashback_relpos_bias(leaf, 5, 7, max_distance=6) * w).sum(), leaf, create_graph=True)[0]
+        assert torch.equal(torch.autograd.grad((first * spread).sum(), w)[0], spread.t()[:, which])
