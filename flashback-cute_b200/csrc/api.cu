@@ -481,19 +481,16 @@ int check_decode(const fb_relpos_decode_args& a) {
   return FB_OK;
 }
 
-bool cluster_of(const fb_relpos_decode_args& a) {
-  return decode_cluster(a.batch, a.heads_kv, a.heads_q / a.heads_kv * a.seqlen_q, a.seqlen_k);
-}
-int splits_of(const fb_relpos_decode_args& a) {
-  return decode_splits(a.batch, a.heads_kv, a.heads_q / a.heads_kv * a.seqlen_q, a.seqlen_k);
+DecodeShape shape_of(const fb_relpos_decode_args& a) {
+  return decode_shape(a.batch, a.heads_kv, a.heads_q / a.heads_kv * a.seqlen_q, a.seqlen_k);
 }
 
 }  // namespace
 
 extern "C" size_t fb_relpos_decode_workspace_bytes(const fb_relpos_decode_args* a) {
   if (!a || check_decode(*a) != FB_OK || a->batch == 0 || a->seqlen_q == 0) return 0;
-  const size_t splits = (size_t)splits_of(*a);
-  return splits == 1 || cluster_of(*a) ? 0 : (size_t)a->batch * a->seqlen_q * a->heads_q * splits * (a->head_dim + 2) * sizeof(float);
+  const DecodeShape shape = shape_of(*a);
+  return shape.splits == 1 || shape.cluster ? 0 : (size_t)a->batch * a->seqlen_q * a->heads_q * (size_t)shape.splits * (a->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int fb_relpos_decode(const fb_relpos_decode_args* a, fb_stream_t stream) {
@@ -516,8 +513,9 @@ extern "C" int fb_relpos_decode(const fb_relpos_decode_args* a, fb_stream_t stre
   p.v = CacheT{a->v.ptr, a->v.batch_stride, a->v.row_stride, a->v.head_stride};
   p.lens = a->lens;
   p.out = a->out;
-  p.splits = splits_of(*a);
-  p.cluster = cluster_of(*a) ? 1 : 0;
+  const DecodeShape shape = shape_of(*a);
+  p.splits = shape.splits;
+  p.cluster = shape.cluster ? 1 : 0;
   if (p.splits > 1 && !p.cluster) {
     if (!a->workspace) return FB_ERR_NULL_ARG;
     p.part = a->workspace;  // row length head_dim floats: the (maximum, sum) pairs behind them stay 8-byte aligned

@@ -469,11 +469,11 @@ int decode_dispatch(DecodeParams& p, RelPos& rel, cudaStream_t s) {
 
 }  // namespace
 
-// Slices of a sequence's keys: enough CTAs for a few waves on the whole GPU, slices of at least one round of the CTA's warps. A
+// Slices of a sequence's keys and how they are joined: enough CTAs for a few waves on the whole GPU, slices of at least one round of the CTA's warps. A
 // power of two up to 8 (a cluster: one launch) for small batches whose slices then have at most 8 rounds; otherwise a workspace and a
 // second launch, since a cluster holds its SMs until its last CTA is done: 48 sequences of up to 8192 keys, 8 kv heads of 128
 // in 4 slices each: 171 us as clusters, 152 + 5 us through the workspace.
-int decode_splits(int batch, int heads_kv, int rows, int seqlen_k) {
+DecodeShape decode_shape(int batch, int heads_kv, int rows, int seqlen_k) {
   const int per = rows <= 16 ? 16 : 32;
   const int64_t base = (int64_t)batch * heads_kv * ((rows + per - 1) / per);
   const int64_t want = (148 * 2 * 4 + base - 1) / base;
@@ -482,15 +482,10 @@ int decode_splits(int batch, int heads_kv, int rows, int seqlen_k) {
   if (base < 2 * 148 && rounds8 <= 8 * kMaxCluster) {
     int n = 1;
     while (n < kMaxCluster && n < want && 2 * n <= rounds8) n *= 2;
-    return n;
+    return {n, n > 1};
   }
   const int64_t n = want < rounds ? want : rounds;
-  return (int)(n < 1 ? 1 : n > 128 ? 128 : n);
-}
-bool decode_cluster(int batch, int heads_kv, int rows, int seqlen_k) {
-  const int per = rows <= 16 ? 16 : 32;
-  const int n = decode_splits(batch, heads_kv, rows, seqlen_k);
-  return n > 1 && n <= kMaxCluster && (int64_t)batch * heads_kv * ((rows + per - 1) / per) < 2 * 148;
+  return {(int)(n < 1 ? 1 : n > 128 ? 128 : n), false};
 }
 
 int launch_decode(int dtype, DecodeParams& p, RelPos& rel, cudaStream_t s) {

@@ -230,8 +230,11 @@ int launch_relpos_fill(int dtype, const RelPos& rel, int heads, int sq, int sk, 
 int launch_relpos_grad(int dtype, const RelPos& rel, int heads, int sq, int sk, const void* grad, void* dtable, int64_t bucket_stride,
                        int64_t head_stride, cudaStream_t stream);
 int64_t relpos_bias_parts(int dtype, int heads, int sq, int sk);  // partial table gradients per head of launch_relpos_grad
-int decode_splits(int batch, int heads_kv, int rows, int seqlen_k);
-bool decode_cluster(int batch, int heads_kv, int rows, int seqlen_k);  // those slices are one cluster (and need no workspace)
+struct DecodeShape {
+  int splits;    // slices of a sequence's keys
+  bool cluster;  // they are one cluster (and need no workspace)
+};
+DecodeShape decode_shape(int batch, int heads_kv, int rows, int seqlen_k);
 constexpr int kDecodeMaxTable = 4096;  // query heads per kv head x buckets
 int launch_decode(int dtype, DecodeParams& p, RelPos& rel, cudaStream_t stream);
 constexpr int kTcOwnerRows = 128, kSimtOwnerRows = 16;  // query rows per partial table gradient

@@ -686,3 +686,9 @@ def test_bias_tensor_of_a_broadcast_table():
     leaf, w, spread = column.expand(-1, 3).detach().requires_grad_(), _mk((3, 40, 50), F32, 2).requires_grad_(), _mk((32, 3), F32, 3)
     first = torch.autograd.grad((flashback_relpos_bias(leaf, 40, 50) * w).sum(), leaf, create_graph=True)[0]
     assert torch.equal(torch.autograd.grad((first * spread).sum(), w)[0], spread.t()[:, which])
+
+
+def test_decode_long_caches_of_mid_sized_batches():
+    """148 to 295 (sequence, kv head) pairs and caches beyond 8192 rows; most sequences short."""
+    for b, hkv, s, long in ((24, 8, 8200, 8200), (37, 4, 9001, 3000), (40, 7, 16500, 5000)):
+        _check_decode(BF16, 64, hkv, hkv, 1, s, [long] + [1 + 37 * i % 301 for i in range(b - 1)])

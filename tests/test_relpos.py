@@ -187,3 +187,22 @@ def test_oracle_gradients_are_the_formulas():
     want = (out, *torch.autograd.grad(out, (a, b, c, t), do.double()))
     for x, y in zip(ref[:5], want):
         assert torch.allclose(x, y, rtol=1e-11, atol=1e-11)
+
+
+def test_decode_long_caches_join_through_the_workspace():
+    """Beyond 8192 cache rows the slices are joined by a second launch, never by a cluster (whose sizes are 2, 4 and 8)."""
+    lib = _lib.load()
+    c = _lib.FbCache(0x1000, 1024, 128, 64)
+
+    def floats(batch, hkv, sk, d=64):
+        a = _lib.FbRelposDecodeArgs(dtype=0, batch=batch, heads_q=2 * hkv, heads_kv=hkv, head_dim=d, seqlen_q=1, seqlen_k=sk, softmax_scale=0.125,
+                                    bias=_bias(), q=c, k=c, v=c, out=0x1000)
+        return lib.fb_relpos_decode_workspace_bytes(ctypes.byref(a)) // 4 / (batch * 2 * hkv * (d + 2))
+
+    for batch, hkv in ((1, 1), (24, 8), (37, 4), (32, 8), (200, 1), (295, 1), (296, 1)):
+        base = batch * hkv
+        for sk in (8193, 16384, 32768, 1 << 20):
+            assert floats(batch, hkv, sk) == min(128, -(-148 * 8 // base), -(-sk // 64)), (base, sk)  # the slices of a sequence
+        for sk in (40, 1000, 8192):
+            if base < 296:
+                assert floats(batch, hkv, sk) == 0
