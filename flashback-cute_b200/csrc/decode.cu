@@ -226,13 +226,14 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int x = e >> 1, j = j0 + 8 * n + 2 * (lane & 3) + (e & 1);
-            float bias = far_bias[mt][x];
-            if (mode != 0) {
+            if (mode == 0) {
+              s[mt][n][e] = fmaf(s[mt][n][e], scale2, far_bias[mt][x]);
+            } else {
               const int r = j - pos[mt][x];
-              bias = row_tab[mt][x][mode == 1 ? bucket_of.near(min(r, 0)) : bucket_of(min(r, 0))];
-              if (r > 0 || j >= k1) bias = -INFINITY;
+              const float bias = row_tab[mt][x][mode == 1 ? bucket_of.near(min(r, 0)) : bucket_of(min(r, 0))];
+              // selected, not added: the key of a later token may hold infinities or NaN
+              s[mt][n][e] = r > 0 || j >= k1 ? -INFINITY : fmaf(s[mt][n][e], scale2, bias);
             }
-            s[mt][n][e] = fmaf(s[mt][n][e], scale2, bias);
             mx[mt][x] = fmaxf(mx[mt][x], s[mt][n][e]);
           }
       }

@@ -692,3 +692,19 @@ def test_decode_long_caches_of_mid_sized_batches():
     """148 to 295 (sequence, kv head) pairs and caches beyond 8192 rows; most sequences short."""
     for b, hkv, s, long in ((24, 8, 8200, 8200), (37, 4, 9001, 3000), (40, 7, 16500, 5000)):
         _check_decode(BF16, 64, hkv, hkv, 1, s, [long] + [1 + 37 * i % 301 for i in range(b - 1)])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_decode_keys_of_later_tokens_may_hold_anything(d):
+    """Infinities and NaN in the key of a drafted token: the tokens before it do not see it."""
+    from flashback_cute import flashback_attn_relpos_decode
+
+    q, k, v, table = _mk((2, 4, 8, d), BF16, 0), _mk((2, 300, 2, d), BF16, 1), _mk((2, 300, 2, d), BF16, 2), _mk((32, 8), BF16, 3)
+    lens = [300, 77]
+    want, tol = _decode_ref(q, k, v, lens, table, 128, False, d ** -0.5)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        broken = k.clone()
+        for i, n in enumerate(lens):
+            broken[i, n - 2:n] = bad  # the keys of tokens 2 and 3
+        got = flashback_attn_relpos_decode(q, broken, v, torch.tensor(lens, dtype=torch.int32, device=DEV), table)
+        _within("out", got[:, :2], want[:, :2], tol[:, :2])
