@@ -325,6 +325,10 @@ int convert_relpos(RelPos& r, const fb_relpos& b, bool need_table) {
     r.starts[t] = b.starts[t];
   }
   r.far = r.starts[r.side - 2];
+  for (int t = 0; t < r.nb; ++t) {  // r > 0 starts at distance 1
+    const int side = t >= r.side, x = t - side * r.side, first = x > 0 ? r.starts[x - 1] : 0, end = x < r.side - 1 ? r.starts[x] : INT32_MAX;
+    if (end > (side && first < 1 ? 1 : first)) r.used[t / 32] |= 1u << (t % 32);
+  }
   uint8_t* bytes = reinterpret_cast<uint8_t*>(r.near_words);
   for (int t = 0, n = 0; t < r.side; ++t) {
     const int end = t < r.side - 1 && r.starts[t] < kRelNear ? r.starts[t] : kRelNear;
@@ -374,6 +378,7 @@ extern "C" int fb_relpos_fwd(const fb_relpos_fwd_args* a, fb_stream_t stream) {
   FB_TRY(device_setup(&p.status));
   p.q = cvt(a->q); p.k = cvt(a->k); p.v = cvt(a->v); p.o = cvt(a->out); p.od = cvt(a->out_low);
   p.lse = a->lse;
+  rel.shift = a->shift;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   int n = use_tensor_cores(a->prob) ? launch_tc_fwd_rel(p, rel, s) : launch_simt_fwd_rel(p, rel, s);
   if (n < 0) { if (n == FB_ERR_CUDA) record_cuda(cudaGetLastError()); return n; }
@@ -393,6 +398,8 @@ extern "C" int fb_relpos_bwd(const fb_relpos_bwd_args* a, fb_stream_t stream) {
   if (!a->lse || !a->workspace) return FB_ERR_NULL_ARG;
   if (reinterpret_cast<uintptr_t>(a->workspace) % 16 != 0) return FB_ERR_ALIGNMENT;
   if (a->prob.total_q == 0 || a->prob.total_k == 0) return FB_ERR_SHAPE;
+  if (!a->shift) return FB_ERR_NULL_ARG;
+  rel.shift = const_cast<float*>(a->shift);
   Params p;
   fill_problem(p, a->prob);
   FB_TRY(device_setup(&p.status));

@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
   // the table's columns of this kv head's query heads
   for (int at = threadIdx.x; at < p.G * rel.nb; at += NT) {
     const int g = at / rel.nb, t = at - g * rel.nb;
-    tab[at] = relpos_entry<T>(rel, t, hk * p.G + g) * kLog2e;
+    tab[at] = relpos_log2(relpos_entry<T>(rel, t, hk * p.G + g));
   }
   // the queries: row x of the CTA is new token (rt * R + x) / G, query head hk * G + (rt * R + x) % G
   for (int at = threadIdx.x; at < R * U; at += NT) {
@@ -151,7 +151,7 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
   const RelFn bucket_of(rel, buckets);
   int pos[MT][2];
   const float* row_tab[MT][2];
-  float far_bias[MT][2], m[MT][2], l[MT][2];
+  float far_bias[MT][2], shift[MT][2], m[MT][2], l[MT][2];
   float o[MT][D / 8][4];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt) {
@@ -161,7 +161,15 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
       const int t = row / p.G;
       row_tab[mt][x] = tab + (row - t * p.G) * rel.nb;
       pos[mt][x] = len - p.Sq + t;  // the new token's place in its sequence
-      far_bias[mt][x] = row_tab[mt][x][rel.side - 1];
+      // the row's shift (relpos_shift): the largest entry of the buckets up to its first key's; the four lanes of a row share the work
+      float top = -INFINITY;
+      if (pos[mt][x] >= 0)
+        for (int u = lane & 3, last = bucket_of(-pos[mt][x]); u <= last; u += 4)
+          if (rel.used[u >> 5] >> (u & 31) & 1u) top = fmaxf(top, row_tab[mt][x][u]);
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      shift[mt][x] = top == -INFINITY ? 0.f : top;
+      far_bias[mt][x] = row_tab[mt][x][rel.side - 1] - shift[mt][x];
       m[mt][x] = -INFINITY;
       l[mt][x] = 0.f;
     }
@@ -230,7 +238,7 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
               s[mt][n][e] = fmaf(s[mt][n][e], scale2, far_bias[mt][x]);
             } else {
               const int r = j - pos[mt][x];
-              const float bias = row_tab[mt][x][mode == 1 ? bucket_of.near(min(r, 0)) : bucket_of(min(r, 0))];
+              const float bias = row_tab[mt][x][mode == 1 ? bucket_of.near(min(r, 0)) : bucket_of(min(r, 0))] - shift[mt][x];
               // selected, not added: the key of a later token may hold infinities or NaN
               s[mt][n][e] = r > 0 || j >= k1 ? -INFINITY : fmaf(s[mt][n][e], scale2, bias);
             }

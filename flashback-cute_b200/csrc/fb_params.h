@@ -74,6 +74,8 @@ struct RelPos {
   int64_t bucket_stride, head_stride;
   int nb, side, two;  // buckets in all / per side, 1 = both sides have buckets of their own
   float* dpart;       // backward: partial table gradients [(batch, query head)][query tile][nb], or nullptr
+  float* shift;       // the rows' shifts (forward: out, may be nullptr; backward: in)
+  uint32_t used[FB_RELPOS_MAX_BUCKETS / 32];  // bit t: some distance falls in bucket t
   int far;            // distances from here on lie in the last bucket of their side
   int starts[FB_RELPOS_MAX_BUCKETS - 1];  // side - 1 entries
   uint32_t near_words[256];  // the buckets of distances 0 .. 1023, a byte each
@@ -126,6 +128,50 @@ template <typename T>
 __device__ __forceinline__ float relpos_entry(const RelPos& rel, int bucket, int head) {
   const float x = to_f<T>(reinterpret_cast<const T*>(rel.table)[bucket * rel.bucket_stride + head * rel.head_stride]);
   return x <= kRelHidden ? -INFINITY : x;
+}
+// An entry in log2 units, as the tensor-core kernels add it: finite stays finite (3e38 log2(e) is beyond float32).
+__device__ __forceinline__ float relpos_log2(float x) {
+  const float y = x * 1.4426950408889634f;
+  return y == INFINITY && x != INFINITY ? 3.402823466e38f : y;
+}
+// The shift of a row: the largest entry that its keys have. Scores are formed as c q.k + (entry - shift): the difference is exact where it
+// matters, while beside an entry of 1e6 the sum would have no room for c q.k, and neither would a log-sum-exp for what the backward needs.
+//
+// Prefix maxima of a head's entries over the buckets of each side that some distance falls in, by one warp.
+template <typename T>
+__device__ __forceinline__ void relpos_prefix(float* pre, const RelPos& rel, int head, int lane) {
+  for (int first = 0; first < rel.nb; first += rel.side) {
+    float carry = -INFINITY;
+    for (int t0 = 0; t0 < rel.side; t0 += 32) {
+      const int t = t0 + lane, b = first + t;
+      float x = -INFINITY;
+      if (t < rel.side && (rel.used[b >> 5] >> (b & 31) & 1u)) x = relpos_entry<T>(rel, b, head);
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const float y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x = fmaxf(x, y);
+      }
+      x = fmaxf(x, carry);
+      if (t < rel.side) pre[b] = x;
+      carry = __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+}
+// The shift of a row whose keys lie at positions lo .. hi, hi >= 0.
+template <typename T>
+__device__ __forceinline__ float relpos_shift(const float* pre, const RelPos& rel, const RelFn& bucket_of, int head, int lo, int hi) {
+  float x = -INFINITY;
+  if (!rel.two || lo <= 0) x = pre[bucket_of(min(lo, 0))];  // distances 0 .. -lo (r > 0 counts as 0 when one side has buckets)
+  if (rel.two && hi > 0) {
+    const int last = bucket_of(hi);
+    if (lo <= 1) {
+      x = fmaxf(x, pre[last]);
+    } else {  // a row ahead of the first key
+      for (int b = bucket_of(lo); b <= last; ++b)
+        if (rel.used[b >> 5] >> (b & 31) & 1u) x = fmaxf(x, relpos_entry<T>(rel, b, head));
+    }
+  }
+  return x == -INFINITY ? 0.f : x;
 }
 // Fills `b`, thread `i` of `n`. Only what the search will look at: bytes up to the first far distance.
 __device__ __forceinline__ void relpos_load_buckets(RelBuckets& b, const RelPos& rel, int i, int n) {

@@ -1,6 +1,6 @@
 // Forward of attention with a learned relative position bias on the tensor cores (16-bit types).
 //
-// Online softmax, in log2 units: V_ij = c log2(e) (Q K^T)_ij + log2(e) T[bucket], P = 2^(V - m), O = P V / l.
+// Online softmax, in log2 units: V_ij = c log2(e) (Q K^T)_ij + log2(e) (T[bucket] - shift_i), P = 2^(V - m), O = P V / l (the shift: fb_params.h).
 //
 // What bounds it: per 128 x 64 scores, S = Q K^T and O += P V keep the tensor pipe busy for 384 + 256 clk (head_dim 128; 192 +
 // 128 at 64), the 8192 exponentials the special-function units for 512 clk, and the softmax warps need about 1100 clk from
@@ -70,7 +70,8 @@ enum {
   M_SLOT = 256,                       // TMEM address, abort flag
   M_UNI = M_SLOT + 16,                // [2 buffers][2 tiles] flags, then the same of biases
   M_TAB = M_UNI + 32 + 208,           // 512: table column in log2 units
-  M_BUCKETS = M_TAB + FB_RELPOS_MAX_BUCKETS * 4,  // RelBuckets
+  M_PRE = M_TAB + FB_RELPOS_MAX_BUCKETS * 4,      // prefix maxima of the entries (relpos_prefix)
+  M_BUCKETS = M_PRE + FB_RELPOS_MAX_BUCKETS * 4,  // RelBuckets
   M_BIAS = M_BUCKETS + (int)sizeof(RelBuckets),   // [2][4][kCopyStride]
   M_BYTES = M_BIAS + 2 * 4 * kCopyStride * 4
 };
@@ -284,8 +285,9 @@ struct RelFwd {
     float* tab = reinterpret_cast<float*>(misc + M_TAB);
     RelBuckets& buckets = *reinterpret_cast<RelBuckets*>(misc + M_BUCKETS);
     for (int t = w * 32 + lane; t < rel.nb; t += 64)
-      tab[t] = relpos_entry<T>(rel, t, head) * kLog2e;
+      tab[t] = relpos_log2(relpos_entry<T>(rel, t, head));
     relpos_load_buckets(buckets, rel, w * 32 + lane, 64);
+    if (w == 1) relpos_prefix<T>(reinterpret_cast<float*>(misc + M_PRE), rel, head, lane);
     named_barrier_sync(1, 64);
     const RelFn bucket_of(rel, buckets);
     for (int it = 0; it < n_it; ++it) {
@@ -370,7 +372,7 @@ struct RelFwd {
     const float scale2 = p.scale * kLog2e;
     const float2 sc2 = make_float2(scale2, scale2);
     const int n = t ? n_of[1] : n_of[0];  // (a dynamic index would put the array into local memory)
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f, shift = 0.f, nshift2 = 0.f;
     // this row's staged biases: entry a + column, read 4 at a time from the copy that is aligned for it
     const int a = 2 * BM - 1 - (t * BM + row);
     const float* bias_row = reinterpret_cast<const float*>(misc + M_BIAS) + (a & 3) * kCopyStride + (a & ~3);
@@ -384,12 +386,19 @@ struct RelFwd {
         cmax = min(cmax, orow + off - c0);
       }
       warp_wait(BAR_S_FULL + 2 * t + buf, (it >> 1) & 1);
+      if (it == 0) {  // (both bias warps' tables are complete when they hand over block 0)
+        if (row_ok && (!p.causal || orow + off >= 0)) {
+          shift = relpos_shift<T>(reinterpret_cast<const float*>(misc + M_PRE), rel, RelFn(rel, *reinterpret_cast<const RelBuckets*>(misc + M_BUCKETS)), head,
+                                  -(orow + off), p.causal ? 0 : si.sk - 1 - (orow + off));
+          nshift2 = -relpos_log2(shift);
+        }
+      }
       tc_fence_after();
       uint32_t raw[BN / 32][32];
 #pragma unroll
       for (int q = 0; q < BN / 32; ++q) tmem_ld32(s_cols(t, buf) + lane_off + q * 32, raw[q]);
       const bool uni = reinterpret_cast<const int*>(misc + M_UNI)[2 * buf + t] != 0;
-      const float ub = reinterpret_cast<const float*>(misc + M_UNI + 16)[2 * buf + t];
+      const float ub = reinterpret_cast<const float*>(misc + M_UNI + 16)[2 * buf + t] + nshift2;
       tmem_ld_wait();
       float v[BN], mx;
 #pragma unroll
@@ -403,11 +412,12 @@ struct RelFwd {
         mx = row_max(v);
       } else {
         const float4* b4 = reinterpret_cast<const float4*>(bias_row + buf * 4 * kCopyStride);
+        const float2 ns2 = make_float2(nshift2, nshift2);
 #pragma unroll
         for (int c = 0; c < BN / 4; ++c) {
           const float4 b = b4[c];
-          const float2 x = __ffma2_rn(make_float2(v[4 * c], v[4 * c + 1]), sc2, make_float2(b.x, b.y));
-          const float2 y = __ffma2_rn(make_float2(v[4 * c + 2], v[4 * c + 3]), sc2, make_float2(b.z, b.w));
+          const float2 x = __ffma2_rn(make_float2(v[4 * c], v[4 * c + 1]), sc2, __fadd2_rn(make_float2(b.x, b.y), ns2));
+          const float2 y = __ffma2_rn(make_float2(v[4 * c + 2], v[4 * c + 3]), sc2, __fadd2_rn(make_float2(b.z, b.w), ns2));
           v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = y.x; v[4 * c + 3] = y.y;
         }
         if (need_mask) {
@@ -475,7 +485,11 @@ struct RelFwd {
     const float inv = l > 0.f ? 1.f / l : 0.f;
     const bool staged = r0 + (t + 1) * BM <= si.sq;
     const int64_t grow_ = si.q0 + orow;
-    if (p.lse && row_ok) p.lse[(int64_t)head * p.Tq + grow_] = l > 0.f ? m * kLn2 + logf(l) : -INFINITY;
+    if (p.lse && row_ok) {
+      const float lse = l > 0.f ? m * kLn2 + logf(l) : -INFINITY;  // less the shift
+      p.lse[(int64_t)head * p.Tq + grow_] = rel.shift ? lse : lse + shift;
+      if (rel.shift) rel.shift[(int64_t)head * p.Tq + grow_] = shift;
+    }
     write_out(t, row, lane_off, inv, staged, row_ok, grow_, n > 0, false);
     if (p.od.ptr) write_out(t, row, lane_off, inv, staged, row_ok, grow_, n > 0, true);
     tc_fence_before();

@@ -64,6 +64,7 @@ __device__ __forceinline__ void store_row(const SeqT& t, int head, int64_t row, 
 // table's gradient, one accumulator per warp and bucket.
 struct RelSmem {
   float tab[FB_RELPOS_MAX_BUCKETS];
+  float pre[FB_RELPOS_MAX_BUCKETS];  // forward: prefix maxima of the entries
   RelBuckets buckets;
   float acc[kWarps][FB_RELPOS_MAX_BUCKETS];
 };
@@ -108,6 +109,17 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
   if (p.causal) n_end = max(0, min(si.sk, m0 + kOwn + causal_off(p, si, m0 + kOwn - 1)));
 
   float lse[kRowsPerWarp];
+  [[maybe_unused]] float shift[kRowsPerWarp];  // see relpos_shift
+  if constexpr (BIAS) {
+    if (warp == 0) relpos_prefix<T>(rs->pre, rel, h, lane);
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kRowsPerWarp; ++r) {
+      const int at = m0 + warp * kRowsPerWarp + r + si.sk - si.sq;  // the row's position among the keys
+      shift[r] = 0.f;
+      if (at < si.sk && si.sk > 0 && (!p.causal || at >= 0)) shift[r] = relpos_shift<T>(rs->pre, rel, RelFn(rel, rs->buckets), h, -at, p.causal ? 0 : si.sk - 1 - at);
+    }
+  }
   if (p.lse_known) {
 #pragma unroll
     for (int r = 0; r < kRowsPerWarp; ++r) {
@@ -130,7 +142,7 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
         s *= p.scale;
         bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j));
         if constexpr (BIAS) {
-          if (ok) s += rs->tab[RelFn(rel, rs->buckets)(j - i - (si.sk - si.sq))];
+          if (ok) s += rs->tab[RelFn(rel, rs->buckets)(j - i - (si.sk - si.sq))] - shift[r];
           ok = ok && s != -INFINITY;  // a bias of -inf hides the pair
         }
         if (ok) {
@@ -178,7 +190,7 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
       s *= p.scale; sd *= p.scale;
       bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j)) && lse[r] != -INFINITY;
       if constexpr (BIAS) {
-        if (ok) s += rs->tab[RelFn(rel, rs->buckets)(j - i - (si.sk - si.sq))];
+        if (ok) s += rs->tab[RelFn(rel, rs->buckets)(j - i - (si.sk - si.sq))] - shift[r];
       }
       float pr = ok ? expf(s - lse[r]) : 0.f;
       float w = pr * sd;
@@ -218,7 +230,12 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
           store_row<T, D>(p.od, h, row, lane, low, 1.f);
         }
       }
-      if (lane == 0 && (!BIAS || p.lse)) p.lse[srow] = lse[r];
+      if constexpr (BIAS) {
+        if (lane == 0 && p.lse) p.lse[srow] = rel.shift ? lse[r] : lse[r] + shift[r];
+        if (lane == 0 && rel.shift) rel.shift[srow] = shift[r];
+      } else {
+        if (lane == 0) p.lse[srow] = lse[r];
+      }
     }
     float od[NC];
     if (TANGENT) {
@@ -298,12 +315,14 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p, const __gri
   if (p.causal) n_end = max(0, min(si.sk, m0 + kOwn + causal_off(p, si, m0 + kOwn - 1)));
 
   float lse[kRowsPerWarp], dps[kRowsPerWarp], z1[kRowsPerWarp], ddt[kRowsPerWarp];
+  [[maybe_unused]] float shift[kRowsPerWarp];
 #pragma unroll
   for (int r = 0; r < kRowsPerWarp; ++r) {
     int i = m0 + warp * kRowsPerWarp + r;
     bool ok = i < si.sq;
     int64_t srow = (int64_t)h * p.Tq + si.q0 + i;
     lse[r] = ok ? p.lse[srow] : -INFINITY;
+    if constexpr (BIAS) shift[r] = ok ? rel.shift[srow] : 0.f;
     if constexpr (BIAS) {  // D = rowsum(dO * O), also for the dK/dV kernel
       float d = 0.f;
       if (ok) {
@@ -362,7 +381,7 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p, const __gri
       [[maybe_unused]] int bucket = 0;
       if constexpr (BIAS) {
         bucket = RelFn(rel, rs->buckets)(j - i - (si.sk - si.sq));
-        if (ok) s += rs->tab[bucket];
+        if (ok) s += rs->tab[bucket] - shift[r];
       }
       float pr = ok ? expf(s - lse[r]) : 0.f;
       float a = dp - dps[r];
@@ -425,7 +444,7 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(Params p, const __gr
   float* qds = qs + kTile * LD;
   float* dos = qds + kTile * LD;
   float* dods = dos + kTile * LD;
-  float* st = dods + kTile * LD;  // [4][kTile]: lse, dpsum, z1, ddot
+  float* st = dods + kTile * LD;  // [4][kTile]: lse, dpsum, z1 (with a bias: shift), ddot
 
   const int b = blockIdx.z, hk = blockIdx.y, G = p.Hq / p.Hkv;
   const SeqInfo si = seq_info(p, b);
@@ -469,7 +488,8 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(Params p, const __gr
         int64_t srow = (int64_t)h * p.Tq + si.q0 + i;
         st[0 * kTile + threadIdx.x] = ok ? p.lse[srow] : -INFINITY;
         st[1 * kTile + threadIdx.x] = ok ? p.dpsum[srow] : 0.f;
-        st[2 * kTile + threadIdx.x] = (ok && TANGENT) ? p.z1[srow] : 0.f;
+        if constexpr (BIAS) st[2 * kTile + threadIdx.x] = ok ? rel.shift[srow] : 0.f;
+        else st[2 * kTile + threadIdx.x] = (ok && TANGENT) ? p.z1[srow] : 0.f;
         st[3 * kTile + threadIdx.x] = (ok && TANGENT) ? p.ddot[srow] : 0.f;
       }
       __syncthreads();
@@ -492,7 +512,7 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(Params p, const __gr
         const float lse = st[lane];
         bool ok = i < si.sq && j < si.sk && (!p.causal || j <= i + pair_off(p, si, i, j)) && lse != -INFINITY;
         if constexpr (BIAS) {
-          if (ok) s += rs->tab[RelFn(rel, rs->buckets)(j - i - (si.sk - si.sq))];
+          if (ok) s += rs->tab[RelFn(rel, rs->buckets)(j - i - (si.sk - si.sq))] - st[2 * kTile + lane];
         }
         float pr = ok ? expf(s - lse) : 0.f;
         float a = dp - st[kTile + lane];

@@ -405,6 +405,7 @@ struct TcCta {
   float m_used, l_sum, z_sum;   // FWD (l_sum, z_sum: this warpgroup's columns only)
   float lse2, dps, z1v, ddt;    // LSE-known FWD and DQ
   long long pw_wait, pw_work, pw_ld0, pw_st;
+  float nshift2;     // KIND_DQ with a bias: this row's shift, negated, in log2 units
   float2 rel_sum;    // KIND_DQ with a bias: running sum of dS over blocks that lie in bucket rel_cur altogether
   int rel_cur;
   int64_t rel_part;  // this tile's row of the partial table gradients
@@ -853,7 +854,7 @@ struct TcCta {
   }
 
   // ====================================== statistics stager (DKV only) ======================================
-  // Streamed query rows of block `it`: -lse*log2e, -dpsum, -z1, -ddot into one of two shared-memory
+  // Streamed query rows of block `it`: -lse*log2e, -dpsum, -z1 (with a bias -shift*log2e), -ddot into one of two shared-memory
   // buffers, handed to the pointwise warps through the block's S_FULL mbarrier (no separate wait, no
   // CTA-wide barrier in the main loop).
   // The global loads of block it+1 are issued before the wait for block it's buffer, so their latency
@@ -870,6 +871,7 @@ struct TcCta {
         v[r].x = p.lse[sr];
         v[r].y = p.dpsum[sr];
         if (TANGENT) { v[r].z = p.z1[sr]; v[r].w = p.ddot[sr]; }
+        if constexpr (BIAS) v[r].z = relpos_log2(rel->shift[sr]);
       }
     }
   }
@@ -878,7 +880,7 @@ struct TcCta {
   __device__ __forceinline__ void rel_load_table(int h) {
     float* tab = reinterpret_cast<float*>(rel_area + REL_TAB);
     for (int t = lane; t < rel->nb; t += 32)
-      tab[t] = relpos_entry<T>(*rel, t, h) * kLog2e;
+      tab[t] = relpos_log2(relpos_entry<T>(*rel, t, h));
     __syncwarp();
   }
   // BIAS: the biases of a block's positions. Entry u belongs to the pairs with (streamed row in block) - (owner row in
@@ -1347,7 +1349,9 @@ struct TcCta {
             if (c % 4 == 0) b4 = bias[(gi * CW + c) / 4];
             b2 = c % 4 == 0 ? make_float2(b4.x, b4.y) : make_float2(b4.z, b4.w);
           }
-          nl2 = __fadd2_rn(nl2, b2);
+          // the shift first: entry - shift is exact where it matters
+          const float2 ns2 = kDkv ? *reinterpret_cast<const float2*>(&stats[2 * BN + col]) : make_float2(nshift2, nshift2);
+          nl2 = __fadd2_rn(nl2, __fadd2_rn(b2, ns2));
         }
         const float2 e = __ffma2_rn(make_float2(__uint_as_float(bs[buf][c]), __uint_as_float(bs[buf][c + 1])), sc2, nl2);
         float2 pe = exp2_pair(e, c2, !need_mask);
@@ -1506,10 +1510,12 @@ struct TcCta {
 
     m_used = -INFINITY; l_sum = 0.f; z_sum = 0.f;
     lse2 = INFINITY; dps = 0.f; z1v = 0.f; ddt = 0.f;
+    nshift2 = 0.f;
     if ((kFwd && !FIRST) || kDq) {
       if (row_ok) {
         float lse = p.lse[srow];
         lse2 = (lse == -INFINITY) ? INFINITY : lse * kLog2e;
+        if constexpr (BIAS) nshift2 = -relpos_log2(rel->shift[srow]);
         if (kDq && !BIAS) {
           dps = p.dpsum[srow];
           if (TANGENT) { z1v = p.z1[srow]; ddt = p.ddot[srow]; }

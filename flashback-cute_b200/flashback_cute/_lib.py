@@ -121,6 +121,7 @@ class FbRelposFwdArgs(ctypes.Structure):
     _fields_ = [
         ("prob", FbProblem), ("bias", FbRelpos),
         ("q", FbTensor), ("k", FbTensor), ("v", FbTensor), ("out", FbTensor), ("out_low", FbTensor), ("lse", ctypes.c_void_p),
+        ("shift", ctypes.c_void_p),
     ]
 
 
@@ -131,7 +132,7 @@ class FbRelposBwdArgs(ctypes.Structure):
         ("lse", ctypes.c_void_p),
         ("dq", FbTensor), ("dk", FbTensor), ("dv", FbTensor),
         ("dtable", ctypes.c_void_p), ("dtable_bucket_stride", ctypes.c_int64), ("dtable_head_stride", ctypes.c_int64),
-        ("workspace", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("shift", ctypes.c_void_p),
     ]
 
 

@@ -152,9 +152,9 @@ def _address():
 
 _F, _B = _lib.FbRelposFwdArgs, _lib.FbRelposBwdArgs
 _FW = {n: _lib.word(_F, n, "ptr") for n in ("q", "k", "v", "out", "out_low")}
-_FW.update(table=_lib.word(_F, "bias", "table"), lse=_lib.word(_F, "lse"), cu_q=_lib.word(_F, "prob", "cu_seqlens_q"), cu_k=_lib.word(_F, "prob", "cu_seqlens_k"))
+_FW.update(table=_lib.word(_F, "bias", "table"), lse=_lib.word(_F, "lse"), shift=_lib.word(_F, "shift"), cu_q=_lib.word(_F, "prob", "cu_seqlens_q"), cu_k=_lib.word(_F, "prob", "cu_seqlens_k"))
 _BW = {n: _lib.word(_B, n, "ptr") for n in ("q", "k", "v", "out", "dout", "out_low", "dq", "dk", "dv")}
-_BW.update(table=_lib.word(_B, "bias", "table"), lse=_lib.word(_B, "lse"), cu_q=_lib.word(_B, "prob", "cu_seqlens_q"), cu_k=_lib.word(_B, "prob", "cu_seqlens_k"),
+_BW.update(table=_lib.word(_B, "bias", "table"), lse=_lib.word(_B, "lse"), shift=_lib.word(_B, "shift"), cu_q=_lib.word(_B, "prob", "cu_seqlens_q"), cu_k=_lib.word(_B, "prob", "cu_seqlens_k"),
            dtable=_lib.word(_B, "dtable"), work=_lib.word(_B, "workspace"))
 
 
@@ -181,7 +181,7 @@ class _AttnPlan:
         else:
             b, sq, sk = q_shape[0], q_shape[1], k_shape[1]
             total_q, total_k = b * sq, b * sk
-        self.total_q = total_q
+        self.total_q, self.stat_bytes = total_q, 4 * self.heads * total_q
         self.empty = 0 in q_shape or 0 in k_shape  # nothing is read, whatever the layouts
         self.copies = not (self.empty or (_strides_ok(q_shape, q_stride) and _strides_ok(k_shape, k_stride) and _strides_ok(k_shape, v_stride)))
         self.low = dtype != torch.float32
@@ -199,27 +199,28 @@ class _AttnPlan:
         self.work = _lib.load().fb_relpos_workspace_bytes(ctypes.byref(prob), table_shape[0]) // 4
 
     def forward(self, q, k, v, table, cu_q, cu_k, train: bool):
-        """(out, low, lse); the last two are None unless `train` (low: never for float32)."""
+        """(out, low, stats); the last two are None unless `train` (low: never for float32). stats: the rows' log-sum-exps and shifts."""
         out = torch.empty(self.q_shape, dtype=self.dtype, device=self.device)
-        low = lse = None
+        low = stats = None
         if train:
-            lse = torch.empty((self.heads, self.total_q), dtype=torch.float32, device=self.device)
+            stats = torch.empty((2, self.heads, self.total_q), dtype=torch.float32, device=self.device)
             if self.low:
                 low = torch.empty(self.q_shape, dtype=self.dtype, device=self.device)
         if self.empty:
-            return out.zero_(), low, lse
+            return out.zero_(), low, stats
         ptr, w, i = _address(), self.fwd[:], _FW
         w[i["q"]], w[i["k"]], w[i["v"]], w[i["table"]], w[i["out"]] = ptr(q), ptr(k), ptr(v), ptr(table), ptr(out)
-        if lse is not None:
-            w[i["lse"]] = ptr(lse)
+        if stats is not None:
+            w[i["lse"]] = at = ptr(stats)
+            w[i["shift"]] = at + self.stat_bytes
         if low is not None:
             w[i["out_low"]] = ptr(low)
         if cu_q is not None:
             w[i["cu_q"]], w[i["cu_k"]] = ptr(cu_q), ptr(cu_k)
         _lib.call_words("fb_relpos_fwd", w, self.index)
-        return out, low, lse
+        return out, low, stats
 
-    def backward(self, q, k, v, table, cu_q, cu_k, out, low, lse, dout, want):
+    def backward(self, q, k, v, table, cu_q, cu_k, out, low, stats, dout, want):
         """[dq, dk, dv, dtable], None where not wanted."""
         grads = [torch.empty(t.shape, dtype=self.dtype, device=self.device) if x else None for t, x in zip((q, k, v, table), want)]
         if self.empty:
@@ -230,7 +231,8 @@ class _AttnPlan:
         work = torch.empty(self.work, dtype=torch.float32, device=self.device)
         w, i = self.bwd[:], _BW
         w[i["q"]], w[i["k"]], w[i["v"]], w[i["table"]], w[i["out"]] = ptr(q), ptr(k), ptr(v), ptr(table), ptr(out)
-        w[i["dout"]], w[i["lse"]], w[i["work"]] = ptr(dout), ptr(lse), ptr(work)
+        at = ptr(stats)
+        w[i["dout"]], w[i["lse"]], w[i["shift"]], w[i["work"]] = ptr(dout), at, at + self.stat_bytes, ptr(work)
         if low is not None:
             w[i["out_low"]] = ptr(low)
         if cu_q is not None:
@@ -250,16 +252,16 @@ class _RelposAttnFunc(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, table, cu_q, cu_k, plan):
-        out, low, lse = plan.forward(q, k, v, table, cu_q, cu_k, True)
-        ctx.save_for_backward(q, k, v, table, cu_q, cu_k, out, low, lse)
+        out, low, stats = plan.forward(q, k, v, table, cu_q, cu_k, True)
+        ctx.save_for_backward(q, k, v, table, cu_q, cu_k, out, low, stats)
         ctx.plan = plan
         return out
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dout):
-        q, k, v, table, cu_q, cu_k, out, low, lse = ctx.saved_tensors
-        return (*ctx.plan.backward(q, k, v, table, cu_q, cu_k, out, low, lse, dout, ctx.needs_input_grad[:4]), None, None, None)
+        q, k, v, table, cu_q, cu_k, out, low, stats = ctx.saved_tensors
+        return (*ctx.plan.backward(q, k, v, table, cu_q, cu_k, out, low, stats, dout, ctx.needs_input_grad[:4]), None, None, None)
 
 
 class _RelposAttnTransformed(torch.autograd.Function):
@@ -278,8 +280,8 @@ class _RelposAttnTransformed(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, dout, *_):
-        q, k, v, table, cu_q, cu_k, out, low, lse = map(_raw, ctx.saved_tensors)
-        return (*ctx.plan.backward(q, k, v, table, cu_q, cu_k, out, low, lse, _raw(dout), ctx.needs_input_grad[:4]), None, None, None)
+        q, k, v, table, cu_q, cu_k, out, low, stats = map(_raw, ctx.saved_tensors)
+        return (*ctx.plan.backward(q, k, v, table, cu_q, cu_k, out, low, stats, _raw(dout), ctx.needs_input_grad[:4]), None, None, None)
 
 
 def _attention(q, k, v, table, cu_q, cu_k, max_q, max_k, max_distance, scale, causal, two):

@@ -315,9 +315,14 @@ typedef struct {
   fb_tensor out;     /* out */
   fb_tensor out_low; /* out, optional */
   float* lse;        /* out, optional, [heads_q][total_q], -inf on fully masked rows */
+  float* shift;      /* out, optional, [heads_q][total_q], see below */
 } fb_relpos_fwd_args;
 
 int fb_relpos_fwd(const fb_relpos_fwd_args* args, fb_stream_t stream);
+
+/* shift: the largest table entry that the row's keys have (0 where they have none but hidden ones). With it, `lse` is the log-sum-exp
+ * of the row's scores LESS its shift; without it, of the scores. The kernels work on scores less the shift throughout, and the backward wants the two
+ * numbers apart: beside an entry of 1e6 a float32 has no room for the scores. */
 
 /* First-order backward (total_q, total_k > 0). dq, dk, dv and dtable (problem dtype, the table's shape) are optional outputs. `workspace`
  * (fb_relpos_workspace_bytes, 16-byte aligned, contents irrelevant before and after) holds D = rowsum(dO * (out + out_low)) and the
@@ -332,6 +337,7 @@ typedef struct {
   void* dtable;            /* out, optional */
   int64_t dtable_bucket_stride, dtable_head_stride;
   float* workspace;
+  const float* shift;      /* in, of the forward that wrote lse */
 } fb_relpos_bwd_args;
 
 int fb_relpos_bwd(const fb_relpos_bwd_args* args, fb_stream_t stream);

@@ -14,6 +14,10 @@ also what D is computed from).
     D                       dD = u rowsum(|dO| |O|) + (1 + u) (rowsum(|dO| (u + ep + n e) P|V|) + d e |dO| |O|)
     dS                      ds = |dS| ep + P (dD + d e |dO|.|V| )
     dQ                      c (ds + (u + n e) |dS|) |K| + u |dQ|;  dK, dV, dT alike (dT has no operand rounding)
+`apart`: the scores are formed as c q.k + (T - top), top the largest entry that the row's keys have, so that |T - top| takes the place of |T|:
+    |dS_ij| <= es_ij = (d + 8) e c |q|.|k| + 2^10 e |T - top|     two entries that differ do so by 2^-8 (bf16) of the larger or more, so that their own
+                                                                   roundings to log2 units, 2 e |T| each, are within 2^9 e |T - top| each
+    P, relative             ep_ij = es_ij + sum_j P_ij es_ij + 16 e
 float16 operands (P, dS) below 2^-14 are subnormal: their rounding is off by up to half a step of 2^-24, an absolute w = 2^-25 beside
 the relative u. It adds w rowsum(|V|) to O, c w rowsum(|K|) to dQ, and so on; 0 for the other types, whose range is float32's.
 """
@@ -59,7 +63,7 @@ class Head(NamedTuple):
     tol_dt: Optional[torch.Tensor]
 
 
-def head(q, k, v, table, which, scale, causal, u, dout=None, w=0.0) -> Head:
+def head(q, k, v, table, which, scale, causal, u, dout=None, w=0.0, apart=False) -> Head:
     """q (sq, d), k/v (sk, d), table (num,), which (sq, sk) long; everything float64 on one device."""
     e = 2.0 ** -24
     sq, sk, d = q.shape[0], k.shape[0], q.shape[1]
@@ -75,10 +79,16 @@ def head(q, k, v, table, which, scale, causal, u, dout=None, w=0.0) -> Head:
     out = p @ v
     mag = (abs(scale) * (q.abs() @ k.abs().T) + b.abs()).masked_fill(hidden | (s == -math.inf), 0.0)
     es = (d + 8) * e * mag
+    if apart:
+        seen_b = b.masked_fill(hidden | (s == -math.inf), -math.inf)
+        top = seen_b.amax(-1, keepdim=True) if sk else torch.zeros(sq, 1, dtype=q.dtype, device=q.device)
+        es = (d + 8) * e * abs(scale) * (q.abs() @ k.abs().T) + 2.0 ** 10 * e * (b - top).abs()
+        es = es.masked_fill(seen_b == -math.inf, 0.0)
     ep = (2 * es.amax(-1, keepdim=True) + 16 * e) if sk else torch.zeros(sq, 1, dtype=q.dtype, device=q.device)
-    pv = p @ v.abs()
+    if apart:
+        ep = es + (p * es).sum(-1, keepdim=True) + 16 * e
     seen = (p > 0).to(q.dtype)
-    tol_out = (u + ep + sk * e) * pv + w * (seen @ v.abs()) + u * out.abs() * (1 + 2 * u)
+    tol_out = (p * (u + ep + sk * e)) @ v.abs() + w * (seen @ v.abs()) + u * out.abs() * (1 + 2 * u)
     if dout is None:
         return Head(out, None, None, None, None, tol_out, None, None, None, None)
     g = dout
@@ -109,7 +119,7 @@ class Result(NamedTuple):
     tol: tuple  # bounds for (out, dq, dk, dv, dt)
 
 
-def attention(q, k, v, table, far, two, scale, causal, dout=None, lens_q=None, lens_k=None) -> Result:
+def attention(q, k, v, table, far, two, scale, causal, dout=None, lens_q=None, lens_k=None, apart=False) -> Result:
     """Dense (b, s, h, d), or packed (total, h, d) with lens_q, lens_k; inputs of any type, results float64."""
     u = torch.finfo(q.dtype).eps / 2
     packed = q.dim() == 3
@@ -132,7 +142,7 @@ def attention(q, k, v, table, far, two, scale, causal, dout=None, lens_q=None, l
         sl, kl = slice(iq, iq + nq), slice(ik, ik + nk)
         for h in range(q.shape[1]):
             hk = h // group
-            r = head(q[sl, h], k[kl, hk], v[kl, hk], table[:, h], which, scale, causal, u, None if dout is None else dout[sl, h], w)
+            r = head(q[sl, h], k[kl, hk], v[kl, hk], table[:, h], which, scale, causal, u, None if dout is None else dout[sl, h], w, apart)
             out[sl, h], tol_out[sl, h] = r.out, r.tol_out
             if dout is not None:
                 dq[sl, h], tol_dq[sl, h] = r.dq, r.tol_dq

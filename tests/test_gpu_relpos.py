@@ -708,3 +708,86 @@ def test_decode_keys_of_later_tokens_may_hold_anything(d):
             broken[i, n - 2:n] = bad  # the keys of tokens 2 and 3
         got = flashback_attn_relpos_decode(q, broken, v, torch.tensor(lens, dtype=torch.int32, device=DEV), table)
         _within("out", got[:, :2], want[:, :2], tol[:, :2])
+
+
+# ---------------------------------------------------------------------------------------------
+# very large entries
+# ---------------------------------------------------------------------------------------------
+LARGE = {BF16: (1e3, 1e5, -1e9, -1.2e30, 3e38), F16: (3e3, -6e4, 65504.0), F32: (1e5 + 0.3, -1e9, -1.2e30, 3.3e38)}
+
+
+def _results(dtype, d, hq, hkv, causal, sq, sk, table, two, packed=None):
+    if packed:
+        q, k, v, do = (_mk((sum(n), h, d), dtype, i) for i, (n, h) in enumerate(zip((packed, packed, packed, packed), (hq, hkv, hkv, hq))))
+        cu = torch.tensor([0, *itertools.accumulate(packed)], dtype=torch.int32, device=DEV)
+        call = lambda *a: flashback_attn_relpos_varlen_func(*a, cu, cu, max(packed), max(packed), causal=causal, bidirectional=two)  # noqa: E731
+    else:
+        q, k, v, do = (_mk((2, s, h, d), dtype, i) for i, (s, h) in enumerate(((sq, hq), (sk, hkv), (sk, hkv), (sq, hq))))
+        call = lambda *a: flashback_attn_relpos_func(*a, causal=causal, bidirectional=two)  # noqa: E731
+    leaves = [t.requires_grad_() for t in (q, k, v, table.clone())]
+    out = call(*leaves)
+    return (q, k, v, do), (out.detach(), *torch.autograd.grad(out, leaves, do))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_a_constant_table_is_no_bias(dtype, d):
+    """Softmax does not see a constant: the same bits as without a bias, however large the constant."""
+    for causal, two, sq, sk, packed in ((True, False, 150, 211, None), (False, True, 211, 150, None), (False, False, 90, 300, None), (True, False, 0, 0, [70, 1, 130])):
+        zero = torch.zeros(32, 4, dtype=dtype, device=DEV)
+        want = _results(dtype, d, 4, 2, causal, sq, sk, zero, two, packed)[1]
+        for c in LARGE[dtype]:
+            got = _results(dtype, d, 4, 2, causal, sq, sk, zero + torch.tensor(c, dtype=dtype), two, packed)[1]
+            assert all(torch.equal(a, b) for a, b in zip(got, want)), c
+
+
+def large_tables(dtype, num, heads):
+    """Entries that hide softly, that only some rows' keys have, that no key has, and a mixture of all sizes."""
+    big = 6e4 if dtype == F16 else 1e6
+    first, near, last, mixed = (_mk((num, heads), dtype, 20 + i) for i in range(4))
+    first[0] = -big                       # the query's own position: the first causal row sees nothing else
+    near[num // 2 + 1] = big              # r = 1: rows far ahead of the first key do not see it
+    near[num - 1] = -big
+    last[num // 2 - 1], last[num - 1] = big, -0.5 * big
+    sizes = torch.tensor([0.0, 1.0, -1.0, big, -big, 0.1 * big, -0.1 * big, 0.01 * big], device=DEV)
+    mixed = (mixed.float() + sizes[torch.randint(8, mixed.shape, generator=torch.Generator(device=DEV).manual_seed(5), device=DEV)]).clamp(-65504, 65504 if dtype == F16 else 1e7).to(dtype)
+    return [first, near, last, mixed]
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_large_entries(dtype, d):
+    """Rows whose keys all have entries of about the same size, whatever it is: bounds that do not grow with it."""
+    for which in range(4):
+        for causal, two, sq, sk in ((True, False, 150, 150), (True, True, 70, 200), (False, True, 200, 70), (False, True, 130, 260), (False, False, 120, 90)):
+            table = large_tables(dtype, 32, 4)[which]
+            (q, k, v, do), got = _results(dtype, d, 4, 2, causal, sq, sk, table, two)
+            ref = orc.attention(q, k, v, table, 128, two, d ** -0.5, causal, do, apart=True)
+            for name, a, b, tol in zip(("out", "dq", "dk", "dv", "dtable"), got, ref[:5], ref.tol):
+                _within(f"{name} table {which} causal {causal} two {two} {sq} x {sk}", a, b, tol)
+
+
+def test_the_first_row_under_a_large_own_entry():
+    """It sees one key: P = 1, O = V, and dV has all of dO."""
+    for dtype in (BF16, F16, F32):
+        for c in LARGE[dtype]:
+            table = torch.zeros(32, 4, dtype=dtype, device=DEV)
+            table[0] = c
+            (q, k, v, do), (out, dq, dk, dv, dt) = _results(dtype, 64, 4, 4, True, 1, 1, table, False)
+            assert torch.equal(out, v.detach()) and torch.equal(dv, do)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_decode_large_entries(dtype):
+    from flashback_cute import flashback_attn_relpos_decode
+
+    q, k, v, lens = _mk((3, 3, 8, 64), dtype, 0), _mk((3, 9000, 2, 64), dtype, 1), _mk((3, 9000, 2, 64), dtype, 2), [9000, 2, 140]
+    on = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    want = flashback_attn_relpos_decode(q, k, v, on, torch.zeros(32, 8, dtype=dtype, device=DEV))
+    for c in LARGE[dtype]:
+        assert torch.equal(flashback_attn_relpos_decode(q, k, v, on, torch.full((32, 8), c, dtype=dtype, device=DEV)), want), c
+    for table in large_tables(dtype, 32, 8):
+        got = flashback_attn_relpos_decode(q[1:], k[1:], v[1:], on[1:], table)
+        for i, n in enumerate(lens[1:]):
+            r = orc.attention(q[1 + i:2 + i], k[1 + i:2 + i, :n], v[1 + i:2 + i, :n], table, 128, False, 0.125, True, apart=True)
+            _within("out", got[i:i + 1], r.out, r.tol[0])

@@ -206,3 +206,21 @@ def test_decode_long_caches_join_through_the_workspace():
         for sk in (40, 1000, 8192):
             if base < 296:
                 assert floats(batch, hkv, sk) == 0
+
+
+def test_the_backward_wants_the_shifts():
+    lib = _lib.load()
+    t = _lib.FbTensor(0x1000, 128, 64)
+    bwd = _lib.FbRelposBwdArgs(prob=_prob(), bias=_bias(), q=t, k=t, v=t, out=t, dout=t, lse=0x1000, dtable=0x1000, workspace=0x1000)
+    assert lib.fb_relpos_bwd(ctypes.byref(bwd), None) == -1
+
+
+def test_bounds_apart_from_the_entries_size():
+    """The oracle's bounds for scores less the row's largest entry: those of a table without the common part, where the others grow with it."""
+    torch.manual_seed(1)
+    q, k, v, do = torch.randn(1, 9, 2, 64), torch.randn(1, 13, 2, 64), torch.randn(1, 13, 2, 64), torch.randn(1, 9, 2, 64)
+    table = torch.randn(8, 2).bfloat16().float()
+    far = lambda c, apart: orc.attention(q, k, v, table.double() + c, 5, True, 0.125, False, do, apart=apart).tol  # noqa: E731
+    small, large = far(0.0, True), far(2.0 ** 24, True)
+    for a, b, loose in zip(small, large, far(2.0 ** 24, False)):
+        assert torch.allclose(a, b, rtol=1e-6) and (loose >= 10 * b).all()  # (buckets without a pair: 0)
