@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
   uint8_t* const qs = smem;                       // [R][D]
   uint8_t* const stages = smem + R * D * 2;       // per warp [kStages][K, V]
   __shared__ RelBuckets buckets;
-  __shared__ float s_m[NW][R], s_l[NW][R];
+  __shared__ float s_m[NW][R], s_l[NW][R], s_shift[R];
   __shared__ float2 joint_ml[R];
   float* const tab = reinterpret_cast<float*>(smem + R * D * 2 + NW * kWarpBytes);  // [heads of the CTA's rows][nb], log2 units
 
@@ -130,9 +130,12 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
   for (int i = 0; i < kStages - 1; ++i) load(i);
 
   // the table's columns of this kv head's query heads
+  bool large = false;
   for (int at = threadIdx.x; at < p.G * rel.nb; at += NT) {
     const int g = at / rel.nb, t = at - g * rel.nb;
-    tab[at] = relpos_log2(relpos_entry<T>(rel, t, hk * p.G + g));
+    const float x = relpos_entry<T>(rel, t, hk * p.G + g);
+    large = large || relpos_large(x);
+    tab[at] = relpos_log2(x);
   }
   // the queries: row x of the CTA is new token (rt * R + x) / G, query head hk * G + (rt * R + x) % G
   for (int at = threadIdx.x; at < R * U; at += NT) {
@@ -144,11 +147,28 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
     }
     *reinterpret_cast<uint4*>(qs + unit_off<D>(x, u)) = v;
   }
-  __syncthreads();
+  large = __syncthreads_or(large) != 0;
+
+  const RelFn bucket_of(rel, buckets);
+  if (large) {  // the rows' shifts (fb_params.h): the largest entry of the buckets up to the first key's, a warp per row
+#pragma unroll 1
+    for (int x = warp; x < R; x += NW) {
+      const int row = min(rt * R + x, rows - 1), t = row / p.G, at = len - p.Sq + t;
+      float top = -INFINITY;
+      if (at >= 0) {
+        const int last = bucket_of(-at);
+        for (int u = lane; u <= last; u += 32)
+          if (rel.used[u >> 5] >> (u & 31) & 1u) top = fmaxf(top, tab[(row - t * p.G) * rel.nb + u]);
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (lane == 0) s_shift[x] = top == -INFINITY ? 0.f : top;
+    }
+    __syncthreads();
+  }
 
   // this thread's rows of the MMA fragments: lane / 4 and lane / 4 + 8 of every 16
   const float scale2 = p.scale * kLog2e;
-  const RelFn bucket_of(rel, buckets);
   int pos[MT][2];
   const float* row_tab[MT][2];
   float far_bias[MT][2], shift[MT][2], m[MT][2], l[MT][2];
@@ -161,14 +181,7 @@ __global__ void __launch_bounds__(NW * 32) decode_kernel(const __grid_constant__
       const int t = row / p.G;
       row_tab[mt][x] = tab + (row - t * p.G) * rel.nb;
       pos[mt][x] = len - p.Sq + t;  // the new token's place in its sequence
-      // the row's shift (relpos_shift): the largest entry of the buckets up to its first key's; the four lanes of a row share the work
-      float top = -INFINITY;
-      if (pos[mt][x] >= 0)
-        for (int u = lane & 3, last = bucket_of(-pos[mt][x]); u <= last; u += 4)
-          if (rel.used[u >> 5] >> (u & 31) & 1u) top = fmaxf(top, row_tab[mt][x][u]);
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      shift[mt][x] = top == -INFINITY ? 0.f : top;
+      shift[mt][x] = large ? s_shift[mt * 16 + lane / 4 + 8 * x] : 0.f;
       far_bias[mt][x] = row_tab[mt][x][rel.side - 1] - shift[mt][x];
       m[mt][x] = -INFINITY;
       l[mt][x] = 0.f;

@@ -137,6 +137,10 @@ __device__ __forceinline__ float relpos_log2(float x) {
 // The shift of a row: the largest entry that its keys have. Scores are formed as c q.k + (entry - shift): the difference is exact where it
 // matters, while beside an entry of 1e6 the sum would have no room for c q.k, and neither would a log-sum-exp for what the backward needs.
 //
+// Where no entry of the head is larger than kRelLarge the shifts are 0: there the sum is good to 2^-18, and the look-ups (they cost 4 % of a
+// packed prompt's time, and 15 % of the drafted tokens') are left out.
+constexpr float kRelLarge = 64.f;
+__device__ __forceinline__ bool relpos_large(float x) { return fabsf(x) > kRelLarge && fabsf(x) != INFINITY; }
 // Prefix maxima of a head's entries over the buckets of each side that some distance falls in, by one warp.
 template <typename T>
 __device__ __forceinline__ void relpos_prefix(float* pre, const RelPos& rel, int head, int lane) {

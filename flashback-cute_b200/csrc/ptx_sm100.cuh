@@ -291,6 +291,13 @@ __device__ __forceinline__ float2 ex2_poly2(float2 x) {
 __device__ __forceinline__ void named_barrier_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }
+// The same; true where any of the threads passes true.
+__device__ __forceinline__ bool named_barrier_or(int id, int nthreads, bool x) {
+  int r;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.s32 p, %3, 0;\n\tbarrier.cta.red.or.pred q, %1, %2, p;\n\tselp.s32 %0, 1, 0, q;\n\t}"
+               : "=r"(r) : "r"(id), "r"(nthreads), "r"((int)x) : "memory");
+  return r != 0;
+}
 __device__ __forceinline__ void named_barrier_arrive(int id, int nthreads) {
   asm volatile("bar.arrive %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
 }

@@ -68,12 +68,14 @@ enum {
 // Bytes behind the tiles
 enum {
   M_SLOT = 256,                       // TMEM address, abort flag
-  M_UNI = M_SLOT + 16,                // [2 buffers][2 tiles] flags, then the same of biases
+  M_UNI = M_SLOT + 16,                // [2 buffers][2 tiles] kinds of blocks, then the same of biases
+  M_LARGE = M_UNI + 32,               // 1: the rows have shifts
   M_TAB = M_UNI + 32 + 208,           // 512: table column in log2 units
   M_PRE = M_TAB + FB_RELPOS_MAX_BUCKETS * 4,      // prefix maxima of the entries (relpos_prefix)
   M_BUCKETS = M_PRE + FB_RELPOS_MAX_BUCKETS * 4,  // RelBuckets
   M_BIAS = M_BUCKETS + (int)sizeof(RelBuckets),   // [2][4][kCopyStride]
-  M_BYTES = M_BIAS + 2 * 4 * kCopyStride * 4
+  M_SHIFT = M_BIAS + 2 * 4 * kCopyStride * 4,     // [2 tiles][BM] the rows' shifts, negated, in log2 units (each read by the thread that wrote it)
+  M_BYTES = M_SHIFT + 2 * BM * 4
 };
 static_assert(M_TAB == 512 && M_BIAS % 16 == 0, "layout");
 
@@ -87,6 +89,9 @@ struct FwdCfg {
   static_assert(smemBytes <= 232448, "shared memory");
   static constexpr int tmemCols = 512;  // 2 x (2 x 64 scores + D): 384 at head_dim 64, and allocations are powers of two
 };
+
+// Kinds of blocks: one bias for all pairs; the rows have shifts
+enum { BLK_SHIFTED = 1, BLK_ONE = 2 };
 
 struct FwdMaps {
   CUtensorMap q, k, v, o, lo;
@@ -284,11 +289,19 @@ struct RelFwd {
   __device__ __forceinline__ void bias_warp(int w) {
     float* tab = reinterpret_cast<float*>(misc + M_TAB);
     RelBuckets& buckets = *reinterpret_cast<RelBuckets*>(misc + M_BUCKETS);
-    for (int t = w * 32 + lane; t < rel.nb; t += 64)
-      tab[t] = relpos_log2(relpos_entry<T>(rel, t, head));
+    bool large = false;
+    for (int t = w * 32 + lane; t < rel.nb; t += 64) {
+      const float x = relpos_entry<T>(rel, t, head);
+      large = large || relpos_large(x);
+      tab[t] = relpos_log2(x);
+    }
     relpos_load_buckets(buckets, rel, w * 32 + lane, 64);
-    if (w == 1) relpos_prefix<T>(reinterpret_cast<float*>(misc + M_PRE), rel, head, lane);
-    named_barrier_sync(1, 64);
+    large = named_barrier_or(1, 64, large);
+    if (w == 1) {
+      if (large) relpos_prefix<T>(reinterpret_cast<float*>(misc + M_PRE), rel, head, lane);
+      if (lane == 0) *reinterpret_cast<int*>(misc + M_LARGE) = large;
+    }
+    const int shifted = large ? BLK_SHIFTED : 0;
     const RelFn bucket_of(rel, buckets);
     for (int it = 0; it < n_it; ++it) {
       const int buf = it & 1;
@@ -320,7 +333,7 @@ struct RelFwd {
       if (w == 0 && lane == 0) {
         int* flag = reinterpret_cast<int*>(misc + M_UNI) + 2 * buf;
         float* val = reinterpret_cast<float*>(misc + M_UNI + 16) + 2 * buf;
-        flag[0] = uni0; flag[1] = uni1;
+        flag[0] = (uni0 ? BLK_ONE : 0) | shifted; flag[1] = (uni1 ? BLK_ONE : 0) | shifted;
         val[0] = v0; val[1] = v1;
       }
       if (!(uni0 && uni1)) {
@@ -372,7 +385,8 @@ struct RelFwd {
     const float scale2 = p.scale * kLog2e;
     const float2 sc2 = make_float2(scale2, scale2);
     const int n = t ? n_of[1] : n_of[0];  // (a dynamic index would put the array into local memory)
-    float m = -INFINITY, l = 0.f, shift = 0.f, nshift2 = 0.f;
+    float m = -INFINITY, l = 0.f;
+    float* const nshift2 = reinterpret_cast<float*>(misc + M_SHIFT) + t * BM + row;
     // this row's staged biases: entry a + column, read 4 at a time from the copy that is aligned for it
     const int a = 2 * BM - 1 - (t * BM + row);
     const float* bias_row = reinterpret_cast<const float*>(misc + M_BIAS) + (a & 3) * kCopyStride + (a & ~3);
@@ -386,19 +400,17 @@ struct RelFwd {
         cmax = min(cmax, orow + off - c0);
       }
       warp_wait(BAR_S_FULL + 2 * t + buf, (it >> 1) & 1);
-      if (it == 0) {  // (both bias warps' tables are complete when they hand over block 0)
-        if (row_ok && (!p.causal || orow + off >= 0)) {
-          shift = relpos_shift<T>(reinterpret_cast<const float*>(misc + M_PRE), rel, RelFn(rel, *reinterpret_cast<const RelBuckets*>(misc + M_BUCKETS)), head,
-                                  -(orow + off), p.causal ? 0 : si.sk - 1 - (orow + off));
-          nshift2 = -relpos_log2(shift);
-        }
-      }
       tc_fence_after();
       uint32_t raw[BN / 32][32];
 #pragma unroll
       for (int q = 0; q < BN / 32; ++q) tmem_ld32(s_cols(t, buf) + lane_off + q * 32, raw[q]);
-      const bool uni = reinterpret_cast<const int*>(misc + M_UNI)[2 * buf + t] != 0;
-      const float ub = reinterpret_cast<const float*>(misc + M_UNI + 16)[2 * buf + t] + nshift2;
+      const int kind = reinterpret_cast<const int*>(misc + M_UNI)[2 * buf + t];
+      const bool uni = (kind & BLK_ONE) != 0;
+      float ub = reinterpret_cast<const float*>(misc + M_UNI + 16)[2 * buf + t];
+      if (kind & BLK_SHIFTED) {
+        if (it == 0) *nshift2 = -relpos_log2(row_shift(orow));  // (both bias warps' tables are complete when they hand over block 0)
+        ub += *nshift2;
+      }
       tmem_ld_wait();
       float v[BN], mx;
 #pragma unroll
@@ -412,14 +424,20 @@ struct RelFwd {
         mx = row_max(v);
       } else {
         const float4* b4 = reinterpret_cast<const float4*>(bias_row + buf * 4 * kCopyStride);
-        const float2 ns2 = make_float2(nshift2, nshift2);
+        auto add_bias = [&](auto shifted) {
+          const float2 ns2 = decltype(shifted)::value ? make_float2(*nshift2, *nshift2) : make_float2(0.f, 0.f);
 #pragma unroll
-        for (int c = 0; c < BN / 4; ++c) {
-          const float4 b = b4[c];
-          const float2 x = __ffma2_rn(make_float2(v[4 * c], v[4 * c + 1]), sc2, __fadd2_rn(make_float2(b.x, b.y), ns2));
-          const float2 y = __ffma2_rn(make_float2(v[4 * c + 2], v[4 * c + 3]), sc2, __fadd2_rn(make_float2(b.z, b.w), ns2));
-          v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = y.x; v[4 * c + 3] = y.y;
-        }
+          for (int c = 0; c < BN / 4; ++c) {
+            const float4 b = b4[c];
+            float2 lo = make_float2(b.x, b.y), hi = make_float2(b.z, b.w);
+            if (decltype(shifted)::value) { lo = __fadd2_rn(lo, ns2); hi = __fadd2_rn(hi, ns2); }
+            const float2 x = __ffma2_rn(make_float2(v[4 * c], v[4 * c + 1]), sc2, lo);
+            const float2 y = __ffma2_rn(make_float2(v[4 * c + 2], v[4 * c + 3]), sc2, hi);
+            v[4 * c] = x.x; v[4 * c + 1] = x.y; v[4 * c + 2] = y.x; v[4 * c + 3] = y.y;
+          }
+        };
+        if (kind & BLK_SHIFTED) add_bias(std::true_type{});
+        else add_bias(std::false_type{});
         if (need_mask) {
 #pragma unroll
           for (int c = 0; c < BN; ++c) if (c > cmax) v[c] = -INFINITY;
@@ -486,13 +504,19 @@ struct RelFwd {
     const bool staged = r0 + (t + 1) * BM <= si.sq;
     const int64_t grow_ = si.q0 + orow;
     if (p.lse && row_ok) {
-      const float lse = l > 0.f ? m * kLn2 + logf(l) : -INFINITY;  // less the shift
+      const float lse = l > 0.f ? m * kLn2 + logf(l) : -INFINITY, shift = n > 0 ? row_shift(orow) : 0.f;  // less the shift
       p.lse[(int64_t)head * p.Tq + grow_] = rel.shift ? lse : lse + shift;
       if (rel.shift) rel.shift[(int64_t)head * p.Tq + grow_] = shift;
     }
     write_out(t, row, lane_off, inv, staged, row_ok, grow_, n > 0, false);
     if (p.od.ptr) write_out(t, row, lane_off, inv, staged, row_ok, grow_, n > 0, true);
     tc_fence_before();
+  }
+  // The shift of query row `i` of the sequence (0 for a row behind it).
+  __device__ __forceinline__ float row_shift(int i) const {
+    if (*reinterpret_cast<const int*>(misc + M_LARGE) == 0 || i >= si.sq || (p.causal && i + off < 0)) return 0.f;
+    return relpos_shift<T>(reinterpret_cast<const float*>(misc + M_PRE), rel, RelFn(rel, *reinterpret_cast<const RelBuckets*>(misc + M_BUCKETS)), head,
+                           -(i + off), p.causal ? 0 : si.sk - 1 - (i + off));
   }
   __device__ __forceinline__ static float row_max(const float (&v)[BN]) {
     float mx[4] = {v[0], v[1], v[2], v[3]};

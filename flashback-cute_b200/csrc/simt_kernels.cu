@@ -111,13 +111,16 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
   float lse[kRowsPerWarp];
   [[maybe_unused]] float shift[kRowsPerWarp];  // see relpos_shift
   if constexpr (BIAS) {
-    if (warp == 0) relpos_prefix<T>(rs->pre, rel, h, lane);
-    __syncthreads();
+    const bool large = __syncthreads_or((int)threadIdx.x < rel.nb && relpos_large(rs->tab[threadIdx.x]));  // (each thread its own entry)
+    if (large) {
+      if (warp == 0) relpos_prefix<T>(rs->pre, rel, h, lane);
+      __syncthreads();
+    }
 #pragma unroll
     for (int r = 0; r < kRowsPerWarp; ++r) {
       const int at = m0 + warp * kRowsPerWarp + r + si.sk - si.sq;  // the row's position among the keys
       shift[r] = 0.f;
-      if (at < si.sk && si.sk > 0 && (!p.causal || at >= 0)) shift[r] = relpos_shift<T>(rs->pre, rel, RelFn(rel, rs->buckets), h, -at, p.causal ? 0 : si.sk - 1 - at);
+      if (large && at < si.sk && si.sk > 0 && (!p.causal || at >= 0)) shift[r] = relpos_shift<T>(rs->pre, rel, RelFn(rel, rs->buckets), h, -at, p.causal ? 0 : si.sk - 1 - at);
     }
   }
   if (p.lse_known) {

@@ -71,7 +71,8 @@ enum {                             // byte offsets in the bias area behind the m
   REL_TAB = 0,                                     // this head's table column, in log2 units
   REL_BUCKETS = REL_TAB + FB_RELPOS_MAX_BUCKETS * 4,  // RelBuckets
   REL_UNI = REL_BUCKETS + (int)sizeof(RelBuckets),  // [2] the bucket all pairs of the block fall in, or -1; [2] its bias
-  REL_BIAS = REL_UNI + 16,                         // [2][4][kRelCopy]: four copies, each shifted by one entry more
+  REL_SHIFTED = REL_UNI + 16,                      // [2] whether the block's rows have shifts
+  REL_BIAS = REL_SHIFTED + 16,                     // [2][4][kRelCopy]: four copies, each shifted by one entry more
   REL_IDS = REL_BIAS + 2 * 4 * kRelCopy * 4,       // [2][kRelSpan] (KIND_DQ)
   REL_DIAG = REL_IDS + 2 * kRelSpan * 4,           // [pointwise warps][32] (KIND_DQ)
   REL_ROWDOT = REL_DIAG + NWG * 4 * 32 * 4,        // [BM] (KIND_DQ)
@@ -877,11 +878,16 @@ struct TcCta {
   }
   // BIAS: this head's column of the table (in log2 units) and the bucket starts, once per head. A DKV CTA walks
   // through the query heads of its kv head.
-  __device__ __forceinline__ void rel_load_table(int h) {
+  // Returns whether the head's rows have shifts (as the forward decided from the same entries).
+  __device__ __forceinline__ bool rel_load_table(int h) {
     float* tab = reinterpret_cast<float*>(rel_area + REL_TAB);
-    for (int t = lane; t < rel->nb; t += 32)
-      tab[t] = relpos_log2(relpos_entry<T>(*rel, t, h));
-    __syncwarp();
+    bool large = false;
+    for (int t = lane; t < rel->nb; t += 32) {
+      const float x = relpos_entry<T>(*rel, t, h);
+      large = large || relpos_large(x);
+      tab[t] = relpos_log2(x);
+    }
+    return __any_sync(0xffffffffu, large) != 0;
   }
   // BIAS: the biases of a block's positions. Entry u belongs to the pairs with (streamed row in block) - (owner row in
   // tile) = u - (BM - 1). Where the block's first and last position share a bucket all pairs do (the usual case far from
@@ -915,8 +921,9 @@ struct TcCta {
       for (int i = 0; i < kRelSpan / 32; ++i) o.bias[i] = tab[o.ids[i]];
     }
   }
-  __device__ __forceinline__ void rel_store_staged(int buf, const RelStaged& o) const {
+  __device__ __forceinline__ void rel_store_staged(int buf, const RelStaged& o, bool shifted) const {
     if (lane == 0) {
+      reinterpret_cast<int*>(rel_area + REL_SHIFTED)[buf] = shifted;
       reinterpret_cast<int*>(rel_area + REL_UNI)[buf] = o.uni;
       reinterpret_cast<float*>(rel_area + REL_UNI)[2 + buf] = o.value;
     }
@@ -1042,6 +1049,7 @@ struct TcCta {
   __device__ __forceinline__ void bias_stager() {
     static_assert(ST == 2 || !BIAS, "the wait for the buffer implies the previous phase of S_FULL");
     int table_head = -1;
+    bool shifted = false;
     relpos_load_buckets(*reinterpret_cast<RelBuckets*>(rel_area + REL_BUCKETS), *rel, lane, 32);
     __syncwarp();
     const RelFn bucket_of(*rel, *reinterpret_cast<const RelBuckets*>(rel_area + REL_BUCKETS));
@@ -1050,14 +1058,14 @@ struct TcCta {
       const int h = kDkv ? head * G + g : head;
       if (h != table_head) {
         __syncwarp();
-        rel_load_table(h);
+        shifted = rel_load_table(h);
         table_head = h;
       }
       RelStaged staged;
       rel_look_up(kDkv ? blk_begin + gi - g * blk_count : it, bucket_of, staged);
       warp_wait(BAR_ST_EMPTY + (it & 1), ((it >> 1) & 1) ^ 1);
       if (aborted()) break;
-      rel_store_staged(it & 1, staged);
+      rel_store_staged(it & 1, staged, shifted);
       __syncwarp();
       if (lane == 0) mbar_arrive(bar(BAR_S_FULL + it % ST));
       if (is_tail(it)) zero_tail(it);
@@ -1301,8 +1309,9 @@ struct TcCta {
   // First-order dQ / dK,dV, one block (kernels with tangents take pw_two_phase_block): 16 streamed
   // columns at a time from the S and dP tiles, the TMEM loads of the next group in flight while
   // the current one is processed.
-  // With a bias: UNI = all pairs of the block share a bucket, MASK = some are masked (without one need_mask says so at run time).
-  template <bool UNI, bool MASK>
+  // With a bias: UNI = all pairs of the block share a bucket, MASK = some are masked (without one need_mask says so at run time),
+  // SHIFTED = the rows have shifts (fb_params.h).
+  template <bool UNI, bool MASK, bool SHIFTED>
   __device__ __forceinline__ void pw_bwd_block(int it, int st, bool need_mask_, int cmin, int cmax, const float* stats,
                                                float (&dsv)[BIAS && kDq ? HC : 1]) {
     const bool need_mask = BIAS ? MASK : need_mask_;
@@ -1349,9 +1358,10 @@ struct TcCta {
             if (c % 4 == 0) b4 = bias[(gi * CW + c) / 4];
             b2 = c % 4 == 0 ? make_float2(b4.x, b4.y) : make_float2(b4.z, b4.w);
           }
-          // the shift first: entry - shift is exact where it matters
-          const float2 ns2 = kDkv ? *reinterpret_cast<const float2*>(&stats[2 * BN + col]) : make_float2(nshift2, nshift2);
-          nl2 = __fadd2_rn(nl2, __fadd2_rn(b2, ns2));
+          float2 sb2 = b2;
+          if constexpr (SHIFTED)  // the shift first: entry - shift is exact where it matters
+            sb2 = __fadd2_rn(b2, kDkv ? *reinterpret_cast<const float2*>(&stats[2 * BN + col]) : make_float2(nshift2, nshift2));
+          nl2 = __fadd2_rn(nl2, sb2);
         }
         const float2 e = __ffma2_rn(make_float2(__uint_as_float(bs[buf][c]), __uint_as_float(bs[buf][c + 1])), sc2, nl2);
         float2 pe = exp2_pair(e, c2, !need_mask);
@@ -1572,13 +1582,16 @@ struct TcCta {
         else if constexpr (BIAS) {
           float dsv[kDq ? HC : 1];
           const int uni = reinterpret_cast<const int*>(rel_area + REL_UNI)[it & 1];
+          const bool shifted = reinterpret_cast<const int*>(rel_area + REL_SHIFTED)[it & 1] != 0;
           if (uni >= 0) {
             if constexpr (kDq) rel_flush(uni);
-            if (need_mask) pw_bwd_block<true, true>(it, st, true, cmin, cmax, stats, dsv);
-            else pw_bwd_block<true, false>(it, st, false, cmin, cmax, stats, dsv);
+            if (shifted) pw_bwd_block<true, true, true>(it, st, true, cmin, cmax, stats, dsv);
+            else if (need_mask) pw_bwd_block<true, true, false>(it, st, true, cmin, cmax, stats, dsv);
+            else pw_bwd_block<true, false, false>(it, st, false, cmin, cmax, stats, dsv);
           } else {
-            if (need_mask) pw_bwd_block<false, true>(it, st, true, cmin, cmax, stats, dsv);
-            else pw_bwd_block<false, false>(it, st, false, cmin, cmax, stats, dsv);
+            if (shifted) pw_bwd_block<false, true, true>(it, st, true, cmin, cmax, stats, dsv);
+            else if (need_mask) pw_bwd_block<false, true, false>(it, st, true, cmin, cmax, stats, dsv);
+            else pw_bwd_block<false, false, false>(it, st, false, cmin, cmax, stats, dsv);
             if constexpr (kDq) {
               pw_publish(BAR_P_FULL + st, it, false);
               rel_diagonals(it, dsv);
@@ -1588,7 +1601,7 @@ struct TcCta {
           }
         } else {
           float none[1];
-          pw_bwd_block<false, false>(it, st, need_mask, cmin, cmax, stats, none);
+          pw_bwd_block<false, false, false>(it, st, need_mask, cmin, cmax, stats, none);
         }
         const long long tq1 = prof ? clock64() : 0;
         pw_publish(BAR_P_FULL + st, it, true);
