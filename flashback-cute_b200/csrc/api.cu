@@ -375,6 +375,7 @@ extern "C" int fb_relpos_fwd(const fb_relpos_fwd_args* a, fb_stream_t stream) {
   if (a->prob.total_k == 0) return FB_ERR_SHAPE;
   Params p;
   fill_problem(p, a->prob);
+  rel.zero_rest = (a->prob.flags & FB_FLAG_ZERO_REST) && a->prob.cu_seqlens_q ? 1 : 0;
   FB_TRY(device_setup(&p.status));
   p.q = cvt(a->q); p.k = cvt(a->k); p.v = cvt(a->v); p.o = cvt(a->out); p.od = cvt(a->out_low);
   p.lse = a->lse;
@@ -402,6 +403,7 @@ extern "C" int fb_relpos_bwd(const fb_relpos_bwd_args* a, fb_stream_t stream) {
   rel.shift = const_cast<float*>(a->shift);
   Params p;
   fill_problem(p, a->prob);
+  rel.zero_rest = (a->prob.flags & FB_FLAG_ZERO_REST) && a->prob.cu_seqlens_q ? 1 : 0;
   FB_TRY(device_setup(&p.status));
   p.q = cvt(a->q); p.k = cvt(a->k); p.v = cvt(a->v); p.dout = cvt(a->dout);
   p.o = cvt(a->out); p.od = cvt(a->out_low);

@@ -609,6 +609,11 @@ template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 relpos_fwd_kernel(const __grid_constant__ FwdMaps maps, const __grid_constant__ Params p, const __grid_constant__ RelPos rel) {
   extern __shared__ __align__(1024) uint8_t smem[];
+  if (rel.zero_rest > 0 && blockIdx.x >= gridDim.x - (unsigned)rel.zero_rest) {
+    grid_dependency_wait();
+    rel_zero_rest<T>(p, p.o, p.cu_q, p.Tq, p.Hq, (int)(gridDim.x - 1 - blockIdx.x), rel.zero_rest);
+    return;
+  }
   RelFwd<T, D> cta(maps, p, rel, smem);
   if (!cta.setup()) return;
   cta.run_role();
@@ -632,9 +637,11 @@ int launch_typed(const Params& p_in, const RelPos& rel, cudaStream_t s) {
   p.ntiles = (p.Sq + 2 * BM - 1) / (2 * BM);
   p.group = tc_choose_group(p, false, p.ntiles, sms);
   const long long ctas = (long long)p.ntiles * p.Hq * p.B;
-  if (ctas <= 0 || ctas > 0x7fffffffll) return FB_ERR_TOO_LARGE;
+  RelPos bias = rel;
+  bias.zero_rest = rel.zero_rest ? kRestCtas : 0;
+  if (ctas <= 0 || ctas + bias.zero_rest > 0x7fffffffll) return FB_ERR_TOO_LARGE;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+  cfg.gridDim = dim3((unsigned)(ctas + bias.zero_rest), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = C::smemBytes;
   cfg.stream = s;
@@ -643,7 +650,7 @@ int launch_typed(const Params& p_in, const RelPos& rel, cudaStream_t s) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kern, maps, p, rel) == cudaSuccess ? 1 : FB_ERR_CUDA;
+  return cudaLaunchKernelEx(&cfg, kern, maps, p, bias) == cudaSuccess ? 1 : FB_ERR_CUDA;
 }
 
 }  // namespace

@@ -98,6 +98,9 @@ __global__ void __launch_bounds__(kThreads) simt_fwd_kernel(Params p, const __gr
 
   const int b = blockIdx.z, h = blockIdx.y, hk = h / (p.Hq / p.Hkv);
   const SeqInfo si = seq_info(p, b);
+  if constexpr (BIAS) {
+    if (rel.zero_rest && b == 0) rel_zero_rest<T>(p, p.o, p.cu_q, p.Tq, p.Hq, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
+  }
   const int m0 = blockIdx.x * kOwn;
   if (m0 >= si.sq) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -295,6 +298,9 @@ __global__ void __launch_bounds__(kThreads) simt_dq_kernel(Params p, const __gri
 
   const int b = blockIdx.z, h = blockIdx.y, hk = h / (p.Hq / p.Hkv);
   const SeqInfo si = seq_info(p, b);
+  if constexpr (BIAS) {
+    if (rel.zero_rest && b == 0) rel_zero_rest<T>(p, p.dq, p.cu_q, p.Tq, p.Hq, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
+  }
   const int m0 = blockIdx.x * kOwn;
   if (m0 >= si.sq) {
     if constexpr (BIAS) {
@@ -451,6 +457,12 @@ __global__ void __launch_bounds__(kThreads) simt_dkv_kernel(Params p, const __gr
 
   const int b = blockIdx.z, hk = blockIdx.y, G = p.Hq / p.Hkv;
   const SeqInfo si = seq_info(p, b);
+  if constexpr (BIAS) {
+    if (rel.zero_rest && b == 0) {
+      rel_zero_rest<T>(p, p.dk, p.cu_k, p.Tk, p.Hkv, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
+      rel_zero_rest<T>(p, p.dv, p.cu_k, p.Tk, p.Hkv, blockIdx.y * gridDim.x + blockIdx.x, gridDim.x * gridDim.y);
+    }
+  }
   const int n0 = blockIdx.x * kOwn;
   if (n0 >= si.sk) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;

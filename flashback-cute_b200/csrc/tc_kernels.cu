@@ -1945,6 +1945,17 @@ template <typename T, int KIND, int D>
 __global__ void __launch_bounds__(kThreads, 1)
 tc_rel_kernel(const __grid_constant__ TmaMaps maps, const __grid_constant__ Params p, const __grid_constant__ RelPos rel) {
   extern __shared__ __align__(1024) uint8_t smem[];
+  if (rel.zero_rest > 0 && blockIdx.x >= gridDim.x - (unsigned)rel.zero_rest) {  // (whole clusters)
+    const int part = (int)(gridDim.x - 1 - blockIdx.x);
+    grid_dependency_wait();
+    if (KIND == KIND_DQ) {
+      rel_zero_rest<T>(p, p.dq, p.cu_q, p.Tq, p.Hq, part, rel.zero_rest);
+    } else {
+      rel_zero_rest<T>(p, p.dk, p.cu_k, p.Tk, p.Hkv, part, rel.zero_rest);
+      rel_zero_rest<T>(p, p.dv, p.cu_k, p.Tk, p.Hkv, part, rel.zero_rest);
+    }
+    return;
+  }
   TcCta<T, KIND, D, false, true, false, false, true> cta(maps, p, smem);
   cta.rel = &rel;
   if (!cta.setup()) return;
@@ -2159,10 +2170,17 @@ int launch_one(const TmaMaps& maps, const Params& p_in, cudaStream_t stream, con
   p.split = KIND == KIND_DKV ? choose_split(p, p.ntiles, device_sm_count(dev)) : 1;
   p.group = choose_group(p, KIND == KIND_DKV, p.ntiles, device_sm_count(dev));
   const long long ctas = (long long)p.ntiles * (KIND == KIND_DKV ? p.Hkv : p.Hq) * p.B * p.split;
-  if (ctas <= 0 || ctas > 0x7fffffffll) return FB_ERR_TOO_LARGE;
+  RelPos bias;
+  int rest = 0;
+  if constexpr (BIAS) {
+    bias = *rel;
+    bias.zero_rest = rest = rel->zero_rest ? kRestCtas : 0;
+    static_assert(kRestCtas % 8 == 0, "whole clusters");
+  }
+  if (ctas <= 0 || ctas + rest > 0x7fffffffll) return FB_ERR_TOO_LARGE;
 
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+  cfg.gridDim = dim3((unsigned)(ctas + rest), 1, 1);
   cfg.blockDim = dim3(kThreads, 1, 1);
   cfg.dynamicSmemBytes = C::smemBytes;
   cfg.stream = stream;
@@ -2183,7 +2201,7 @@ int launch_one(const TmaMaps& maps, const Params& p_in, cudaStream_t stream, con
   }
   cfg.attrs = attrs;
   cfg.numAttrs = na;
-  if constexpr (BIAS) return cudaLaunchKernelEx(&cfg, kern, maps, p, *rel) == cudaSuccess ? 1 : FB_ERR_CUDA;
+  if constexpr (BIAS) return cudaLaunchKernelEx(&cfg, kern, maps, p, bias) == cudaSuccess ? 1 : FB_ERR_CUDA;
   else return cudaLaunchKernelEx(&cfg, kern, maps, p) == cudaSuccess ? 1 : FB_ERR_CUDA;
 }
 

@@ -26,6 +26,7 @@ FB_FLAG_FORCE_SIMT = 1
 FB_FLAG_TILE_MAJOR = 2
 FB_FLAG_KV_OUT_F32 = 4       # hvp_bwd: dk, dv, dk_dot, dv_dot are float32 tensors ...
 FB_FLAG_KV_ACCUMULATE = 8    # ... and results are added to their contents
+FB_FLAG_ZERO_REST = 32       # relpos_fwd, relpos_bwd: rows of no packed sequence are zeroed
 FB_FLAG_SEG_KEYS = 16        # fb_problem.seg_rows / seg_shift describe the key rows (dK/dV-side kernels only)
 
 

@@ -182,14 +182,15 @@ class _AttnPlan:
             b, sq, sk = q_shape[0], q_shape[1], k_shape[1]
             total_q, total_k = b * sq, b * sk
         self.total_q, self.stat_bytes = total_q, 4 * self.heads * total_q
-        self.empty = 0 in q_shape or 0 in k_shape  # nothing is read, whatever the layouts
+        self.empty = 0 in q_shape or 0 in k_shape or 0 in (sq, sk)  # nothing is read, whatever the layouts
         self.copies = not (self.empty or (_strides_ok(q_shape, q_stride) and _strides_ok(k_shape, k_stride) and _strides_ok(k_shape, v_stride)))
         self.low = dtype != torch.float32
         if self.copies or self.empty:
             return
         cu = 16 if packed else None  # an address to come: a problem with cu_seqlens is a packed one
         prob = _lib.FbProblem(
-            _lib._DTYPES[dtype], b, self.heads, k_shape[-2], q_shape[-1], sq, sk, int(causal), total_q, total_k, cu, cu, scale, _lib.DEFAULT_FLAGS,
+            _lib._DTYPES[dtype], b, self.heads, k_shape[-2], q_shape[-1], sq, sk, int(causal), total_q, total_k, cu, cu, scale,
+            _lib.DEFAULT_FLAGS | (_lib.FB_FLAG_ZERO_REST if packed else 0),
         )
         bias = _bias(table_shape, table_stride, two, max_distance)
         t = lambda stride: _lib.FbTensor(None, stride[-3], stride[-2])  # noqa: E731
@@ -487,7 +488,8 @@ def flashback_attn_relpos_varlen_func(
     causal: bool = False,
     bidirectional: Optional[bool] = None,
 ) -> torch.Tensor:
-    """The same for packed sequences: q (total_q, hq, d), k/v (total_k, hkv, d), cu_seqlens int32 (b+1,)."""
+    """The same for packed sequences: q (total_q, hq, d), k/v (total_k, hkv, d), cu_seqlens int32 (b+1,). Rows that belong to no
+    sequence (behind cu_seqlens[b]) are not read; their results and gradients are zeros."""
     return _attention(
         q, k, v, bias_table, cu_seqlens_q, cu_seqlens_k, max_seqlen_q, max_seqlen_k, max_distance, softmax_scale, causal, bidirectional
     )

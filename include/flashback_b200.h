@@ -128,6 +128,9 @@ typedef struct {
 #define FB_FLAG_KV_ACCUMULATE 8
 /* fb_problem.seg_rows / seg_shift describe the key rows instead of the query rows (see there). */
 #define FB_FLAG_SEG_KEYS 16
+/* fb_relpos_fwd, fb_relpos_bwd, packed problems: rows of out, dq, dk, dv that belong to no sequence (before cu_seqlens[0], from
+ * cu_seqlens[batch] on) are set to zero; without it they are left as they are. */
+#define FB_FLAG_ZERO_REST 32
 
 /*
  * JVP forward. Replaces the reference's K1 launch `_jvp_fwd` (interface.py:122-148,

@@ -64,14 +64,20 @@ class Calls(list):
     def fb_relpos_fwd(self, a):
         p, dtype = a.prob, TYPES[a.prob.dtype]
         r, n, _ = self._attention(a)
-        _seq(a.out, p.total_q, p.heads_q, p.head_dim, dtype)[:n] = r.out.to(dtype)
+        out = _seq(a.out, p.total_q, p.heads_q, p.head_dim, dtype)
+        out[:n] = r.out.to(dtype)
+        if p.flags & _lib.FB_FLAG_ZERO_REST:
+            out[n:] = 0
 
     def fb_relpos_bwd(self, a):
         p, dtype = a.prob, TYPES[a.prob.dtype]
         r, nq, nk = self._attention(a, a.dout)
         for t, g, n, heads, rows in ((a.dq, r.dq, nq, p.heads_q, p.total_q), (a.dk, r.dk, nk, p.heads_kv, p.total_k), (a.dv, r.dv, nk, p.heads_kv, p.total_k)):
             if t.ptr:
-                _seq(t, rows, heads, p.head_dim, dtype)[:n] = g.to(dtype)
+                out = _seq(t, rows, heads, p.head_dim, dtype)
+                out[:n] = g.to(dtype)
+                if p.flags & _lib.FB_FLAG_ZERO_REST:
+                    out[n:] = 0
         if a.dtable:
             memory(a.dtable, (a.bias.num_buckets, p.heads_q), (a.dtable_bucket_stride, a.dtable_head_stride), dtype).copy_(r.dt.to(dtype))
 

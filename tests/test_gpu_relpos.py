@@ -791,3 +791,31 @@ def test_decode_large_entries(dtype):
         for i, n in enumerate(lens[1:]):
             r = orc.attention(q[1 + i:2 + i], k[1 + i:2 + i, :n], v[1 + i:2 + i, :n], table, 128, False, 0.125, True, apart=True)
             _within("out", got[i:i + 1], r.out, r.tol[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_rows_of_no_sequence_get_zeros(dtype):
+    """Packed tensors with rows before the first sequence and behind the last: results and gradients there are zeros, whatever the memory held."""
+    def poison():
+        torch.cuda.synchronize()
+        hold = [torch.full((n,), float("nan"), device=DEV) for n in (1 << 24, 1 << 20, 1 << 18, 1 << 16, 1 << 14) for _ in range(6)]
+        del hold
+
+    for lead, lens, rest, causal in ((0, [70, 1, 130], 41, True), (37, [20], 3000, False), (5, [0, 129, 0], 300, True), (9, [0, 0], 20, False)):
+        total = lead + sum(lens) + rest
+        cu = torch.tensor([lead, *(lead + n for n in itertools.accumulate(lens))], dtype=torch.int32, device=DEV)
+        full = [_mk((total, h, 64), dtype, i) for i, h in enumerate((4, 2, 2, 4))]
+        inside = slice(lead, lead + sum(lens))
+        for t in full:
+            t[:lead], t[inside.stop:] = float("nan"), float("nan")
+        leaves = [t.requires_grad_() for t in (*full[:3], _mk((32, 4), dtype, 9))]
+        poison()
+        out = flashback_attn_relpos_varlen_func(*leaves, cu, cu, max(lens), max(lens), causal=causal)
+        poison()
+        grads = torch.autograd.grad(out, leaves, full[3])
+        for t in (out, *grads[:3]):
+            assert (t[:lead] == 0).all() and (t[inside.stop:] == 0).all()
+        q, k, v, do = (t.detach()[inside] for t in full)
+        ref = orc.attention(q, k, v, leaves[3].detach(), 128, not causal, 0.125, causal, do, lens, lens)
+        for name, got, want, tol in zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(), *grads), ref[:5], ref.tol):
+            _within(name, got if name == "dtable" else got[inside], want, tol)

@@ -154,3 +154,23 @@ def test_derivatives_of_the_bias_of_a_broadcast_table(monkeypatch):
         assert leaf.stride() == (1, 0)
         first = torch.autograd.grad((flashback_relpos_bias(leaf, 5, 7, max_distance=6) * w).sum(), leaf, create_graph=True)[0]
         assert torch.equal(torch.autograd.grad((first * spread).sum(), w)[0], spread.t()[:, which])
+
+
+# ---------------------------------------------------------------------------------------------
+# packed tensors longer than their sequences
+# ---------------------------------------------------------------------------------------------
+def test_rows_of_no_sequence_get_zeros(monkeypatch):
+    """Results and gradients come from memory that may hold anything; the call asks for zeros in the rows that no sequence has."""
+    fresh = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **kw: fresh(*a, **kw).fill_(float("nan")))
+    q, k, v, do, table = _mk((50, 4, 64), 0), _mk((50, 2, 64), 1), _mk((50, 2, 64), 2), _mk((50, 4, 64), 3), _mk((32, 4), 4)
+    for t in (q, k, v, do):
+        t[30:] = float("nan")
+    for lens in ([20, 10], [30, 0], [0, 0]):
+        cu = torch.tensor([0, lens[0], sum(lens)], dtype=torch.int32)
+        leaves = [t.clone().requires_grad_() for t in (q, k, v, table)]
+        with double.library():
+            out = flashback_attn_relpos_varlen_func(*leaves, cu, cu, max(lens), max(lens), causal=True)
+            grads = torch.autograd.grad(out, leaves, do)
+        assert all((t[sum(lens):] == 0).all() for t in (out, *grads[:3]))
+        assert all(torch.isfinite(t).all() for t in (out, *grads))
