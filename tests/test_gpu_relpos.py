@@ -819,3 +819,49 @@ def test_rows_of_no_sequence_get_zeros(dtype):
         ref = orc.attention(q, k, v, leaves[3].detach(), 128, not causal, 0.125, causal, do, lens, lens)
         for name, got, want, tol in zip(("out", "dq", "dk", "dv", "dtable"), (out.detach(), *grads), ref[:5], ref.tol):
             _within(name, got if name == "dtable" else got[inside], want, tol)
+
+
+# ---------------------------------------------------------------------------------------------
+# the bias tensor at sizes whose tiles are the largest ones
+# ---------------------------------------------------------------------------------------------
+def _which(sq, sk, num, far, two):
+    """(sq, sk) buckets on the GPU, from the oracle's bucket function by distance."""
+    side = num // 2 if two else num
+    dist = torch.tensor([orc.bucket(min(n, far), side, far) for n in range(max(sq, sk) + abs(sk - sq) + 1)], device=DEV)
+    r = torch.arange(sk, device=DEV)[None, :] - (torch.arange(sq, device=DEV)[:, None] + sk - sq)
+    return torch.where(r <= 0, dist[r.abs()], side + dist[r.abs()] if two else dist[0])
+
+
+@pytest.mark.parametrize("heads,sq,sk", [(8, 1537, 2051), (16, 2047, 4099), (12, 3001, 1030)])
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_bias_tensor_full_tiles(dtype, heads, sq, sk):
+    """CTAs of up to 256 rows (gradient) and 128 rows (fill): every element of the bias, every entry of the table's gradient."""
+    for num, far, two in ((32, 128, True), (64, 1500, False)):
+        table, which = _mk((num, heads), dtype, 0).requires_grad_(), _which(sq, sk, num, far, two)
+        bias = flashback_relpos_bias(table, sq, sk, max_distance=far, bidirectional=two)
+        grad = _mk(bias.shape, dtype, 1)
+        got = torch.autograd.grad(bias, table, grad)[0]
+        want, size = (torch.zeros(num, heads, dtype=torch.float64, device=DEV) for _ in range(2))
+        for h in range(heads):
+            assert torch.equal(bias[h].detach(), table.detach()[:, h][which])
+            want[:, h].index_add_(0, which.flatten(), grad[h].double().flatten())
+            size[:, h].index_add_(0, which.flatten(), grad[h].double().abs().flatten())
+        # float32 sums: 256 rows by 8 warps along a diagonal and a cut row at each end, 8 warps, a run of up to 32 neighbours (5 steps), 8 warps; then 64 bits; one rounding
+        u = torch.finfo(dtype).eps / 2
+        _within("dtable", got, want, (256 / 8 + 2 + 8 + 5 + 8) * 2.0 ** -24 * size * (1 + u) + u * want.abs())
+
+
+@pytest.mark.parametrize("sq,sk", [(70000, 1), (20011, 3), (4099, 17), (1, 70000), (5, 30001)])
+def test_bias_tensor_tall_and_wide(sq, sk):
+    for dtype, two in ((BF16, True), (F32, False)):
+        table, which = _mk((32, 3), dtype, 0).requires_grad_(), _which(sq, sk, 32, 128, two)
+        bias = flashback_relpos_bias(table, sq, sk, bidirectional=two)
+        grad = _mk(bias.shape, dtype, 1)
+        got = torch.autograd.grad(bias, table, grad)[0]
+        want, size = (torch.zeros(32, 3, dtype=torch.float64, device=DEV) for _ in range(2))
+        for h in range(3):
+            assert torch.equal(bias[h].detach(), table.detach()[:, h][which])
+            want[:, h].index_add_(0, which.flatten(), grad[h].double().flatten())
+            size[:, h].index_add_(0, which.flatten(), grad[h].double().abs().flatten())
+        u = torch.finfo(dtype).eps / 2
+        _within("dtable", got, want, (256 / 8 + 2 + 8 + 5 + 8) * 2.0 ** -24 * size * (1 + u) + u * want.abs())
