@@ -76,7 +76,7 @@ __global__ void __launch_bounds__(kThreads) relpos_fill_kernel(const __grid_cons
 // ---------------------------------------------------------------------------------------------------
 // The sum over a bucket is a sum over diagonals. Diagonal c = j - i + (sq - 1) of row i sits at flat offset
 // i * (sk + 1) + c - (sq - 1): rows that are VEC = 16 bytes / element apart keep their place relative to a 16-byte
-// boundary. So a CTA takes kSpan diagonals x a stretch of rows, each of VEC residues of the row index gets an equal share of
+// boundary. So a CTA takes kSpan of the diagonals that meet a stretch of rows, each of VEC residues of the row index gets an equal share of
 // the warps, and a thread adds up VEC neighbouring diagonals in registers over its rows with 16-byte loads: no
 // atomics, no reordering, every element read once. At the end the CTA adds up its warps' diagonals, then those of
 // each bucket (neighbours), and leaves one number per bucket in the workspace.
@@ -99,9 +99,9 @@ __global__ void __launch_bounds__(kThreads) relpos_grad_kernel(const __grid_cons
   __shared__ float acc[FB_RELPOS_MAX_BUCKETS];
   __shared__ RelBuckets buckets;
   const int h = blockIdx.z;
-  const int c0 = blockIdx.x * kSpan;  // first diagonal
-  const int ndiag = sq + sk - 1;
   int i_lo = blockIdx.y * rows_per_cta, i_hi = min(sq, i_lo + rows_per_cta);
+  const int c0 = sq - i_hi + blockIdx.x * kSpan;  // first diagonal; the stretch's first is that of its last row's first column
+  const int ndiag = sq + sk - 1;
   float* out = rel.dpart + (((int64_t)h * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x) * rel.nb;
   // rows whose columns j = c - (sq - 1) + i meet [0, sk) for some diagonal of the CTA
   i_lo = max(i_lo, sq - 1 - (c0 + kSpan - 1));
@@ -262,11 +262,11 @@ struct GradShape {
 GradShape grad_shape(int dtype, int heads, int sq, int sk) {
   GradShape g;
   const int span = 32 * (dtype == FB_F32 ? 4 : 8);
-  g.spans = (sq + sk - 1 + span - 1) / span;
-  g.rows = 256;
-  while (g.rows > 32 && (int64_t)g.spans * heads * ((sq + g.rows - 1) / g.rows) < 148 * 8) g.rows /= 2;
-  g.row_blocks = (sq + g.rows - 1) / g.rows;
-  return g;
+  for (g.rows = 256;; g.rows /= 2) {
+    g.spans = (g.rows + sk - 1 + span - 1) / span;  // of a stretch of rows
+    g.row_blocks = (sq + g.rows - 1) / g.rows;
+    if (g.rows <= 32 || (int64_t)g.spans * heads * g.row_blocks >= 148 * 8) return g;
+  }
 }
 
 template <typename T>

@@ -224,3 +224,16 @@ def test_bounds_apart_from_the_entries_size():
     small, large = far(0.0, True), far(2.0 ** 24, True)
     for a, b, loose in zip(small, large, far(2.0 ** 24, False)):
         assert torch.allclose(a, b, rtol=1e-6) and (loose >= 10 * b).all()  # (buckets without a pair: 0)
+
+
+def test_workspace_of_the_bias_gradient_follows_the_tensor():
+    """Partial sums only for diagonals that a block of rows has: no more than a few bytes per element, however tall the tensor."""
+    lib = _lib.load()
+    for dtype, size in ((0, 2), (2, 4)):
+        for heads in (1, 16):
+            for sq, sk in ((1 << 20, 1), (1 << 20, 64), (1 << 18, 1000), (70000, 1), (4095, 4099), (1 << 15, 1 << 15)):
+                n = lib.fb_relpos_bias_workspace_bytes(dtype, heads, sq, sk, 32)
+                # one part of 32 float32 per 256 rows and 128 or 256 diagonals, of which 256 + sk - 1 at most; small tensors: down to 32 rows
+                parts = lambda rows: -(-sq // rows) * -(-(rows + sk - 1) // (64 * 8 // size))  # noqa: E731
+                assert 0 < n <= heads * parts(32) * 32 * 4, (heads, sq, sk, n)
+                assert heads * sq * sk < 1 << 26 or n == heads * parts(256) * 32 * 4, (heads, sq, sk, n)
