@@ -887,6 +887,7 @@ struct TcCta {
       large = large || relpos_large(x);
       tab[t] = relpos_log2(x);
     }
+    __syncwarp();  // (a vote orders no memory)
     return __any_sync(0xffffffffu, large) != 0;
   }
   // BIAS: the biases of a block's positions. Entry u belongs to the pairs with (streamed row in block) - (owner row in
