@@ -167,6 +167,7 @@ class FbRelposDecodeArgs(ctypes.Structure):
 
 NOALLOC_MAX_STAT_FLOATS = 1 << 20
 RELPOS_MAX_BUCKETS = 128
+DECODE_MAX_TABLE = 4096  # query heads per kv head x buckets
 
 EXPORTS = (
     "fb_jvp_fwd", "fb_bwd_row_stats", "fb_hvp_bwd", "fb_bwd_noalloc", "fb_last_launch_count", "fb_check_device_status",

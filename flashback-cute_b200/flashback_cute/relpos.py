@@ -513,8 +513,11 @@ class _DecodePlan:
             if lens.shape != q.shape[:1] or lens.device != q.device or not lens.is_contiguous():
                 raise ValueError("cache_seqlens must be contiguous, of shape (batch,) and on the device of q")
         q_shape, k_shape, table_shape, dtype = tuple(q.shape), tuple(k.shape), tuple(table.shape), q.dtype
-        q_stride, k_stride, v_stride, table_stride = q.stride(), k.stride(), v.stride(), table.stride()
+        table_stride = table.stride()
+        q_stride, k_stride, v_stride = (tuple(0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride())) + t.stride()[3:] for t in (q, k, v))  # (of one entry: any)
         _check_buckets(table_shape[0], two, max_distance)
+        if q_shape[2] // k_shape[2] * table_shape[0] > _lib.DECODE_MAX_TABLE:
+            raise ValueError(f"decoding takes at most {_lib.DECODE_MAX_TABLE} table entries per kv head: (heads_q / heads_kv) * num_buckets")
         ok = lambda s: s[3] == 1 and all(x >= 0 and x % 8 == 0 for x in s[:3])  # noqa: E731
         if not (ok(k_stride) and ok(v_stride)):
             raise ValueError("caches need unit stride on head_dim and strides that are multiples of 8 elements")
@@ -542,7 +545,7 @@ def flashback_attn_relpos_decode(
 ) -> torch.Tensor:
     """Attention of the newest tokens of every sequence: q (b, sq, hq, d) against caches (b, s, hkv, d) that already hold
     their keys and values. cache_seqlens, int32 (b,) on the device of q: keys per sequence, the new tokens included (None: s each; values are
-    clamped to [0, s]). Causal: token t of sequence i sits at position cache_seqlens[i] - sq + t. Cache rows at or behind a
+    clamped to [0, s]). (hq / hkv) * num_buckets is at most 4096. Causal: token t of sequence i sits at position cache_seqlens[i] - sq + t. Cache rows at or behind a
     sequence's length are not read. bfloat16 or float16; meant for one to a few tokens (every 16 or 32 (token, head) pairs of a kv head read the
     cache once). No autograd graph."""
     max_distance, softmax_scale = _numbers(max_distance, softmax_scale)

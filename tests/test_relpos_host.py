@@ -174,3 +174,28 @@ def test_rows_of_no_sequence_get_zeros(monkeypatch):
             grads = torch.autograd.grad(out, leaves, do)
         assert all((t[sum(lens):] == 0).all() for t in (out, *grads[:3]))
         assert all(torch.isfinite(t).all() for t in (out, *grads))
+
+
+# ---------------------------------------------------------------------------------------------
+# decoding: strides of dimensions of size one, the table's limit
+# ---------------------------------------------------------------------------------------------
+def test_decode_strides_of_single_entries_do_not_matter():
+    """One sequence or one head out of buffers with odd strides between them."""
+    buf = _mk((9 * 4 * 64 + 3,), 0)
+    k = buf[: 9 * 4 * 64].as_strided((1, 9, 4, 64), (9 * 4 * 64 + 3, 256, 64, 1))
+    one = _mk((2, 9, 64), 1).as_strided((2, 9, 1, 64), (576, 64, 3, 1))
+    q, table = _mk((1, 1, 8, 64), 2), _mk((32, 8), 3)
+    with double.library() as calls:
+        assert torch.equal(flashback_attn_relpos_decode(q, k, k, None, table), _decode_want(q, k, k, table))
+        q2 = _mk((2, 1, 8, 64), 4)
+        assert torch.equal(flashback_attn_relpos_decode(q2, one, one, None, table), _decode_want(q2, one, one, table))
+    assert all(s % 8 == 0 for _, a in calls for t in (a.q, a.k, a.v) for s in (t.batch_stride, t.row_stride, t.head_stride))
+    odd = buf.as_strided((2, 3, 4, 64), (771, 256, 64, 1))
+    with double.library(), pytest.raises(ValueError):  # between several of them: the kernel's loads need the alignment
+        flashback_attn_relpos_decode(q2, odd, odd, None, table)
+
+
+def test_decode_refuses_tables_beyond_shared_memory():
+    k = _mk((1, 3, 1, 64), 0)
+    with double.library(), pytest.raises(ValueError, match="4096"):
+        flashback_attn_relpos_decode(_mk((1, 1, 64, 64), 1), k, k, None, _mk((128, 64), 2))
