@@ -236,10 +236,9 @@ __device__ __forceinline__ SeqInfo seq_info(const Params& p, int b) {
 
 // CTAs for that (beside the last tiles).
 constexpr int kRestCtas = 16;
-// Zeroes the rows of `t` that belong to no sequence (before cu[0], from cu[B] on); this CTA as part `part` of `parts`. A call: inlined at the entry of the
-// tensor-core kernels it cost every launch 2 us (12 packed prompts of up to 2048: 197.0 us, 195.0 as a call, 194.8 without).
+// Zeroes the rows of `t` that belong to no sequence (before cu[0], from cu[B] on); this CTA as part `part` of `parts`.
 template <typename T>
-__device__ __noinline__ void rel_zero_rest(const Params& p, const SeqT& t, const int32_t* cu, int64_t total, int heads, int part, int parts) {
+__device__ __forceinline__ void rel_zero_rest(const Params& p, const SeqT& t, const int32_t* cu, int64_t total, int heads, int part, int parts) {
   if (!t.ptr) return;
   constexpr int VEC = 16 / sizeof(T);
   const int units = p.D / VEC;
@@ -249,6 +248,12 @@ __device__ __noinline__ void rel_zero_rest(const Params& p, const SeqT& t, const
     const int64_t r = x / units / heads, row = r < lead ? r : end + r - lead;
     *reinterpret_cast<uint4*>(reinterpret_cast<T*>(t.ptr) + row * t.row_stride + (int64_t)h * t.head_stride + u * VEC) = make_uint4(0, 0, 0, 0);
   }
+}
+// The same as a call, for the tensor-core kernels: inlined at their entry it cost every launch 2 us (12 packed prompts of up to 2048: 197.0 us, 195.0 as a
+// call, 194.8 without). The CUDA-core kernels inline it: a call costs them registers (training step B2 S200, 4 heads of 64: 163 us, 142 inlined).
+template <typename T>
+__device__ __noinline__ void rel_zero_rest_call(const Params& p, const SeqT& t, const int32_t* cu, int64_t total, int heads, int part, int parts) {
+  rel_zero_rest<T>(p, t, cu, total, heads, part, parts);
 }
 
 // Shift of sequence-local row `row` of the segmented side (fb_problem.seg_rows / seg_shift).

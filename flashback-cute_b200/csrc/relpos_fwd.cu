@@ -110,6 +110,14 @@ template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t u);
 template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t u) { return __bfloat1622float2(*reinterpret_cast<__nv_bfloat162*>(&u)); }
 template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t u) { return __half22float2(*reinterpret_cast<__half2*>(&u)); }
 
+// The two parts of the shifts as calls: heads without large entries jump over them, and code in their place cost every CTA's set-up and epilogue.
+template <typename T>
+__device__ __noinline__ void prefix_call(float* pre, const RelPos& rel, int head, int lane) { relpos_prefix<T>(pre, rel, head, lane); }
+template <typename T>
+__device__ __noinline__ float shift_call(const float* pre, const RelBuckets& buckets, const RelPos& rel, int head, int lo, int hi) {
+  return relpos_shift<T>(pre, rel, RelFn(rel, buckets), head, lo, hi);
+}
+
 template <typename T, int D>
 struct RelFwd {
   using C = FwdCfg<D>;
@@ -298,7 +306,7 @@ struct RelFwd {
     relpos_load_buckets(buckets, rel, w * 32 + lane, 64);
     large = named_barrier_or(1, 64, large);
     if (w == 1) {
-      if (large) relpos_prefix<T>(reinterpret_cast<float*>(misc + M_PRE), rel, head, lane);
+      if (large) prefix_call<T>(reinterpret_cast<float*>(misc + M_PRE), rel, head, lane);
       if (lane == 0) *reinterpret_cast<int*>(misc + M_LARGE) = large;
     }
     const int shifted = large ? BLK_SHIFTED : 0;
@@ -515,8 +523,8 @@ struct RelFwd {
   // The shift of query row `i` of the sequence (0 for a row behind it).
   __device__ __forceinline__ float row_shift(int i) const {
     if (*reinterpret_cast<const int*>(misc + M_LARGE) == 0 || i >= si.sq || (p.causal && i + off < 0)) return 0.f;
-    return relpos_shift<T>(reinterpret_cast<const float*>(misc + M_PRE), rel, RelFn(rel, *reinterpret_cast<const RelBuckets*>(misc + M_BUCKETS)), head,
-                           -(i + off), p.causal ? 0 : si.sk - 1 - (i + off));
+    return shift_call<T>(reinterpret_cast<const float*>(misc + M_PRE), *reinterpret_cast<const RelBuckets*>(misc + M_BUCKETS), rel, head,
+                         -(i + off), p.causal ? 0 : si.sk - 1 - (i + off));
   }
   __device__ __forceinline__ static float row_max(const float (&v)[BN]) {
     float mx[4] = {v[0], v[1], v[2], v[3]};
@@ -611,7 +619,7 @@ relpos_fwd_kernel(const __grid_constant__ FwdMaps maps, const __grid_constant__ 
   extern __shared__ __align__(1024) uint8_t smem[];
   if (rel.zero_rest > 0 && blockIdx.x >= gridDim.x - (unsigned)rel.zero_rest) {
     grid_dependency_wait();
-    rel_zero_rest<T>(p, p.o, p.cu_q, p.Tq, p.Hq, (int)(gridDim.x - 1 - blockIdx.x), rel.zero_rest);
+    rel_zero_rest_call<T>(p, p.o, p.cu_q, p.Tq, p.Hq, (int)(gridDim.x - 1 - blockIdx.x), rel.zero_rest);
     return;
   }
   RelFwd<T, D> cta(maps, p, rel, smem);

@@ -872,7 +872,7 @@ struct TcCta {
         v[r].x = p.lse[sr];
         v[r].y = p.dpsum[sr];
         if (TANGENT) { v[r].z = p.z1[sr]; v[r].w = p.ddot[sr]; }
-        if constexpr (BIAS) v[r].z = relpos_log2(rel->shift[sr]);
+        if constexpr (BIAS) v[r].z = rel->shift[sr];
       }
     }
   }
@@ -1034,7 +1034,7 @@ struct TcCta {
       for (int r = 0; r < BN / 32; ++r) {
         const int rr = lane + 32 * r;
         dst[rr] = (fabsf(cur[r].x) == INFINITY) ? -INFINITY : -cur[r].x * kLog2e;  // a fully masked row has lse = -inf
-        dst[BN + rr] = -cur[r].y; dst[2 * BN + rr] = -cur[r].z; dst[3 * BN + rr] = -cur[r].w;
+        dst[BN + rr] = -cur[r].y; dst[2 * BN + rr] = BIAS ? -relpos_log2(cur[r].z) : -cur[r].z; dst[3 * BN + rr] = -cur[r].w;
       }
       __syncwarp();
       if (lane == 0) {
@@ -1583,16 +1583,18 @@ struct TcCta {
         else if constexpr (BIAS) {
           float dsv[kDq ? HC : 1];
           const int uni = reinterpret_cast<const int*>(rel_area + REL_UNI)[it & 1];
-          const bool shifted = reinterpret_cast<const int*>(rel_area + REL_SHIFTED)[it & 1] != 0;
+          // KIND_DKV: one shift per streamed column, an addition per pair, left out where there are none; KIND_DQ: one per thread, always
+          // (B2 Hq16 Hkv4 S4096 D128: dK/dV 551 us and 566 with the additions, dQ 497, and 492 without them, causal 264 and 271)
+          const bool shifted = kDkv && reinterpret_cast<const int*>(rel_area + REL_SHIFTED)[it & 1] != 0;
           if (uni >= 0) {
             if constexpr (kDq) rel_flush(uni);
             if (shifted) pw_bwd_block<true, true, true>(it, st, true, cmin, cmax, stats, dsv);
-            else if (need_mask) pw_bwd_block<true, true, false>(it, st, true, cmin, cmax, stats, dsv);
-            else pw_bwd_block<true, false, false>(it, st, false, cmin, cmax, stats, dsv);
+            else if (need_mask) pw_bwd_block<true, true, kDq>(it, st, true, cmin, cmax, stats, dsv);
+            else pw_bwd_block<true, false, kDq>(it, st, false, cmin, cmax, stats, dsv);
           } else {
             if (shifted) pw_bwd_block<false, true, true>(it, st, true, cmin, cmax, stats, dsv);
-            else if (need_mask) pw_bwd_block<false, true, false>(it, st, true, cmin, cmax, stats, dsv);
-            else pw_bwd_block<false, false, false>(it, st, false, cmin, cmax, stats, dsv);
+            else if (need_mask) pw_bwd_block<false, true, kDq>(it, st, true, cmin, cmax, stats, dsv);
+            else pw_bwd_block<false, false, kDq>(it, st, false, cmin, cmax, stats, dsv);
             if constexpr (kDq) {
               pw_publish(BAR_P_FULL + st, it, false);
               rel_diagonals(it, dsv);
@@ -1950,10 +1952,10 @@ tc_rel_kernel(const __grid_constant__ TmaMaps maps, const __grid_constant__ Para
     const int part = (int)(gridDim.x - 1 - blockIdx.x);
     grid_dependency_wait();
     if (KIND == KIND_DQ) {
-      rel_zero_rest<T>(p, p.dq, p.cu_q, p.Tq, p.Hq, part, rel.zero_rest);
+      rel_zero_rest_call<T>(p, p.dq, p.cu_q, p.Tq, p.Hq, part, rel.zero_rest);
     } else {
-      rel_zero_rest<T>(p, p.dk, p.cu_k, p.Tk, p.Hkv, part, rel.zero_rest);
-      rel_zero_rest<T>(p, p.dv, p.cu_k, p.Tk, p.Hkv, part, rel.zero_rest);
+      rel_zero_rest_call<T>(p, p.dk, p.cu_k, p.Tk, p.Hkv, part, rel.zero_rest);
+      rel_zero_rest_call<T>(p, p.dv, p.cu_k, p.Tk, p.Hkv, part, rel.zero_rest);
     }
     return;
   }
