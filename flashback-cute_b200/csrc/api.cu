@@ -578,7 +578,7 @@ extern "C" const char* fb_status_string(int status) {
 
 extern "C" const char* fb_last_cuda_error(void) { return tl_cuda_error; }
 
-extern "C" int fb_version(void) { return 100; }
+extern "C" int fb_version(void) { return 200; }
 
 extern "C" int fb_debug_profile(long long* out16) { return out16 ? read_profile(out16) : FB_ERR_NULL_ARG; }
 

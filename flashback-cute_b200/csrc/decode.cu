@@ -4,15 +4,15 @@
 // rows = (new tokens) x (query heads per kv head) sharing them need. So the rows of a kv head form ONE 16-row operand (two for
 // more rows) of warp-level MMAs, and the kernel is built around keeping loads in flight:
 //
-//   * a CTA of 4 warps takes a slice of one (sequence, kv head)'s keys; every warp is a flash-attention of its own over every 4th
-//     group of 16 keys (own running maximum, sum and accumulator; own shared-memory stages filled by cp.async), so nothing in
+//   * a CTA of 4 warps (8 in a cluster) takes a slice of one (sequence, kv head)'s keys; every warp is a flash-attention of its own over every
+//     4th (8th) group of 16 keys (own running maximum, sum and accumulator; own shared-memory stages filled by cp.async), so nothing in
 //     the main loop waits for another warp;
 //   * the slices divide the sequence's OWN length, so ragged batches stay balanced. Up to 8 slices are one thread-block cluster: its CTAs
 //     leave their partial results (float32, unnormalised, with maximum and sum) in shared memory and join them through
 //     distributed shared memory, each a part of the rows. More slices (few sequences with long caches) go through a
 //     workspace and a second kernel. Fixed order either way.
 //
-// Measured: 48 sequences of up to 8192 keys, 32 / 8 heads of 128, bf16 (897 MB): 141 + 7 us, 6.0 TB/s, 92 % of the measured copy bandwidth.
+// Measured: 48 sequences of up to 8192 keys, 32 / 8 heads of 128, bf16 (897 MB): 139 + 5 us, 150 us a call, 6.0 TB/s, 91 % of the measured copy bandwidth.
 //
 // Far from the newest token all keys of a group share the last bucket and the bias is one number per row.
 #include "fb_params.h"
@@ -494,7 +494,7 @@ int decode_dispatch(DecodeParams& p, RelPos& rel, cudaStream_t s) {
 // Slices of a sequence's keys and how they are joined: enough CTAs for a few waves on the whole GPU, slices of at least one round of the CTA's warps. A
 // power of two up to 8 (a cluster: one launch) for small batches whose slices then have at most 8 rounds; otherwise a workspace and a
 // second launch, since a cluster holds its SMs until its last CTA is done: 48 sequences of up to 8192 keys, 8 kv heads of 128
-// in 4 slices each: 171 us as clusters, 152 + 5 us through the workspace.
+// in 4 slices each: 171 us as clusters, 152 + 5 us through the workspace; 24 sequences of 9000 keys, 8 kv heads of 128 in 7 slices: 222 and 141 us.
 DecodeShape decode_shape(int batch, int heads_kv, int rows, int seqlen_k) {
   const int per = rows <= 16 ? 16 : 32;
   const int64_t base = (int64_t)batch * heads_kv * ((rows + per - 1) / per);

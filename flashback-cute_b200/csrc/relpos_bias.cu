@@ -81,9 +81,9 @@ __global__ void __launch_bounds__(kThreads) relpos_fill_kernel(const __grid_cons
 // atomics, no reordering, every element read once. At the end the CTA adds up its warps' diagonals, then those of
 // each bucket (neighbours), and leaves one number per bucket in the workspace.
 // A warp reads one 16-byte vector per lane and row, 512 bytes of it; 4 rows in flight, 256 rows per CTA. Measured on 16 x 4095 x 4099 bf16
-// (537 MB): 140 us; 8 rows in flight 153; 512 / 1024 rows per CTA 178 / 196; 1 KB of a row per warp 158, 2 KB 222. Many small
+// (537 MB): 141 us; 8 rows in flight 153; 512 / 1024 rows per CTA 178 / 196; 1 KB of a row per warp 158, 2 KB 222. Many small
 // CTAs that read one region of the tensor at a time beat fewer, longer ones. Interior rows without predicates and packed
-// additions: 154 -> 142 us on a slower GPU (71 % of the issue slots before).
+// additions were worth 8 %.
 
 template <typename T> struct Vec;
 template <> struct Vec<__nv_bfloat16> { static constexpr int n = 8; };

@@ -21,8 +21,8 @@
 // read neighbouring entries; four copies, each shifted by one entry, let every thread fetch four columns with one
 // 16-byte load whatever its row.
 //
-// Measured: non-causal B2 Hq16 Hkv4 S4096 bf16, 287 us at head_dim 128 (958 TFLOP/s, 0.58 of the measured cuBLAS burst rate) and 248 at 64;
-// causal at 128, 162 us. Per block the softmax warps wait 400 of 1900 clk for scores, spend 350 on the maximum and 800 on exponentials.
+// Measured: non-causal B2 Hq16 Hkv4 S4096 bf16, 281 us at head_dim 128 (978 TFLOP/s, 0.59 of the measured cuBLAS burst rate) and 253 at 64;
+// causal at 128, 146 us (300, 264 and 160 within a training step, with the outputs that the backward wants). Per block the softmax warps wait 400 of 1900 clk for scores, spend 350 on the maximum and 800 on exponentials.
 // Tried (non-causal B2 Hq16 Hkv4 S4096 D128, at a clock where this version takes 317): blocks of 128 keys with one buffer of scores per tile 340 us (a tile waits 1550 of 3800 clk
 // for its scores); the same with the exponentials started on the maximum known so far, 348 us; two CTAs per SM with one
 // tile each and two warps per row, 372 us.
