@@ -234,7 +234,7 @@ __device__ __forceinline__ SeqInfo seq_info(const Params& p, int b) {
   return s;
 }
 
-// CTAs for that (beside the last tiles).
+// CTAs of a tensor-core launch that zero the rows of no sequence, behind those of the tiles.
 constexpr int kRestCtas = 16;
 // Zeroes the rows of `t` that belong to no sequence (before cu[0], from cu[B] on); this CTA as part `part` of `parts`.
 template <typename T>
